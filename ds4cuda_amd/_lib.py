@@ -105,6 +105,15 @@ SIGNATURES: dict[str, list] = {
     "ds4hip_session_emit_f32": [_vp, _i, _i, _vp, _vp, _vp, _vp],
     "ds4hip_session_save_to_disk": [_vp, _vp, _i, C.c_char_p],
     "ds4hip_session_load_from_disk": [_vp, C.c_char_p, C.POINTER(_i), C.POINTER(_i)],
+    "ds4hip_kv_pages_init": [_vp, _vp],
+    "ds4hip_kv_pages_workspace_bytes": [_vp],
+    "ds4hip_kv_pages_extend": [_vp, _vp, _vp, _i, _vp, _i, _vp],
+    "ds4hip_kv_pages_append": [_vp, _i, _vp, _i, _vp, _vp],
+    "ds4hip_kv_pages_fork": [_vp, _vp, _vp, _vp, _i, _i, _vp, _sz, _vp],
+    "ds4hip_kv_pages_free": [_vp, _vp, _vp, _i, _vp],
+    "ds4hip_kv_pages_compact": [_vp, _vp, _vp, _sz, _vp],
+    "ds4hip_flash_attn_window_fp8_workspace_bytes": [_i, _i, _i],
+    "ds4hip_flash_attn_window_fp8": [_vp, _vp, _sz, _vp],
     "ds4hip_ds4cudak_probe": [C.c_char_p, _vp],
     "ds4hip_session_import_ds4cudak": [_vp, C.c_char_p, C.POINTER(_i), C.POINTER(_i)],
     "ds4hip_session_export_ds4cudak": [_vp, _vp, _i, C.c_char_p],
@@ -115,6 +124,8 @@ RESTYPES = {"ds4hip_indexer_select_scratch_bytes": C.c_size_t,
             "ds4hip_flash_attn_prefill_fp8_workspace_size": C.c_size_t,
             "ds4hip_flash_attn_prefill_fp8_workspace_for": C.c_size_t,
             "ds4hip_session_state_arena_bytes": C.c_size_t,
+            "ds4hip_kv_pages_workspace_bytes": C.c_size_t,
+            "ds4hip_flash_attn_window_fp8_workspace_bytes": C.c_size_t,
             "ds4hip_session_chunk_step_workspace_bytes": C.c_size_t,
             "ds4hip_mul_mm_workspace_bytes": C.c_size_t,
             "ds4hip_compressor_batch_scratch_bytes": C.c_size_t,
@@ -128,7 +139,7 @@ _lib = None
 
 class Ds4HipError(RuntimeError):
     def __init__(self, name: str, code: int):
-        kind = "invalid argument" if code == -22 else (
+        kind = "invalid argument" if code == -22 else "no room" if code == -28 else (
             f"hip error {-1000 - code}" if code <= -1000 else "error")
         super().__init__(f"{name} failed: {code} ({kind})")
         self.code = code

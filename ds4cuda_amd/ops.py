@@ -286,6 +286,81 @@ def flash_attn_prefill_fp8(q, sinks, out, cache: Fp8KVCache, n_q, n_cached, row0
     return workspace
 
 
+class WindowAttn(C.Structure):
+    """ds4hip_window_attn (include/ds4hip_pages.h)."""
+    _fields_ = [("q", C.c_void_p), ("out", C.c_void_p), ("io_f32", C.c_int), ("sinks", C.c_void_p),
+                ("codes", C.c_void_p), ("sexp", C.c_void_p), ("tail", C.c_void_p), ("n_cache_rows", C.c_longlong),
+                ("table", C.c_void_p), ("rows", C.c_void_p), ("n_slots", C.c_int), ("table_stride", C.c_int),
+                ("page_rows", C.c_int), ("q_start", C.c_void_p), ("seq_ids", C.c_void_p), ("n_seqs", C.c_int),
+                ("n_q", C.c_int), ("n_head", C.c_int), ("window", C.c_int), ("n_first", C.c_int)]
+
+
+def window_workspace_bytes(n_seqs, n_q, n_head) -> int:
+    return lib().ds4hip_flash_attn_window_fp8_workspace_bytes(n_seqs, n_q, n_head)
+
+
+def _on_stream(stream, device):
+    """Context in which tensors are allocated for work on `stream` (None: the
+    device's current stream)."""
+    if stream is None:
+        return torch.cuda.device(device)
+    if not isinstance(stream, torch.cuda.Stream):
+        stream = torch.cuda.ExternalStream(int(getattr(stream, "value", stream) or 0), device=device)
+    return torch.cuda.stream(stream)
+
+
+def flash_attn_window_fp8(q, cache: Fp8KVCache, page_table, seq_rows, *, page_rows, window=0, n_first=0, sinks=None,
+                          q_start=None, seq_ids=None, out=None, workspace=None, stream=None):
+    """Attention over the pages of a paged FP8 cache, in a sliding window with the
+    first rows kept visible; returns out.
+
+    q [n_q, n_head, 512] bf16 or fp32 (out has its type; n_head 8, 16, 32, 64 or
+    128); page_table int32 [slots, entries] and seq_rows int32 [slots]: the pages of
+    `page_rows` rows and the rows of every sequence. Entry s is the sequence in
+    slot seq_ids[s] (or s); its last tokens are the queries q_start[s] ..
+    q_start[s + 1] - 1 (int32 [entries + 1]), or one query each where q_start is
+    None. The query at position p sees row k where k <= p and (window == 0 or k >
+    p - window or k < n_first); sinks [n_head] fp32: a sink logit per head.
+    All lengths are read on the device: a captured call follows them.
+    """
+    if q.dim() != 3 or q.shape[2] != HEAD_DIM or q.dtype not in (torch.bfloat16, torch.float32):
+        raise Ds4HipError("q must be bf16 or fp32 [n_q, n_head, 512]", -22)
+    n_q, n_head = q.shape[0], q.shape[1]
+    _check(q, q.dtype, None, "q")
+    if page_table.dim() != 2:
+        raise Ds4HipError("page_table must be [slots, entries]", -22)
+    slots, stride = page_table.shape
+    _check(page_table, torch.int32, None, "page_table")
+    _check(seq_rows, torch.int32, slots, "seq_rows")
+    _check(sinks, torch.float32, n_head, "sinks")
+    _check(q_start, torch.int32, 1, "q_start")
+    _check(seq_ids, torch.int32, None, "seq_ids")
+    _check(cache.codes, torch.uint8, cache.n_rows * N_NOPE, "codes")
+    _check(cache.sexp, torch.int8, cache.n_rows * 8, "sexp")
+    _check(cache.tail, cache.tail.dtype, cache.n_rows * N_ROT, "tail")
+    if cache.tail.element_size() != 2:
+        raise Ds4HipError("tail: expected f16 values or their bits", -22)
+    n_seqs = q_start.numel() - 1 if q_start is not None else n_q
+    if seq_ids is not None and seq_ids.numel() != n_seqs:
+        raise Ds4HipError(f"seq_ids: {n_seqs} entries expected, got {seq_ids.numel()}", -22)
+    with _on_stream(stream, q.device):
+        if out is None:
+            out = torch.empty_like(q)
+        _check(out, q.dtype, q.numel(), "out")
+        if n_q == 0 or n_seqs == 0:
+            return out
+        need = window_workspace_bytes(n_seqs, n_q, n_head)
+        if workspace is None:
+            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+        _dev(workspace, "workspace", need)
+        a = WindowAttn(_ptr(q), _ptr(out), int(q.dtype == torch.float32), _ptr(sinks), _ptr(cache.codes),
+                       _ptr(cache.sexp), _ptr(cache.tail), cache.n_rows, _ptr(page_table), _ptr(seq_rows), slots, stride,
+                       int(page_rows), _ptr(q_start), _ptr(seq_ids), n_seqs, n_q, n_head, int(window), int(n_first))
+        call("ds4hip_flash_attn_window_fp8", C.byref(a), _ptr(workspace), workspace.numel() * workspace.element_size(),
+             _stream(stream))
+    return out
+
+
 # ---- tail RoPE (cuda/rope.cuh:51, cuda/attn_out.cuh:52) ----------------------------------
 
 def launch_tail_rope_yarn_f32(x_in, x_out, n_heads, head_dim, n_rot, pos, il, stream=None):

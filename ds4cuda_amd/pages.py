@@ -1,0 +1,163 @@
+"""A paged FP8 KV cache (include/ds4hip_pages.h).
+
+`PagePool` holds pages of FP8 rows for all layers, the sequences' page tables
+and the pages' reference counts, all on the device: sequences are extended,
+forked (pages shared or copied), cut and freed, and the pool is compacted,
+without a wait for the host. What a call finds wrong on the device (too few free
+pages, a sequence that is not there) goes to `status`; `check()` reads it.
+"""
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from ._lib import Ds4HipError, call, lib
+from .ops import HEAD_DIM, N_NOPE, N_ROT, Fp8KVCache, _check, _on_stream, _ptr, _stream, flash_attn_window_fp8
+
+MAX_JOBS = 1024    # sequences of one call
+
+
+class KvPages(C.Structure):
+    """ds4hip_kv_pages."""
+    _fields_ = [("codes", C.c_void_p), ("sexp", C.c_void_p), ("tail", C.c_void_p), ("layer_rows", C.c_longlong),
+                ("n_layers", C.c_int), ("n_pages", C.c_int), ("page_rows", C.c_int), ("table_stride", C.c_int),
+                ("n_seqs", C.c_int), ("refs", C.c_void_p), ("table", C.c_void_p), ("rows", C.c_void_p),
+                ("status", C.c_void_p)]
+
+
+class PagePool:
+    """Pages of `page_rows` rows (a power of two) for every layer.
+
+    codes uint8 [layers, pages * page_rows, 448], sexp int8 [.., 8], tail f16 (or
+    its bits) [.., 64]; refs int32 [pages], table int32 [sequences, entries], rows
+    int32 [sequences]. The pool works on these tensors; entries of `table` past a
+    sequence's rows have no meaning. Calls on one pool are ordered on one stream.
+    """
+
+    def __init__(self, codes, sexp, tail, refs, table, rows, page_rows, status=None):
+        if codes.dim() != 3 or table.dim() != 2:
+            raise Ds4HipError("codes must be [layers, rows, 448] and table [sequences, entries]", -22)
+        layers, n_rows = codes.shape[0], codes.shape[1]
+        n_pages = refs.numel()
+        _check(codes, torch.uint8, layers * n_rows * N_NOPE, "codes")
+        _check(sexp, torch.int8, layers * n_rows * 8, "sexp")
+        _check(tail, tail.dtype, layers * n_rows * N_ROT, "tail")
+        _check(refs, torch.int32, None, "refs")
+        _check(table, torch.int32, None, "table")
+        _check(rows, torch.int32, table.shape[0], "rows")
+        if codes.shape[2] != N_NOPE or tail.element_size() != 2 or n_rows != n_pages * int(page_rows):
+            raise Ds4HipError("codes, tail or refs do not fit pages of that many rows", -22)
+        with torch.cuda.device(codes.device):
+            self.status = torch.zeros(1, dtype=torch.int32, device=codes.device) if status is None else status
+        _check(self.status, torch.int32, 1, "status")
+        self.codes, self.sexp, self.tail = codes, sexp, tail
+        self.refs, self.table, self.rows = refs, table, rows
+        self.page_rows, self.n_layers, self.n_pages, self.n_seqs = int(page_rows), layers, n_pages, table.shape[0]
+        self.device = codes.device
+        self.c = KvPages(_ptr(codes), _ptr(sexp), _ptr(tail), n_rows, layers, n_pages, self.page_rows, table.shape[1],
+                         self.n_seqs, _ptr(refs), _ptr(table), _ptr(rows), _ptr(self.status))
+        self._workspace = None
+
+    @classmethod
+    def empty(cls, n_pages, page_rows, n_seqs, max_rows, n_layers=1, device="cuda"):
+        """A pool with every page free, for sequences of up to max_rows rows."""
+        n = n_pages * page_rows
+        pool = cls(torch.zeros((n_layers, n, N_NOPE), dtype=torch.uint8, device=device),
+                   torch.zeros((n_layers, n, 8), dtype=torch.int8, device=device),
+                   torch.zeros((n_layers, n, N_ROT), dtype=torch.int16, device=device),
+                   torch.empty(n_pages, dtype=torch.int32, device=device),
+                   torch.empty((n_seqs, -(-max_rows // page_rows)), dtype=torch.int32, device=device),
+                   torch.empty(n_seqs, dtype=torch.int32, device=device), page_rows)
+        with torch.cuda.device(pool.device):
+            call("ds4hip_kv_pages_init", C.byref(pool.c), _stream(None))
+        return pool
+
+    def layer(self, layer) -> Fp8KVCache:
+        """The rows of one layer, as the other FP8 launchers take them."""
+        return Fp8KVCache(self.codes[layer], self.sexp[layer], self.tail[layer])
+
+    def check(self):
+        """Waits for the device; raises Ds4HipError where a call was refused there
+        since the last check (-22 or -28), and resets the status."""
+        code = int(self.status.item())
+        if code:
+            self.status.zero_()
+            raise Ds4HipError("PagePool", code)
+
+    def _jobs(self, ids, name, n=None):
+        if ids is None:
+            return 0
+        _check(ids, torch.int32, n, name)
+        if n is not None and ids.numel() != n:
+            raise Ds4HipError(f"{name}: {n} entries expected, got {ids.numel()}", -22)
+        return ids.numel()
+
+    def _ws(self, stream):
+        need = lib().ds4hip_kv_pages_workspace_bytes(C.byref(self.c))
+        if self._workspace is None:
+            with _on_stream(stream, self.device):
+                self._workspace = torch.empty(need, dtype=torch.uint8, device=self.device)
+        return self._workspace
+
+    def extend(self, seqs, n_new, n_dst, dst_rows=None, stream=None):
+        """n_new[j] more rows for sequence seqs[j] (int32 device tensors): takes the
+        lowest free pages and returns the rows' places, int64 [n_dst], job after job
+        (-1 past the last job's rows, or everywhere where the call is refused)."""
+        n = self._jobs(seqs, "seqs")
+        self._jobs(n_new, "n_new", n)
+        with _on_stream(stream, self.device):
+            if dst_rows is None:
+                dst_rows = torch.empty(n_dst, dtype=torch.int64, device=self.device)
+            _check(dst_rows, torch.int64, n_dst, "dst_rows")
+            call("ds4hip_kv_pages_extend", C.byref(self.c), _ptr(seqs), _ptr(n_new), n, _ptr(dst_rows), int(n_dst),
+                 _stream(stream))
+        return dst_rows
+
+    def append(self, kv, dst_rows, layer=0, stream=None):
+        """Quantizes fp32 rows kv [n, 512] into the layer at dst_rows (extend's); a row
+        whose place is -1 is skipped."""
+        n = kv.shape[0]
+        _check(kv, torch.float32, n * HEAD_DIM, "kv")
+        _check(dst_rows, torch.int64, n, "dst_rows")
+        with _on_stream(stream, self.device):
+            call("ds4hip_kv_pages_append", C.byref(self.c), int(layer), _ptr(kv), n, _ptr(dst_rows), _stream(stream))
+
+    def fork(self, parents, children, n_rows=None, deep=False, stream=None):
+        """children[j] (empty sequences) become copies of the first n_rows[j] rows (None
+        or negative: all) of parents[j]: full pages shared and a partly filled last page
+        copied, or every page copied (deep)."""
+        n = self._jobs(parents, "parents")
+        self._jobs(children, "children", n)
+        self._jobs(n_rows, "n_rows", n)
+        ws = self._ws(stream)
+        with _on_stream(stream, self.device):
+            call("ds4hip_kv_pages_fork", C.byref(self.c), _ptr(parents), _ptr(children), _ptr(n_rows), n, int(bool(deep)),
+                 _ptr(ws), ws.numel(), _stream(stream))
+
+    def free(self, seqs, keep=None, stream=None):
+        """Cuts sequences seqs[j] down to keep[j] rows (None: to nothing) and releases
+        their other pages."""
+        n = self._jobs(seqs, "seqs")
+        self._jobs(keep, "keep", n)
+        with _on_stream(stream, self.device):
+            call("ds4hip_kv_pages_free", C.byref(self.c), _ptr(seqs), _ptr(keep), n, _stream(stream))
+
+    def compact(self, n_live=None, stream=None):
+        """Moves the held pages to the front of the pool; returns their number, an int32
+        device scalar."""
+        ws = self._ws(stream)
+        with _on_stream(stream, self.device):
+            if n_live is None:
+                n_live = torch.empty((), dtype=torch.int32, device=self.device)
+            _check(n_live, torch.int32, 1, "n_live")
+            call("ds4hip_kv_pages_compact", C.byref(self.c), _ptr(n_live), _ptr(ws), ws.numel(), _stream(stream))
+        return n_live
+
+    def attend(self, q, *, seqs=None, q_start=None, window=0, n_first=0, sinks=None, layer=0, out=None, workspace=None,
+               stream=None):
+        """ops.flash_attn_window_fp8 over this pool's pages of one layer: the sequences
+        seqs (None: slots 0, 1, ..)."""
+        return flash_attn_window_fp8(q, self.layer(layer), self.table, self.rows, page_rows=self.page_rows, window=window,
+                                     n_first=n_first, sinks=sinks, q_start=q_start, seq_ids=seqs, out=out,
+                                     workspace=workspace, stream=stream)
