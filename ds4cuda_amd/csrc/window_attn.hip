@@ -24,10 +24,12 @@ using namespace ds4hip;
 
 namespace {
 
-constexpr int kM = 64;               // rows (queries x heads) of a problem
-constexpr int kWgs = 512;            // workgroups the line of tiles is cut for
+constexpr int kLogRows = 6, kRows = 1 << kLogRows;   // rows (queries x heads) of a problem
+constexpr int kWgs = 256;            // workgroups the line of tiles is cut for: one per CU
 constexpr int kMinTiles = 4;         // tiles of a part
+constexpr int kWhole = 8;            // tiles of a problem that is never cut
 constexpr int kMaxSeqs = 4096;
+constexpr int kInlineProbs = 512;    // problems that a workgroup lays out itself
 // P = 2^((s - m) kq + kTop) with s and the row's reference m as the matrix
 // instructions leave them and kq its scale to log2: their difference is exact where P
 // is large, at any magnitude. The reference moves only where P would pass 2^(kTop +
@@ -46,13 +48,14 @@ struct WinArgs {
     int n_seqs, n_slots, n_q, log_head, window, first, stride, shift, n_pages;
     // workspace
     int prob_cap;
+    long long *line;         // [2] tiles in all, tiles per workgroup
     int *n_prob;
-    int2 *prob;              // [prob_cap] sequence and tile of its rows
+    int4 *prob;              // [prob_cap] records
     long long *pre;          // [prob_cap + 1] tiles before each problem
     long long *wg_tile;      // [kWgs + 1] first tile of each workgroup
     int *wg_prob;            // [kWgs + 1] the problem it lies in
-    float *part_ml;          // [2 kWgs][3][kM] references, sums and scales to log2
-    float *part_o;           // [2 kWgs][kM][kD] unnormalized outputs
+    float *part_ml;          // [2 kWgs][3][kRows] references, sums and scales to log2
+    float *part_o;           // [2 kWgs][kRows][kD] unnormalized outputs
 };
 
 // The queries of sequence s: their first packed index and their number, whatever
@@ -63,35 +66,42 @@ __device__ inline int2 queries_of(const WinArgs &A, int s) {
     return make_int2(b, max(e - b, 0));
 }
 
+// The heads of a query in one problem.
+__device__ inline int log_hpt(const WinArgs &A) { return min(A.log_head, kLogRows); }
+
+// Problem `tile` of sequence s as the plan keeps it: its table row (-1: not a sequence of
+// the table, or one with more rows than its table row holds), first packed query, number of
+// queries and first head (times 256), position of its first query.
+__device__ inline int4 record_of(const WinArgs &A, int s, int tile) {
+    const int lh = log_hpt(A), lg = A.log_head - lh, qpt = kRows >> lh;
+    const int2 qs = queries_of(A, s);
+    const int q = (tile >> lg) * qpt, slot = A.seq_ids ? A.seq_ids[s] : s;
+    const bool in = slot >= 0 && slot < A.n_slots;
+    const int rows = in ? max(A.rows[slot], 0) : 0;
+    return make_int4(in && ((rows - 1) >> A.shift) < A.stride ? slot : -1, qs.x + q,
+                     min(qpt, qs.y - q) | ((tile & ((1 << lg) - 1)) << lh) << 8, rows - qs.y + q);
+}
+
 struct Problem {
-    int slot;       // table row; -1: not a sequence of the table
+    int slot;       // table row; -1: names rows that the table does not hold
     int q0, n;      // first packed query and the queries of the tile
     int head0;      // first head
-    int pos0, pos1; // positions of the first and the last query
+    int pos0, pos1; // positions of the first and the last query; pos1 < 0: it sees nothing
     int n_first, t_window, tiles;   // tiles of the first rows, first tile of the window, all tiles
-    bool bad;       // names rows that the table does not hold
+    int whole_a, whole_b, whole_c;  // tiles t < a, or b <= t, of those t < c, are seen whole by every query
 };
 
-// The rows of a tile: hpt heads (a power of two) of kM / hpt queries.
-__device__ inline int log_hpt(const WinArgs &A) { return min(A.log_head, 6); }
-
-__device__ inline Problem problem_of(const WinArgs &A, int s, int tile) {
+__device__ inline Problem problem_of(const WinArgs &A, int4 rec) {
     Problem P;
-    const int lh = log_hpt(A), groups = 1 << (A.log_head - lh), qpt = kM >> lh;
-    const int2 qs = queries_of(A, s);
-    const int q = (tile >> (A.log_head - lh)) * qpt;
-    P.q0 = qs.x + q;
-    P.n = min(qpt, qs.y - q);
-    P.head0 = (tile & (groups - 1)) << lh;
-    P.slot = A.seq_ids ? A.seq_ids[s] : s;
-    P.bad = P.slot < 0 || P.slot >= A.n_slots;
-    const int rows = P.bad ? 0 : max(A.rows[P.slot], 0);
-    P.bad = P.bad || ((rows - 1) >> A.shift) >= A.stride;
-    P.pos0 = rows - qs.y + q;
+    P.slot = rec.x;
+    P.q0 = rec.y;
+    P.n = rec.z & 255;
+    P.head0 = rec.z >> 8;
+    P.pos0 = rec.w;
     P.pos1 = P.pos0 + P.n - 1;
-    if (P.bad || P.pos1 < 0) {   // one tile that sees nothing
+    P.n_first = P.t_window = P.whole_a = P.whole_b = P.whole_c = 0;
+    if (P.slot < 0 || P.pos1 < 0) {   // one tile that sees nothing
         P.pos1 = -1;
-        P.n_first = P.t_window = 0;
         P.tiles = 1;
         return P;
     }
@@ -100,13 +110,14 @@ __device__ inline Problem problem_of(const WinArgs &A, int s, int tile) {
     P.t_window = lo / kTile;
     if (P.n_first >= P.t_window) P.n_first = P.t_window = 0;   // they meet: one run of tiles from row 0
     P.tiles = P.n_first + P.pos1 / kTile - P.t_window + 1;
+    P.whole_a = A.first / kTile;
+    P.whole_b = A.window > 0 && P.pos1 >= A.window ? (P.pos1 - A.window) / kTile + 1 : 0;
+    P.whole_c = max(P.pos0 + 1, 0) / kTile;
     return P;
 }
 
-// First key of the problem's tile i.
-__device__ inline int tile_key(const Problem &P, int i) {
-    return kTile * (i < P.n_first ? i : P.t_window + i - P.n_first);
-}
+// Tile of the keys that the problem's i-th one is.
+__device__ inline int tile_at(const Problem &P, int i) { return i < P.n_first ? i : P.t_window + i - P.n_first; }
 
 __device__ inline bool sees(const WinArgs &A, int pos, int key) {
     return key <= pos && (A.window <= 0 || key > pos - A.window || key < A.first);
@@ -114,23 +125,23 @@ __device__ inline bool sees(const WinArgs &A, int pos, int key) {
 
 // ---- plan ------------------------------------------------------------------------
 
-// Exclusive sum of v over the 1024 threads; *total receives the sum.
-template <typename T>
-__device__ inline T block_scan(T v, T *sums, T *total) {
+// Exclusive sum of v over the workgroup's kThreads threads; *total receives the sum.
+template <int kThreads>
+__device__ inline long long block_scan(long long v, long long *sums, long long *total) {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    T x = v;
+    long long x = v;
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
-        const T y = __shfl_up(x, off);
+        const long long y = __shfl_up(x, off);
         if (lane >= off) x += y;
     }
     __syncthreads();
     if (lane == 63) sums[w] = x;
     __syncthreads();
-    T before = 0, all = 0;
+    long long before = 0, all = 0;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        const T y = sums[i];
+    for (int i = 0; i < kThreads / 64; ++i) {
+        const long long y = sums[i];
         before += i < w ? y : 0;
         all += y;
     }
@@ -138,60 +149,112 @@ __device__ inline T block_scan(T v, T *sums, T *total) {
     return before + x - v;
 }
 
-__global__ __launch_bounds__(1024) void plan_kernel(const WinArgs A) {
-    __shared__ int first_s[kMaxSeqs];   // problems before each sequence
-    __shared__ int sums_i[16];
-    __shared__ long long sums_l[16];
+// put(i, record, tiles before) for every problem; returns their number and *tiles. All
+// threads of the workgroup; first_s: [n_seqs].
+template <int kThreads, typename Put>
+__device__ inline int lay_line(const WinArgs &A, int *first_s, long long *sums, long long *tiles, Put put) {
     const int tid = threadIdx.x;
-    const int lh = log_hpt(A), qpt = kM >> lh;
-    int n_prob = 0;
-    for (int s0 = 0; s0 < A.n_seqs; s0 += 1024) {
-        const int s = s0 + tid;
-        int n = s < A.n_seqs ? ((queries_of(A, s).y + qpt - 1) / qpt) << (A.log_head - lh) : 0;
-        int all;
-        const int before = n_prob + block_scan(n, sums_i, &all);
-        if (s < A.n_seqs) first_s[s] = before;
-        n_prob += all;
+    const int lh = log_hpt(A), lg = A.log_head - lh, qpt = kRows >> lh;
+    long long n_all = 0, t_all = 0;
+    if (A.q_start) {
+        for (int s0 = 0; s0 < A.n_seqs; s0 += kThreads) {
+            const int s = s0 + tid;
+            const long long n = s < A.n_seqs ? (long long)((queries_of(A, s).y + qpt - 1) / qpt) << lg : 0;
+            long long all;
+            const long long before = n_all + block_scan<kThreads>(n, sums, &all);
+            if (s < A.n_seqs) first_s[s] = (int)min(before, (long long)A.prob_cap);
+            n_all += all;
+        }
+        __syncthreads();
+    } else {
+        n_all = (long long)A.n_seqs << lg;
     }
-    __syncthreads();
-    n_prob = min(n_prob, A.prob_cap);   // (only a q_start that goes back names more)
-    long long tiles = 0;
-    for (int i0 = 0; i0 < n_prob; i0 += 1024) {
+    const int n_prob = (int)min(n_all, (long long)A.prob_cap);   // (only a q_start that goes back names more)
+    for (int i0 = 0; i0 < n_prob; i0 += kThreads) {
         const int i = i0 + tid;
+        int4 rec = make_int4(-1, 0, 0, 0);
         int n = 0;
         if (i < n_prob) {
-            int lo = 0, hi = A.n_seqs;   // the last sequence whose first problem is at most i
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) >> 1;
-                if (first_s[mid] <= i) lo = mid; else hi = mid;
+            int s = i >> lg, first = s << lg;
+            if (A.q_start) {
+                int hi = A.n_seqs;   // the last sequence whose first problem is at most i
+                s = 0;
+                while (hi - s > 1) {
+                    const int mid = (s + hi) >> 1;
+                    if (first_s[mid] <= i) s = mid; else hi = mid;
+                }
+                first = first_s[s];
             }
-            A.prob[i] = make_int2(lo, i - first_s[lo]);
-            n = problem_of(A, lo, i - first_s[lo]).tiles;
+            rec = record_of(A, s, i - first);
+            n = problem_of(A, rec).tiles;
         }
         long long all;
-        const long long before = tiles + block_scan<long long>(n, sums_l, &all);
-        if (i < n_prob) A.pre[i] = before;
-        tiles += all;
+        const long long before = t_all + block_scan<kThreads>(n, sums, &all);
+        if (i < n_prob) put(i, rec, before);
+        t_all += all;
     }
-    if (tid == 0) {
+    *tiles = t_all;
+    return n_prob;
+}
+
+__device__ inline long long tiles_per_wg(long long tiles) { return max((tiles + kWgs - 1) / kWgs, (long long)kMinTiles); }
+
+// Where a cut at tile t of the line falls that lies in the problem [begin, end): a short
+// problem stays whole (its parts would cost more than it does) and moves the cut to its nearer end.
+__device__ inline long long settle_cut(long long t, long long begin, long long end) {
+    return end - begin > kWhole ? t : 2 * t <= begin + end ? begin : end;
+}
+
+__global__ __launch_bounds__(1024) void plan_kernel(const WinArgs A) {
+    __shared__ int first_s[kMaxSeqs];   // problems before each sequence
+    __shared__ long long sums[16];
+    long long tiles;
+    const int n_prob = lay_line<1024>(A, first_s, sums, &tiles, [&](int i, int4 rec, long long before) {
+        A.prob[i] = rec;
+        A.pre[i] = before;
+    });
+    const long long per = tiles_per_wg(tiles);
+    if (threadIdx.x == 0) {
         A.pre[n_prob] = tiles;
         *A.n_prob = n_prob;
+        A.line[0] = tiles;
+        A.line[1] = per;
     }
     __syncthreads();
-    const long long per = max((tiles + kWgs - 1) / kWgs, (long long)kMinTiles);
-    for (int b = tid; b <= kWgs; b += 1024) {
-        const long long t = min(b * per, tiles);
-        int lo = 0, hi = n_prob;
+    const int b = threadIdx.x;
+    if (b > kWgs) return;
+    const long long t = b * per;
+    int lo = n_prob;
+    long long cut = tiles;
+    if (t < tiles) {
+        int hi = n_prob;
+        lo = 0;
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
             if (A.pre[mid] <= t) lo = mid; else hi = mid;
         }
-        A.wg_tile[b] = t;
-        A.wg_prob[b] = lo;
+        cut = settle_cut(t, A.pre[lo], A.pre[lo + 1]);
+        lo += cut == A.pre[lo + 1];
     }
+    A.wg_tile[b] = cut;
+    A.wg_prob[b] = lo;
 }
 
 // ---- attention -------------------------------------------------------------------
+
+// The 64-row kernel's order of dims in an LDS row: the first dim of 8-dim granule p. A
+// thread's 16-byte code chunk becomes two granules; the first ones of 16 threads lie
+// side by side and so do the second ones, so that no LDS write meets another's banks.
+__device__ inline int dim_of(int p) {
+    const int i = p >> 5, h = p >> 4 & 1, j = p & 15;
+    return i == 0 || j < 12 ? 256 * i + 16 * j + 8 * h : kNope + 8 * (j - 12) + 32 * h;
+}
+
+// The largest of the lanes 16 and 32 apart.
+__device__ inline uint32_t umax_16_32(uint32_t v) {
+    v = max(v, (uint32_t)__shfl_xor((int)v, 16));
+    return max(v, (uint32_t)__shfl_xor((int)v, 32));
+}
 
 // One of the workgroup's 16-row query tiles as f16 fragments (hi, and for fp32
 // queries lo): lane (n16, g) holds row n16's dims 32 s + 8 g .. + 8. Each row is
@@ -203,38 +266,58 @@ __device__ inline float load_q(const WinArgs &A, const Problem &P, int row, int 
     const int lh = log_hpt(A);
     const int qi = row >> lh, head = P.head0 + (row & ((1 << lh) - 1));
     const bool ok = qi < P.n;
-    const size_t at = (((size_t)(P.q0 + (ok ? qi : 0)) << A.log_head) + head) * kD + 8 * g;
-    float x[16][8];
-    float amax = 0.0f;
+    const size_t at = (((size_t)(P.q0 + (ok ? qi : 0)) << A.log_head) + head) * kD;
+    // first dim of the row's fragment s
+    auto dim = [&](int s) { return dim_of(4 * s + g); };
+    // (a row of zeros, or with a value that is not finite, is left as it is)
+    auto power = [](uint32_t amax) { return amax && amax < 0x7F800000u ? 7 - ilogbf(__uint_as_float(amax)) : 0; };
+    int e;
+    if constexpr (kF32) {
+        const float *src = static_cast<const float *>(A.q) + at;
+        float4_t x[16][2];
+        uint32_t amax = 0;   // bits of |x| compare as the values do
 #pragma unroll
-    for (int s = 0; s < 16; ++s) {
-        if (kF32) {
-            const float *src = static_cast<const float *>(A.q) + at + 32 * s;
-            const float4_t a = *reinterpret_cast<const float4_t *>(src), b = *reinterpret_cast<const float4_t *>(src + 4);
+        for (int s = 0; s < 16; ++s)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[s][i] = a[i], x[s][4 + i] = b[i];
-        } else {
-            const uint4_t v = *reinterpret_cast<const uint4_t *>(static_cast<const uint16_t *>(A.q) + at + 32 * s);
+            for (int h = 0; h < 2; ++h) x[s][h] = *reinterpret_cast<const float4_t *>(src + dim(s) + 4 * h);
+        __builtin_amdgcn_sched_barrier(0);   // all in flight before the first is used
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                x[s][2 * i] = bf16_to_f32((uint16_t)(v[i] & 0xFFFF));
-                x[s][2 * i + 1] = bf16_to_f32((uint16_t)(v[i] >> 16));
+        for (int s = 0; s < 16; ++s)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) amax = max(amax, __float_as_uint(x[s][h][i]) & 0x7FFFFFFFu);
             }
-        }
+        e = power(umax_16_32(amax));
 #pragma unroll
-        for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(x[s][i]));
+        for (int s = 0; s < 16; ++s)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float v = ok ? ldexpf(x[s][i >> 2][i & 3], e) : 0.0f;
+                hi[s][i] = (half_t)v;
+                lo[s][i] = (half_t)(v - (float)hi[s][i]);
+            }
+    } else {
+        const uint16_t *src = static_cast<const uint16_t *>(A.q) + at;
+        uint4_t x[16];
+        uint32_t amax = 0;
+#pragma unroll
+        for (int s = 0; s < 16; ++s) x[s] = *reinterpret_cast<const uint4_t *>(src + dim(s));
+        __builtin_amdgcn_sched_barrier(0);   // all in flight before the first is used
+#pragma unroll
+        for (int s = 0; s < 16; ++s) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) amax = max(max(amax, x[s][i] << 16 & 0x7FFF0000u), x[s][i] & 0x7FFF0000u);
+        }
+        e = power(umax_16_32(amax));
+#pragma unroll
+        for (int s = 0; s < 16; ++s)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float v = __uint_as_float(i & 1 ? x[s][i >> 1] & 0xFFFF0000u : x[s][i >> 1] << 16);
+                hi[s][i] = (half_t)(ok ? ldexpf(v, e) : 0.0f);
+            }
     }
-    amax = xmax_16_32(amax);
-    // (a row of zeros, or with an infinity, is left as it is)
-    const int e = amax > 0.0f && amax < INFINITY ? 7 - ilogbf(amax) : 0;
-#pragma unroll
-    for (int s = 0; s < 16; ++s)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float v = ok ? ldexpf(x[s][i], e) : 0.0f;
-            hi[s][i] = (half_t)v;
-            if (kF32) lo[s][i] = (half_t)(v - (float)hi[s][i]);
-        }
     return ldexpf(1.0f, -e);
 }
 
@@ -243,242 +326,509 @@ __device__ inline float sink_term(const WinArgs &A, int head, float m, float kq)
     return A.sinks ? __builtin_amdgcn_exp2f(fmaf(-m, kq, fmaf(A.sinks[head], kLog2e, kTop))) : 0.0f;
 }
 
+// Four outputs, rounded to bf16 unless the call's type is fp32.
 template <bool kF32>
-__global__ __launch_bounds__(256) void window_kernel(const WinArgs A) {
-    __shared__ __attribute__((aligned(16))) uint8_t stage[kStageB];
-    __shared__ __attribute__((aligned(16))) half8_t pb[2][4][64];   // [hi, lo][row tile][lane]
-    __shared__ float fac_s[kM], m_s[kM], l_s[kM], kq_s[kM];
-    __shared__ uint32_t odd_s[4];   // keys whose scores are not finite, per wave
-    __shared__ int bad_s;
-
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-    const int n16 = lane & 15, g = lane >> 4;
-    const int wg = blockIdx.x;
-    const int n_prob = *A.n_prob;
-    long long t = A.wg_tile[wg];
-    const long long t_end = A.wg_tile[wg + 1];
-    uint32_t ka[2], va[2];
-#pragma unroll
-    for (int kt = 0; kt < 2; ++kt) {
-        const int r = pi_key(16 * kt + n16);
-        ka[kt] = r * kRowB + ((16 * g) ^ row_swz(r));
-        const int v = pi_key(16 * kt + 4 * g + (n16 >> 2));
-        va[kt] = lds_addr(stage) + v * kRowB + 256 * w + ((8 * (n16 & 3)) ^ row_swz(v));
-    }
-
-    for (int pi = A.wg_prob[wg]; t < t_end && pi < n_prob; ++pi) {
-        const long long p_begin = A.pre[pi], p_end = A.pre[pi + 1];
-        const int2 id = A.prob[pi];
-        const Problem P = problem_of(A, id.x, id.y);
-        const bool begins = t == p_begin, ends = p_end <= t_end;
-        const int i0 = (int)(t - p_begin), i1 = (int)(min(p_end, t_end) - p_begin);
-        t = min(p_end, t_end);
-        const int row = 16 * w + n16, lh = log_hpt(A);
-        const int pos = P.pos0 + min(row >> lh, P.n - 1);   // (rows past the queries repeat the last one's)
-        half8_t qh[16], ql[16];
-        const float unit = load_q<kF32>(A, P, row, g, qh, ql);
-        const float kq = unit * (kLog2e / 22.62741699796952f);   // 1 / sqrt(512), in the exp2 domain
-        float4_t o[4][8];
-#pragma unroll
-        for (int a = 0; a < 4; ++a)
-#pragma unroll
-            for (int b = 0; b < 8; ++b) o[a][b] = float4_t{0, 0, 0, 0};
-        float m = -INFINITY, l = 0.0f;
-        bool bad = P.bad;
-        if (tid == 0) bad_s = 0;
-        for (int i = i0; i < i1 && P.pos1 >= 0; ++i) {
-            const int key0 = tile_key(P, i);
-            {
-                const int r = min(key0 + (tid >> 3), P.pos1);
-                int page = A.table[(long long)P.slot * A.stride + (r >> A.shift)];
-                if (page < 0 || page >= A.n_pages) {
-                    bad = true;
-                    page = 0;
-                }
-                Raw R;
-                load_raw_row(A.codes, A.sexp, A.tail,
-                             ((long long)page << A.shift) + (r & ((1 << A.shift) - 1)), tid & 7, R);
-                __syncthreads();   // the last tile's readers are done
-                store_tile(stage, tid, R);
-            }
-            __syncthreads();
-            float4_t acc[2];
-#pragma unroll
-            for (int kt = 0; kt < 2; ++kt) {
-                acc[kt] = float4_t{0, 0, 0, 0};
-#pragma unroll
-                for (int s = 0; s < 16; ++s) {
-                    const half8_t k = *reinterpret_cast<const half8_t *>(stage + ka[kt] + 64 * s);
-                    acc[kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh[s], acc[kt], 0, 0, 0);
-                    if (kF32) acc[kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql[s], acc[kt], 0, 0, 0);
-                }
-            }
-            const bool edge = !(key0 + kTile - 1 <= P.pos0 &&
-                                (A.window <= 0 || key0 > P.pos1 - A.window || key0 + kTile - 1 < A.first));
-            float mx = -INFINITY;
-            if (edge) {
-                uint32_t odd = 0;
-#pragma unroll
-                for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const int k = pi_key(16 * kt + 4 * g + r);
-                        const uint64_t b = __ballot(!(fabsf(acc[kt][r]) < INFINITY));
-                        if (((b >> (16 * g)) & 0xFFFF) == 0xFFFF) odd |= 1u << k;
-                        if (!sees(A, pos, key0 + k))
-                            acc[kt][r] = -INFINITY;
-                        else if (!(fabsf(acc[kt][r]) < INFINITY))
-                            acc[kt][r] = __builtin_nanf("");
-                    }
-                odd |= __shfl_xor(odd, 16);
-                odd |= __shfl_xor(odd, 32);
-                if (lane == 0) odd_s[w] = odd;
-            }
-#pragma unroll
-            for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) mx = fmaxf(mx, acc[kt][r]);
-            mx = xmax_16_32(mx);
-            float fac = 1.0f;
-            if ((mx - m) * kq > kLazy) {   // (m is -inf before the first key seen)
-                fac = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - mx) * kq);
-                m = mx;
-            }
-            l *= fac;
-            half8_t ph, pl;
-#pragma unroll
-            for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const float p = acc[kt][r] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(fmaf(acc[kt][r] - m, kq, kTop));
-                    const half_t h = (half_t)p;
-                    ph[4 * kt + r] = h;
-                    if (kF32) pl[4 * kt + r] = (half_t)(p - (float)h);
-                    l += kF32 ? p : (float)h;
-                }
-            pb[0][w][lane] = ph;
-            if (kF32) pb[1][w][lane] = pl;
-            if (g == 0) fac_s[row] = fac;
-            __syncthreads();
-            if (edge) {
-                uint32_t odd = odd_s[0] & odd_s[1] & odd_s[2] & odd_s[3];
-                // A row that is not finite and that some query must not see: zeroed in this
-                // wave's own dims (0 x inf would reach it). Queries that see it have a P that is not finite.
-                while (odd) {
-                    const int k = __builtin_ctz(odd);
-                    odd &= odd - 1;
-                    *reinterpret_cast<uint32_t *>(stage + k * kRowB + 256 * w + ((4 * lane) ^ row_swz(k))) = 0;
-                }
-                asm volatile("" ::: "memory");   // before the reads below, which are asm
-            }
-            half8_t vb[8];
-            read_vt4<0>(va[0], va[1], vb);
-            read_vt4<4>(va[0], va[1], vb + 4);
-#pragma unroll
-            for (int rt = 0; rt < 4; ++rt) {
-                const half8_t h = pb[0][rt][lane];
-                float f[4];
-#pragma unroll
-                for (int r = 0; r < 4; ++r) f[r] = fac_s[16 * rt + 4 * g + r];
-#pragma unroll
-                for (int dt = 0; dt < 8; ++dt) {
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) o[rt][dt][r] *= f[r];
-                    o[rt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(h, vb[dt], o[rt][dt], 0, 0, 0);
-                    if (kF32)
-                        o[rt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(pb[1][rt][lane], vb[dt], o[rt][dt], 0, 0, 0);
-                }
-            }
-        }
-        __syncthreads();
-        l = xsum_16_32(l);
-        if (g == 0) {
-            m_s[row] = m;
-            l_s[row] = l;
-            kq_s[row] = kq;
-        }
-        if (__any(bad) && lane == 0) bad_s = 1;
-        __syncthreads();
-        const float nan = bad_s ? __builtin_nanf("") : 0.0f;
-        if (begins && ends) {
-#pragma unroll
-            for (int rt = 0; rt < 4; ++rt)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int rr = 16 * rt + 4 * g + r, qi = rr >> lh, head = P.head0 + (rr & ((1 << lh) - 1));
-                    if (qi >= P.n) continue;
-                    const float mm = m_s[rr];
-                    const float sink = sink_term(A, head, mm, kq_s[rr]);
-                    const float inv = mm == -INFINITY ? nan : 1.0f / (l_s[rr] + sink) + nan;
-                    const size_t at = (((size_t)(P.q0 + qi) << A.log_head) + head) * kD + 128 * w + n16;
-#pragma unroll
-                    for (int dt = 0; dt < 8; ++dt) {
-                        const float v = o[rt][dt][r] * inv;
-                        if (kF32)
-                            static_cast<float *>(A.out)[at + 16 * dt] = v;
-                        else
-                            static_cast<__bf16 *>(A.out)[at + 16 * dt] = (__bf16)v;
-                    }
-                }
-        } else {
-            const int slot = 2 * wg + (begins ? 1 : 0);
-            if (tid < kM) {
-                float *ml = A.part_ml + (size_t)slot * 3 * kM + tid;
-                ml[0] = m_s[tid];
-                ml[kM] = l_s[tid] + nan;
-                ml[2 * kM] = kq_s[tid];
-            }
-            float *dst = A.part_o + ((size_t)slot * kM + 4 * g) * kD + 128 * w + n16;
-#pragma unroll
-            for (int rt = 0; rt < 4; ++rt)
-#pragma unroll
-                for (int dt = 0; dt < 8; ++dt)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) dst[(16 * rt + r) * kD + 16 * dt] = o[rt][dt][r];
-        }
-        __syncthreads();   // bad_s, m_s and l_s are free again
+__device__ inline void store_out(void *out, size_t at, float4_t v) {
+    if (kF32) {
+        *reinterpret_cast<float4_t *>(static_cast<float *>(out) + at) = v;
+    } else {
+        typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+        *reinterpret_cast<bf16x4 *>(static_cast<__bf16 *>(out) + at) = __builtin_convertvector(v, bf16x4);
     }
 }
 
-// The parts of each problem that a cut falls into, in order, and the sink. One
-// workgroup per four rows and first cut of a problem; a lane's eight dims.
-template <bool kF32>
-__global__ __launch_bounds__(256) void window_merge_kernel(const WinArgs A) {
-    const int b = blockIdx.x / (kM / 4), row = 4 * (blockIdx.x % (kM / 4)) + (threadIdx.x >> 6), lane = threadIdx.x & 63;
-    const int n_prob = *A.n_prob, pi = A.wg_prob[b + 1];
+// v, as a value the compiler does not know: what rare paths derive from it is computed
+// there again, not kept in registers through the loop (where a spilled one's reload would
+// wait for every copy in flight).
+__device__ inline int again(int v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
+
+// ---- 64 rows ----------------------------------------------------------------------
+//
+// bf16: eight waves, two per SIMD, so that one's matrix instructions run under the other's
+// vector instructions and waits (four waves of twice the work each: 2.07 us a tile, eight
+// 1.6). fp32: four waves, whose queries' hi and lo halves and outputs take the registers of
+// two. Wave w has rows 16 (w % 4) .. + 16 and one half of the tile's keys (of eight waves; else both) for
+// scores and softmax, and an equal share of the dims of all rows for O += P V.
+
+// The thread's share of a tile: of row tid / 16, code chunks j and (j < 12) j + 16 of 16
+// bytes, j = tid % 16, the row's exponents and its tail's dims 4 j .. + 4.
+struct Part {
+    uint4_t c[2];
+    uint2_t t, e;
+};
+
+__device__ inline void load_part(const WinArgs &A, long long row, int j, Part &R) {
+    const uint8_t *cp = A.codes + row * kNope + 16 * j;
+    R.c[0] = *reinterpret_cast<const uint4_t *>(cp);
+    // (every thread loads, so that the counts of loads in flight are the same on all paths)
+    R.c[1] = *reinterpret_cast<const uint4_t *>(cp + (j < 12 ? 256 : 0));
+    R.e = *reinterpret_cast<const uint2_t *>(A.sexp + row * 8);
+    R.t = *reinterpret_cast<const uint2_t *>(A.tail + row * kRot + 4 * j);
+}
+
+__device__ inline void store_part(uint8_t *stage, int tid, const Part &R) {
+    const int row = tid >> 4, j = tid & 15;   // (of the 16 or 32 rows at stage)
+    uint8_t *rp = stage + row * kRowB;
+    const uint32_t x = row_swz(row);
+    uint8_t *p = rp + ((16 * j) ^ x);   // dim_of's order
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        if (i == 1 && j >= 12) break;
+        const int e = (int)(int8_t)(R.e[i] >> (8 * (j >> 2)));   // block j / 4 + 4 i
+        const float sc = __uint_as_float((uint32_t)(e + 127) << 23);
+        half2_t h[8];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            h[2 * k] = cvt2<false>(R.c[i][k], sc);
+            h[2 * k + 1] = cvt2<true>(R.c[i][k], sc);
+        }
+        *reinterpret_cast<half8_t *>(p + 512 * i) = half8_t{h[0][0], h[0][1], h[1][0], h[1][1], h[2][0], h[2][1], h[3][0], h[3][1]};
+        *reinterpret_cast<half8_t *>(p + 512 * i + 256) = half8_t{h[4][0], h[4][1], h[5][0], h[5][1], h[6][0], h[6][1], h[7][0], h[7][1]};
+    }
+    const int u = j >> 1;   // tail granule
+    *reinterpret_cast<uint2_t *>(rp + ((512 + 16 * (12 + (u & 3)) + 256 * (u >> 2) + 8 * (j & 1)) ^ x)) = R.t;
+}
+
+// Iteration i, with one barrier: scores of tile i | tile i + 1 dequantized, a later one
+// fetched | P of tile i | O += P V of tile i - 1. P is computed against the references of the
+// tile before. Where a row outgrows its reference, P's tile is marked, and before it is
+// used all waves agree on new references, rescale and compute it again from its scores:
+// always on the first tile, seldom after it.
+template <bool kF32, bool kInline>
+__global__ __launch_bounds__(kF32 ? 256 : 512, kF32 ? 1 : 2) void window_kernel(const WinArgs A) {
+    constexpr int kW = kF32 ? 4 : 8;     // waves
+    constexpr int kN = 8 / kW;           // key halves of a wave, and thread rows of a tile
+    constexpr int kDT = 4 * kN;          // dim tiles of a wave
+    constexpr int kDB = 1024 / kW;       // its bytes of an f16 row
+    __shared__ __attribute__((aligned(16))) uint8_t stages[3][kStageB];
+    __shared__ __attribute__((aligned(16))) half4_t pb[2][kF32 ? 2 : 1][4][64][2];   // [buffer][hi, lo][row tile][lane][key half]
+    __shared__ float top_s[2][kRows], l_s[2][kRows], m_s[kRows], kq_s[kRows];
+    __shared__ uint32_t odd_s[2][8];   // keys whose scores are not finite, per wave
+    __shared__ __attribute__((aligned(16))) int moved_s[2][8];   // whether a row of the wave's outgrew its reference
+    __shared__ int bad_s;
+
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    const int n16 = lane & 15, g = lane >> 4, row = 16 * (w & 3) + n16;
+    const int kh = w >> 2;   // the wave's (first) key half
+    const int wg = blockIdx.x;
+    // Few problems: every workgroup lays out the line itself, and the first one leaves it
+    // to the merge; else the plan kernel did.
+    __shared__ __attribute__((aligned(16))) int4 prob_s[kInline ? kInlineProbs : 1];
+    __shared__ long long pre_s[kInline ? kInlineProbs + 1 : 1], sums_s[kInline ? 8 : 1];
+    __shared__ int first_s[kInline ? kInlineProbs : 1];
+    int n_prob, pi;
+    long long t, t_end;
+    if constexpr (kInline) {
+        long long tiles;
+        n_prob = lay_line<64 * kW>(A, first_s, sums_s, &tiles, [&](int i, int4 rec, long long before) {
+            prob_s[i] = rec;
+            pre_s[i] = before;
+        });
+        if (tid == 0) pre_s[n_prob] = tiles;
+        __syncthreads();
+        const long long per = tiles_per_wg(tiles);
+        if (wg == 0) {
+            for (int i = tid; i < n_prob; i += 64 * kW) {
+                A.prob[i] = prob_s[i];
+                A.pre[i] = pre_s[i];
+            }
+            if (tid == 0) {
+                A.pre[n_prob] = tiles;
+                *A.n_prob = n_prob;
+                A.line[0] = tiles;
+                A.line[1] = per;
+            }
+        }
+        long long cut[2];
+        pi = 0;
+#pragma unroll
+        for (int e = 1; e >= 0; --e) {   // (the workgroup's first problem is found last)
+            const long long at = (wg + e) * per;
+            cut[e] = tiles;
+            if (at < tiles) {
+                int hi = n_prob;
+                pi = 0;
+                while (hi - pi > 1) {
+                    const int mid = (pi + hi) >> 1;
+                    if (pre_s[mid] <= at) pi = mid; else hi = mid;
+                }
+                cut[e] = settle_cut(at, pre_s[pi], pre_s[pi + 1]);
+                pi += cut[e] == pre_s[pi + 1];
+            }
+        }
+        t = cut[0];
+        t_end = cut[1];
+    } else {
+        n_prob = *A.n_prob;
+        pi = A.wg_prob[wg];
+        t = A.wg_tile[wg];
+        t_end = A.wg_tile[wg + 1];
+    }
+    const int lh = log_hpt(A);
+    uint32_t ka[kN], va[2];
+    {
+#pragma unroll
+        for (int u = 0; u < kN; ++u) {
+            const int r = pi_key(16 * (kh + u) + n16);
+            ka[u] = r * kRowB + ((16 * g) ^ row_swz(r));
+        }
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) {
+            const int v = pi_key(16 * kt + 4 * g + (n16 >> 2));
+            va[kt] = lds_addr(stages[0]) + v * kRowB + kDB * w + ((8 * (n16 & 3)) ^ row_swz(v));
+        }
+    }
+    // first of the lane's four dims of the wave's dim tile dt
+    auto out_dim = [&](int dt) { return dim_of(kDB / 16 * w + 2 * dt + (g >> 1)) + 4 * (g & 1); };
+
+    for (; t < t_end && pi < n_prob; ++pi) {
+        const long long p_begin = kInline ? pre_s[kInline ? pi : 0] : A.pre[pi], p_end = kInline ? pre_s[kInline ? pi + 1 : 0] : A.pre[pi + 1];
+        const int4 rec = kInline ? prob_s[kInline ? pi : 0] : A.prob[pi];
+        const Problem P = problem_of(A, make_int4(__builtin_amdgcn_readfirstlane(rec.x), __builtin_amdgcn_readfirstlane(rec.y),
+                                                  __builtin_amdgcn_readfirstlane(rec.z), __builtin_amdgcn_readfirstlane(rec.w)));
+        const bool begins = t == p_begin, ends = p_end <= t_end;
+        const int i0 = __builtin_amdgcn_readfirstlane((int)(t - p_begin)), i1 = __builtin_amdgcn_readfirstlane((int)(min(p_end, t_end) - p_begin));
+        t = min(p_end, t_end);
+        bool bad = P.slot < 0;
+        float4_t o[4][kDT];
+#pragma unroll
+        for (int a = 0; a < 4; ++a)
+#pragma unroll
+            for (int b = 0; b < kDT; ++b) o[a][b] = float4_t{0, 0, 0, 0};
+        if (tid == 0) bad_s = 0;
+        if (P.pos1 >= 0) {   // else its one tile sees nothing
+            // row tiles in use; the waves of the others only share the rest
+            const int n_rt = ((P.n << lh) + 15) >> 4;
+            const bool scores_mine = (w & 3) < n_rt;
+            // the thread's u-th row of tile i (past the last row seen: that row again, masked), and its page
+            auto row_of = [&](int i, int u) { return min(kTile * tile_at(P, min(i, i1 - 1)) + (tid >> 4) + 16 * u, P.pos1); };
+            auto page_of = [&](int i, int u) { return A.table[(long long)P.slot * A.stride + (row_of(i, u) >> A.shift)]; };
+            Part R[kN];
+            int page[kN];
+            // fetches tile i + 2 (the pages after it first: waiting for a page must not wait for the
+            // rows). An entry outside the pool reads row 0
+            auto advance = [&](int i) {
+                int next[kN];
+#pragma unroll
+                for (int u = 0; u < kN; ++u) next[u] = page_of(i + 3, u);
+#pragma unroll
+                for (int u = 0; u < kN; ++u) {
+                    if (page[u] < 0 || page[u] >= A.n_pages) {
+                        bad = true;
+                        page[u] = 0;
+                    }
+                    load_part(A, ((long long)page[u] << A.shift) + (row_of(i + 2, u) & ((1 << A.shift) - 1)), tid & 15, R[u]);
+                    page[u] = next[u];
+                }
+            };
+            auto store = [&](int stage) {
+#pragma unroll
+                for (int u = 0; u < kN; ++u) store_part(stages[0] + stage + 16 * u * kRowB, tid, R[u]);
+            };
+#pragma unroll
+            for (int u = 0; u < kN; ++u) page[u] = page_of(i0, u);
+            advance(i0 - 2);
+            half8_t qh[16], ql[kF32 ? 16 : 1];
+            const float kq = load_q<kF32>(A, P, row, g, qh, ql) * (kLog2e / 22.62741699796952f);   // 1 / sqrt(512)
+            const int pos = P.pos0 + min(row >> lh, P.n - 1);   // (rows past the queries repeat the last one's)
+            float m = -INFINITY, l = 0.0f, sum = 0.0f;
+            float ref = 0.0f;   // m, or 0 while there is none
+            store(0);
+            advance(i0 - 1);
+            int sp = 2 * kStageB, sc = 0, sn = kStageB;   // stages of tiles i - 1, i, i + 1
+            int buf = 0;                                  // P's of tile i
+            float4_t acc[kN];                             // scores of the tile whose P is the newest
+
+            // P of the scores in acc into buffer b
+            auto weights = [&](int b) {
+                sum = 0.0f;
+#pragma unroll
+                for (int u = 0; u < kN; ++u) {
+                    half4_t ph, pl;
+                    float p[4];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        p[r] = __builtin_amdgcn_exp2f(fmaf(acc[u][r] - ref, kq, kTop));
+                        ph[r] = (half_t)p[r];
+                        if (kF32) pl[r] = (half_t)(p[r] - (float)ph[r]);
+                    }
+                    if (kF32) {
+                        sum += (p[0] + p[1]) + (p[2] + p[3]);
+                    } else {   // of the rounded values: the output stays an average
+                        const half2_t one = {(half_t)1.0f, (half_t)1.0f};
+                        sum = __builtin_amdgcn_fdot2(half2_t{ph[0], ph[1]}, one, sum, false);
+                        sum = __builtin_amdgcn_fdot2(half2_t{ph[2], ph[3]}, one, sum, false);
+                    }
+                    pb[b][0][w & 3][lane][kh + u] = ph;
+                    if (kF32) pb[b][kF32 ? 1 : 0][w & 3][lane][kh + u] = pl;
+                }
+            };
+            auto top_of = [&]() {
+                float x = -INFINITY;
+#pragma unroll
+                for (int u = 0; u < kN; ++u) x = fmaxf(x, fmaxf(fmaxf(acc[u][0], acc[u][1]), fmaxf(acc[u][2], acc[u][3])));
+                return x;
+            };
+
+            // O += P V of the tile in stage sp, whose P lies in buffer b (after a barrier)
+            auto settle = [&](int b, int4 f0, int4 f1) {
+                int any = f0.x | f0.y | f0.z | f0.w;
+                if (kW == 8) any |= f1.x | f1.y | f1.z | f1.w;
+                if (__builtin_amdgcn_readfirstlane(any)) {
+                    const int lane_r = again(lane), n_r = lane_r & 15, row_r = 16 * (w & 3) + n_r;
+                    const float top = xmax_16_32(top_of());   // (all lanes take part)
+                    if (lane_r < 16 && scores_mine) top_s[kh][row_r] = top;
+                    lds_barrier();
+                    // every lane: its own row's reference, and those of its output rows
+                    auto renew = [&](int r, float &old, float scale) {
+                        const float top = kW == 8 ? fmaxf(top_s[0][r], top_s[1][r]) : top_s[0][r];
+                        float f = 1.0f;
+                        if ((top - old) * scale > kLazy) {   // (-inf before the first key seen)
+                            f = old == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((old - top) * scale);
+                            old = top;
+                        }
+                        return f;
+                    };
+#pragma unroll
+                    for (int rt = 0; rt < 4; ++rt) {
+                        if (rt >= n_rt) break;
+                        float old = m_s[16 * rt + n_r];
+                        const float f = renew(16 * rt + n_r, old, kq_s[16 * rt + n_r]);
+#pragma unroll
+                        for (int dt = 0; dt < kDT; ++dt) o[rt][dt] *= f;
+                    }
+                    if (scores_mine) {
+                        l *= renew(row_r, m, kq);
+                        ref = m == -INFINITY ? 0.0f : m;
+                        weights(b);
+                    }
+                    lds_barrier();
+                    if (scores_mine && kh == 0 && lane_r < 16) m_s[row_r] = m;   // (read again after more barriers)
+                }
+                l += sum;
+            };
+            auto add = [&](int b, bool edge) {
+                if (edge) {
+                    uint32_t odd = odd_s[b][0] & odd_s[b][1] & odd_s[b][2] & odd_s[b][3];
+                    if (kW == 8) odd |= odd_s[b][4] & odd_s[b][5] & odd_s[b][6] & odd_s[b][7];
+                    odd = __builtin_amdgcn_readfirstlane(odd);
+                    // A row that is not finite and that some query must not see: zeroed in this wave's own
+                    // dims (0 x inf would reach it). Queries that see it have a P that is not finite.
+                    while (odd) {
+                        const int k = __builtin_ctz(odd);
+                        odd &= odd - 1;
+                        if (4 * lane < kDB)
+                            *reinterpret_cast<uint32_t *>(stages[0] + sp + k * kRowB + kDB * w + ((4 * lane) ^ row_swz(k))) = 0;
+                    }
+                    asm volatile("" ::: "memory");   // before the reads below, which are asm
+                }
+#pragma unroll
+                for (int d0 = 0; d0 < kDT; d0 += 4) {
+                    half8_t vb[4];
+                    if (d0 == 0)
+                        read_vt4<0>(va[0] + sp, va[1] + sp, vb);
+                    else
+                        read_vt4<4>(va[0] + sp, va[1] + sp, vb);
+#pragma unroll
+                    for (int rt = 0; rt < 4; ++rt) {
+                        if (rt >= n_rt) break;
+                        const half8_t h = *reinterpret_cast<const half8_t *>(&pb[b][0][rt][lane][0]);
+#pragma unroll
+                        for (int dt = 0; dt < 4; ++dt)
+                            o[rt][d0 + dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vb[dt], h, o[rt][d0 + dt], 0, 0, 0);
+                        if (kF32) {
+                            const half8_t lo = *reinterpret_cast<const half8_t *>(&pb[b][kF32 ? 1 : 0][rt][lane][0]);
+#pragma unroll
+                            for (int dt = 0; dt < 4; ++dt)
+                                o[rt][d0 + dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vb[dt], lo, o[rt][d0 + dt], 0, 0, 0);
+                        }
+                    }
+                }
+            };
+
+            if (kh == 0 && g == 0) {
+                m_s[row] = m;
+                kq_s[row] = kq;
+            }
+            bool edge_before = false;
+            auto step = [&](int i) {
+                const bool live = i < i1;
+                lds_barrier();
+                const int4 f0 = *reinterpret_cast<const int4 *>(&moved_s[buf ^ 1][0]), f1 = *reinterpret_cast<const int4 *>(&moved_s[buf ^ 1][4]);
+                float4_t a[kN][2];   // two chains each
+                if (live && scores_mine) {
+                    const uint8_t *st = stages[0] + sc;
+#pragma unroll
+                    for (int u = 0; u < kN; ++u) a[u][0] = a[u][1] = float4_t{0, 0, 0, 0};
+                    half8_t k[2][kN][2];   // K fragments, read two steps ahead
+#pragma unroll
+                    for (int u = 0; u < kN; ++u)
+#pragma unroll
+                        for (int v = 0; v < 2; ++v) k[0][u][v] = *reinterpret_cast<const half8_t *>(st + ka[u] + 64 * v);
+#pragma unroll
+                    for (int s0 = 0; s0 < 16; s0 += 2) {
+                        const int now = (s0 / 2) & 1;
+#pragma unroll
+                        for (int u = 0; u < kN; ++u)
+#pragma unroll
+                            for (int v = 0; v < 2; ++v)
+                                if (s0 < 14) k[now ^ 1][u][v] = *reinterpret_cast<const half8_t *>(st + ka[u] + 64 * (s0 + 2 + v));
+#pragma unroll
+                        for (int u = 0; u < kN; ++u)
+#pragma unroll
+                            for (int v = 0; v < 2; ++v)
+                                a[u][v] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[now][u][v], qh[s0 + v], a[u][v], 0, 0, 0);
+                        if (kF32)
+#pragma unroll
+                            for (int u = 0; u < kN; ++u)
+#pragma unroll
+                                for (int v = 0; v < 2; ++v)
+                                    a[u][v] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[now][u][v], ql[kF32 ? s0 + v : 0], a[u][v], 0, 0, 0);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                }
+                if (i > i0) {
+                    settle(buf ^ 1, f0, f1);   // (acc: still the scores of the tile before)
+                    add(buf ^ 1, edge_before);
+                }
+                if (!live) return;
+                store(sn);
+                advance(i);
+#pragma unroll
+                for (int u = 0; u < kN; ++u) acc[u] = a[u][0] + a[u][1];
+                const int tile = tile_at(P, i), key0 = kTile * tile;
+                const bool edge = !(tile < P.whole_c && (tile >= P.whole_b || tile < P.whole_a));
+                if (edge) {
+                    uint32_t odd = 0;
+                    const int lane_r = again(lane), g_r = lane_r >> 4;
+#pragma unroll
+                    for (int u = 0; u < kN; ++u)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const int k = pi_key(16 * (kh + u) + 4 * g_r + r);
+                            const bool fine = fabsf(acc[u][r]) < INFINITY;
+                            if (((__ballot(!fine) >> (16 * g_r)) & 0xFFFF) == 0xFFFF) odd |= 1u << k;
+                            acc[u][r] = !sees(A, pos, key0 + k) ? -INFINITY : fine ? acc[u][r] : __builtin_nanf("");
+                        }
+                    odd |= __shfl_xor(odd, 16);
+                    odd |= __shfl_xor(odd, 32);
+                    if (lane_r == 0) odd_s[buf][w] = scores_mine ? odd : ~0u;
+                }
+                const bool moved = scores_mine && __any((top_of() - m) * kq > kLazy);
+                if (lane == 0) moved_s[buf][w] = moved;
+                if (scores_mine) weights(buf);
+                edge_before = edge;
+                buf ^= 1;
+                const int free = sp;
+                sp = sc;
+                sc = sn;
+                sn = free;
+            };
+            for (int i = i0; i <= i1; ++i) step(i);   // (the last one only adds the tile before: the code of settle and add stands once)
+            l = xsum_16_32(l);
+            if (g == 0) l_s[kh][row] = l;
+        } else if (tid < kRows) {
+            m_s[tid] = -INFINITY;
+        }
+        if (__any(bad) && lane == 0) bad_s = 1;
+        lds_barrier();
+        const float nan = bad_s ? __builtin_nanf("") : 0.0f;
+        if (begins && ends) {
+#pragma unroll
+            for (int rt = 0; rt < 4; ++rt) {
+                const int rr = 16 * rt + n16, qi = rr >> lh, head = P.head0 + (rr & ((1 << lh) - 1));
+                if (qi >= P.n) continue;
+                const float mm = m_s[rr];
+                const float sum = kW == 8 ? l_s[0][rr] + l_s[1][rr] : l_s[0][rr];
+                const float inv = mm == -INFINITY ? nan : 1.0f / (sum + sink_term(A, head, mm, kq_s[rr])) + nan;
+                const size_t at = (((size_t)(P.q0 + qi) << A.log_head) + head) * kD;
+#pragma unroll
+                for (int dt = 0; dt < kDT; ++dt) store_out<kF32>(A.out, at + out_dim(dt), o[rt][dt] * inv);
+            }
+        } else {
+            const int slot = 2 * wg + (begins ? 1 : 0);
+            if (tid < kRows) {
+                float *ml = A.part_ml + (size_t)slot * 3 * kRows + tid;
+                ml[0] = m_s[tid];
+                ml[kRows] = (kW == 8 ? l_s[0][tid] + l_s[1][tid] : l_s[0][tid]) + nan;
+                ml[2 * kRows] = kq_s[tid];
+            }
+            float *dst = A.part_o + ((size_t)slot * kRows + n16) * kD;
+#pragma unroll
+            for (int rt = 0; rt < 4; ++rt) {
+                if (16 * rt >= P.n << lh) break;
+#pragma unroll
+                for (int dt = 0; dt < kDT; ++dt) *reinterpret_cast<float4_t *>(dst + 16 * rt * kD + out_dim(dt)) = o[rt][dt];
+            }
+        }
+        lds_barrier();   // what is shared is free again
+    }
+}
+
+// The parts of a problem that cuts fall into, in order, and the sink: one workgroup per
+// row. Waves 2 k and 2 k + 1 take the halves of parts k, k + 4, .., a lane four dims, sixteen
+// parts in flight; the four sums are joined in order.
+// kInline: workgroup b has row b % kRows of problem b / kRows; else of the problem that cut
+// b / kRows + 1 falls into, if that is its first cut.
+template <bool kF32, bool kInline>
+__global__ __launch_bounds__(512) void window_merge_kernel(const WinArgs A) {
+    __shared__ float f_s[kWgs];   // each part's factor
+    __shared__ float4_t o_s[3][128];
+    const int tid = threadIdx.x, row = blockIdx.x % kRows, n_prob = *A.n_prob;
+    const long long per = A.line[1];
+    int pi = blockIdx.x / kRows;
+    if (!kInline) pi = A.wg_prob[pi + 1];
     if (pi >= n_prob) return;
-    const long long begin = A.pre[pi], end = A.pre[pi + 1], cut = A.wg_tile[b + 1];
-    if (cut <= begin || cut >= end || A.wg_tile[b] > begin) return;
-    const int2 id = A.prob[pi];
-    const Problem P = problem_of(A, id.x, id.y);
+    const long long begin = A.pre[pi], end = A.pre[pi + 1];
+    const long long b0 = begin / per;   // the workgroup of its first tile; the first cut is the next one's
+    if (end - begin <= kWhole || (b0 + 1) * per >= end) return;
+    if (!kInline && b0 != blockIdx.x / kRows) return;
+    const Problem P = problem_of(A, A.prob[pi]);
     const int lh = log_hpt(A), qi = row >> lh, head = P.head0 + (row & ((1 << lh) - 1));
     if (qi >= P.n) return;
-    int last = b + 1;
-    while (last + 1 < kWgs && A.wg_tile[last + 1] < end) ++last;
+    const int parts = (int)((end - 1) / per - b0) + 1;
+    // (the first part is its workgroup's last one, the others their workgroups' first)
+    auto slot = [&](int c) { return (size_t)(2 * (b0 + c) + (c == 0)); };
+    const float *ml = A.part_ml + row;
+    const int lane = tid & 63, w = tid >> 6;
     float mx = -INFINITY;
-    for (int c = b; c <= last; ++c) mx = fmaxf(mx, A.part_ml[(size_t)(c == b ? 2 * c + 1 : 2 * c) * 3 * kM + row]);
-    const float kq = A.part_ml[(size_t)(2 * b + 1) * 3 * kM + 2 * kM + row];
-    float den = 0.0f, o[8] = {};
-    for (int c = b; c <= last; ++c) {
-        const size_t slot = c == b ? 2 * c + 1 : 2 * c;
-        const float m = A.part_ml[slot * 3 * kM + row], l = A.part_ml[slot * 3 * kM + kM + row];
-        const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m - mx) * kq);
-        den += l * f;
-        const float *src = A.part_o + (slot * kM + row) * kD + 8 * lane;
+    for (int c = lane; c < parts; c += 64) mx = fmaxf(mx, ml[slot(c) * 3 * kRows]);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) o[i] += src[i] * f;
+    for (int off = 32; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor(mx, off));
+    const float kq = ml[slot(0) * 3 * kRows + 2 * kRows];
+    float den = 0.0f;   // every wave its own, the same sums
+    for (int c = lane; c < parts; c += 64) {
+        const float *x = ml + slot(c) * 3 * kRows;
+        const float f = x[0] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((x[0] - mx) * kq);
+        den += x[kRows] * f;
+        if (w == 0) f_s[c] = f;
     }
-    const float sink = sink_term(A, head, mx, kq);
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) den += __shfl_xor(den, off);
+    __syncthreads();
+    float4_t o = {0, 0, 0, 0};
+    const int d = 256 * (w & 1) + 4 * lane;
+    const float *src = A.part_o + (size_t)row * kD + d;
+    for (int c0 = w >> 1; c0 < parts; c0 += 64) {
+        float4_t v[16];
+#pragma unroll
+        for (int u = 0; u < 16; ++u)
+            v[u] = *reinterpret_cast<const float4_t *>(src + slot(min(c0 + 4 * u, parts - 1)) * kRows * kD);
+#pragma unroll
+        for (int u = 0; u < 16; ++u)
+            if (c0 + 4 * u < parts) o += v[u] * f_s[c0 + 4 * u];
+    }
+    if (w >= 2) o_s[(w >> 1) - 1][64 * (w & 1) + lane] = o;
+    __syncthreads();
+    if (w >= 2) return;
+#pragma unroll
+    for (int k = 0; k < 3; ++k) o += o_s[k][64 * (w & 1) + lane];
     // (a part whose rows could not be read has a NaN sum)
-    const float inv = mx == -INFINITY && den == 0.0f ? 0.0f : 1.0f / (den + sink);
-    const size_t at = (((size_t)(P.q0 + qi) << A.log_head) + head) * kD + 8 * lane;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        if (kF32)
-            static_cast<float *>(A.out)[at + i] = o[i] * inv;
-        else
-            static_cast<__bf16 *>(A.out)[at + i] = (__bf16)(o[i] * inv);
-    }
+    const float inv = mx == -INFINITY && den == 0.0f ? 0.0f : 1.0f / (den + sink_term(A, head, mx, kq));
+    store_out<kF32>(A.out, (((size_t)(P.q0 + qi) << A.log_head) + head) * kD + d, o * inv);
 }
 
 size_t up256(size_t b) { return (b + 255) & ~(size_t)255; }
@@ -491,8 +841,8 @@ int log2_heads(int n_head) {
 
 // Problems that n_seqs sequences of n_q queries in all can make.
 long long prob_cap(int n_seqs, int n_q, int log_head) {
-    const int lh = std::min(log_head, 6);
-    return ((long long)n_q / (kM >> lh) + n_seqs) << (log_head - lh);
+    const int lh = std::min(log_head, kLogRows);
+    return ((long long)(n_q >> (kLogRows - lh)) + n_seqs) << (log_head - lh);
 }
 
 // The workspace, laid out from `base` (or only measured).
@@ -503,13 +853,15 @@ size_t lay_out(WinArgs *A, char *base, long long cap) {
         at += up256(bytes);
         return p;
     };
-    char *n_prob = take(sizeof(int)), *prob = take(sizeof(int2) * cap), *pre = take(sizeof(long long) * (cap + 1)),
-         *wg_tile = take(sizeof(long long) * (kWgs + 1)), *wg_prob = take(sizeof(int) * (kWgs + 1)),
-         *ml = take(sizeof(float) * 2 * kWgs * 3 * kM), *o = take(sizeof(float) * 2 * kWgs * kM * kD);
+    char *line = take(2 * sizeof(long long)), *n_prob = take(sizeof(int)), *prob = take(sizeof(int4) * cap),
+         *pre = take(sizeof(long long) * (cap + 1)), *wg_tile = take(sizeof(long long) * (kWgs + 1)),
+         *wg_prob = take(sizeof(int) * (kWgs + 1)), *ml = take(sizeof(float) * 2 * kWgs * 3 * kRows),
+         *o = take(sizeof(float) * 2 * kWgs * kRows * kD);
     if (A) {
         A->prob_cap = (int)cap;
+        A->line = reinterpret_cast<long long *>(line);
         A->n_prob = reinterpret_cast<int *>(n_prob);
-        A->prob = reinterpret_cast<int2 *>(prob);
+        A->prob = reinterpret_cast<int4 *>(prob);
         A->pre = reinterpret_cast<long long *>(pre);
         A->wg_tile = reinterpret_cast<long long *>(wg_tile);
         A->wg_prob = reinterpret_cast<int *>(wg_prob);
@@ -541,7 +893,7 @@ extern "C" int ds4hip_flash_attn_window_fp8(const ds4hip_window_attn *a, void *w
     if (!a->q || !a->out || !a->codes || !a->sexp || !a->tail || !a->table || !a->rows || a->table_stride <= 0 ||
         a->n_slots <= 0 || a->n_cache_rows < a->page_rows || (a->n_cache_rows >> shift) > 0x7FFFFFFF || !workspace ||
         (!a->q_start && a->n_q < a->n_seqs) || (!a->seq_ids && a->n_slots < a->n_seqs) || !aligned(a->q, 16) ||
-        !aligned(a->out, a->io_f32 ? 16 : 8) || !aligned(a->codes, 8) || !aligned(a->sexp, 8) || !aligned(a->tail, 16) ||
+        !aligned(a->out, a->io_f32 ? 16 : 8) || !aligned(a->codes, 16) || !aligned(a->sexp, 8) || !aligned(a->tail, 16) ||
         !aligned(workspace, 16))
         return ds4hip_set_last_error(kEINVAL);
     WinArgs A = {};
@@ -567,14 +919,20 @@ extern "C" int ds4hip_flash_attn_window_fp8(const ds4hip_window_attn *a, void *w
     A.shift = shift;
     A.n_pages = (int)(a->n_cache_rows >> shift);
     const hipStream_t st = (hipStream_t)stream;
-    hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(1024), 0, st, A);
-    const dim3 merge((kWgs - 1) * (kM / 4));
-    if (a->io_f32) {
-        hipLaunchKernelGGL(window_kernel<true>, dim3(kWgs), dim3(256), 0, st, A);
-        hipLaunchKernelGGL(window_merge_kernel<true>, merge, dim3(256), 0, st, A);
-    } else {
-        hipLaunchKernelGGL(window_kernel<false>, dim3(kWgs), dim3(256), 0, st, A);
-        hipLaunchKernelGGL(window_merge_kernel<false>, merge, dim3(256), 0, st, A);
+    const bool f32 = a->io_f32, in = A.prob_cap <= kInlineProbs;
+    if (!in) hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(1024), 0, st, A);
+    auto *main = f32 ? in ? window_kernel<true, true> : window_kernel<true, false>
+                     : in ? window_kernel<false, true> : window_kernel<false, false>;
+    hipLaunchKernelGGL(main, dim3(kWgs), dim3(f32 ? 256 : 512), 0, st, A);
+    // no problem is cut where none can have that many tiles: of rows that the table can name, or of
+    // the window, the queries' own span and the first rows, with their ends inside tiles
+    const long long held = (long long)a->table_stride << shift;
+    const long long span = std::min<long long>(held, (long long)a->window + (kRows >> std::min(lh, kLogRows)));
+    const long long most = a->window > 0 ? span / kTile + 2 + (std::min<long long>(a->n_first, held) + kTile - 1) / kTile : held / kTile + 1;
+    if (most > kWhole) {
+        auto *merge = f32 ? in ? window_merge_kernel<true, true> : window_merge_kernel<true, false>
+                          : in ? window_merge_kernel<false, true> : window_merge_kernel<false, false>;
+        hipLaunchKernelGGL(merge, dim3((in ? A.prob_cap : kWgs - 1) * kRows), dim3(512), 0, st, A);
     }
     return ds4hip_set_last_error(hip_status(hipGetLastError()));
 }

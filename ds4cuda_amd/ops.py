@@ -29,7 +29,8 @@ def _ptr(t):
 
 def _stream(stream):
     if stream is None:
-        return C.c_void_p(torch.cuda.current_stream().cuda_stream)
+        # (the handle of torch.cuda.current_stream(), without the object around it)
+        return C.c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
     if isinstance(stream, torch.cuda.Stream):
         return C.c_void_p(stream.cuda_stream)
     return C.c_void_p(stream)
@@ -295,15 +296,33 @@ class WindowAttn(C.Structure):
                 ("n_q", C.c_int), ("n_head", C.c_int), ("window", C.c_int), ("n_first", C.c_int)]
 
 
+def _addr(t):
+    return None if t is None else t.data_ptr()
+
+
 def window_workspace_bytes(n_seqs, n_q, n_head) -> int:
     return lib().ds4hip_flash_attn_window_fp8_workspace_bytes(n_seqs, n_q, n_head)
 
 
+class _Here:
+    """The context that changes nothing (the common case: the work's device and
+    stream are the current ones)."""
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE = _Here()
+
+
 def _on_stream(stream, device):
-    """Context in which tensors are allocated for work on `stream` (None: the
-    device's current stream)."""
+    """Context in which tensors are allocated, and launches made, for work on
+    `stream` of `device` (None: its current stream)."""
     if stream is None:
-        return torch.cuda.device(device)
+        return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
     if not isinstance(stream, torch.cuda.Stream):
         stream = torch.cuda.ExternalStream(int(getattr(stream, "value", stream) or 0), device=device)
     return torch.cuda.stream(stream)
@@ -323,42 +342,60 @@ def flash_attn_window_fp8(q, cache: Fp8KVCache, page_table, seq_rows, *, page_ro
     p - window or k < n_first); sinks [n_head] fp32: a sink logit per head.
     All lengths are read on the device: a captured call follows them.
     """
-    if q.dim() != 3 or q.shape[2] != HEAD_DIM or q.dtype not in (torch.bfloat16, torch.float32):
-        raise Ds4HipError("q must be bf16 or fp32 [n_q, n_head, 512]", -22)
-    n_q, n_head = q.shape[0], q.shape[1]
-    _check(q, q.dtype, None, "q")
-    if page_table.dim() != 2:
-        raise Ds4HipError("page_table must be [slots, entries]", -22)
-    slots, stride = page_table.shape
-    _check(page_table, torch.int32, None, "page_table")
-    _check(seq_rows, torch.int32, slots, "seq_rows")
-    _check(sinks, torch.float32, n_head, "sinks")
-    _check(q_start, torch.int32, 1, "q_start")
-    _check(seq_ids, torch.int32, None, "seq_ids")
-    _check(cache.codes, torch.uint8, cache.n_rows * N_NOPE, "codes")
-    _check(cache.sexp, torch.int8, cache.n_rows * 8, "sexp")
-    _check(cache.tail, cache.tail.dtype, cache.n_rows * N_ROT, "tail")
-    if cache.tail.element_size() != 2:
-        raise Ds4HipError("tail: expected f16 values or their bits", -22)
-    n_seqs = q_start.numel() - 1 if q_start is not None else n_q
-    if seq_ids is not None and seq_ids.numel() != n_seqs:
-        raise Ds4HipError(f"seq_ids: {n_seqs} entries expected, got {seq_ids.numel()}", -22)
-    with _on_stream(stream, q.device):
-        if out is None:
-            out = torch.empty_like(q)
-        _check(out, q.dtype, q.numel(), "out")
-        if n_q == 0 or n_seqs == 0:
-            return out
-        need = window_workspace_bytes(n_seqs, n_q, n_head)
-        if workspace is None:
-            workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
-        _dev(workspace, "workspace", need)
-        a = WindowAttn(_ptr(q), _ptr(out), int(q.dtype == torch.float32), _ptr(sinks), _ptr(cache.codes),
-                       _ptr(cache.sexp), _ptr(cache.tail), cache.n_rows, _ptr(page_table), _ptr(seq_rows), slots, stride,
-                       int(page_rows), _ptr(q_start), _ptr(seq_ids), n_seqs, n_q, n_head, int(window), int(n_first))
-        call("ds4hip_flash_attn_window_fp8", C.byref(a), _ptr(workspace), workspace.numel() * workspace.element_size(),
-             _stream(stream))
-    return out
+    view = WindowView(cache, page_table, seq_rows, page_rows)
+    return view.attend(q, window=window, n_first=n_first, sinks=sinks, q_start=q_start, seq_ids=seq_ids, out=out,
+                       workspace=workspace, stream=stream)
+
+
+class WindowView:
+    """The checked arguments of flash_attn_window_fp8 that stay the same from call to call:
+    a cache, its page table and its sequences' rows."""
+
+    def __init__(self, cache: Fp8KVCache, page_table, seq_rows, page_rows):
+        if page_table.dim() != 2:
+            raise Ds4HipError("page_table must be [slots, entries]", -22)
+        slots, stride = page_table.shape
+        _check(page_table, torch.int32, None, "page_table")
+        _check(seq_rows, torch.int32, slots, "seq_rows")
+        _check(cache.codes, torch.uint8, cache.n_rows * N_NOPE, "codes")
+        _check(cache.sexp, torch.int8, cache.n_rows * 8, "sexp")
+        _check(cache.tail, cache.tail.dtype, cache.n_rows * N_ROT, "tail")
+        if cache.tail.element_size() != 2:
+            raise Ds4HipError("tail: expected f16 values or their bits", -22)
+        self.keep = (cache, page_table, seq_rows)
+        self.fixed = dict(codes=cache.codes.data_ptr(), sexp=cache.sexp.data_ptr(), tail=cache.tail.data_ptr(),
+                          n_cache_rows=cache.n_rows, table=page_table.data_ptr(), rows=seq_rows.data_ptr(), n_slots=slots,
+                          table_stride=stride, page_rows=int(page_rows))
+
+    def attend(self, q, *, window=0, n_first=0, sinks=None, q_start=None, seq_ids=None, out=None, workspace=None, stream=None):
+        if q.dim() != 3 or q.shape[2] != HEAD_DIM or q.dtype not in (torch.bfloat16, torch.float32):
+            raise Ds4HipError("q must be bf16 or fp32 [n_q, n_head, 512]", -22)
+        n_q, n_head = q.shape[0], q.shape[1]
+        _check(q, q.dtype, None, "q")
+        _check(sinks, torch.float32, n_head, "sinks")
+        _check(q_start, torch.int32, 1, "q_start")
+        _check(seq_ids, torch.int32, None, "seq_ids")
+        n_seqs = q_start.numel() - 1 if q_start is not None else n_q
+        if seq_ids is not None and seq_ids.numel() != n_seqs:
+            raise Ds4HipError(f"seq_ids: {n_seqs} entries expected, got {seq_ids.numel()}", -22)
+        with _on_stream(stream, q.device):
+            if out is None:
+                out = torch.empty_like(q)
+            else:
+                _check(out, q.dtype, q.numel(), "out")
+            if n_q == 0 or n_seqs == 0:
+                return out
+            need = window_workspace_bytes(n_seqs, n_q, n_head)
+            if workspace is None:
+                workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+            else:
+                _dev(workspace, "workspace", need)
+            a = WindowAttn(q=q.data_ptr(), out=out.data_ptr(), io_f32=q.dtype == torch.float32, sinks=_addr(sinks),
+                           q_start=_addr(q_start), seq_ids=_addr(seq_ids), n_seqs=n_seqs, n_q=n_q, n_head=n_head,
+                           window=int(window), n_first=int(n_first), **self.fixed)
+            call("ds4hip_flash_attn_window_fp8", C.byref(a), workspace.data_ptr(),
+                 workspace.numel() * workspace.element_size(), _stream(stream))
+        return out
 
 
 # ---- tail RoPE (cuda/rope.cuh:51, cuda/attn_out.cuh:52) ----------------------------------

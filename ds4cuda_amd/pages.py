@@ -13,7 +13,7 @@ import ctypes as C
 import torch
 
 from ._lib import Ds4HipError, call, lib
-from .ops import HEAD_DIM, N_NOPE, N_ROT, Fp8KVCache, _check, _on_stream, _ptr, _stream, flash_attn_window_fp8
+from .ops import HEAD_DIM, N_NOPE, N_ROT, Fp8KVCache, WindowView, _check, _on_stream, _ptr, _stream
 
 MAX_JOBS = 1024    # sequences of one call
 
@@ -58,6 +58,7 @@ class PagePool:
         self.c = KvPages(_ptr(codes), _ptr(sexp), _ptr(tail), n_rows, layers, n_pages, self.page_rows, table.shape[1],
                          self.n_seqs, _ptr(refs), _ptr(table), _ptr(rows), _ptr(self.status))
         self._workspace = None
+        self._views = {}
 
     @classmethod
     def empty(cls, n_pages, page_rows, n_seqs, max_rows, n_layers=1, device="cuda"):
@@ -94,8 +95,8 @@ class PagePool:
         return ids.numel()
 
     def _ws(self, stream):
-        need = lib().ds4hip_kv_pages_workspace_bytes(C.byref(self.c))
         if self._workspace is None:
+            need = lib().ds4hip_kv_pages_workspace_bytes(C.byref(self.c))
             with _on_stream(stream, self.device):
                 self._workspace = torch.empty(need, dtype=torch.uint8, device=self.device)
         return self._workspace
@@ -158,6 +159,8 @@ class PagePool:
                stream=None):
         """ops.flash_attn_window_fp8 over this pool's pages of one layer: the sequences
         seqs (None: slots 0, 1, ..)."""
-        return flash_attn_window_fp8(q, self.layer(layer), self.table, self.rows, page_rows=self.page_rows, window=window,
-                                     n_first=n_first, sinks=sinks, q_start=q_start, seq_ids=seqs, out=out,
-                                     workspace=workspace, stream=stream)
+        view = self._views.get(layer)
+        if view is None:
+            view = self._views[layer] = WindowView(self.layer(layer), self.table, self.rows, self.page_rows)
+        return view.attend(q, window=window, n_first=n_first, sinks=sinks, q_start=q_start, seq_ids=seqs, out=out,
+                           workspace=workspace, stream=stream)

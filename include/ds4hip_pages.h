@@ -106,7 +106,7 @@ int ds4hip_kv_pages_compact(const ds4hip_kv_pages *p, int32_t *n_live, void *wor
  * nothing; outputs of queries that no entry names are left as they were.
  * n_head: 8, 16, 32, 64 or 128. io_f32 0: q and out are bf16, and P is rounded to one
  * f16 (2^-12 relative); 1: both are fp32, with q and P as f16 hi + lo halves.
- * All arrays are device memory (q and out 16-byte aligned): the lengths are read on
+ * All arrays are device memory (q, out, codes and tail 16-byte aligned, sexp 8-byte): the lengths are read on
  * the device, so a captured call follows them. No entry outside the table and no row
  * outside [0, n_cache_rows) is read; a query of a sequence that names one is NaN. A
  * row that is not finite reaches only the queries that see it. */
