@@ -28,14 +28,19 @@ constexpr int kLogRows = 6, kRows = 1 << kLogRows;   // rows (queries x heads) o
 constexpr int kWgs = 256;            // workgroups the line of tiles is cut for: one per CU
 constexpr int kMinTiles = 4;         // tiles of a part
 constexpr int kWhole = 8;            // tiles of a problem that is never cut
+constexpr int kPart = 12;            // tiles whose time a cut costs: its parts' 256 KB and their merge
 constexpr int kMaxSeqs = 4096;
 constexpr int kInlineProbs = 512;    // problems that a workgroup lays out itself
-// P = 2^((s - m) kq + kTop) with s and the row's reference m as the matrix
-// instructions leave them and kq its scale to log2: their difference is exact where P
-// is large, at any magnitude. The reference moves only where P would pass 2^(kTop +
-// kLazy) = 2^15 (f16 ends at 2^16), so outputs are rescaled on few tiles.
-constexpr float kTop = 8.0f;
-constexpr float kLazy = 7.0f;
+// P = 2^((s - m) kq + top) with s and the row's reference m as the matrix
+// instructions leave them and kq its scale to log2: their difference is exact where P is
+// large, at any magnitude. The reference moves only where P would pass 2^15 (f16 ends at
+// 2^16). One f16 (bf16 outputs) starts at 2^-8: a row may gain 23 bits before it moves
+// (moving costs half a tile: rows of which 1% are eight times as large moved in 9 of 32 tiles from
+// 2^8 on), and weights under 2^-6 of the largest are off by up to 2^-17 of it. hi + lo (fp32) start at 2^8: 2^-32.
+template <bool kF32>
+constexpr float kTop = kF32 ? 8.0f : -8.0f;
+template <bool kF32>
+constexpr float kLazy = 15.0f - kTop<kF32>;
 
 struct WinArgs {
     const void *q;
@@ -48,7 +53,7 @@ struct WinArgs {
     int n_seqs, n_slots, n_q, log_head, window, first, stride, shift, n_pages;
     // workspace
     int prob_cap;
-    long long *line;         // [2] tiles in all, tiles per workgroup
+    long long *line;         // [2] tiles per workgroup, tiles of a problem that stays whole
     int *n_prob;
     int4 *prob;              // [prob_cap] records
     long long *pre;          // [prob_cap + 1] tiles before each problem
@@ -149,10 +154,10 @@ __device__ inline long long block_scan(long long v, long long *sums, long long *
     return before + x - v;
 }
 
-// put(i, record, tiles before) for every problem; returns their number and *tiles. All
-// threads of the workgroup; first_s: [n_seqs].
+// put(i, record, tiles before) for every problem; returns their number, *tiles and, in
+// *longest (shared, 0 before), the most of one. All threads of the workgroup; first_s: [n_seqs].
 template <int kThreads, typename Put>
-__device__ inline int lay_line(const WinArgs &A, int *first_s, long long *sums, long long *tiles, Put put) {
+__device__ inline int lay_line(const WinArgs &A, int *first_s, long long *sums, int *longest, long long *tiles, Put put) {
     const int tid = threadIdx.x;
     const int lh = log_hpt(A), lg = A.log_head - lh, qpt = kRows >> lh;
     long long n_all = 0, t_all = 0;
@@ -192,52 +197,86 @@ __device__ inline int lay_line(const WinArgs &A, int *first_s, long long *sums, 
         const long long before = t_all + block_scan<kThreads>(n, sums, &all);
         if (i < n_prob) put(i, rec, before);
         t_all += all;
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1) n = max(n, __shfl_xor(n, off));
+        if ((tid & 63) == 0 && n) atomicMax(longest, n);
     }
+    __syncthreads();
     *tiles = t_all;
     return n_prob;
 }
 
-__device__ inline long long tiles_per_wg(long long tiles) { return max((tiles + kWgs - 1) / kWgs, (long long)kMinTiles); }
+// How the line is cut. Where every workgroup can have a problem of its own and the longest
+// costs less than parts and their merge would (about kPart tiles), nothing is cut; else at
+// every `per` tiles, but not through short problems.
+struct Cuts {
+    long long tiles, per;
+    int whole;   // tiles of a problem that stays whole; < 0: workgroup b has problem b
+};
 
-// Where a cut at tile t of the line falls that lies in the problem [begin, end): a short
-// problem stays whole (its parts would cost more than it does) and moves the cut to its nearer end.
-__device__ inline long long settle_cut(long long t, long long begin, long long end) {
-    return end - begin > kWhole ? t : 2 * t <= begin + end ? begin : end;
+__device__ inline Cuts cuts_of(long long tiles, int n_prob, int longest) {
+    Cuts C;
+    C.tiles = tiles;
+    C.per = max((tiles + kWgs - 1) / kWgs, (long long)kMinTiles);
+    C.whole = (int)min(max((long long)kWhole, C.per / 8), 1LL << 30);
+    if (n_prob <= kWgs && longest <= C.per + kPart) {
+        C.whole = -1;
+        C.per = tiles + 1;   // (no cut inside the line)
+    }
+    return C;
+}
+
+// Tile and problem at which workgroup b begins.
+template <typename Pre>
+__device__ inline long long begin_of(const Cuts &C, int b, int n_prob, Pre pre, int *prob) {
+    if (C.whole < 0) {
+        *prob = min(b, n_prob);
+        return pre(*prob);
+    }
+    const long long t = b * C.per;
+    *prob = n_prob;
+    if (t >= C.tiles) return C.tiles;
+    int lo = 0, hi = n_prob;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (pre(mid) <= t) lo = mid; else hi = mid;
+    }
+    *prob = lo;
+    const long long begin = pre(lo), end = pre(lo + 1);
+    if (end - begin > C.whole) return t;
+    if (2 * t <= begin + end) return begin;   // a short problem goes to the side that has more of it
+    *prob = lo + 1;
+    return end;
+}
+
+// What the merge needs of the plan, besides the problems.
+__device__ inline void leave(const WinArgs &A, const Cuts &C, int n_prob) {
+    *A.n_prob = n_prob;
+    A.line[0] = C.per;
+    A.line[1] = C.whole;
 }
 
 __global__ __launch_bounds__(1024) void plan_kernel(const WinArgs A) {
     __shared__ int first_s[kMaxSeqs];   // problems before each sequence
     __shared__ long long sums[16];
     long long tiles;
-    const int n_prob = lay_line<1024>(A, first_s, sums, &tiles, [&](int i, int4 rec, long long before) {
+    __shared__ int longest;
+    if (threadIdx.x == 0) longest = 0;
+    const int n_prob = lay_line<1024>(A, first_s, sums, &longest, &tiles, [&](int i, int4 rec, long long before) {
         A.prob[i] = rec;
         A.pre[i] = before;
     });
-    const long long per = tiles_per_wg(tiles);
+    const Cuts C = cuts_of(tiles, n_prob, longest);
     if (threadIdx.x == 0) {
         A.pre[n_prob] = tiles;
-        *A.n_prob = n_prob;
-        A.line[0] = tiles;
-        A.line[1] = per;
+        leave(A, C, n_prob);
     }
     __syncthreads();
     const int b = threadIdx.x;
     if (b > kWgs) return;
-    const long long t = b * per;
-    int lo = n_prob;
-    long long cut = tiles;
-    if (t < tiles) {
-        int hi = n_prob;
-        lo = 0;
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (A.pre[mid] <= t) lo = mid; else hi = mid;
-        }
-        cut = settle_cut(t, A.pre[lo], A.pre[lo + 1]);
-        lo += cut == A.pre[lo + 1];
-    }
-    A.wg_tile[b] = cut;
-    A.wg_prob[b] = lo;
+    int prob;
+    A.wg_tile[b] = begin_of(C, b, n_prob, [&](int i) { return A.pre[i]; }, &prob);
+    A.wg_prob[b] = prob;
 }
 
 // ---- attention -------------------------------------------------------------------
@@ -322,8 +361,9 @@ __device__ inline float load_q(const WinArgs &A, const Problem &P, int row, int 
 }
 
 // The sink's part of a denominator with reference m.
+template <bool kF32>
 __device__ inline float sink_term(const WinArgs &A, int head, float m, float kq) {
-    return A.sinks ? __builtin_amdgcn_exp2f(fmaf(-m, kq, fmaf(A.sinks[head], kLog2e, kTop))) : 0.0f;
+    return A.sinks ? __builtin_amdgcn_exp2f(fmaf(-m, kq, fmaf(A.sinks[head], kLog2e, kTop<kF32>))) : 0.0f;
 }
 
 // Four outputs, rounded to bf16 unless the call's type is fp32.
@@ -372,8 +412,7 @@ __device__ inline void load_part(const WinArgs &A, long long row, int j, Part &R
 __device__ inline void store_part(uint8_t *stage, int tid, const Part &R) {
     const int row = tid >> 4, j = tid & 15;   // (of the 16 or 32 rows at stage)
     uint8_t *rp = stage + row * kRowB;
-    const uint32_t x = row_swz(row);
-    uint8_t *p = rp + ((16 * j) ^ x);   // dim_of's order
+    uint8_t *p = rp + 16 * j;   // dim_of's order
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         if (i == 1 && j >= 12) break;
@@ -389,7 +428,7 @@ __device__ inline void store_part(uint8_t *stage, int tid, const Part &R) {
         *reinterpret_cast<half8_t *>(p + 512 * i + 256) = half8_t{h[4][0], h[4][1], h[5][0], h[5][1], h[6][0], h[6][1], h[7][0], h[7][1]};
     }
     const int u = j >> 1;   // tail granule
-    *reinterpret_cast<uint2_t *>(rp + ((512 + 16 * (12 + (u & 3)) + 256 * (u >> 2) + 8 * (j & 1)) ^ x)) = R.t;
+    *reinterpret_cast<uint2_t *>(rp + 512 + 16 * (12 + (u & 3)) + 256 * (u >> 2) + 8 * (j & 1)) = R.t;
 }
 
 // Iteration i, with one barrier: scores of tile i | tile i + 1 dequantized, a later one
@@ -403,6 +442,7 @@ __global__ __launch_bounds__(kF32 ? 256 : 512, kF32 ? 1 : 2) void window_kernel(
     constexpr int kN = 8 / kW;           // key halves of a wave, and thread rows of a tile
     constexpr int kDT = 4 * kN;          // dim tiles of a wave
     constexpr int kDB = 1024 / kW;       // its bytes of an f16 row
+    constexpr int kAhead = kF32 ? 1 : 2; // tiles in flight to registers
     __shared__ __attribute__((aligned(16))) uint8_t stages[3][kStageB];
     __shared__ __attribute__((aligned(16))) half4_t pb[2][kF32 ? 2 : 1][4][64][2];   // [buffer][hi, lo][row tile][lane][key half]
     __shared__ float top_s[2][kRows], l_s[2][kRows], m_s[kRows], kq_s[kRows];
@@ -422,45 +462,26 @@ __global__ __launch_bounds__(kF32 ? 256 : 512, kF32 ? 1 : 2) void window_kernel(
     int n_prob, pi;
     long long t, t_end;
     if constexpr (kInline) {
+        __shared__ int longest;
+        if (tid == 0) longest = 0;
         long long tiles;
-        n_prob = lay_line<64 * kW>(A, first_s, sums_s, &tiles, [&](int i, int4 rec, long long before) {
+        n_prob = lay_line<64 * kW>(A, first_s, sums_s, &longest, &tiles, [&](int i, int4 rec, long long before) {
             prob_s[i] = rec;
             pre_s[i] = before;
         });
         if (tid == 0) pre_s[n_prob] = tiles;
         __syncthreads();
-        const long long per = tiles_per_wg(tiles);
+        const Cuts C = cuts_of(tiles, n_prob, longest);
         if (wg == 0) {
-            for (int i = tid; i < n_prob; i += 64 * kW) {
-                A.prob[i] = prob_s[i];
+            for (int i = tid; i <= n_prob; i += 64 * kW) {
+                if (i < n_prob) A.prob[i] = prob_s[i];
                 A.pre[i] = pre_s[i];
             }
-            if (tid == 0) {
-                A.pre[n_prob] = tiles;
-                *A.n_prob = n_prob;
-                A.line[0] = tiles;
-                A.line[1] = per;
-            }
+            if (tid == 0) leave(A, C, n_prob);
         }
-        long long cut[2];
-        pi = 0;
-#pragma unroll
-        for (int e = 1; e >= 0; --e) {   // (the workgroup's first problem is found last)
-            const long long at = (wg + e) * per;
-            cut[e] = tiles;
-            if (at < tiles) {
-                int hi = n_prob;
-                pi = 0;
-                while (hi - pi > 1) {
-                    const int mid = (pi + hi) >> 1;
-                    if (pre_s[mid] <= at) pi = mid; else hi = mid;
-                }
-                cut[e] = settle_cut(at, pre_s[pi], pre_s[pi + 1]);
-                pi += cut[e] == pre_s[pi + 1];
-            }
-        }
-        t = cut[0];
-        t_end = cut[1];
+        auto pre = [&](int i) { return pre_s[i]; };
+        t_end = begin_of(C, wg + 1, n_prob, pre, &pi);
+        t = begin_of(C, wg, n_prob, pre, &pi);
     } else {
         n_prob = *A.n_prob;
         pi = A.wg_prob[wg];
@@ -473,14 +494,22 @@ __global__ __launch_bounds__(kF32 ? 256 : 512, kF32 ? 1 : 2) void window_kernel(
 #pragma unroll
         for (int u = 0; u < kN; ++u) {
             const int r = pi_key(16 * (kh + u) + n16);
-            ka[u] = r * kRowB + ((16 * g) ^ row_swz(r));
+            ka[u] = r * kRowB + 16 * g;
         }
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt) {
             const int v = pi_key(16 * kt + 4 * g + (n16 >> 2));
-            va[kt] = lds_addr(stages[0]) + v * kRowB + kDB * w + ((8 * (n16 & 3)) ^ row_swz(v));
+            va[kt] = lds_addr(stages[0]) + v * kRowB + kDB * w + 8 * (n16 & 3);
         }
     }
+    // The next problem's queries, brought to L2 while this one's tiles run (3 us from HBM
+    // otherwise, with nothing beside them): a word of each 128 bytes is read.
+    auto warm_q = [&](int next) {
+        const int4 rec = kInline ? prob_s[kInline ? next : 0] : A.prob[next];
+        const size_t item = kF32 ? 4 : 2, row0 = ((size_t)rec.y << A.log_head) + (rec.z >> 8), n = (size_t)((rec.z & 255) << lh) * kD * item;
+        const char *q = static_cast<const char *>(A.q) + row0 * kD * item;
+        for (size_t b = 128 * tid; b < n; b += 128 * 64 * kW) (void)*reinterpret_cast<const volatile int *>(q + b);
+    };
     // first of the lane's four dims of the wave's dim tile dt
     auto out_dim = [&](int dt) { return dim_of(kDB / 16 * w + 2 * dt + (g >> 1)) + 4 * (g & 1); };
 
@@ -506,38 +535,45 @@ __global__ __launch_bounds__(kF32 ? 256 : 512, kF32 ? 1 : 2) void window_kernel(
             // the thread's u-th row of tile i (past the last row seen: that row again, masked), and its page
             auto row_of = [&](int i, int u) { return min(kTile * tile_at(P, min(i, i1 - 1)) + (tid >> 4) + 16 * u, P.pos1); };
             auto page_of = [&](int i, int u) { return A.table[(long long)P.slot * A.stride + (row_of(i, u) >> A.shift)]; };
-            Part R[kN];
+            Part R[kAhead][kN];
             int page[kN];
-            // fetches tile i + 2 (the pages after it first: waiting for a page must not wait for the
-            // rows). An entry outside the pool reads row 0
-            auto advance = [&](int i) {
+            // fetches tile i + 1 + kAhead (the pages after it first: waiting for a page must not wait for
+            // the rows). An entry outside the pool reads row 0
+            auto advance = [&](int i, Part (&R)[kN]) {
                 int next[kN];
 #pragma unroll
-                for (int u = 0; u < kN; ++u) next[u] = page_of(i + 3, u);
+                for (int u = 0; u < kN; ++u) next[u] = page_of(i + 2 + kAhead, u);
 #pragma unroll
                 for (int u = 0; u < kN; ++u) {
                     if (page[u] < 0 || page[u] >= A.n_pages) {
                         bad = true;
                         page[u] = 0;
                     }
-                    load_part(A, ((long long)page[u] << A.shift) + (row_of(i + 2, u) & ((1 << A.shift) - 1)), tid & 15, R[u]);
+                    load_part(A, ((long long)page[u] << A.shift) + (row_of(i + 1 + kAhead, u) & ((1 << A.shift) - 1)), tid & 15, R[u]);
                     page[u] = next[u];
                 }
             };
-            auto store = [&](int stage) {
+            auto store = [&](int stage, Part (&R)[kN]) {
 #pragma unroll
                 for (int u = 0; u < kN; ++u) store_part(stages[0] + stage + 16 * u * kRowB, tid, R[u]);
             };
 #pragma unroll
             for (int u = 0; u < kN; ++u) page[u] = page_of(i0, u);
-            advance(i0 - 2);
+            advance(i0 - 1 - kAhead, R[0]);
             half8_t qh[16], ql[kF32 ? 16 : 1];
             const float kq = load_q<kF32>(A, P, row, g, qh, ql) * (kLog2e / 22.62741699796952f);   // 1 / sqrt(512)
             const int pos = P.pos0 + min(row >> lh, P.n - 1);   // (rows past the queries repeat the last one's)
             float m = -INFINITY, l = 0.0f, sum = 0.0f;
             float ref = 0.0f;   // m, or 0 while there is none
-            store(0);
-            advance(i0 - 1);
+            store(0, R[0]);
+            // (in the loop's order: its waits count the loads behind the one they wait for)
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                __builtin_amdgcn_sched_barrier(0);
+                advance(i0 - kAhead + u, R[u]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            if (t < t_end && pi + 1 < n_prob) warm_q(pi + 1);
             int sp = 2 * kStageB, sc = 0, sn = kStageB;   // stages of tiles i - 1, i, i + 1
             int buf = 0;                                  // P's of tile i
             float4_t acc[kN];                             // scores of the tile whose P is the newest
@@ -551,7 +587,7 @@ __global__ __launch_bounds__(kF32 ? 256 : 512, kF32 ? 1 : 2) void window_kernel(
                     float p[4];
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        p[r] = __builtin_amdgcn_exp2f(fmaf(acc[u][r] - ref, kq, kTop));
+                        p[r] = __builtin_amdgcn_exp2f(fmaf(acc[u][r] - ref, kq, kTop<kF32>));
                         ph[r] = (half_t)p[r];
                         if (kF32) pl[r] = (half_t)(p[r] - (float)ph[r]);
                     }
@@ -586,7 +622,7 @@ __global__ __launch_bounds__(kF32 ? 256 : 512, kF32 ? 1 : 2) void window_kernel(
                     auto renew = [&](int r, float &old, float scale) {
                         const float top = kW == 8 ? fmaxf(top_s[0][r], top_s[1][r]) : top_s[0][r];
                         float f = 1.0f;
-                        if ((top - old) * scale > kLazy) {   // (-inf before the first key seen)
+                        if ((top - old) * scale > kLazy<kF32>) {   // (-inf before the first key seen)
                             f = old == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((old - top) * scale);
                             old = top;
                         }
@@ -621,7 +657,7 @@ __global__ __launch_bounds__(kF32 ? 256 : 512, kF32 ? 1 : 2) void window_kernel(
                         const int k = __builtin_ctz(odd);
                         odd &= odd - 1;
                         if (4 * lane < kDB)
-                            *reinterpret_cast<uint32_t *>(stages[0] + sp + k * kRowB + kDB * w + ((4 * lane) ^ row_swz(k))) = 0;
+                            *reinterpret_cast<uint32_t *>(stages[0] + sp + k * kRowB + kDB * w + 4 * lane) = 0;
                     }
                     asm volatile("" ::: "memory");   // before the reads below, which are asm
                 }
@@ -654,9 +690,9 @@ __global__ __launch_bounds__(kF32 ? 256 : 512, kF32 ? 1 : 2) void window_kernel(
                 kq_s[row] = kq;
             }
             bool edge_before = false;
-            auto step = [&](int i) {
+            auto step = [&](int i, Part (&R)[kN]) {
                 const bool live = i < i1;
-                lds_barrier();
+                if (i <= i1) lds_barrier();
                 const int4 f0 = *reinterpret_cast<const int4 *>(&moved_s[buf ^ 1][0]), f1 = *reinterpret_cast<const int4 *>(&moved_s[buf ^ 1][4]);
                 float4_t a[kN][2];   // two chains each
                 if (live && scores_mine) {
@@ -690,13 +726,13 @@ __global__ __launch_bounds__(kF32 ? 256 : 512, kF32 ? 1 : 2) void window_kernel(
                         __builtin_amdgcn_sched_barrier(0);
                     }
                 }
-                if (i > i0) {
+                if (i > i0 && i <= i1) {
                     settle(buf ^ 1, f0, f1);   // (acc: still the scores of the tile before)
                     add(buf ^ 1, edge_before);
                 }
+                if (live) store(sn, R);
+                advance(i, R);
                 if (!live) return;
-                store(sn);
-                advance(i);
 #pragma unroll
                 for (int u = 0; u < kN; ++u) acc[u] = a[u][0] + a[u][1];
                 const int tile = tile_at(P, i), key0 = kTile * tile;
@@ -717,7 +753,7 @@ __global__ __launch_bounds__(kF32 ? 256 : 512, kF32 ? 1 : 2) void window_kernel(
                     odd |= __shfl_xor(odd, 32);
                     if (lane_r == 0) odd_s[buf][w] = scores_mine ? odd : ~0u;
                 }
-                const bool moved = scores_mine && __any((top_of() - m) * kq > kLazy);
+                const bool moved = scores_mine && __any((top_of() - m) * kq > kLazy<kF32>);
                 if (lane == 0) moved_s[buf][w] = moved;
                 if (scores_mine) weights(buf);
                 edge_before = edge;
@@ -727,7 +763,13 @@ __global__ __launch_bounds__(kF32 ? 256 : 512, kF32 ? 1 : 2) void window_kernel(
                 sc = sn;
                 sn = free;
             };
-            for (int i = i0; i <= i1; ++i) step(i);   // (the last one only adds the tile before: the code of settle and add stands once)
+            // The last step only adds the tile before (the code of settle and add stands once). One past
+            // it only loads: the loads behind one that a step waits for are the same on all paths, else the
+            // compiler would wait for all.
+            for (int i = i0; i <= i1; i += kAhead) {
+#pragma unroll
+                for (int u = 0; u < kAhead; ++u) step(i + u, R[u]);
+            }
             l = xsum_16_32(l);
             if (g == 0) l_s[kh][row] = l;
         } else if (tid < kRows) {
@@ -737,16 +779,30 @@ __global__ __launch_bounds__(kF32 ? 256 : 512, kF32 ? 1 : 2) void window_kernel(
         lds_barrier();
         const float nan = bad_s ? __builtin_nanf("") : 0.0f;
         if (begins && ends) {
+            constexpr int kOutB = 2 * kD + 16;   // a bf16 row in LDS
 #pragma unroll
             for (int rt = 0; rt < 4; ++rt) {
                 const int rr = 16 * rt + n16, qi = rr >> lh, head = P.head0 + (rr & ((1 << lh) - 1));
                 if (qi >= P.n) continue;
                 const float mm = m_s[rr];
                 const float sum = kW == 8 ? l_s[0][rr] + l_s[1][rr] : l_s[0][rr];
-                const float inv = mm == -INFINITY ? nan : 1.0f / (sum + sink_term(A, head, mm, kq_s[rr])) + nan;
+                const float inv = mm == -INFINITY ? nan : 1.0f / (sum + sink_term<kF32>(A, head, mm, kq_s[rr])) + nan;
                 const size_t at = (((size_t)(P.q0 + qi) << A.log_head) + head) * kD;
 #pragma unroll
-                for (int dt = 0; dt < kDT; ++dt) store_out<kF32>(A.out, at + out_dim(dt), o[rt][dt] * inv);
+                for (int dt = 0; dt < kDT; ++dt) {
+                    if (kF32)
+                        store_out<true>(A.out, at + out_dim(dt), o[rt][dt] * inv);
+                    else
+                        store_out<false>(stages[0], (rr * kOutB) / 2 + out_dim(dt), o[rt][dt] * inv);
+                }
+            }
+            if (!kF32) {   // whole rows of 1 KB (eight bytes a lane from the accumulators: 2 us more)
+                lds_barrier();
+                for (int rr = w; rr < P.n << lh; rr += kW) {
+                    const size_t at = (((size_t)(P.q0 + (rr >> lh)) << A.log_head) + P.head0 + (rr & ((1 << lh) - 1))) * kD + 8 * lane;
+                    *reinterpret_cast<uint4_t *>(static_cast<uint16_t *>(A.out) + at) =
+                        *reinterpret_cast<const uint4_t *>(stages[0] + rr * kOutB + 16 * lane);
+                }
             }
         } else {
             const int slot = 2 * wg + (begins ? 1 : 0);
@@ -768,67 +824,81 @@ __global__ __launch_bounds__(kF32 ? 256 : 512, kF32 ? 1 : 2) void window_kernel(
     }
 }
 
-// The parts of a problem that cuts fall into, in order, and the sink: one workgroup per
-// row. Waves 2 k and 2 k + 1 take the halves of parts k, k + 4, .., a lane four dims, sixteen
-// parts in flight; the four sums are joined in order.
-// kInline: workgroup b has row b % kRows of problem b / kRows; else of the problem that cut
-// b / kRows + 1 falls into, if that is its first cut.
-template <bool kF32, bool kInline>
-__global__ __launch_bounds__(512) void window_merge_kernel(const WinArgs A) {
-    __shared__ float f_s[kWgs];   // each part's factor
-    __shared__ float4_t o_s[3][128];
-    const int tid = threadIdx.x, row = blockIdx.x % kRows, n_prob = *A.n_prob;
-    const long long per = A.line[1];
-    int pi = blockIdx.x / kRows;
+// The parts of a problem that cuts fall into, in order, and the sink. A workgroup has
+// kShare rows: one, whose parts its four waves share (parts w, w + 4, .., then their sums in
+// order), or four, a wave each; a lane has eight dims, eight parts in flight.
+// kInline: the workgroups' problems are 0, 1, ..; else those that cuts 1, 2, .. fall into, each at its first cut.
+template <bool kF32, bool kInline, int kShare>
+__global__ __launch_bounds__(256) void window_merge_kernel(const WinArgs A) {
+    constexpr int kWg = kRows / kShare, kStep = kShare == 1 ? 4 : 1;
+    __shared__ float f_s[4][kWgs];   // each wave's parts' factors
+    __shared__ float4_t o_s[3][64][2];
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, n_prob = *A.n_prob;
+    const int row = kShare == 1 ? blockIdx.x % kWg : 4 * (blockIdx.x % kWg) + w;
+    const long long per = A.line[0], whole = A.line[1];
+    int pi = blockIdx.x / kWg;
     if (!kInline) pi = A.wg_prob[pi + 1];
     if (pi >= n_prob) return;
     const long long begin = A.pre[pi], end = A.pre[pi + 1];
     const long long b0 = begin / per;   // the workgroup of its first tile; the first cut is the next one's
-    if (end - begin <= kWhole || (b0 + 1) * per >= end) return;
-    if (!kInline && b0 != blockIdx.x / kRows) return;
+    if (end - begin <= whole || (b0 + 1) * per >= end) return;
+    if (!kInline && b0 != blockIdx.x / kWg) return;
     const Problem P = problem_of(A, A.prob[pi]);
     const int lh = log_hpt(A), qi = row >> lh, head = P.head0 + (row & ((1 << lh) - 1));
-    if (qi >= P.n) return;
+    if (qi >= P.n) return;   // (of four rows, whole waves; one row's waves leave together)
     const int parts = (int)((end - 1) / per - b0) + 1;
     // (the first part is its workgroup's last one, the others their workgroups' first)
     auto slot = [&](int c) { return (size_t)(2 * (b0 + c) + (c == 0)); };
     const float *ml = A.part_ml + row;
-    const int lane = tid & 63, w = tid >> 6;
     float mx = -INFINITY;
     for (int c = lane; c < parts; c += 64) mx = fmaxf(mx, ml[slot(c) * 3 * kRows]);
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor(mx, off));
     const float kq = ml[slot(0) * 3 * kRows + 2 * kRows];
-    float den = 0.0f;   // every wave its own, the same sums
+    float den = 0.0f;
     for (int c = lane; c < parts; c += 64) {
         const float *x = ml + slot(c) * 3 * kRows;
         const float f = x[0] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((x[0] - mx) * kq);
         den += x[kRows] * f;
-        if (w == 0) f_s[c] = f;
+        f_s[w][c] = f;
     }
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) den += __shfl_xor(den, off);
-    __syncthreads();
-    float4_t o = {0, 0, 0, 0};
-    const int d = 256 * (w & 1) + 4 * lane;
-    const float *src = A.part_o + (size_t)row * kD + d;
-    for (int c0 = w >> 1; c0 < parts; c0 += 64) {
-        float4_t v[16];
+    float4_t o[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+    const float *src = A.part_o + (size_t)row * kD + 8 * lane;
+    for (int c0 = kShare == 1 ? w : 0; c0 < parts; c0 += 8 * kStep) {
+        float4_t v[8][2];
 #pragma unroll
-        for (int u = 0; u < 16; ++u)
-            v[u] = *reinterpret_cast<const float4_t *>(src + slot(min(c0 + 4 * u, parts - 1)) * kRows * kD);
+        for (int u = 0; u < 8; ++u)
 #pragma unroll
-        for (int u = 0; u < 16; ++u)
-            if (c0 + 4 * u < parts) o += v[u] * f_s[c0 + 4 * u];
+            for (int h = 0; h < 2; ++h)
+                v[u][h] = *reinterpret_cast<const float4_t *>(src + slot(min(c0 + kStep * u, parts - 1)) * kRows * kD + 4 * h);
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+            if (c0 + kStep * u < parts) {
+                const float f = f_s[w][c0 + kStep * u];
+                o[0] += v[u][0] * f;
+                o[1] += v[u][1] * f;
+            }
     }
-    if (w >= 2) o_s[(w >> 1) - 1][64 * (w & 1) + lane] = o;
-    __syncthreads();
-    if (w >= 2) return;
+    if (kShare == 1) {
+        if (w > 0) {
+            o_s[w - 1][lane][0] = o[0];
+            o_s[w - 1][lane][1] = o[1];
+        }
+        __syncthreads();
+        if (w > 0) return;
 #pragma unroll
-    for (int k = 0; k < 3; ++k) o += o_s[k][64 * (w & 1) + lane];
+        for (int k = 0; k < 3; ++k) {
+            o[0] += o_s[k][lane][0];
+            o[1] += o_s[k][lane][1];
+        }
+    }
     // (a part whose rows could not be read has a NaN sum)
-    const float inv = mx == -INFINITY && den == 0.0f ? 0.0f : 1.0f / (den + sink_term(A, head, mx, kq));
-    store_out<kF32>(A.out, (((size_t)(P.q0 + qi) << A.log_head) + head) * kD + d, o * inv);
+    const float inv = mx == -INFINITY && den == 0.0f ? 0.0f : 1.0f / (den + sink_term<kF32>(A, head, mx, kq));
+    const size_t at = (((size_t)(P.q0 + qi) << A.log_head) + head) * kD + 8 * lane;
+    store_out<kF32>(A.out, at, o[0] * inv);
+    store_out<kF32>(A.out, at + 4, o[1] * inv);
 }
 
 size_t up256(size_t b) { return (b + 255) & ~(size_t)255; }
@@ -930,9 +1000,11 @@ extern "C" int ds4hip_flash_attn_window_fp8(const ds4hip_window_attn *a, void *w
     const long long span = std::min<long long>(held, (long long)a->window + (kRows >> std::min(lh, kLogRows)));
     const long long most = a->window > 0 ? span / kTile + 2 + (std::min<long long>(a->n_first, held) + kTile - 1) / kTile : held / kTile + 1;
     if (most > kWhole) {
-        auto *merge = f32 ? in ? window_merge_kernel<true, true> : window_merge_kernel<true, false>
-                          : in ? window_merge_kernel<false, true> : window_merge_kernel<false, false>;
-        hipLaunchKernelGGL(merge, dim3((in ? A.prob_cap : kWgs - 1) * kRows), dim3(512), 0, st, A);
+        const int n = in ? A.prob_cap : kWgs - 1;
+        auto *merge = n > 64 ? f32 ? in ? window_merge_kernel<true, true, 4> : window_merge_kernel<true, false, 4>
+                                   : in ? window_merge_kernel<false, true, 4> : window_merge_kernel<false, false, 4>
+                             : f32 ? window_merge_kernel<true, true, 1> : window_merge_kernel<false, true, 1>;
+        hipLaunchKernelGGL(merge, dim3(n * (n > 64 ? kRows / 4 : kRows)), dim3(256), 0, st, A);
     }
     return ds4hip_set_last_error(hip_status(hipGetLastError()));
 }

@@ -33,14 +33,15 @@ def row_values(codes, sexp, tail):
 
 def attend_64(q, kv, positions, window, first, sinks):
     """q [n, heads, 512] at `positions` over one sequence's rows kv, in 64 bits: the
-    outputs, the same averages of |value|, and how far each head's scores may be off."""
+    outputs, the same averages of |value|, how far each head's scores may be off, and the
+    largest weight times the sum of |value|."""
     n = q.shape[0]
     k = torch.arange(kv.shape[0], device=q.device)[None]
     p = torch.as_tensor(positions, device=q.device)[:, None]
     seen = k <= p
     if window:
         seen &= (k > p - window) | (k < first)
-    out, size, err = torch.zeros_like(q, dtype=torch.float64), torch.zeros_like(q, dtype=torch.float64), []
+    out, size, all_of, err = *(torch.zeros_like(q, dtype=torch.float64) for _ in range(3)), []
     for i in range(n):
         rows = kv[seen[i]]
         if rows.shape[0] == 0:
@@ -53,18 +54,23 @@ def attend_64(q, kv, positions, window, first, sinks):
         w = torch.softmax(s, -1)[:, :rows.shape[0]]
         out[i] = w @ rows
         size[i] = w @ rows.abs()
+        all_of[i] = w.amax(-1, keepdim=True) * rows.abs().sum(0)
         # |error of a score| <= 42 steps of 2^-23 (16 matrix instructions a score, each sum
         # of 32 products in 5 levels, truncated at worst) of the sum of |q k|
         err.append(42 * 2.0 ** -23 * (x.abs() @ rows.abs().T / math.sqrt(DIM)).amax(-1) + 2.0 ** -22 * s.abs().amax(-1))
-    return out, size, torch.stack(err) if err else torch.zeros((0, q.shape[1]), dtype=torch.float64, device=q.device)
+    return out, (size, all_of), torch.stack(err) if err else torch.zeros((0, q.shape[1]), dtype=torch.float64, device=q.device)
 
 
 def bound_of(ref, size, err, f32):
     """A weight is off by its own rounding (one f16: 2^-11; hi + lo: 2^-22) and by its
     score's error, as a share of itself; numerator and denominator each, so twice the
-    average |value|. Then the result's own rounding (bf16 2^-8, fp32 2^-24)."""
+    average |value|. One that is subnormal in f16 is off by up to 2^-25 instead, where the largest weight is
+    2^-8 or more (hi + lo: 2^8): by 2^-17 (2^-33) of the largest, for each row. Then the
+    result's own rounding (bf16 2^-8, fp32 2^-24)."""
+    size, all_of = size
     weight = (2.0 ** -22 if f32 else 2.0 ** -11) + err[..., None]
-    return 2 * weight * size + (2.0 ** -24 if f32 else 2.0 ** -8) * ref.abs() + 1e-30
+    return 2 * weight * size + 2 * (2.0 ** -33 if f32 else 2.0 ** -17) * all_of + \
+        (2.0 ** -24 if f32 else 2.0 ** -8) * ref.abs() + 1e-30
 
 
 class PoolModel:
