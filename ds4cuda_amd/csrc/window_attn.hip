@@ -442,7 +442,6 @@ __global__ __launch_bounds__(kF32 ? 256 : 512, kF32 ? 1 : 2) void window_kernel(
     constexpr int kN = 8 / kW;           // key halves of a wave, and thread rows of a tile
     constexpr int kDT = 4 * kN;          // dim tiles of a wave
     constexpr int kDB = 1024 / kW;       // its bytes of an f16 row
-    constexpr int kAhead = kF32 ? 1 : 2; // tiles in flight to registers
     __shared__ __attribute__((aligned(16))) uint8_t stages[3][kStageB];
     __shared__ __attribute__((aligned(16))) half4_t pb[2][kF32 ? 2 : 1][4][64][2];   // [buffer][hi, lo][row tile][lane][key half]
     __shared__ float top_s[2][kRows], l_s[2][kRows], m_s[kRows], kq_s[kRows];
@@ -502,16 +501,6 @@ __global__ __launch_bounds__(kF32 ? 256 : 512, kF32 ? 1 : 2) void window_kernel(
             va[kt] = lds_addr(stages[0]) + v * kRowB + kDB * w + 8 * (n16 & 3);
         }
     }
-    // The next problem's queries, brought to L2 while this one's tiles run (3 us from HBM
-    // otherwise, with nothing beside them): a word of each 128 bytes is read.
-    auto warm_q = [&](int next) {
-        const int4 rec = kInline ? prob_s[kInline ? next : 0] : A.prob[next];
-        const size_t item = kF32 ? 4 : 2, row0 = ((size_t)rec.y << A.log_head) + (rec.z >> 8), n = (size_t)((rec.z & 255) << lh) * kD * item;
-        const char *q = static_cast<const char *>(A.q) + row0 * kD * item;
-        for (size_t b = 128 * tid; b < n; b += 128 * 64 * kW) (void)*reinterpret_cast<const volatile int *>(q + b);
-    };
-    // first of the lane's four dims of the wave's dim tile dt
-    auto out_dim = [&](int dt) { return dim_of(kDB / 16 * w + 2 * dt + (g >> 1)) + 4 * (g & 1); };
 
     for (; t < t_end && pi < n_prob; ++pi) {
         const long long p_begin = kInline ? pre_s[kInline ? pi : 0] : A.pre[pi], p_end = kInline ? pre_s[kInline ? pi + 1 : 0] : A.pre[pi + 1];
@@ -535,45 +524,38 @@ __global__ __launch_bounds__(kF32 ? 256 : 512, kF32 ? 1 : 2) void window_kernel(
             // the thread's u-th row of tile i (past the last row seen: that row again, masked), and its page
             auto row_of = [&](int i, int u) { return min(kTile * tile_at(P, min(i, i1 - 1)) + (tid >> 4) + 16 * u, P.pos1); };
             auto page_of = [&](int i, int u) { return A.table[(long long)P.slot * A.stride + (row_of(i, u) >> A.shift)]; };
-            Part R[kAhead][kN];
+            Part R[kN];
             int page[kN];
-            // fetches tile i + 1 + kAhead (the pages after it first: waiting for a page must not wait for
-            // the rows). An entry outside the pool reads row 0
-            auto advance = [&](int i, Part (&R)[kN]) {
+            // fetches tile i + 2 (the pages after it first: waiting for a page must not wait for the
+            // rows). An entry outside the pool reads row 0
+            auto advance = [&](int i) {
                 int next[kN];
 #pragma unroll
-                for (int u = 0; u < kN; ++u) next[u] = page_of(i + 2 + kAhead, u);
+                for (int u = 0; u < kN; ++u) next[u] = page_of(i + 3, u);
 #pragma unroll
                 for (int u = 0; u < kN; ++u) {
                     if (page[u] < 0 || page[u] >= A.n_pages) {
                         bad = true;
                         page[u] = 0;
                     }
-                    load_part(A, ((long long)page[u] << A.shift) + (row_of(i + 1 + kAhead, u) & ((1 << A.shift) - 1)), tid & 15, R[u]);
+                    load_part(A, ((long long)page[u] << A.shift) + (row_of(i + 2, u) & ((1 << A.shift) - 1)), tid & 15, R[u]);
                     page[u] = next[u];
                 }
             };
-            auto store = [&](int stage, Part (&R)[kN]) {
+            auto store = [&](int stage) {
 #pragma unroll
                 for (int u = 0; u < kN; ++u) store_part(stages[0] + stage + 16 * u * kRowB, tid, R[u]);
             };
 #pragma unroll
             for (int u = 0; u < kN; ++u) page[u] = page_of(i0, u);
-            advance(i0 - 1 - kAhead, R[0]);
+            advance(i0 - 2);
             half8_t qh[16], ql[kF32 ? 16 : 1];
             const float kq = load_q<kF32>(A, P, row, g, qh, ql) * (kLog2e / 22.62741699796952f);   // 1 / sqrt(512)
             const int pos = P.pos0 + min(row >> lh, P.n - 1);   // (rows past the queries repeat the last one's)
             float m = -INFINITY, l = 0.0f, sum = 0.0f;
             float ref = 0.0f;   // m, or 0 while there is none
-            store(0, R[0]);
-            // (in the loop's order: its waits count the loads behind the one they wait for)
-#pragma unroll
-            for (int u = 0; u < kAhead; ++u) {
-                __builtin_amdgcn_sched_barrier(0);
-                advance(i0 - kAhead + u, R[u]);
-            }
-            __builtin_amdgcn_sched_barrier(0);
-            if (t < t_end && pi + 1 < n_prob) warm_q(pi + 1);
+            store(0);
+            advance(i0 - 1);
             int sp = 2 * kStageB, sc = 0, sn = kStageB;   // stages of tiles i - 1, i, i + 1
             int buf = 0;                                  // P's of tile i
             float4_t acc[kN];                             // scores of the tile whose P is the newest
@@ -690,9 +672,9 @@ __global__ __launch_bounds__(kF32 ? 256 : 512, kF32 ? 1 : 2) void window_kernel(
                 kq_s[row] = kq;
             }
             bool edge_before = false;
-            auto step = [&](int i, Part (&R)[kN]) {
+            auto step = [&](int i) {
                 const bool live = i < i1;
-                if (i <= i1) lds_barrier();
+                lds_barrier();
                 const int4 f0 = *reinterpret_cast<const int4 *>(&moved_s[buf ^ 1][0]), f1 = *reinterpret_cast<const int4 *>(&moved_s[buf ^ 1][4]);
                 float4_t a[kN][2];   // two chains each
                 if (live && scores_mine) {
@@ -726,13 +708,13 @@ __global__ __launch_bounds__(kF32 ? 256 : 512, kF32 ? 1 : 2) void window_kernel(
                         __builtin_amdgcn_sched_barrier(0);
                     }
                 }
-                if (i > i0 && i <= i1) {
+                if (i > i0) {
                     settle(buf ^ 1, f0, f1);   // (acc: still the scores of the tile before)
                     add(buf ^ 1, edge_before);
                 }
-                if (live) store(sn, R);
-                advance(i, R);
                 if (!live) return;
+                store(sn);
+                advance(i);
 #pragma unroll
                 for (int u = 0; u < kN; ++u) acc[u] = a[u][0] + a[u][1];
                 const int tile = tile_at(P, i), key0 = kTile * tile;
@@ -763,13 +745,8 @@ __global__ __launch_bounds__(kF32 ? 256 : 512, kF32 ? 1 : 2) void window_kernel(
                 sc = sn;
                 sn = free;
             };
-            // The last step only adds the tile before (the code of settle and add stands once). One past
-            // it only loads: the loads behind one that a step waits for are the same on all paths, else the
-            // compiler would wait for all.
-            for (int i = i0; i <= i1; i += kAhead) {
-#pragma unroll
-                for (int u = 0; u < kAhead; ++u) step(i + u, R[u]);
-            }
+            // the last step only adds the tile before: the code of settle and add stands once
+            for (int i = i0; i <= i1; ++i) step(i);
             l = xsum_16_32(l);
             if (g == 0) l_s[kh][row] = l;
         } else if (tid < kRows) {
@@ -778,11 +755,14 @@ __global__ __launch_bounds__(kF32 ? 256 : 512, kF32 ? 1 : 2) void window_kernel(
         if (__any(bad) && lane == 0) bad_s = 1;
         lds_barrier();
         const float nan = bad_s ? __builtin_nanf("") : 0.0f;
+        const int lane_e = again(lane), n_e = lane_e & 15, g_e = lane_e >> 4;
+        // first of the lane's four dims of the wave's dim tile dt
+        auto out_dim = [&](int dt) { return dim_of(kDB / 16 * w + 2 * dt + (g_e >> 1)) + 4 * (g_e & 1); };
         if (begins && ends) {
             constexpr int kOutB = 2 * kD + 16;   // a bf16 row in LDS
 #pragma unroll
             for (int rt = 0; rt < 4; ++rt) {
-                const int rr = 16 * rt + n16, qi = rr >> lh, head = P.head0 + (rr & ((1 << lh) - 1));
+                const int rr = 16 * rt + n_e, qi = rr >> lh, head = P.head0 + (rr & ((1 << lh) - 1));
                 if (qi >= P.n) continue;
                 const float mm = m_s[rr];
                 const float sum = kW == 8 ? l_s[0][rr] + l_s[1][rr] : l_s[0][rr];
@@ -799,9 +779,9 @@ __global__ __launch_bounds__(kF32 ? 256 : 512, kF32 ? 1 : 2) void window_kernel(
             if (!kF32) {   // whole rows of 1 KB (eight bytes a lane from the accumulators: 2 us more)
                 lds_barrier();
                 for (int rr = w; rr < P.n << lh; rr += kW) {
-                    const size_t at = (((size_t)(P.q0 + (rr >> lh)) << A.log_head) + P.head0 + (rr & ((1 << lh) - 1))) * kD + 8 * lane;
+                    const size_t at = (((size_t)(P.q0 + (rr >> lh)) << A.log_head) + P.head0 + (rr & ((1 << lh) - 1))) * kD + 8 * lane_e;
                     *reinterpret_cast<uint4_t *>(static_cast<uint16_t *>(A.out) + at) =
-                        *reinterpret_cast<const uint4_t *>(stages[0] + rr * kOutB + 16 * lane);
+                        *reinterpret_cast<const uint4_t *>(stages[0] + rr * kOutB + 16 * lane_e);
                 }
             }
         } else {
@@ -812,7 +792,7 @@ __global__ __launch_bounds__(kF32 ? 256 : 512, kF32 ? 1 : 2) void window_kernel(
                 ml[kRows] = (kW == 8 ? l_s[0][tid] + l_s[1][tid] : l_s[0][tid]) + nan;
                 ml[2 * kRows] = kq_s[tid];
             }
-            float *dst = A.part_o + ((size_t)slot * kRows + n16) * kD;
+            float *dst = A.part_o + ((size_t)slot * kRows + n_e) * kD;
 #pragma unroll
             for (int rt = 0; rt < 4; ++rt) {
                 if (16 * rt >= P.n << lh) break;

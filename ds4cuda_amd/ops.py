@@ -300,6 +300,11 @@ def _addr(t):
     return None if t is None else t.data_ptr()
 
 
+def _ready(t, dtype, index):
+    """Whether t is a contiguous tensor of that type on GPU `index`."""
+    return t.dtype is dtype and t.get_device() == index and t.is_contiguous()
+
+
 def window_workspace_bytes(n_seqs, n_q, n_head) -> int:
     return lib().ds4hip_flash_attn_window_fp8_workspace_bytes(n_seqs, n_q, n_head)
 
@@ -362,6 +367,9 @@ class WindowView:
         _check(cache.tail, cache.tail.dtype, cache.n_rows * N_ROT, "tail")
         if cache.tail.element_size() != 2:
             raise Ds4HipError("tail: expected f16 values or their bits", -22)
+        self.index = cache.codes.get_device()
+        if {page_table.get_device(), seq_rows.get_device(), cache.sexp.get_device(), cache.tail.get_device()} != {self.index}:
+            raise Ds4HipError("the cache, its page table and its rows must be on one GPU", -22)
         self.keep = (cache, page_table, seq_rows)
         self.fixed = dict(codes=cache.codes.data_ptr(), sexp=cache.sexp.data_ptr(), tail=cache.tail.data_ptr(),
                           n_cache_rows=cache.n_rows, table=page_table.data_ptr(), rows=seq_rows.data_ptr(), n_slots=slots,
@@ -371,10 +379,11 @@ class WindowView:
         if q.dim() != 3 or q.shape[2] != HEAD_DIM or q.dtype not in (torch.bfloat16, torch.float32):
             raise Ds4HipError("q must be bf16 or fp32 [n_q, n_head, 512]", -22)
         n_q, n_head = q.shape[0], q.shape[1]
-        _check(q, q.dtype, None, "q")
-        _check(sinks, torch.float32, n_head, "sinks")
-        _check(q_start, torch.int32, 1, "q_start")
-        _check(seq_ids, torch.int32, None, "seq_ids")
+        for t, dtype, n, name in ((q, q.dtype, None, "q"), (sinks, torch.float32, n_head, "sinks"),
+                                  (q_start, torch.int32, 1, "q_start"), (seq_ids, torch.int32, None, "seq_ids")):
+            if t is not None and (not _ready(t, dtype, self.index) or (n and t.numel() < n)):
+                _check(t, dtype, n, name)
+                raise Ds4HipError(f"{name}: on {t.device}, the cache is on GPU {self.index}", -22)
         n_seqs = q_start.numel() - 1 if q_start is not None else n_q
         if seq_ids is not None and seq_ids.numel() != n_seqs:
             raise Ds4HipError(f"seq_ids: {n_seqs} entries expected, got {seq_ids.numel()}", -22)

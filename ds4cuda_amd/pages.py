@@ -13,7 +13,7 @@ import ctypes as C
 import torch
 
 from ._lib import Ds4HipError, call, lib
-from .ops import HEAD_DIM, N_NOPE, N_ROT, Fp8KVCache, WindowView, _check, _on_stream, _ptr, _stream
+from .ops import HEAD_DIM, N_NOPE, N_ROT, Fp8KVCache, WindowView, _addr, _check, _on_stream, _ptr, _ready, _stream
 
 MAX_JOBS = 1024    # sequences of one call
 
@@ -38,6 +38,8 @@ class PagePool:
     def __init__(self, codes, sexp, tail, refs, table, rows, page_rows, status=None):
         if codes.dim() != 3 or table.dim() != 2:
             raise Ds4HipError("codes must be [layers, rows, 448] and table [sequences, entries]", -22)
+        if len({t.device for t in (codes, sexp, tail, refs, table, rows)}) > 1:
+            raise Ds4HipError("the pool's tensors must be on one device", -22)
         layers, n_rows = codes.shape[0], codes.shape[1]
         n_pages = refs.numel()
         _check(codes, torch.uint8, layers * n_rows * N_NOPE, "codes")
@@ -54,9 +56,10 @@ class PagePool:
         self.codes, self.sexp, self.tail = codes, sexp, tail
         self.refs, self.table, self.rows = refs, table, rows
         self.page_rows, self.n_layers, self.n_pages, self.n_seqs = int(page_rows), layers, n_pages, table.shape[0]
-        self.device = codes.device
+        self.device, self.index = codes.device, codes.device.index
         self.c = KvPages(_ptr(codes), _ptr(sexp), _ptr(tail), n_rows, layers, n_pages, self.page_rows, table.shape[1],
                          self.n_seqs, _ptr(refs), _ptr(table), _ptr(rows), _ptr(self.status))
+        self._c = C.byref(self.c)
         self._workspace = None
         self._views = {}
 
@@ -71,7 +74,7 @@ class PagePool:
                    torch.empty((n_seqs, -(-max_rows // page_rows)), dtype=torch.int32, device=device),
                    torch.empty(n_seqs, dtype=torch.int32, device=device), page_rows)
         with torch.cuda.device(pool.device):
-            call("ds4hip_kv_pages_init", C.byref(pool.c), _stream(None))
+            call("ds4hip_kv_pages_init", pool._c, _stream(None))
         return pool
 
     def layer(self, layer) -> Fp8KVCache:
@@ -89,17 +92,28 @@ class PagePool:
     def _jobs(self, ids, name, n=None):
         if ids is None:
             return 0
-        _check(ids, torch.int32, n, name)
-        if n is not None and ids.numel() != n:
-            raise Ds4HipError(f"{name}: {n} entries expected, got {ids.numel()}", -22)
-        return ids.numel()
+        if not _ready(ids, torch.int32, self.index):
+            _check(ids, torch.int32, None, name)
+            raise Ds4HipError(f"{name}: on {ids.device}, the pool is on {self.device}", -22)
+        k = ids.numel()
+        if n is not None and k != n:
+            raise Ds4HipError(f"{name}: {n} entries expected, got {k}", -22)
+        return k
+
+    def _call(self, name, stream, *args):
+        with _on_stream(stream, self.device):
+            call(name, self._c, *args, _stream(stream))
+
+    def _empty(self, size, dtype, stream):
+        with _on_stream(stream, self.device):
+            return torch.empty(size, dtype=dtype, device=self.device)
 
     def _ws(self, stream):
         if self._workspace is None:
-            need = lib().ds4hip_kv_pages_workspace_bytes(C.byref(self.c))
-            with _on_stream(stream, self.device):
-                self._workspace = torch.empty(need, dtype=torch.uint8, device=self.device)
-        return self._workspace
+            need = lib().ds4hip_kv_pages_workspace_bytes(self._c)
+            self._workspace = self._empty(need, torch.uint8, stream)
+            self._ws_args = (self._workspace.data_ptr(), need)
+        return self._ws_args
 
     def extend(self, seqs, n_new, n_dst, dst_rows=None, stream=None):
         """n_new[j] more rows for sequence seqs[j] (int32 device tensors): takes the
@@ -107,12 +121,11 @@ class PagePool:
         (-1 past the last job's rows, or everywhere where the call is refused)."""
         n = self._jobs(seqs, "seqs")
         self._jobs(n_new, "n_new", n)
-        with _on_stream(stream, self.device):
-            if dst_rows is None:
-                dst_rows = torch.empty(n_dst, dtype=torch.int64, device=self.device)
+        if dst_rows is None:
+            dst_rows = self._empty(n_dst, torch.int64, stream)
+        else:
             _check(dst_rows, torch.int64, n_dst, "dst_rows")
-            call("ds4hip_kv_pages_extend", C.byref(self.c), _ptr(seqs), _ptr(n_new), n, _ptr(dst_rows), int(n_dst),
-                 _stream(stream))
+        self._call("ds4hip_kv_pages_extend", stream, _addr(seqs), _addr(n_new), n, dst_rows.data_ptr(), int(n_dst))
         return dst_rows
 
     def append(self, kv, dst_rows, layer=0, stream=None):
@@ -121,8 +134,7 @@ class PagePool:
         n = kv.shape[0]
         _check(kv, torch.float32, n * HEAD_DIM, "kv")
         _check(dst_rows, torch.int64, n, "dst_rows")
-        with _on_stream(stream, self.device):
-            call("ds4hip_kv_pages_append", C.byref(self.c), int(layer), _ptr(kv), n, _ptr(dst_rows), _stream(stream))
+        self._call("ds4hip_kv_pages_append", stream, int(layer), kv.data_ptr(), n, dst_rows.data_ptr())
 
     def fork(self, parents, children, n_rows=None, deep=False, stream=None):
         """children[j] (empty sequences) become copies of the first n_rows[j] rows (None
@@ -131,28 +143,24 @@ class PagePool:
         n = self._jobs(parents, "parents")
         self._jobs(children, "children", n)
         self._jobs(n_rows, "n_rows", n)
-        ws = self._ws(stream)
-        with _on_stream(stream, self.device):
-            call("ds4hip_kv_pages_fork", C.byref(self.c), _ptr(parents), _ptr(children), _ptr(n_rows), n, int(bool(deep)),
-                 _ptr(ws), ws.numel(), _stream(stream))
+        self._call("ds4hip_kv_pages_fork", stream, _addr(parents), _addr(children), _addr(n_rows), n, int(bool(deep)),
+                   *self._ws(stream))
 
     def free(self, seqs, keep=None, stream=None):
         """Cuts sequences seqs[j] down to keep[j] rows (None: to nothing) and releases
         their other pages."""
         n = self._jobs(seqs, "seqs")
         self._jobs(keep, "keep", n)
-        with _on_stream(stream, self.device):
-            call("ds4hip_kv_pages_free", C.byref(self.c), _ptr(seqs), _ptr(keep), n, _stream(stream))
+        self._call("ds4hip_kv_pages_free", stream, _addr(seqs), _addr(keep), n)
 
     def compact(self, n_live=None, stream=None):
         """Moves the held pages to the front of the pool; returns their number, an int32
         device scalar."""
-        ws = self._ws(stream)
-        with _on_stream(stream, self.device):
-            if n_live is None:
-                n_live = torch.empty((), dtype=torch.int32, device=self.device)
+        if n_live is None:
+            n_live = self._empty((), torch.int32, stream)
+        else:
             _check(n_live, torch.int32, 1, "n_live")
-            call("ds4hip_kv_pages_compact", C.byref(self.c), _ptr(n_live), _ptr(ws), ws.numel(), _stream(stream))
+        self._call("ds4hip_kv_pages_compact", stream, n_live.data_ptr(), *self._ws(stream))
         return n_live
 
     def attend(self, q, *, seqs=None, q_start=None, window=0, n_first=0, sinks=None, layer=0, out=None, workspace=None,
