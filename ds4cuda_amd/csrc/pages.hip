@@ -61,11 +61,13 @@ __device__ inline void scan_jobs(Plan &S, long long v, int *out, int n_jobs) {
         if (lane >= off) x += y;
     }
     x = x < kMost ? x : kMost;
-    __syncthreads();
-    if (lane == 63) S.sums[w] = (int)x;
-    __syncthreads();
-    for (int i = 0; i < w; ++i) x += S.sums[i];
-    x = x < kMost ? x : kMost;
+    if (n_jobs > 64) {   // (else the first wave has all)
+        __syncthreads();
+        if (lane == 63) S.sums[w] = (int)x;
+        __syncthreads();
+        for (int i = 0; i < w; ++i) x += S.sums[i];
+        x = x < kMost ? x : kMost;
+    }
     if (tid < n_jobs) out[tid + 1] = (int)x;
     if (tid == 0) out[0] = 0;
     __syncthreads();
@@ -100,19 +102,30 @@ __device__ inline bool failed(Plan &S, const ds4hip_kv_pages &P) {
 
 __device__ inline void fail(Plan &S, int code) { atomicOr(&S.fail, code == kEINVAL ? 1 : 2); }
 
+// The thread's counts of a step of the search below, from page p0 on. A kernel loads the
+// first ones before anything else: they arrive while it checks its jobs.
+struct Counts {
+    int c[kScan];
+};
+__device__ inline Counts counts_from(const ds4hip_kv_pages &P, int p0) {
+    Counts C;
+#pragma unroll
+    for (int u = 0; u < kScan; ++u) {
+        const int p = p0 + u * kThreads + (int)threadIdx.x;
+        C.c[u] = p < P.n_pages ? P.refs[p] : 1;
+    }
+    return C;
+}
+
 // use(k, page) for the `want` lowest free pages, k = 0, 1, ... in order; false where
 // there are fewer. 8192 counts a step, from the front, until there are enough.
 template <typename Use>
-__device__ inline bool lowest_free(Plan &S, const ds4hip_kv_pages &P, int want, Use use) {
+__device__ inline bool lowest_free(Plan &S, const ds4hip_kv_pages &P, Counts C, int want, Use use) {
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
     int found = 0;
     for (int p0 = 0; p0 < P.n_pages && found < want; p0 += kScan * kThreads) {
-        int c[kScan];
-#pragma unroll
-        for (int u = 0; u < kScan; ++u) {
-            const int p = p0 + u * kThreads + tid;
-            c[u] = p < P.n_pages ? P.refs[p] : 1;
-        }
+        if (p0) C = counts_from(P, p0);
+        const int (&c)[kScan] = C.c;
         uint64_t b[kScan];
         __syncthreads();
 #pragma unroll
@@ -168,6 +181,7 @@ __global__ __launch_bounds__(kThreads) void extend_kernel(const ds4hip_kv_pages 
     __shared__ Plan S;
     __shared__ int rows_s[kJobs];
     const int tid = threadIdx.x;
+    const Counts counts = counts_from(P, 0);
     start(S, P.n_seqs);
     int seq = -1, n = 0, r0 = 0, need = 0;
     if (tid < n_jobs) {
@@ -203,7 +217,7 @@ __global__ __launch_bounds__(kThreads) void extend_kernel(const ds4hip_kv_pages 
     bool refused = failed(S, P);
     if (!refused) {
         // into the tables, where entries past the rows mean nothing yet
-        const bool enough = lowest_free(S, P, want, [&](int k, int page) {
+        const bool enough = lowest_free(S, P, counts, want, [&](int k, int page) {
             const int j = job_of(S.base, n_jobs, k);
             *entry(P, S.at[j], pages_of(P, rows_s[j]) + k - S.base[j]) = page;
         });
@@ -242,6 +256,7 @@ __global__ __launch_bounds__(kThreads) void fork_kernel(const ds4hip_kv_pages P,
     __shared__ Plan S;
     __shared__ int child_s[kJobs], rows_s[kJobs];
     const int tid = threadIdx.x, page_rows = P.page_rows;
+    const Counts counts = counts_from(P, 0);
     start(S, P.n_seqs);
     int child = -1, r = 0;
     if (tid < n_jobs) {
@@ -275,7 +290,7 @@ __global__ __launch_bounds__(kThreads) void fork_kernel(const ds4hip_kv_pages P,
         refused = failed(S, P);
     }
     if (!refused) {
-        const bool enough = lowest_free(S, P, want, [&](int k, int page) {
+        const bool enough = lowest_free(S, P, counts, want, [&](int k, int page) {
             const int j = job_of(S.base, n_jobs, k);
             const int i = deep ? k - S.base[j] : pages_of(P, rows_s[j]) - 1;
             M.src[k] = *entry(P, S.at[j], i);

@@ -24,7 +24,6 @@ using namespace ds4hip;
 
 namespace {
 
-constexpr int kLogRows = 6, kRows = 1 << kLogRows;   // rows (queries x heads) of a problem
 constexpr int kWgs = 256;            // workgroups the line of tiles is cut for: one per CU
 constexpr int kMinTiles = 4;         // tiles of a part
 constexpr int kWhole = 8;            // tiles of a problem that is never cut
@@ -51,6 +50,7 @@ struct WinArgs {
     const uint16_t *tail;
     const int32_t *table, *rows, *q_start, *seq_ids;
     int n_seqs, n_slots, n_q, log_head, window, first, stride, shift, n_pages;
+    int log_rows;            // a problem has 2^log_rows rows (queries x heads)
     // workspace
     int prob_cap;
     long long *line;         // [2] tiles per workgroup, tiles of a problem that stays whole
@@ -59,8 +59,8 @@ struct WinArgs {
     long long *pre;          // [prob_cap + 1] tiles before each problem
     long long *wg_tile;      // [kWgs + 1] first tile of each workgroup
     int *wg_prob;            // [kWgs + 1] the problem it lies in
-    float *part_ml;          // [2 kWgs][3][kRows] references, sums and scales to log2
-    float *part_o;           // [2 kWgs][kRows][kD] unnormalized outputs
+    float *part_ml;          // [2 kWgs][3][rows] references, sums and scales to log2
+    float *part_o;           // [2 kWgs][rows][kD] unnormalized outputs
 };
 
 // The queries of sequence s: their first packed index and their number, whatever
@@ -72,13 +72,13 @@ __device__ inline int2 queries_of(const WinArgs &A, int s) {
 }
 
 // The heads of a query in one problem.
-__device__ inline int log_hpt(const WinArgs &A) { return min(A.log_head, kLogRows); }
+__device__ inline int log_hpt(const WinArgs &A) { return min(A.log_head, A.log_rows); }
 
 // Problem `tile` of sequence s as the plan keeps it: its table row (-1: not a sequence of
 // the table, or one with more rows than its table row holds), first packed query, number of
 // queries and first head (times 256), position of its first query.
 __device__ inline int4 record_of(const WinArgs &A, int s, int tile) {
-    const int lh = log_hpt(A), lg = A.log_head - lh, qpt = kRows >> lh;
+    const int lh = log_hpt(A), lg = A.log_head - lh, qpt = (1 << A.log_rows) >> lh;
     const int2 qs = queries_of(A, s);
     const int q = (tile >> lg) * qpt, slot = A.seq_ids ? A.seq_ids[s] : s;
     const bool in = slot >= 0 && slot < A.n_slots;
@@ -159,7 +159,7 @@ __device__ inline long long block_scan(long long v, long long *sums, long long *
 template <int kThreads, typename Put>
 __device__ inline int lay_line(const WinArgs &A, int *first_s, long long *sums, int *longest, long long *tiles, Put put) {
     const int tid = threadIdx.x;
-    const int lh = log_hpt(A), lg = A.log_head - lh, qpt = kRows >> lh;
+    const int lh = log_hpt(A), lg = A.log_head - lh, qpt = (1 << A.log_rows) >> lh;
     long long n_all = 0, t_all = 0;
     if (A.q_start) {
         for (int s0 = 0; s0 < A.n_seqs; s0 += kThreads) {
@@ -217,7 +217,8 @@ struct Cuts {
 __device__ inline Cuts cuts_of(long long tiles, int n_prob, int longest) {
     Cuts C;
     C.tiles = tiles;
-    C.per = max((tiles + kWgs - 1) / kWgs, (long long)kMinTiles);
+    // at least sqrt(longest / 16) tiles: a long problem's merge takes 0.09 us a part, a tile 1.5
+    C.per = max((tiles + kWgs - 1) / kWgs, (long long)max(kMinTiles, (int)sqrtf((float)longest * 0.0625f)));
     C.whole = (int)min(max((long long)kWhole, C.per / 8), 1LL << 30);
     if (n_prob <= kWgs && longest <= C.per + kPart) {
         C.whole = -1;
@@ -431,20 +432,23 @@ __device__ inline void store_part(uint8_t *stage, int tid, const Part &R) {
     *reinterpret_cast<uint2_t *>(rp + 512 + 16 * (12 + (u & 3)) + 256 * (u >> 2) + 8 * (j & 1)) = R.t;
 }
 
+constexpr int waves_of(bool f32, int row_tiles) { return f32 && row_tiles == 4 ? 4 : 8; }
+
 // Iteration i, with one barrier: scores of tile i | tile i + 1 dequantized, a later one
 // fetched | P of tile i | O += P V of tile i - 1. P is computed against the references of the
 // tile before. Where a row outgrows its reference, P's tile is marked, and before it is
 // used all waves agree on new references, rescale and compute it again from its scores:
 // always on the first tile, seldom after it.
-template <bool kF32, bool kInline>
-__global__ __launch_bounds__(kF32 ? 256 : 512, kF32 ? 1 : 2) void window_kernel(const WinArgs A) {
-    constexpr int kW = kF32 ? 4 : 8;     // waves
+template <bool kF32, int kRT, bool kInline>
+__global__ __launch_bounds__(waves_of(kF32, kRT) * 64, waves_of(kF32, kRT) / 4) void window_kernel(const WinArgs A) {
+    constexpr int kRows = 16 * kRT;      // rows of a problem
+    constexpr int kW = waves_of(kF32, kRT);
     constexpr int kN = 8 / kW;           // key halves of a wave, and thread rows of a tile
     constexpr int kDT = 4 * kN;          // dim tiles of a wave
     constexpr int kDB = 1024 / kW;       // its bytes of an f16 row
     __shared__ __attribute__((aligned(16))) uint8_t stages[3][kStageB];
-    __shared__ __attribute__((aligned(16))) half4_t pb[2][kF32 ? 2 : 1][4][64][2];   // [buffer][hi, lo][row tile][lane][key half]
-    __shared__ float top_s[2][kRows], l_s[2][kRows], m_s[kRows], kq_s[kRows];
+    __shared__ __attribute__((aligned(16))) half4_t pb[2][kF32 ? 2 : 1][kRT][64][2];   // [buffer][hi, lo][row tile][lane][key half]
+    __shared__ float top_s[2][64], l_s[2][64], m_s[64], kq_s[64];
     __shared__ uint32_t odd_s[2][8];   // keys whose scores are not finite, per wave
     __shared__ __attribute__((aligned(16))) int moved_s[2][8];   // whether a row of the wave's outgrew its reference
     __shared__ int bad_s;
@@ -511,9 +515,9 @@ __global__ __launch_bounds__(kF32 ? 256 : 512, kF32 ? 1 : 2) void window_kernel(
         const int i0 = __builtin_amdgcn_readfirstlane((int)(t - p_begin)), i1 = __builtin_amdgcn_readfirstlane((int)(min(p_end, t_end) - p_begin));
         t = min(p_end, t_end);
         bool bad = P.slot < 0;
-        float4_t o[4][kDT];
+        float4_t o[kRT][kDT];
 #pragma unroll
-        for (int a = 0; a < 4; ++a)
+        for (int a = 0; a < kRT; ++a)
 #pragma unroll
             for (int b = 0; b < kDT; ++b) o[a][b] = float4_t{0, 0, 0, 0};
         if (tid == 0) bad_s = 0;
@@ -550,7 +554,8 @@ __global__ __launch_bounds__(kF32 ? 256 : 512, kF32 ? 1 : 2) void window_kernel(
             for (int u = 0; u < kN; ++u) page[u] = page_of(i0, u);
             advance(i0 - 2);
             half8_t qh[16], ql[kF32 ? 16 : 1];
-            const float kq = load_q<kF32>(A, P, row, g, qh, ql) * (kLog2e / 22.62741699796952f);   // 1 / sqrt(512)
+            float kq = 0.0f;
+            if (scores_mine) kq = load_q<kF32>(A, P, row, g, qh, ql) * (kLog2e / 22.62741699796952f);   // 1 / sqrt(512)
             const int pos = P.pos0 + min(row >> lh, P.n - 1);   // (rows past the queries repeat the last one's)
             float m = -INFINITY, l = 0.0f, sum = 0.0f;
             float ref = 0.0f;   // m, or 0 while there is none
@@ -580,8 +585,8 @@ __global__ __launch_bounds__(kF32 ? 256 : 512, kF32 ? 1 : 2) void window_kernel(
                         sum = __builtin_amdgcn_fdot2(half2_t{ph[0], ph[1]}, one, sum, false);
                         sum = __builtin_amdgcn_fdot2(half2_t{ph[2], ph[3]}, one, sum, false);
                     }
-                    pb[b][0][w & 3][lane][kh + u] = ph;
-                    if (kF32) pb[b][kF32 ? 1 : 0][w & 3][lane][kh + u] = pl;
+                    pb[b][0][w & (kRT - 1)][lane][kh + u] = ph;
+                    if (kF32) pb[b][kF32 ? 1 : 0][w & (kRT - 1)][lane][kh + u] = pl;
                 }
             };
             auto top_of = [&]() {
@@ -611,7 +616,7 @@ __global__ __launch_bounds__(kF32 ? 256 : 512, kF32 ? 1 : 2) void window_kernel(
                         return f;
                     };
 #pragma unroll
-                    for (int rt = 0; rt < 4; ++rt) {
+                    for (int rt = 0; rt < kRT; ++rt) {
                         if (rt >= n_rt) break;
                         float old = m_s[16 * rt + n_r];
                         const float f = renew(16 * rt + n_r, old, kq_s[16 * rt + n_r]);
@@ -651,7 +656,7 @@ __global__ __launch_bounds__(kF32 ? 256 : 512, kF32 ? 1 : 2) void window_kernel(
                     else
                         read_vt4<4>(va[0] + sp, va[1] + sp, vb);
 #pragma unroll
-                    for (int rt = 0; rt < 4; ++rt) {
+                    for (int rt = 0; rt < kRT; ++rt) {
                         if (rt >= n_rt) break;
                         const half8_t h = *reinterpret_cast<const half8_t *>(&pb[b][0][rt][lane][0]);
 #pragma unroll
@@ -667,7 +672,7 @@ __global__ __launch_bounds__(kF32 ? 256 : 512, kF32 ? 1 : 2) void window_kernel(
                 }
             };
 
-            if (kh == 0 && g == 0) {
+            if (kh == 0 && g == 0 && scores_mine) {
                 m_s[row] = m;
                 kq_s[row] = kq;
             }
@@ -748,7 +753,7 @@ __global__ __launch_bounds__(kF32 ? 256 : 512, kF32 ? 1 : 2) void window_kernel(
             // the last step only adds the tile before: the code of settle and add stands once
             for (int i = i0; i <= i1; ++i) step(i);
             l = xsum_16_32(l);
-            if (g == 0) l_s[kh][row] = l;
+            if (g == 0 && scores_mine) l_s[kh][row] = l;
         } else if (tid < kRows) {
             m_s[tid] = -INFINITY;
         }
@@ -761,7 +766,7 @@ __global__ __launch_bounds__(kF32 ? 256 : 512, kF32 ? 1 : 2) void window_kernel(
         if (begins && ends) {
             constexpr int kOutB = 2 * kD + 16;   // a bf16 row in LDS
 #pragma unroll
-            for (int rt = 0; rt < 4; ++rt) {
+            for (int rt = 0; rt < kRT; ++rt) {
                 const int rr = 16 * rt + n_e, qi = rr >> lh, head = P.head0 + (rr & ((1 << lh) - 1));
                 if (qi >= P.n) continue;
                 const float mm = m_s[rr];
@@ -794,7 +799,7 @@ __global__ __launch_bounds__(kF32 ? 256 : 512, kF32 ? 1 : 2) void window_kernel(
             }
             float *dst = A.part_o + ((size_t)slot * kRows + n_e) * kD;
 #pragma unroll
-            for (int rt = 0; rt < 4; ++rt) {
+            for (int rt = 0; rt < kRT; ++rt) {
                 if (16 * rt >= P.n << lh) break;
 #pragma unroll
                 for (int dt = 0; dt < kDT; ++dt) *reinterpret_cast<float4_t *>(dst + 16 * rt * kD + out_dim(dt)) = o[rt][dt];
@@ -810,19 +815,20 @@ __global__ __launch_bounds__(kF32 ? 256 : 512, kF32 ? 1 : 2) void window_kernel(
 // kInline: the workgroups' problems are 0, 1, ..; else those that cuts 1, 2, .. fall into, each at its first cut.
 template <bool kF32, bool kInline, int kShare>
 __global__ __launch_bounds__(256) void window_merge_kernel(const WinArgs A) {
-    constexpr int kWg = kRows / kShare, kStep = kShare == 1 ? 4 : 1;
+    constexpr int kStep = kShare == 1 ? 4 : 1;
+    const int rows = 1 << A.log_rows, wgs = rows / kShare;   // workgroups of a problem
     __shared__ float f_s[4][kWgs];   // each wave's parts' factors
     __shared__ float4_t o_s[3][64][2];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, n_prob = *A.n_prob;
-    const int row = kShare == 1 ? blockIdx.x % kWg : 4 * (blockIdx.x % kWg) + w;
+    const int row = kShare == 1 ? blockIdx.x % wgs : 4 * (blockIdx.x % wgs) + w;
     const long long per = A.line[0], whole = A.line[1];
-    int pi = blockIdx.x / kWg;
+    int pi = blockIdx.x / wgs;
     if (!kInline) pi = A.wg_prob[pi + 1];
     if (pi >= n_prob) return;
     const long long begin = A.pre[pi], end = A.pre[pi + 1];
     const long long b0 = begin / per;   // the workgroup of its first tile; the first cut is the next one's
     if (end - begin <= whole || (b0 + 1) * per >= end) return;
-    if (!kInline && b0 != blockIdx.x / kWg) return;
+    if (!kInline && b0 != blockIdx.x / wgs) return;
     const Problem P = problem_of(A, A.prob[pi]);
     const int lh = log_hpt(A), qi = row >> lh, head = P.head0 + (row & ((1 << lh) - 1));
     if (qi >= P.n) return;   // (of four rows, whole waves; one row's waves leave together)
@@ -831,15 +837,15 @@ __global__ __launch_bounds__(256) void window_merge_kernel(const WinArgs A) {
     auto slot = [&](int c) { return (size_t)(2 * (b0 + c) + (c == 0)); };
     const float *ml = A.part_ml + row;
     float mx = -INFINITY;
-    for (int c = lane; c < parts; c += 64) mx = fmaxf(mx, ml[slot(c) * 3 * kRows]);
+    for (int c = lane; c < parts; c += 64) mx = fmaxf(mx, ml[slot(c) * 3 * rows]);
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor(mx, off));
-    const float kq = ml[slot(0) * 3 * kRows + 2 * kRows];
+    const float kq = ml[slot(0) * 3 * rows + 2 * rows];
     float den = 0.0f;
     for (int c = lane; c < parts; c += 64) {
-        const float *x = ml + slot(c) * 3 * kRows;
+        const float *x = ml + slot(c) * 3 * rows;
         const float f = x[0] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((x[0] - mx) * kq);
-        den += x[kRows] * f;
+        den += x[rows] * f;
         f_s[w][c] = f;
     }
 #pragma unroll
@@ -852,7 +858,7 @@ __global__ __launch_bounds__(256) void window_merge_kernel(const WinArgs A) {
         for (int u = 0; u < 8; ++u)
 #pragma unroll
             for (int h = 0; h < 2; ++h)
-                v[u][h] = *reinterpret_cast<const float4_t *>(src + slot(min(c0 + kStep * u, parts - 1)) * kRows * kD + 4 * h);
+                v[u][h] = *reinterpret_cast<const float4_t *>(src + slot(min(c0 + kStep * u, parts - 1)) * rows * kD + 4 * h);
 #pragma unroll
         for (int u = 0; u < 8; ++u)
             if (c0 + kStep * u < parts) {
@@ -890,13 +896,14 @@ int log2_heads(int n_head) {
 }
 
 // Problems that n_seqs sequences of n_q queries in all can make.
-long long prob_cap(int n_seqs, int n_q, int log_head) {
-    const int lh = std::min(log_head, kLogRows);
-    return ((long long)(n_q >> (kLogRows - lh)) + n_seqs) << (log_head - lh);
+long long prob_cap(int n_seqs, int n_q, int log_head, int log_rows) {
+    const int lh = std::min(log_head, log_rows);
+    return ((long long)(n_q >> (log_rows - lh)) + n_seqs) << (log_head - lh);
 }
 
 // The workspace, laid out from `base` (or only measured).
-size_t lay_out(WinArgs *A, char *base, long long cap) {
+size_t lay_out(WinArgs *A, char *base, long long cap, int log_rows) {
+    const size_t rows = (size_t)1 << log_rows;
     size_t at = 0;
     auto take = [&](size_t bytes) {
         char *p = base + at;
@@ -905,9 +912,10 @@ size_t lay_out(WinArgs *A, char *base, long long cap) {
     };
     char *line = take(2 * sizeof(long long)), *n_prob = take(sizeof(int)), *prob = take(sizeof(int4) * cap),
          *pre = take(sizeof(long long) * (cap + 1)), *wg_tile = take(sizeof(long long) * (kWgs + 1)),
-         *wg_prob = take(sizeof(int) * (kWgs + 1)), *ml = take(sizeof(float) * 2 * kWgs * 3 * kRows),
-         *o = take(sizeof(float) * 2 * kWgs * kRows * kD);
+         *wg_prob = take(sizeof(int) * (kWgs + 1)), *ml = take(sizeof(float) * 2 * kWgs * 3 * rows),
+         *o = take(sizeof(float) * 2 * kWgs * rows * kD);
     if (A) {
+        A->log_rows = log_rows;
         A->prob_cap = (int)cap;
         A->line = reinterpret_cast<long long *>(line);
         A->n_prob = reinterpret_cast<int *>(n_prob);
@@ -921,6 +929,10 @@ size_t lay_out(WinArgs *A, char *base, long long cap) {
     return at;
 }
 
+// Rows of a problem: 64, so that a key tile serves as many as it can; 16 where the
+// sequences have no more on the average, whose outputs then take few registers.
+int rows_log(int n_seqs, int n_q, int log_head) { return ((long long)n_q << log_head) <= 16LL * n_seqs ? 4 : 6; }
+
 bool aligned(const void *p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
 }  // namespace
@@ -928,7 +940,8 @@ bool aligned(const void *p, size_t n) { return (reinterpret_cast<uintptr_t>(p) &
 extern "C" size_t ds4hip_flash_attn_window_fp8_workspace_bytes(int n_seqs, int n_q, int n_head) {
     const int lh = log2_heads(n_head);
     if (lh < 0 || n_seqs <= 0 || n_seqs > kMaxSeqs || n_q <= 0 || n_q > (1 << 24)) return 0;
-    return lay_out(nullptr, nullptr, prob_cap(n_seqs, n_q, lh));
+    const int log_rows = rows_log(n_seqs, n_q, lh);
+    return lay_out(nullptr, nullptr, prob_cap(n_seqs, n_q, lh, log_rows), log_rows);
 }
 
 extern "C" int ds4hip_flash_attn_window_fp8(const ds4hip_window_attn *a, void *workspace, size_t workspace_bytes,
@@ -947,7 +960,8 @@ extern "C" int ds4hip_flash_attn_window_fp8(const ds4hip_window_attn *a, void *w
         !aligned(workspace, 16))
         return ds4hip_set_last_error(kEINVAL);
     WinArgs A = {};
-    if (workspace_bytes < lay_out(&A, static_cast<char *>(workspace), prob_cap(a->n_seqs, a->n_q, lh)))
+    const int log_rows = rows_log(a->n_seqs, a->n_q, lh);
+    if (workspace_bytes < lay_out(&A, static_cast<char *>(workspace), prob_cap(a->n_seqs, a->n_q, lh, log_rows), log_rows))
         return ds4hip_set_last_error(kEINVAL);
     A.q = a->q;
     A.out = a->out;
@@ -969,22 +983,30 @@ extern "C" int ds4hip_flash_attn_window_fp8(const ds4hip_window_attn *a, void *w
     A.shift = shift;
     A.n_pages = (int)(a->n_cache_rows >> shift);
     const hipStream_t st = (hipStream_t)stream;
+    // (one query each: exactly as many problems)
+    if (!a->q_start) A.prob_cap = a->n_seqs << (lh - std::min(lh, log_rows));
     const bool f32 = a->io_f32, in = A.prob_cap <= kInlineProbs;
     if (!in) hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(1024), 0, st, A);
-    auto *main = f32 ? in ? window_kernel<true, true> : window_kernel<true, false>
-                     : in ? window_kernel<false, true> : window_kernel<false, false>;
-    hipLaunchKernelGGL(main, dim3(kWgs), dim3(f32 ? 256 : 512), 0, st, A);
+    if (log_rows == 4) {
+        auto *main = f32 ? in ? window_kernel<true, 1, true> : window_kernel<true, 1, false>
+                         : in ? window_kernel<false, 1, true> : window_kernel<false, 1, false>;
+        hipLaunchKernelGGL(main, dim3(kWgs), dim3(64 * waves_of(f32, 1)), 0, st, A);
+    } else {
+        auto *main = f32 ? in ? window_kernel<true, 4, true> : window_kernel<true, 4, false>
+                         : in ? window_kernel<false, 4, true> : window_kernel<false, 4, false>;
+        hipLaunchKernelGGL(main, dim3(kWgs), dim3(64 * waves_of(f32, 4)), 0, st, A);
+    }
     // no problem is cut where none can have that many tiles: of rows that the table can name, or of
     // the window, the queries' own span and the first rows, with their ends inside tiles
     const long long held = (long long)a->table_stride << shift;
-    const long long span = std::min<long long>(held, (long long)a->window + (kRows >> std::min(lh, kLogRows)));
+    const long long span = std::min<long long>(held, (long long)a->window + ((1 << log_rows) >> std::min(lh, log_rows)));
     const long long most = a->window > 0 ? span / kTile + 2 + (std::min<long long>(a->n_first, held) + kTile - 1) / kTile : held / kTile + 1;
     if (most > kWhole) {
         const int n = in ? A.prob_cap : kWgs - 1;
-        auto *merge = n > 64 ? f32 ? in ? window_merge_kernel<true, true, 4> : window_merge_kernel<true, false, 4>
+        auto *merge = n > 16 ? f32 ? in ? window_merge_kernel<true, true, 4> : window_merge_kernel<true, false, 4>
                                    : in ? window_merge_kernel<false, true, 4> : window_merge_kernel<false, false, 4>
                              : f32 ? window_merge_kernel<true, true, 1> : window_merge_kernel<false, true, 1>;
-        hipLaunchKernelGGL(merge, dim3(n * (n > 64 ? kRows / 4 : kRows)), dim3(256), 0, st, A);
+        hipLaunchKernelGGL(merge, dim3(n << (n > 16 ? log_rows - 2 : log_rows)), dim3(256), 0, st, A);
     }
     return ds4hip_set_last_error(hip_status(hipGetLastError()));
 }
