@@ -24,12 +24,12 @@ using namespace ds4hip;
 
 namespace {
 
-constexpr int kWgs = 256;            // workgroups the line of tiles is cut for: one per CU
+constexpr int kMaxWgs = 512;         // workgroups the line of tiles is cut for: one or two per CU
 constexpr int kMinTiles = 4;         // tiles of a part
 constexpr int kWhole = 8;            // tiles of a problem that is never cut
 constexpr int kPart = 12;            // tiles whose time a cut costs: its parts' 256 KB and their merge
 constexpr int kMaxSeqs = 4096;
-constexpr int kInlineProbs = 512;    // problems that a workgroup lays out itself
+constexpr int kFewProbs = 512, kFewProbs16 = 128;   // problems of 64, 16 rows that a workgroup lays out itself
 // P = 2^((s - m) kq + top) with s and the row's reference m as the matrix
 // instructions leave them and kq its scale to log2: their difference is exact where P is
 // large, at any magnitude. The reference moves only where P would pass 2^15 (f16 ends at
@@ -51,16 +51,17 @@ struct WinArgs {
     const int32_t *table, *rows, *q_start, *seq_ids;
     int n_seqs, n_slots, n_q, log_head, window, first, stride, shift, n_pages;
     int log_rows;            // a problem has 2^log_rows rows (queries x heads)
+    int n_wg;                // workgroups that the line is cut for
     // workspace
     int prob_cap;
     long long *line;         // [2] tiles per workgroup, tiles of a problem that stays whole
     int *n_prob;
     int4 *prob;              // [prob_cap] records
     long long *pre;          // [prob_cap + 1] tiles before each problem
-    long long *wg_tile;      // [kWgs + 1] first tile of each workgroup
-    int *wg_prob;            // [kWgs + 1] the problem it lies in
-    float *part_ml;          // [2 kWgs][3][rows] references, sums and scales to log2
-    float *part_o;           // [2 kWgs][rows][kD] unnormalized outputs
+    long long *wg_tile;      // [n_wg + 1] first tile of each workgroup
+    int *wg_prob;            // [n_wg + 1] the problem it lies in
+    float *part_ml;          // [2 n_wg][3][rows] references, sums and scales to log2
+    float *part_o;           // [2 n_wg][rows][kD] unnormalized outputs
 };
 
 // The queries of sequence s: their first packed index and their number, whatever
@@ -214,13 +215,13 @@ struct Cuts {
     int whole;   // tiles of a problem that stays whole; < 0: workgroup b has problem b
 };
 
-__device__ inline Cuts cuts_of(long long tiles, int n_prob, int longest) {
+__device__ inline Cuts cuts_of(long long tiles, int n_wg, int n_prob, int longest) {
     Cuts C;
     C.tiles = tiles;
     // at least sqrt(longest / 16) tiles: a long problem's merge takes 0.09 us a part, a tile 1.5
-    C.per = max((tiles + kWgs - 1) / kWgs, (long long)max(kMinTiles, (int)sqrtf((float)longest * 0.0625f)));
+    C.per = max((tiles + n_wg - 1) / n_wg, (long long)max(kMinTiles, (int)sqrtf((float)longest * 0.0625f)));
     C.whole = (int)min(max((long long)kWhole, C.per / 8), 1LL << 30);
-    if (n_prob <= kWgs && longest <= C.per + kPart) {
+    if (n_prob <= n_wg && longest <= C.per + kPart) {
         C.whole = -1;
         C.per = tiles + 1;   // (no cut inside the line)
     }
@@ -267,17 +268,88 @@ __global__ __launch_bounds__(1024) void plan_kernel(const WinArgs A) {
         A.prob[i] = rec;
         A.pre[i] = before;
     });
-    const Cuts C = cuts_of(tiles, n_prob, longest);
+    const Cuts C = cuts_of(tiles, A.n_wg, n_prob, longest);
     if (threadIdx.x == 0) {
         A.pre[n_prob] = tiles;
         leave(A, C, n_prob);
     }
     __syncthreads();
     const int b = threadIdx.x;
-    if (b > kWgs) return;
+    if (b > A.n_wg) return;
     int prob;
     A.wg_tile[b] = begin_of(C, b, n_prob, [&](int i) { return A.pre[i]; }, &prob);
     A.wg_prob[b] = prob;
+}
+
+// The workgroup's own copy of a line of at most kFew problems (0: none).
+template <int kFew>
+struct Line {
+    int4 prob[kFew ? kFew : 1];
+    long long pre[kFew + 1], sums[8];
+    int first[kFew ? kFew : 1], longest;
+};
+
+// Where a workgroup stands: its first problem, and the tiles [t, end) of the line.
+struct Place {
+    int n_prob, prob;
+    long long t, end;
+};
+
+// Few problems: every workgroup lays out the line itself (a launch and a wait less), and
+// the first one leaves it to the merge; else the plan kernel did.
+template <int kFew, int kThreads>
+__device__ inline Place take_place(const WinArgs &A, Line<kFew> &L) {
+    const int tid = threadIdx.x, wg = blockIdx.x;
+    Place at;
+    if constexpr (kFew != 0) {
+        if (tid == 0) L.longest = 0;
+        long long tiles;
+        at.n_prob = lay_line<kThreads>(A, L.first, L.sums, &L.longest, &tiles, [&](int i, int4 rec, long long before) {
+            L.prob[i] = rec;
+            L.pre[i] = before;
+        });
+        if (tid == 0) L.pre[at.n_prob] = tiles;
+        __syncthreads();
+        const Cuts C = cuts_of(tiles, A.n_wg, at.n_prob, L.longest);
+        if (wg == 0) {
+            for (int i = tid; i <= at.n_prob; i += kThreads) {
+                if (i < at.n_prob) A.prob[i] = L.prob[i];
+                A.pre[i] = L.pre[i];
+            }
+            if (tid == 0) leave(A, C, at.n_prob);
+        }
+        auto pre = [&](int i) { return L.pre[i]; };
+        at.end = begin_of(C, wg + 1, at.n_prob, pre, &at.prob);
+        at.t = begin_of(C, wg, at.n_prob, pre, &at.prob);
+    } else {
+        at.n_prob = *A.n_prob;
+        at.prob = A.wg_prob[wg];
+        at.t = A.wg_tile[wg];
+        at.end = A.wg_tile[wg + 1];
+    }
+    return at;
+}
+
+// Its next stretch of one problem: tiles [i0, i1) of P; false at the end.
+struct Stretch {
+    Problem P;
+    bool begins, ends;
+    int i0, i1;
+};
+template <int kFew>
+__device__ inline bool next_stretch(const WinArgs &A, const Line<kFew> &L, Place &at, Stretch &S) {
+    if (at.t >= at.end || at.prob >= at.n_prob) return false;
+    const int pi = at.prob++;
+    const long long begin = kFew ? L.pre[kFew ? pi : 0] : A.pre[pi], end = kFew ? L.pre[kFew ? pi + 1 : 0] : A.pre[pi + 1];
+    const int4 rec = kFew ? L.prob[kFew ? pi : 0] : A.prob[pi];
+    S.P = problem_of(A, make_int4(__builtin_amdgcn_readfirstlane(rec.x), __builtin_amdgcn_readfirstlane(rec.y),
+                                  __builtin_amdgcn_readfirstlane(rec.z), __builtin_amdgcn_readfirstlane(rec.w)));
+    S.begins = at.t == begin;
+    S.ends = end <= at.end;
+    S.i0 = __builtin_amdgcn_readfirstlane((int)(at.t - begin));
+    S.i1 = __builtin_amdgcn_readfirstlane((int)(min(end, at.end) - begin));
+    at.t = min(end, at.end);
+    return true;
 }
 
 // ---- attention -------------------------------------------------------------------
@@ -296,6 +368,25 @@ __device__ inline uint32_t umax_16_32(uint32_t v) {
     return max(v, (uint32_t)__shfl_xor((int)v, 32));
 }
 
+// The power of two that brings a row's largest value, of bits `top`, to [2^7, 2^8); none where
+// it is 0 or not finite.
+__device__ inline int power_of(uint32_t top) { return top && top < 0x7F800000u ? 7 - ilogbf(__uint_as_float(top)) : 0; }
+
+// Eight query values from element `at` on.
+template <bool kF32>
+__device__ inline void load_eight(const void *q, size_t at, float *x) {
+    if (kF32) {
+        const float *src = static_cast<const float *>(q) + at;
+        const float4_t a = *reinterpret_cast<const float4_t *>(src), b = *reinterpret_cast<const float4_t *>(src + 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = a[i], x[4 + i] = b[i];
+    } else {
+        const uint4_t v = *reinterpret_cast<const uint4_t *>(static_cast<const uint16_t *>(q) + at);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[2 * i] = __uint_as_float(v[i] << 16), x[2 * i + 1] = __uint_as_float(v[i] & 0xFFFF0000u);
+    }
+}
+
 // One of the workgroup's 16-row query tiles as f16 fragments (hi, and for fp32
 // queries lo): lane (n16, g) holds row n16's dims 32 s + 8 g .. + 8. Each row is
 // scaled by a power of two that brings its largest value to [2^7, 2^8), so that f16
@@ -309,8 +400,6 @@ __device__ inline float load_q(const WinArgs &A, const Problem &P, int row, int 
     const size_t at = (((size_t)(P.q0 + (ok ? qi : 0)) << A.log_head) + head) * kD;
     // first dim of the row's fragment s
     auto dim = [&](int s) { return dim_of(4 * s + g); };
-    // (a row of zeros, or with a value that is not finite, is left as it is)
-    auto power = [](uint32_t amax) { return amax && amax < 0x7F800000u ? 7 - ilogbf(__uint_as_float(amax)) : 0; };
     int e;
     if constexpr (kF32) {
         const float *src = static_cast<const float *>(A.q) + at;
@@ -328,7 +417,7 @@ __device__ inline float load_q(const WinArgs &A, const Problem &P, int row, int 
 #pragma unroll
                 for (int i = 0; i < 4; ++i) amax = max(amax, __float_as_uint(x[s][h][i]) & 0x7FFFFFFFu);
             }
-        e = power(umax_16_32(amax));
+        e = power_of(umax_16_32(amax));
 #pragma unroll
         for (int s = 0; s < 16; ++s)
 #pragma unroll
@@ -349,7 +438,7 @@ __device__ inline float load_q(const WinArgs &A, const Problem &P, int row, int 
 #pragma unroll
             for (int i = 0; i < 4; ++i) amax = max(max(amax, x[s][i] << 16 & 0x7FFF0000u), x[s][i] & 0x7FFF0000u);
         }
-        e = power(umax_16_32(amax));
+        e = power_of(umax_16_32(amax));
 #pragma unroll
         for (int s = 0; s < 16; ++s)
 #pragma unroll
@@ -432,23 +521,21 @@ __device__ inline void store_part(uint8_t *stage, int tid, const Part &R) {
     *reinterpret_cast<uint2_t *>(rp + 512 + 16 * (12 + (u & 3)) + 256 * (u >> 2) + 8 * (j & 1)) = R.t;
 }
 
-constexpr int waves_of(bool f32, int row_tiles) { return f32 && row_tiles == 4 ? 4 : 8; }
-
 // Iteration i, with one barrier: scores of tile i | tile i + 1 dequantized, a later one
 // fetched | P of tile i | O += P V of tile i - 1. P is computed against the references of the
 // tile before. Where a row outgrows its reference, P's tile is marked, and before it is
 // used all waves agree on new references, rescale and compute it again from its scores:
 // always on the first tile, seldom after it.
-template <bool kF32, int kRT, bool kInline>
-__global__ __launch_bounds__(waves_of(kF32, kRT) * 64, waves_of(kF32, kRT) / 4) void window_kernel(const WinArgs A) {
-    constexpr int kRows = 16 * kRT;      // rows of a problem
-    constexpr int kW = waves_of(kF32, kRT);
+template <bool kF32, bool kInline>
+__global__ __launch_bounds__(kF32 ? 256 : 512, kF32 ? 1 : 2) void window_kernel(const WinArgs A) {
+    constexpr int kRT = 4, kRows = 16 * kRT;   // row tiles and rows of a problem
+    constexpr int kW = kF32 ? 4 : 8;     // waves
     constexpr int kN = 8 / kW;           // key halves of a wave, and thread rows of a tile
     constexpr int kDT = 4 * kN;          // dim tiles of a wave
     constexpr int kDB = 1024 / kW;       // its bytes of an f16 row
     __shared__ __attribute__((aligned(16))) uint8_t stages[3][kStageB];
     __shared__ __attribute__((aligned(16))) half4_t pb[2][kF32 ? 2 : 1][kRT][64][2];   // [buffer][hi, lo][row tile][lane][key half]
-    __shared__ float top_s[2][64], l_s[2][64], m_s[64], kq_s[64];
+    __shared__ float top_s[2][kRows], l_s[2][kRows], m_s[kRows], kq_s[kRows];
     __shared__ uint32_t odd_s[2][8];   // keys whose scores are not finite, per wave
     __shared__ __attribute__((aligned(16))) int moved_s[2][8];   // whether a row of the wave's outgrew its reference
     __shared__ int bad_s;
@@ -457,40 +544,9 @@ __global__ __launch_bounds__(waves_of(kF32, kRT) * 64, waves_of(kF32, kRT) / 4) 
     const int n16 = lane & 15, g = lane >> 4, row = 16 * (w & 3) + n16;
     const int kh = w >> 2;   // the wave's (first) key half
     const int wg = blockIdx.x;
-    // Few problems: every workgroup lays out the line itself, and the first one leaves it
-    // to the merge; else the plan kernel did.
-    __shared__ __attribute__((aligned(16))) int4 prob_s[kInline ? kInlineProbs : 1];
-    __shared__ long long pre_s[kInline ? kInlineProbs + 1 : 1], sums_s[kInline ? 8 : 1];
-    __shared__ int first_s[kInline ? kInlineProbs : 1];
-    int n_prob, pi;
-    long long t, t_end;
-    if constexpr (kInline) {
-        __shared__ int longest;
-        if (tid == 0) longest = 0;
-        long long tiles;
-        n_prob = lay_line<64 * kW>(A, first_s, sums_s, &longest, &tiles, [&](int i, int4 rec, long long before) {
-            prob_s[i] = rec;
-            pre_s[i] = before;
-        });
-        if (tid == 0) pre_s[n_prob] = tiles;
-        __syncthreads();
-        const Cuts C = cuts_of(tiles, n_prob, longest);
-        if (wg == 0) {
-            for (int i = tid; i <= n_prob; i += 64 * kW) {
-                if (i < n_prob) A.prob[i] = prob_s[i];
-                A.pre[i] = pre_s[i];
-            }
-            if (tid == 0) leave(A, C, n_prob);
-        }
-        auto pre = [&](int i) { return pre_s[i]; };
-        t_end = begin_of(C, wg + 1, n_prob, pre, &pi);
-        t = begin_of(C, wg, n_prob, pre, &pi);
-    } else {
-        n_prob = *A.n_prob;
-        pi = A.wg_prob[wg];
-        t = A.wg_tile[wg];
-        t_end = A.wg_tile[wg + 1];
-    }
+    constexpr int kFew = kInline ? kFewProbs : 0;
+    __shared__ Line<kFew> line;
+    Place at = take_place<kFew, 64 * kW>(A, line);
     const int lh = log_hpt(A);
     uint32_t ka[kN], va[2];
     {
@@ -506,14 +562,11 @@ __global__ __launch_bounds__(waves_of(kF32, kRT) * 64, waves_of(kF32, kRT) / 4) 
         }
     }
 
-    for (; t < t_end && pi < n_prob; ++pi) {
-        const long long p_begin = kInline ? pre_s[kInline ? pi : 0] : A.pre[pi], p_end = kInline ? pre_s[kInline ? pi + 1 : 0] : A.pre[pi + 1];
-        const int4 rec = kInline ? prob_s[kInline ? pi : 0] : A.prob[pi];
-        const Problem P = problem_of(A, make_int4(__builtin_amdgcn_readfirstlane(rec.x), __builtin_amdgcn_readfirstlane(rec.y),
-                                                  __builtin_amdgcn_readfirstlane(rec.z), __builtin_amdgcn_readfirstlane(rec.w)));
-        const bool begins = t == p_begin, ends = p_end <= t_end;
-        const int i0 = __builtin_amdgcn_readfirstlane((int)(t - p_begin)), i1 = __builtin_amdgcn_readfirstlane((int)(min(p_end, t_end) - p_begin));
-        t = min(p_end, t_end);
+    Stretch S;
+    while (next_stretch(A, line, at, S)) {
+        const Problem P = S.P;
+        const bool begins = S.begins, ends = S.ends;
+        const int i0 = S.i0, i1 = S.i1;
         bool bad = P.slot < 0;
         float4_t o[kRT][kDT];
 #pragma unroll
@@ -585,8 +638,8 @@ __global__ __launch_bounds__(waves_of(kF32, kRT) * 64, waves_of(kF32, kRT) / 4) 
                         sum = __builtin_amdgcn_fdot2(half2_t{ph[0], ph[1]}, one, sum, false);
                         sum = __builtin_amdgcn_fdot2(half2_t{ph[2], ph[3]}, one, sum, false);
                     }
-                    pb[b][0][w & (kRT - 1)][lane][kh + u] = ph;
-                    if (kF32) pb[b][kF32 ? 1 : 0][w & (kRT - 1)][lane][kh + u] = pl;
+                    pb[b][0][w & 3][lane][kh + u] = ph;
+                    if (kF32) pb[b][kF32 ? 1 : 0][w & 3][lane][kh + u] = pl;
                 }
             };
             auto top_of = [&]() {
@@ -772,11 +825,11 @@ __global__ __launch_bounds__(waves_of(kF32, kRT) * 64, waves_of(kF32, kRT) / 4) 
                 const float mm = m_s[rr];
                 const float sum = kW == 8 ? l_s[0][rr] + l_s[1][rr] : l_s[0][rr];
                 const float inv = mm == -INFINITY ? nan : 1.0f / (sum + sink_term<kF32>(A, head, mm, kq_s[rr])) + nan;
-                const size_t at = (((size_t)(P.q0 + qi) << A.log_head) + head) * kD;
+                const size_t to = (((size_t)(P.q0 + qi) << A.log_head) + head) * kD;
 #pragma unroll
                 for (int dt = 0; dt < kDT; ++dt) {
                     if (kF32)
-                        store_out<true>(A.out, at + out_dim(dt), o[rt][dt] * inv);
+                        store_out<true>(A.out, to + out_dim(dt), o[rt][dt] * inv);
                     else
                         store_out<false>(stages[0], (rr * kOutB) / 2 + out_dim(dt), o[rt][dt] * inv);
                 }
@@ -784,8 +837,8 @@ __global__ __launch_bounds__(waves_of(kF32, kRT) * 64, waves_of(kF32, kRT) / 4) 
             if (!kF32) {   // whole rows of 1 KB (eight bytes a lane from the accumulators: 2 us more)
                 lds_barrier();
                 for (int rr = w; rr < P.n << lh; rr += kW) {
-                    const size_t at = (((size_t)(P.q0 + (rr >> lh)) << A.log_head) + P.head0 + (rr & ((1 << lh) - 1))) * kD + 8 * lane_e;
-                    *reinterpret_cast<uint4_t *>(static_cast<uint16_t *>(A.out) + at) =
+                    const size_t to = (((size_t)(P.q0 + (rr >> lh)) << A.log_head) + P.head0 + (rr & ((1 << lh) - 1))) * kD + 8 * lane_e;
+                    *reinterpret_cast<uint4_t *>(static_cast<uint16_t *>(A.out) + to) =
                         *reinterpret_cast<const uint4_t *>(stages[0] + rr * kOutB + 16 * lane_e);
                 }
             }
@@ -809,6 +862,246 @@ __global__ __launch_bounds__(waves_of(kF32, kRT) * 64, waves_of(kF32, kRT) / 4) 
     }
 }
 
+// ---- 16 rows -----------------------------------------------------------------------
+//
+// Single tokens of a slice of the heads: too few rows to share a key tile's scores out by
+// rows (one wave of four would have them all: 3.5 us a tile of fp32). Wave w has dims 128 w .. + 128 of the
+// scores' sums and of the outputs; the four partial sums meet in LDS, and then every wave has all
+// weights in registers, as its matrix instructions take them, with references and sums of
+// its own that agree bit for bit. Two workgroups a CU.
+template <bool kF32, bool kInline>
+__global__ __launch_bounds__(256, 2) void few_rows_kernel(const WinArgs A) {
+    constexpr int kRT = 1, kRows = 16 * kRT;
+    constexpr int kFew = kInline ? kFewProbs16 : 0;
+    __shared__ __attribute__((aligned(16))) uint8_t stages[2][kStageB];
+    __shared__ __attribute__((aligned(16))) float4_t sum_s[4][kRT][2][64];   // [wave][row tile][key half][lane]
+    __shared__ uint32_t top_s[4][kRows];   // bits of the largest query value
+    __shared__ int bad_s;
+    __shared__ Line<kFew> line;
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    const int n16 = lane & 15, g = lane >> 4;
+    Place at = take_place<kFew, 256>(A, line);
+    const int lh = log_hpt(A);
+    uint32_t ka[2], va[2];
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+        ka[kt] = pi_key(16 * kt + n16) * kRowB + 256 * w + 16 * g;
+        va[kt] = lds_addr(stages[0]) + pi_key(16 * kt + 4 * g + (n16 >> 2)) * kRowB + 256 * w + 8 * (n16 & 3);
+    }
+    Stretch S;
+    while (next_stretch(A, line, at, S)) {
+        const Problem P = S.P;
+        const int i0 = S.i0, i1 = S.i1;
+        bool bad = P.slot < 0;
+        float4_t o[kRT][8];
+#pragma unroll
+        for (int a = 0; a < kRT; ++a)
+#pragma unroll
+            for (int b = 0; b < 8; ++b) o[a][b] = float4_t{0, 0, 0, 0};
+        float m[kRT], l[kRT], kq[kRT];
+#pragma unroll
+        for (int rt = 0; rt < kRT; ++rt) m[rt] = -INFINITY, l[rt] = kq[rt] = 0.0f;
+        if (tid == 0) bad_s = 0;
+        if (P.pos1 >= 0) {   // else its one tile sees nothing
+            // the thread's u-th row of tile i (past the last row seen: that row again, masked), and its page
+            auto row_of = [&](int i, int u) { return min(kTile * tile_at(P, min(i, i1 - 1)) + (tid >> 4) + 16 * u, P.pos1); };
+            auto page_of = [&](int i, int u) { return A.table[(long long)P.slot * A.stride + (row_of(i, u) >> A.shift)]; };
+            Part R[2];
+            int page[2] = {page_of(i0, 0), page_of(i0, 1)};
+            // fetches tile i (the next one's pages first: waiting for a page must not wait for the
+            // rows). An entry outside the pool reads row 0
+            auto fetch = [&](int i) {
+                const int next[2] = {page_of(i + 1, 0), page_of(i + 1, 1)};
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    if (page[u] < 0 || page[u] >= A.n_pages) {
+                        bad = true;
+                        page[u] = 0;
+                    }
+                    load_part(A, ((long long)page[u] << A.shift) + (row_of(i, u) & ((1 << A.shift) - 1)), tid & 15, R[u]);
+                    page[u] = next[u];
+                }
+            };
+            auto store = [&](int stage) {
+#pragma unroll
+                for (int u = 0; u < 2; ++u) store_part(stages[stage] + 16 * u * kRowB, tid, R[u]);
+            };
+            fetch(i0);
+            // the wave's quarter of the rows' dims, and its power of two from all quarters' largest values
+            float x[kRT][4][8];
+            int pos[kRT];
+#pragma unroll
+            for (int rt = 0; rt < kRT; ++rt) {
+                const int row = 16 * rt + n16, qi = min(row >> lh, P.n - 1);   // (rows past the queries repeat the last one's)
+                pos[rt] = P.pos0 + qi;
+                const size_t from = (((size_t)(P.q0 + qi) << A.log_head) + P.head0 + (row & ((1 << lh) - 1))) * kD;
+                uint32_t top = 0;
+#pragma unroll
+                for (int s = 0; s < 4; ++s) {
+                    load_eight<kF32>(A.q, from + dim_of(4 * (4 * w + s) + g), x[rt][s]);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) top = max(top, __float_as_uint(x[rt][s][k]) & 0x7FFFFFFFu);
+                }
+                top = umax_16_32(top);
+                if (g == 0) top_s[w][row] = top;
+            }
+            store(0);
+            fetch(i0 + 1);
+            lds_barrier();
+            half8_t qh[kRT][4], ql[kRT][kF32 ? 4 : 1];
+#pragma unroll
+            for (int rt = 0; rt < kRT; ++rt) {
+                const int row = 16 * rt + n16;
+                const int e = power_of(max(max(top_s[0][row], top_s[1][row]), max(top_s[2][row], top_s[3][row])));
+                kq[rt] = ldexpf(kLog2e / 22.62741699796952f, -e);   // 1 / sqrt(512)
+#pragma unroll
+                for (int s = 0; s < 4; ++s)
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const float v = ldexpf(x[rt][s][k], e);
+                        qh[rt][s][k] = (half_t)v;
+                        if (kF32) ql[rt][kF32 ? s : 0][k] = (half_t)(v - (float)qh[rt][s][k]);
+                    }
+            }
+            for (int i = i0; i < i1; ++i) {
+                const int cur = (i - i0) & 1;
+                if (i > i0) lds_barrier();   // the tile is whole, the last one's V and sums are read
+                float4_t acc[kRT][2];
+                {
+                    const uint8_t *st = stages[cur];
+#pragma unroll
+                    for (int rt = 0; rt < kRT; ++rt) acc[rt][0] = acc[rt][1] = float4_t{0, 0, 0, 0};
+#pragma unroll
+                    for (int s = 0; s < 4; ++s)
+#pragma unroll
+                        for (int kt = 0; kt < 2; ++kt) {
+                            const half8_t k = *reinterpret_cast<const half8_t *>(st + ka[kt] + 64 * s);
+#pragma unroll
+                            for (int rt = 0; rt < kRT; ++rt) {
+                                acc[rt][kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qh[rt][s], acc[rt][kt], 0, 0, 0);
+                                if (kF32) acc[rt][kt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, ql[rt][kF32 ? s : 0], acc[rt][kt], 0, 0, 0);
+                            }
+                        }
+                }
+#pragma unroll
+                for (int rt = 0; rt < kRT; ++rt)
+#pragma unroll
+                    for (int kt = 0; kt < 2; ++kt) sum_s[w][rt][kt][lane] = acc[rt][kt];
+                if (i + 1 < i1) store(cur ^ 1);
+                fetch(i + 2);
+                lds_barrier();
+#pragma unroll
+                for (int rt = 0; rt < kRT; ++rt)
+#pragma unroll
+                    for (int kt = 0; kt < 2; ++kt)
+                        acc[rt][kt] = (sum_s[0][rt][kt][lane] + sum_s[1][rt][kt][lane]) + (sum_s[2][rt][kt][lane] + sum_s[3][rt][kt][lane]);
+                const int tile = tile_at(P, i), key0 = kTile * tile;
+                if (!(tile < P.whole_c && (tile >= P.whole_b || tile < P.whole_a))) {
+                    uint32_t odd = 0;   // keys whose scores are not finite in any row
+                    const int g_r = again(lane) >> 4;
+#pragma unroll
+                    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const int k = pi_key(16 * kt + 4 * g_r + r);
+                            bool all = true;
+#pragma unroll
+                            for (int rt = 0; rt < kRT; ++rt) {
+                                const bool fine = fabsf(acc[rt][kt][r]) < INFINITY;
+                                all = all && !fine;
+                                acc[rt][kt][r] = !sees(A, pos[rt], key0 + k) ? -INFINITY : fine ? acc[rt][kt][r] : __builtin_nanf("");
+                            }
+                            if (((__ballot(all) >> (16 * g_r)) & 0xFFFF) == 0xFFFF) odd |= 1u << k;
+                        }
+                    odd |= __shfl_xor(odd, 16);
+                    odd |= __shfl_xor(odd, 32);
+                    odd = __builtin_amdgcn_readfirstlane(odd);
+                    // such a row is zeroed in this wave's own dims (0 x inf would reach queries that must not
+                    // see it). Queries that see it have a P that is not finite.
+                    for (; odd; odd &= odd - 1)
+                        *reinterpret_cast<uint32_t *>(stages[cur] + __builtin_ctz(odd) * kRowB + 256 * w + 4 * lane) = 0;
+                    asm volatile("" ::: "memory");   // before the reads below, which are asm
+                }
+                half8_t ph[kRT], pl[kRT];
+#pragma unroll
+                for (int rt = 0; rt < kRT; ++rt) {
+                    float top = -INFINITY;
+#pragma unroll
+                    for (int kt = 0; kt < 2; ++kt)
+                        top = fmaxf(top, fmaxf(fmaxf(acc[rt][kt][0], acc[rt][kt][1]), fmaxf(acc[rt][kt][2], acc[rt][kt][3])));
+                    top = xmax_16_32(top);
+                    const bool moves = (top - m[rt]) * kq[rt] > kLazy<kF32>;   // (m is -inf before the first key seen)
+                    if (__any(moves)) {
+                        const float f = !moves ? 1.0f : m[rt] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m[rt] - top) * kq[rt]);
+                        if (moves) m[rt] = top;
+                        l[rt] *= f;
+#pragma unroll
+                        for (int dt = 0; dt < 8; ++dt) o[rt][dt] *= f;
+                    }
+                    const float ref = m[rt] == -INFINITY ? 0.0f : m[rt];
+#pragma unroll
+                    for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const float p = __builtin_amdgcn_exp2f(fmaf(acc[rt][kt][r] - ref, kq[rt], kTop<kF32>));
+                            const half_t h = (half_t)p;
+                            ph[rt][4 * kt + r] = h;
+                            if (kF32) pl[rt][4 * kt + r] = (half_t)(p - (float)h);
+                            l[rt] += kF32 ? p : (float)h;   // (of the rounded values: the output stays an average)
+                        }
+                }
+                const uint32_t v0 = va[0] + cur * kStageB, v1 = va[1] + cur * kStageB;
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    half8_t vb[4];
+                    if (half == 0)
+                        read_vt4<0>(v0, v1, vb);
+                    else
+                        read_vt4<4>(v0, v1, vb);
+#pragma unroll
+                    for (int rt = 0; rt < kRT; ++rt)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            float4_t &c = o[rt][4 * half + k];
+                            c = __builtin_amdgcn_mfma_f32_16x16x32_f16(vb[k], ph[rt], c, 0, 0, 0);
+                            if (kF32) c = __builtin_amdgcn_mfma_f32_16x16x32_f16(vb[k], pl[rt], c, 0, 0, 0);
+                        }
+                }
+            }
+#pragma unroll
+            for (int rt = 0; rt < kRT; ++rt) l[rt] = xsum_16_32(l[rt]);
+        }
+        if (__any(bad) && lane == 0) bad_s = 1;
+        lds_barrier();
+        const float nan = bad_s ? __builtin_nanf("") : 0.0f;
+        const int slot = 2 * blockIdx.x + (S.begins ? 1 : 0);
+#pragma unroll
+        for (int rt = 0; rt < kRT; ++rt) {
+            const int row = 16 * rt + n16, qi = row >> lh, head = P.head0 + (row & ((1 << lh) - 1));
+            if (qi >= P.n) continue;
+            if (S.begins && S.ends) {
+                const float inv = m[rt] == -INFINITY ? nan : 1.0f / (l[rt] + sink_term<kF32>(A, head, m[rt], kq[rt])) + nan;
+                const size_t to = (((size_t)(P.q0 + qi) << A.log_head) + head) * kD;
+#pragma unroll
+                for (int dt = 0; dt < 8; ++dt)
+                    store_out<kF32>(A.out, to + dim_of(16 * w + 2 * dt + (g >> 1)) + 4 * (g & 1), o[rt][dt] * inv);
+            } else {
+                if (w == 0 && g == 0) {
+                    float *ml = A.part_ml + (size_t)slot * 3 * kRows + row;
+                    ml[0] = m[rt];
+                    ml[kRows] = l[rt] + nan;
+                    ml[2 * kRows] = kq[rt];
+                }
+                float *to = A.part_o + ((size_t)slot * kRows + row) * kD;
+#pragma unroll
+                for (int dt = 0; dt < 8; ++dt)
+                    *reinterpret_cast<float4_t *>(to + dim_of(16 * w + 2 * dt + (g >> 1)) + 4 * (g & 1)) = o[rt][dt];
+            }
+        }
+        lds_barrier();   // bad_s and the stages are free again
+    }
+}
+
 // The parts of a problem that cuts fall into, in order, and the sink. A workgroup has
 // kShare rows: one, whose parts its four waves share (parts w, w + 4, .., then their sums in
 // order), or four, a wave each; a lane has eight dims, eight parts in flight.
@@ -817,7 +1110,7 @@ template <bool kF32, bool kInline, int kShare>
 __global__ __launch_bounds__(256) void window_merge_kernel(const WinArgs A) {
     constexpr int kStep = kShare == 1 ? 4 : 1;
     const int rows = 1 << A.log_rows, wgs = rows / kShare;   // workgroups of a problem
-    __shared__ float f_s[4][kWgs];   // each wave's parts' factors
+    __shared__ float f_s[4][kMaxWgs];   // each wave's parts' factors
     __shared__ float4_t o_s[3][64][2];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, n_prob = *A.n_prob;
     const int row = kShare == 1 ? blockIdx.x % wgs : 4 * (blockIdx.x % wgs) + w;
@@ -904,6 +1197,7 @@ long long prob_cap(int n_seqs, int n_q, int log_head, int log_rows) {
 // The workspace, laid out from `base` (or only measured).
 size_t lay_out(WinArgs *A, char *base, long long cap, int log_rows) {
     const size_t rows = (size_t)1 << log_rows;
+    const int n_wg = log_rows == 6 ? 256 : 512;
     size_t at = 0;
     auto take = [&](size_t bytes) {
         char *p = base + at;
@@ -911,11 +1205,12 @@ size_t lay_out(WinArgs *A, char *base, long long cap, int log_rows) {
         return p;
     };
     char *line = take(2 * sizeof(long long)), *n_prob = take(sizeof(int)), *prob = take(sizeof(int4) * cap),
-         *pre = take(sizeof(long long) * (cap + 1)), *wg_tile = take(sizeof(long long) * (kWgs + 1)),
-         *wg_prob = take(sizeof(int) * (kWgs + 1)), *ml = take(sizeof(float) * 2 * kWgs * 3 * rows),
-         *o = take(sizeof(float) * 2 * kWgs * rows * kD);
+         *pre = take(sizeof(long long) * (cap + 1)), *wg_tile = take(sizeof(long long) * (n_wg + 1)),
+         *wg_prob = take(sizeof(int) * (n_wg + 1)), *ml = take(sizeof(float) * 2 * n_wg * 3 * rows),
+         *o = take(sizeof(float) * 2 * n_wg * rows * kD);
     if (A) {
         A->log_rows = log_rows;
+        A->n_wg = n_wg;
         A->prob_cap = (int)cap;
         A->line = reinterpret_cast<long long *>(line);
         A->n_prob = reinterpret_cast<int *>(n_prob);
@@ -929,9 +1224,12 @@ size_t lay_out(WinArgs *A, char *base, long long cap, int log_rows) {
     return at;
 }
 
-// Rows of a problem: 64, so that a key tile serves as many as it can; 16 where the
-// sequences have no more on the average, whose outputs then take few registers.
-int rows_log(int n_seqs, int n_q, int log_head) { return ((long long)n_q << log_head) <= 16LL * n_seqs ? 4 : 6; }
+// Rows of a problem: 64, so that a key tile serves as many as it can; 16 where the sequences
+// have no more on the average.
+int rows_log(int n_seqs, int n_q, int log_head) {
+    const long long rows = (long long)n_q << log_head;
+    return rows <= 16LL * n_seqs ? 4 : 6;
+}
 
 bool aligned(const void *p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
@@ -985,24 +1283,20 @@ extern "C" int ds4hip_flash_attn_window_fp8(const ds4hip_window_attn *a, void *w
     const hipStream_t st = (hipStream_t)stream;
     // (one query each: exactly as many problems)
     if (!a->q_start) A.prob_cap = a->n_seqs << (lh - std::min(lh, log_rows));
-    const bool f32 = a->io_f32, in = A.prob_cap <= kInlineProbs;
+    const bool f32 = a->io_f32, in = A.prob_cap <= (log_rows == 4 ? kFewProbs16 : kFewProbs);
     if (!in) hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(1024), 0, st, A);
-    if (log_rows == 4) {
-        auto *main = f32 ? in ? window_kernel<true, 1, true> : window_kernel<true, 1, false>
-                         : in ? window_kernel<false, 1, true> : window_kernel<false, 1, false>;
-        hipLaunchKernelGGL(main, dim3(kWgs), dim3(64 * waves_of(f32, 1)), 0, st, A);
-    } else {
-        auto *main = f32 ? in ? window_kernel<true, 4, true> : window_kernel<true, 4, false>
-                         : in ? window_kernel<false, 4, true> : window_kernel<false, 4, false>;
-        hipLaunchKernelGGL(main, dim3(kWgs), dim3(64 * waves_of(f32, 4)), 0, st, A);
-    }
+    auto *main = log_rows == 4 ? f32 ? in ? few_rows_kernel<true, true> : few_rows_kernel<true, false>
+                                     : in ? few_rows_kernel<false, true> : few_rows_kernel<false, false>
+                                 : f32 ? in ? window_kernel<true, true> : window_kernel<true, false>
+                                       : in ? window_kernel<false, true> : window_kernel<false, false>;
+    hipLaunchKernelGGL(main, dim3(A.n_wg), dim3(log_rows < 6 || f32 ? 256 : 512), 0, st, A);
     // no problem is cut where none can have that many tiles: of rows that the table can name, or of
     // the window, the queries' own span and the first rows, with their ends inside tiles
     const long long held = (long long)a->table_stride << shift;
     const long long span = std::min<long long>(held, (long long)a->window + ((1 << log_rows) >> std::min(lh, log_rows)));
     const long long most = a->window > 0 ? span / kTile + 2 + (std::min<long long>(a->n_first, held) + kTile - 1) / kTile : held / kTile + 1;
     if (most > kWhole) {
-        const int n = in ? A.prob_cap : kWgs - 1;
+        const int n = in ? A.prob_cap : A.n_wg - 1;
         auto *merge = n > 16 ? f32 ? in ? window_merge_kernel<true, true, 4> : window_merge_kernel<true, false, 4>
                                    : in ? window_merge_kernel<false, true, 4> : window_merge_kernel<false, false, 4>
                              : f32 ? window_merge_kernel<true, true, 1> : window_merge_kernel<false, true, 1>;
