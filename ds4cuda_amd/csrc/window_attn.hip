@@ -264,20 +264,24 @@ __global__ __launch_bounds__(1024) void plan_kernel(const WinArgs A) {
     long long tiles;
     __shared__ int longest;
     if (threadIdx.x == 0) longest = 0;
+    constexpr int kHeld = 8192;   // (64 KB; the search below took half the kernel's time in memory)
+    __shared__ long long pre_s[kHeld];
     const int n_prob = lay_line<1024>(A, first_s, sums, &longest, &tiles, [&](int i, int4 rec, long long before) {
         A.prob[i] = rec;
         A.pre[i] = before;
+        if (i < kHeld) pre_s[i] = before;
     });
     const Cuts C = cuts_of(tiles, A.n_wg, n_prob, longest);
     if (threadIdx.x == 0) {
         A.pre[n_prob] = tiles;
+        if (n_prob < kHeld) pre_s[n_prob] = tiles;
         leave(A, C, n_prob);
     }
     __syncthreads();
     const int b = threadIdx.x;
     if (b > A.n_wg) return;
     int prob;
-    A.wg_tile[b] = begin_of(C, b, n_prob, [&](int i) { return A.pre[i]; }, &prob);
+    A.wg_tile[b] = begin_of(C, b, n_prob, [&](int i) { return i < kHeld ? pre_s[i] : A.pre[i]; }, &prob);
     A.wg_prob[b] = prob;
 }
 
@@ -338,7 +342,7 @@ struct Stretch {
 };
 template <int kFew>
 __device__ inline bool next_stretch(const WinArgs &A, const Line<kFew> &L, Place &at, Stretch &S) {
-    if (at.t >= at.end || at.prob >= at.n_prob) return false;
+    if (__builtin_amdgcn_readfirstlane(at.t >= at.end || at.prob >= at.n_prob)) return false;
     const int pi = at.prob++;
     const long long begin = kFew ? L.pre[kFew ? pi : 0] : A.pre[pi], end = kFew ? L.pre[kFew ? pi + 1 : 0] : A.pre[pi + 1];
     const int4 rec = kFew ? L.prob[kFew ? pi : 0] : A.prob[pi];
@@ -362,6 +366,14 @@ __device__ inline int dim_of(int p) {
     return i == 0 || j < 12 ? 256 * i + 16 * j + 8 * h : kNope + 8 * (j - 12) + 32 * h;
 }
 
+// v, as a value the compiler does not know: what rare paths derive from it is computed
+// there again, not kept in registers through the loop (where a spilled one's reload would
+// wait for every copy in flight).
+__device__ inline int again(int v) {
+    asm volatile("" : "+v"(v));
+    return v;
+}
+
 // The largest of the lanes 16 and 32 apart.
 __device__ inline uint32_t umax_16_32(uint32_t v) {
     v = max(v, (uint32_t)__shfl_xor((int)v, 16));
@@ -369,8 +381,11 @@ __device__ inline uint32_t umax_16_32(uint32_t v) {
 }
 
 // The power of two that brings a row's largest value, of bits `top`, to [2^7, 2^8); none where
-// it is 0 or not finite.
-__device__ inline int power_of(uint32_t top) { return top && top < 0x7F800000u ? 7 - ilogbf(__uint_as_float(top)) : 0; }
+// it is 0 or not finite. (At most 2^120, itself an fp32 value: scores of rows under 2^-113 are
+// 0 to all that is done with them, |s| < 2^-88.)
+__device__ inline int power_of(uint32_t top) {
+    return top && top < 0x7F800000u ? min(7 - ilogbf(__uint_as_float(top)), 120) : 0;
+}
 
 // Eight query values from element `at` on.
 template <bool kF32>
@@ -387,67 +402,75 @@ __device__ inline void load_eight(const void *q, size_t at, float *x) {
     }
 }
 
-// One of the workgroup's 16-row query tiles as f16 fragments (hi, and for fp32
-// queries lo): lane (n16, g) holds row n16's dims 32 s + 8 g .. + 8. Each row is
+// A lane's part of a 16-row query tile: lane (n16, g) has row n16's granules g, 4 + g, ..
+template <bool kF32>
+struct QRow {
+    uint4_t x[kF32 ? 32 : 16];
+};
+// (rows past the queries repeat the last one's)
+template <bool kF32>
+__device__ inline void load_row(const WinArgs &A, const Problem &P, int row, int g, QRow<kF32> &q) {
+    const int lh = log_hpt(A);
+    const size_t at = (((size_t)(P.q0 + min(row >> lh, P.n - 1)) << A.log_head) + P.head0 + (row & ((1 << lh) - 1))) * kD;
+    const uint8_t *src = static_cast<const uint8_t *>(A.q) + at * (kF32 ? 4 : 2);
+#pragma unroll
+    for (int s = 0; s < 16; ++s) {
+        const uint4_t *from = reinterpret_cast<const uint4_t *>(src + dim_of(4 * s + g) * (kF32 ? 4 : 2));
+        if (kF32) {
+            q.x[kF32 ? 2 * s : 0] = from[0];
+            q.x[kF32 ? 2 * s + 1 : 0] = from[1];
+        } else {
+            q.x[s] = from[0];
+        }
+    }
+    __builtin_amdgcn_sched_barrier(0);   // all in flight before the first is used
+}
+
+// It as f16 fragments (hi, and for fp32 queries lo). Each row is
 // scaled by a power of two that brings its largest value to [2^7, 2^8), so that f16
 // keeps what bf16 and fp32 rows of any magnitude hold: hi + lo are off by 2^-22 of
-// a value, or 2^-32 of the row's largest. Returns the power's inverse.
+// a value, or 2^-32 of the row's largest; hi alone, from bf16, by 2^-31 of the largest (values that become
+// subnormal, rounded toward zero: one instruction for two; the others are exact). Returns the power's inverse.
 template <bool kF32>
-__device__ inline float load_q(const WinArgs &A, const Problem &P, int row, int g, half8_t *hi, half8_t *lo) {
-    const int lh = log_hpt(A);
-    const int qi = row >> lh, head = P.head0 + (row & ((1 << lh) - 1));
-    const bool ok = qi < P.n;
-    const size_t at = (((size_t)(P.q0 + (ok ? qi : 0)) << A.log_head) + head) * kD;
-    // first dim of the row's fragment s
-    auto dim = [&](int s) { return dim_of(4 * s + g); };
-    int e;
+__device__ inline float fragments_of(const QRow<kF32> &q, half8_t *hi, half8_t *lo) {
     if constexpr (kF32) {
-        const float *src = static_cast<const float *>(A.q) + at;
-        float4_t x[16][2];
-        uint32_t amax = 0;   // bits of |x| compare as the values do
+        float top = 0.0f;
 #pragma unroll
-        for (int s = 0; s < 16; ++s)
+        for (int s = 0; s < 32; ++s)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) x[s][h] = *reinterpret_cast<const float4_t *>(src + dim(s) + 4 * h);
-        __builtin_amdgcn_sched_barrier(0);   // all in flight before the first is used
-#pragma unroll
-        for (int s = 0; s < 16; ++s)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) amax = max(amax, __float_as_uint(x[s][h][i]) & 0x7FFFFFFFu);
-            }
-        e = power_of(umax_16_32(amax));
+            for (int i = 0; i < 4; ++i) top = fmaxf(top, fabsf(__uint_as_float(q.x[s][i])));
+        const int e = power_of(umax_16_32(__float_as_uint(top)));
+        const float scale = ldexpf(1.0f, e);
 #pragma unroll
         for (int s = 0; s < 16; ++s)
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float v = ok ? ldexpf(x[s][i >> 2][i & 3], e) : 0.0f;
+                const float v = __uint_as_float(q.x[2 * s + (i >> 2)][i & 3]) * scale;
                 hi[s][i] = (half_t)v;
                 lo[s][i] = (half_t)(v - (float)hi[s][i]);
             }
+        return ldexpf(1.0f, -e);
     } else {
-        const uint16_t *src = static_cast<const uint16_t *>(A.q) + at;
-        uint4_t x[16];
-        uint32_t amax = 0;
-#pragma unroll
-        for (int s = 0; s < 16; ++s) x[s] = *reinterpret_cast<const uint4_t *>(src + dim(s));
-        __builtin_amdgcn_sched_barrier(0);   // all in flight before the first is used
-#pragma unroll
-        for (int s = 0; s < 16; ++s) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) amax = max(max(amax, x[s][i] << 16 & 0x7FFF0000u), x[s][i] & 0x7FFF0000u);
-        }
-        e = power_of(umax_16_32(amax));
+        typedef uint16_t ushort2_t __attribute__((ext_vector_type(2)));
+        ushort2_t top = {0, 0};   // bits of |x| compare as the values do
 #pragma unroll
         for (int s = 0; s < 16; ++s)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float v = __uint_as_float(i & 1 ? x[s][i >> 1] & 0xFFFF0000u : x[s][i >> 1] << 16);
-                hi[s][i] = (half_t)(ok ? ldexpf(v, e) : 0.0f);
+            for (int i = 0; i < 4; ++i)
+                top = __builtin_elementwise_max(top, __builtin_bit_cast(ushort2_t, q.x[s][i] & 0x7FFF7FFFu));
+        const int e = power_of(umax_16_32((uint32_t)max(top[0], top[1]) << 16));
+        const float scale = ldexpf(1.0f, e);
+#pragma unroll
+        for (int s = 0; s < 16; ++s)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const auto two = __builtin_amdgcn_cvt_pkrtz(__uint_as_float(q.x[s][i] << 16) * scale,
+                                                            __uint_as_float(q.x[s][i] & 0xFFFF0000u) * scale);
+                hi[s][2 * i] = (half_t)two[0];
+                hi[s][2 * i + 1] = (half_t)two[1];
             }
+        return ldexpf(1.0f, -e);
     }
-    return ldexpf(1.0f, -e);
 }
 
 // The sink's part of a denominator with reference m.
@@ -465,14 +488,6 @@ __device__ inline void store_out(void *out, size_t at, float4_t v) {
         typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
         *reinterpret_cast<bf16x4 *>(static_cast<__bf16 *>(out) + at) = __builtin_convertvector(v, bf16x4);
     }
-}
-
-// v, as a value the compiler does not know: what rare paths derive from it is computed
-// there again, not kept in registers through the loop (where a spilled one's reload would
-// wait for every copy in flight).
-__device__ inline int again(int v) {
-    asm volatile("" : "+v"(v));
-    return v;
 }
 
 // ---- 64 rows ----------------------------------------------------------------------
@@ -540,7 +555,7 @@ __global__ __launch_bounds__(kF32 ? 256 : 512, kF32 ? 1 : 2) void window_kernel(
     __shared__ __attribute__((aligned(16))) int moved_s[2][8];   // whether a row of the wave's outgrew its reference
     __shared__ int bad_s;
 
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n16 = lane & 15, g = lane >> 4, row = 16 * (w & 3) + n16;
     const int kh = w >> 2;   // the wave's (first) key half
     const int wg = blockIdx.x;
@@ -562,8 +577,22 @@ __global__ __launch_bounds__(kF32 ? 256 : 512, kF32 ? 1 : 2) void window_kernel(
         }
     }
 
+    // The page of the thread's u-th row of the first tile is looked up before the outputs of the
+    // problem before are stored. (Loading the queries there as well spills 47 registers.)
     Stretch S;
-    while (next_stretch(A, line, at, S)) {
+    int page[kN];
+    auto next = [&]() {
+        if (!next_stretch(A, line, at, S)) return false;
+        const int t = again(tid);
+#pragma unroll
+        for (int u = 0; u < kN; ++u) {
+            const int key = min(kTile * tile_at(S.P, S.i0) + (t >> 4) + 16 * u, S.P.pos1);
+            page[u] = S.P.pos1 < 0 ? -1 : A.table[(long long)S.P.slot * A.stride + (key >> A.shift)];
+        }
+        return true;
+    };
+    bool more = next();
+    while (more) {
         const Problem P = S.P;
         const bool begins = S.begins, ends = S.ends;
         const int i0 = S.i0, i1 = S.i1;
@@ -582,7 +611,6 @@ __global__ __launch_bounds__(kF32 ? 256 : 512, kF32 ? 1 : 2) void window_kernel(
             auto row_of = [&](int i, int u) { return min(kTile * tile_at(P, min(i, i1 - 1)) + (tid >> 4) + 16 * u, P.pos1); };
             auto page_of = [&](int i, int u) { return A.table[(long long)P.slot * A.stride + (row_of(i, u) >> A.shift)]; };
             Part R[kN];
-            int page[kN];
             // fetches tile i + 2 (the pages after it first: waiting for a page must not wait for the
             // rows). An entry outside the pool reads row 0
             auto advance = [&](int i) {
@@ -603,12 +631,14 @@ __global__ __launch_bounds__(kF32 ? 256 : 512, kF32 ? 1 : 2) void window_kernel(
 #pragma unroll
                 for (int u = 0; u < kN; ++u) store_part(stages[0] + stage + 16 * u * kRowB, tid, R[u]);
             };
-#pragma unroll
-            for (int u = 0; u < kN; ++u) page[u] = page_of(i0, u);
             advance(i0 - 2);
             half8_t qh[16], ql[kF32 ? 16 : 1];
             float kq = 0.0f;
-            if (scores_mine) kq = load_q<kF32>(A, P, row, g, qh, ql) * (kLog2e / 22.62741699796952f);   // 1 / sqrt(512)
+            if (scores_mine) {
+                QRow<kF32> q;
+                load_row<kF32>(A, P, row, g, q);
+                kq = fragments_of<kF32>(q, qh, ql) * (kLog2e / 22.62741699796952f);   // 1 / sqrt(512)
+            }
             const int pos = P.pos0 + min(row >> lh, P.n - 1);   // (rows past the queries repeat the last one's)
             float m = -INFINITY, l = 0.0f, sum = 0.0f;
             float ref = 0.0f;   // m, or 0 while there is none
@@ -811,6 +841,7 @@ __global__ __launch_bounds__(kF32 ? 256 : 512, kF32 ? 1 : 2) void window_kernel(
             m_s[tid] = -INFINITY;
         }
         if (__any(bad) && lane == 0) bad_s = 1;
+        more = next();
         lds_barrier();
         const float nan = bad_s ? __builtin_nanf("") : 0.0f;
         const int lane_e = again(lane), n_e = lane_e & 15, g_e = lane_e >> 4;
@@ -1103,15 +1134,15 @@ __global__ __launch_bounds__(256, 2) void few_rows_kernel(const WinArgs A) {
 }
 
 // The parts of a problem that cuts fall into, in order, and the sink. A workgroup has
-// kShare rows: one, whose parts its four waves share (parts w, w + 4, .., then their sums in
+// kShare rows: one, whose parts its eight waves share (parts w, w + 8, .., then their sums in
 // order), or four, a wave each; a lane has eight dims, eight parts in flight.
 // kInline: the workgroups' problems are 0, 1, ..; else those that cuts 1, 2, .. fall into, each at its first cut.
 template <bool kF32, bool kInline, int kShare>
-__global__ __launch_bounds__(256) void window_merge_kernel(const WinArgs A) {
-    constexpr int kStep = kShare == 1 ? 4 : 1;
+__global__ __launch_bounds__(kShare == 1 ? 512 : 256) void window_merge_kernel(const WinArgs A) {
+    constexpr int kWaves = kShare == 1 ? 8 : 4, kStep = kShare == 1 ? 8 : 1;
     const int rows = 1 << A.log_rows, wgs = rows / kShare;   // workgroups of a problem
-    __shared__ float f_s[4][kMaxWgs];   // each wave's parts' factors
-    __shared__ float4_t o_s[3][64][2];
+    __shared__ float f_s[kWaves][kMaxWgs];   // each wave's parts' factors
+    __shared__ float4_t o_s[kShare == 1 ? kWaves - 1 : 1][64][2];
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, n_prob = *A.n_prob;
     const int row = kShare == 1 ? blockIdx.x % wgs : 4 * (blockIdx.x % wgs) + w;
     const long long per = A.line[0], whole = A.line[1];
@@ -1168,7 +1199,7 @@ __global__ __launch_bounds__(256) void window_merge_kernel(const WinArgs A) {
         __syncthreads();
         if (w > 0) return;
 #pragma unroll
-        for (int k = 0; k < 3; ++k) {
+        for (int k = 0; k < kWaves - 1; ++k) {
             o[0] += o_s[k][lane][0];
             o[1] += o_s[k][lane][1];
         }
@@ -1300,7 +1331,7 @@ extern "C" int ds4hip_flash_attn_window_fp8(const ds4hip_window_attn *a, void *w
         auto *merge = n > 16 ? f32 ? in ? window_merge_kernel<true, true, 4> : window_merge_kernel<true, false, 4>
                                    : in ? window_merge_kernel<false, true, 4> : window_merge_kernel<false, false, 4>
                              : f32 ? window_merge_kernel<true, true, 1> : window_merge_kernel<false, true, 1>;
-        hipLaunchKernelGGL(merge, dim3(n << (n > 16 ? log_rows - 2 : log_rows)), dim3(256), 0, st, A);
+        hipLaunchKernelGGL(merge, dim3(n << (n > 16 ? log_rows - 2 : log_rows)), dim3(n > 16 ? 256 : 512), 0, st, A);
     }
     return ds4hip_set_last_error(hip_status(hipGetLastError()));
 }
