@@ -19,6 +19,7 @@
 #include "../../include/ds4hip_pages.h"
 
 #include <algorithm>
+#include <cmath>
 
 using namespace ds4hip;
 
@@ -157,7 +158,7 @@ __device__ inline long long block_scan(long long v, long long *sums, long long *
 
 // put(i, record, tiles before) for every problem; returns their number, *tiles and, in
 // *longest (shared, 0 before), the most of one. All threads of the workgroup; first_s: [n_seqs].
-template <int kThreads, typename Put>
+template <int kThreads, int kEach, typename Put>
 __device__ inline int lay_line(const WinArgs &A, int *first_s, long long *sums, int *longest, long long *tiles, Put put) {
     const int tid = threadIdx.x;
     const int lh = log_hpt(A), lg = A.log_head - lh, qpt = (1 << A.log_rows) >> lh;
@@ -176,31 +177,46 @@ __device__ inline int lay_line(const WinArgs &A, int *first_s, long long *sums, 
         n_all = (long long)A.n_seqs << lg;
     }
     const int n_prob = (int)min(n_all, (long long)A.prob_cap);   // (only a q_start that goes back names more)
-    for (int i0 = 0; i0 < n_prob; i0 += kThreads) {
-        const int i = i0 + tid;
-        int4 rec = make_int4(-1, 0, 0, 0);
-        int n = 0;
-        if (i < n_prob) {
-            int s = i >> lg, first = s << lg;
-            if (A.q_start) {
-                int hi = A.n_seqs;   // the last sequence whose first problem is at most i
-                s = 0;
-                while (hi - s > 1) {
-                    const int mid = (s + hi) >> 1;
-                    if (first_s[mid] <= i) s = mid; else hi = mid;
+    for (int i0 = 0; i0 < n_prob; i0 += kThreads * kEach) {
+        int4 rec[kEach];
+        int n[kEach], sum = 0, most = 0;
+#pragma unroll
+        for (int u = 0; u < kEach; ++u) {
+            const int i = i0 + kEach * tid + u;
+            n[u] = 0;
+            if (i < n_prob) {
+                int s = i >> lg, first = s << lg;
+                if (A.q_start) {
+                    int hi = A.n_seqs;   // the last sequence whose first problem is at most i
+                    s = 0;
+                    while (hi - s > 1) {
+                        const int mid = (s + hi) >> 1;
+                        if (first_s[mid] <= i) s = mid; else hi = mid;
+                    }
+                    first = first_s[s];
                 }
-                first = first_s[s];
+                rec[u] = record_of(A, s, i - first);
             }
-            rec = record_of(A, s, i - first);
-            n = problem_of(A, rec).tiles;
         }
+#pragma unroll
+        for (int u = 0; u < kEach; ++u)
+            if (i0 + kEach * tid + u < n_prob) {
+                n[u] = problem_of(A, rec[u]).tiles;
+                sum += n[u];   // (four problems have under 2^30)
+                most = max(most, n[u]);
+            }
         long long all;
-        const long long before = t_all + block_scan<kThreads>(n, sums, &all);
-        if (i < n_prob) put(i, rec, before);
+        long long before = t_all + block_scan<kThreads>(sum, sums, &all);
+#pragma unroll
+        for (int u = 0; u < kEach; ++u)
+            if (i0 + kEach * tid + u < n_prob) {
+                put(i0 + kEach * tid + u, rec[u], before);
+                before += n[u];
+            }
         t_all += all;
 #pragma unroll
-        for (int off = 32; off > 0; off >>= 1) n = max(n, __shfl_xor(n, off));
-        if ((tid & 63) == 0 && n) atomicMax(longest, n);
+        for (int off = 32; off > 0; off >>= 1) most = max(most, __shfl_xor(most, off));
+        if ((tid & 63) == 0 && most) atomicMax(longest, most);
     }
     __syncthreads();
     *tiles = t_all;
@@ -266,7 +282,8 @@ __global__ __launch_bounds__(1024) void plan_kernel(const WinArgs A) {
     if (threadIdx.x == 0) longest = 0;
     constexpr int kHeld = 8192;   // (64 KB; the search below took half the kernel's time in memory)
     __shared__ long long pre_s[kHeld];
-    const int n_prob = lay_line<1024>(A, first_s, sums, &longest, &tiles, [&](int i, int4 rec, long long before) {
+    // four problems a thread: their loads and one sum for 4096 (12 us; with one a thread 17)
+    const int n_prob = lay_line<1024, 4>(A, first_s, sums, &longest, &tiles, [&](int i, int4 rec, long long before) {
         A.prob[i] = rec;
         A.pre[i] = before;
         if (i < kHeld) pre_s[i] = before;
@@ -308,7 +325,7 @@ __device__ inline Place take_place(const WinArgs &A, Line<kFew> &L) {
     if constexpr (kFew != 0) {
         if (tid == 0) L.longest = 0;
         long long tiles;
-        at.n_prob = lay_line<kThreads>(A, L.first, L.sums, &L.longest, &tiles, [&](int i, int4 rec, long long before) {
+        at.n_prob = lay_line<kThreads, 1>(A, L.first, L.sums, &L.longest, &tiles, [&](int i, int4 rec, long long before) {
             L.prob[i] = rec;
             L.pre[i] = before;
         });
@@ -1134,12 +1151,12 @@ __global__ __launch_bounds__(256, 2) void few_rows_kernel(const WinArgs A) {
 }
 
 // The parts of a problem that cuts fall into, in order, and the sink. A workgroup has
-// kShare rows: one, whose parts its eight waves share (parts w, w + 8, .., then their sums in
+// kShare rows: one, whose parts its four or eight waves share (parts w, w + 4, .., then their sums in
 // order), or four, a wave each; a lane has eight dims, eight parts in flight.
 // kInline: the workgroups' problems are 0, 1, ..; else those that cuts 1, 2, .. fall into, each at its first cut.
-template <bool kF32, bool kInline, int kShare>
-__global__ __launch_bounds__(kShare == 1 ? 512 : 256) void window_merge_kernel(const WinArgs A) {
-    constexpr int kWaves = kShare == 1 ? 8 : 4, kStep = kShare == 1 ? 8 : 1;
+template <bool kF32, bool kInline, int kWaves, int kShare>
+__global__ __launch_bounds__(64 * kWaves) void window_merge_kernel(const WinArgs A) {
+    constexpr int kStep = kShare == 1 ? kWaves : 1;
     const int rows = 1 << A.log_rows, wgs = rows / kShare;   // workgroups of a problem
     __shared__ float f_s[kWaves][kMaxWgs];   // each wave's parts' factors
     __shared__ float4_t o_s[kShare == 1 ? kWaves - 1 : 1][64][2];
@@ -1328,10 +1345,16 @@ extern "C" int ds4hip_flash_attn_window_fp8(const ds4hip_window_attn *a, void *w
     const long long most = a->window > 0 ? span / kTile + 2 + (std::min<long long>(a->n_first, held) + kTile - 1) / kTile : held / kTile + 1;
     if (most > kWhole) {
         const int n = in ? A.prob_cap : A.n_wg - 1;
-        auto *merge = n > 16 ? f32 ? in ? window_merge_kernel<true, true, 4> : window_merge_kernel<true, false, 4>
-                                   : in ? window_merge_kernel<false, true, 4> : window_merge_kernel<false, false, 4>
-                             : f32 ? window_merge_kernel<true, true, 1> : window_merge_kernel<false, true, 1>;
-        hipLaunchKernelGGL(merge, dim3(n << (n > 16 ? log_rows - 2 : log_rows)), dim3(n > 16 ? 256 : 512), 0, st, A);
+        // parts that a problem can have: its share of the workgroups, or as many as `per` leaves. Four rows a
+        // workgroup from 17 problems on; a row's parts are shared by four waves, by eight from
+        // 65 parts on (128 parts: 16.0 us with four, 12.0 with eight; 16 parts: 10.1 and 12.5)
+        const int parts = std::min(A.n_wg / std::max(n, 1), 4 * (int)std::sqrt((double)most));
+        const bool shared = n <= 16, eight = shared && parts > 64;
+        auto *merge = eight    ? f32 ? window_merge_kernel<true, true, 8, 1> : window_merge_kernel<false, true, 8, 1>
+                      : shared ? f32 ? window_merge_kernel<true, true, 4, 1> : window_merge_kernel<false, true, 4, 1>
+                      : f32    ? in ? window_merge_kernel<true, true, 4, 4> : window_merge_kernel<true, false, 4, 4>
+                               : in ? window_merge_kernel<false, true, 4, 4> : window_merge_kernel<false, false, 4, 4>;
+        hipLaunchKernelGGL(merge, dim3(n << (shared ? log_rows : log_rows - 2)), dim3(eight ? 512 : 256), 0, st, A);
     }
     return ds4hip_set_last_error(hip_status(hipGetLastError()));
 }
