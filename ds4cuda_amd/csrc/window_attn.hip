@@ -7,12 +7,20 @@
 //   out = sum_k exp(s_k - M) V_k / (exp(sink_h - M) + sum_k exp(s_k - M)),
 //   s_k = (q_h . K_k) / sqrt(512), K == V (one latent KV head).
 //
-// Work split. A problem is 64 rows (queries x heads of one sequence) and the
-// key tiles any of them sees. The tiles of all problems are one line that is cut
-// into equal parts, one per workgroup, so that ragged lengths, few long
-// sequences and many short ones all fill the chip; a problem that a cut falls
-// into leaves its parts' (O, m, l) to a merge. The lengths live on the device: a
-// plan kernel lays the line out.
+// Work split. A problem is 64 rows (queries x heads of one sequence), or 16 where the
+// sequences have no more on the average, and the key tiles any of them sees. The tiles
+// of all problems are one line that is cut into equal parts, one per workgroup, so that
+// ragged lengths, few long sequences and many short ones all fill the chip; a problem
+// that a cut falls into leaves its parts' (O, m, l) to a merge. The lengths live on the
+// device: where problems are few every workgroup lays the line out for itself, else a plan
+// kernel does.
+//
+// What bounds it. 64 queries x 64 heads over a window of 1024 rows each: matrix
+// instructions, LDS reads and the weights take turns within a tile, 1.3 us where a library
+// product's rate would take 0.9; long lists add the wait for memory (1.9 us). Calls of a few tiles are
+// launch, the queries, the first rows and the outputs one after the other (about 20 us).
+// (A workgroup's place on the line by XCD, so that neighbours share an L2, changed nothing:
+// the rows come from there already.)
 
 #include "attn_tile.h"
 #include "ds4hip_common.h"
@@ -30,6 +38,7 @@ constexpr int kMinTiles = 4;         // tiles of a part
 constexpr int kWhole = 8;            // tiles of a problem that is never cut
 constexpr int kPart = 12;            // tiles whose time a cut costs: its parts' 256 KB and their merge
 constexpr int kMaxSeqs = 4096;
+constexpr int kMaxRows = 0x7FFFFF00; // rows of a sequence: a tile's keys stay in 32 bits
 constexpr int kFewProbs = 512, kFewProbs16 = 128;   // problems of 64, 16 rows that a workgroup lays out itself
 // P = 2^((s - m) kq + top) with s and the row's reference m as the matrix
 // instructions leave them and kq its scale to log2: their difference is exact where P is
@@ -85,7 +94,7 @@ __device__ inline int4 record_of(const WinArgs &A, int s, int tile) {
     const int q = (tile >> lg) * qpt, slot = A.seq_ids ? A.seq_ids[s] : s;
     const bool in = slot >= 0 && slot < A.n_slots;
     const int rows = in ? max(A.rows[slot], 0) : 0;
-    return make_int4(in && ((rows - 1) >> A.shift) < A.stride ? slot : -1, qs.x + q,
+    return make_int4(in && rows <= kMaxRows && ((rows - 1) >> A.shift) < A.stride ? slot : -1, qs.x + q,
                      min(qpt, qs.y - q) | ((tile & ((1 << lg) - 1)) << lh) << 8, rows - qs.y + q);
 }
 
@@ -373,7 +382,7 @@ __device__ inline bool next_stretch(const WinArgs &A, const Line<kFew> &L, Place
     return true;
 }
 
-// ---- attention -------------------------------------------------------------------
+// ---- 64 rows ---------------------------------------------------------------------
 
 // The 64-row kernel's order of dims in an LDS row: the first dim of 8-dim granule p. A
 // thread's 16-byte code chunk becomes two granules; the first ones of 16 threads lie
@@ -1286,8 +1295,10 @@ bool aligned(const void *p, size_t n) { return (reinterpret_cast<uintptr_t>(p) &
 extern "C" size_t ds4hip_flash_attn_window_fp8_workspace_bytes(int n_seqs, int n_q, int n_head) {
     const int lh = log2_heads(n_head);
     if (lh < 0 || n_seqs <= 0 || n_seqs > kMaxSeqs || n_q <= 0 || n_q > (1 << 24)) return 0;
-    const int log_rows = rows_log(n_seqs, n_q, lh);
-    return lay_out(nullptr, nullptr, prob_cap(n_seqs, n_q, lh, log_rows), log_rows);
+    // (of either split: what is enough for some sizes is enough for smaller ones)
+    size_t most = 0;
+    for (int log_rows : {4, 6}) most = std::max(most, lay_out(nullptr, nullptr, prob_cap(n_seqs, n_q, lh, log_rows), log_rows));
+    return most;
 }
 
 extern "C" int ds4hip_flash_attn_window_fp8(const ds4hip_window_attn *a, void *workspace, size_t workspace_bytes,
@@ -1302,7 +1313,7 @@ extern "C" int ds4hip_flash_attn_window_fp8(const ds4hip_window_attn *a, void *w
     if (!a->q || !a->out || !a->codes || !a->sexp || !a->tail || !a->table || !a->rows || a->table_stride <= 0 ||
         a->n_slots <= 0 || a->n_cache_rows < a->page_rows || (a->n_cache_rows >> shift) > 0x7FFFFFFF || !workspace ||
         (!a->q_start && a->n_q < a->n_seqs) || (!a->seq_ids && a->n_slots < a->n_seqs) || !aligned(a->q, 16) ||
-        !aligned(a->out, a->io_f32 ? 16 : 8) || !aligned(a->codes, 16) || !aligned(a->sexp, 8) || !aligned(a->tail, 16) ||
+        !aligned(a->out, 16) || !aligned(a->codes, 16) || !aligned(a->sexp, 8) || !aligned(a->tail, 16) ||
         !aligned(workspace, 16))
         return ds4hip_set_last_error(kEINVAL);
     WinArgs A = {};

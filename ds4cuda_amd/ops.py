@@ -305,6 +305,11 @@ def _ready(t, dtype, index):
     return t.dtype is dtype and t.get_device() == index and t.is_contiguous()
 
 
+def _same_gpu(t, index, name):
+    if t.get_device() != index:
+        raise Ds4HipError(f"{name}: on {t.device}, the cache is on GPU {index}", -22)
+
+
 def window_workspace_bytes(n_seqs, n_q, n_head) -> int:
     return lib().ds4hip_flash_attn_window_fp8_workspace_bytes(n_seqs, n_q, n_head)
 
@@ -383,7 +388,7 @@ class WindowView:
                                   (q_start, torch.int32, 1, "q_start"), (seq_ids, torch.int32, None, "seq_ids")):
             if t is not None and (not _ready(t, dtype, self.index) or (n and t.numel() < n)):
                 _check(t, dtype, n, name)
-                raise Ds4HipError(f"{name}: on {t.device}, the cache is on GPU {self.index}", -22)
+                _same_gpu(t, self.index, name)
         n_seqs = q_start.numel() - 1 if q_start is not None else n_q
         if seq_ids is not None and seq_ids.numel() != n_seqs:
             raise Ds4HipError(f"seq_ids: {n_seqs} entries expected, got {seq_ids.numel()}", -22)
@@ -392,6 +397,7 @@ class WindowView:
                 out = torch.empty_like(q)
             else:
                 _check(out, q.dtype, q.numel(), "out")
+                _same_gpu(out, self.index, "out")
             if n_q == 0 or n_seqs == 0:
                 return out
             need = window_workspace_bytes(n_seqs, n_q, n_head)
@@ -399,6 +405,7 @@ class WindowView:
                 workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
             else:
                 _dev(workspace, "workspace", need)
+                _same_gpu(workspace, self.index, "workspace")
             a = WindowAttn(q=q.data_ptr(), out=out.data_ptr(), io_f32=q.dtype == torch.float32, sinks=_addr(sinks),
                            q_start=_addr(q_start), seq_ids=_addr(seq_ids), n_seqs=n_seqs, n_q=n_q, n_head=n_head,
                            window=int(window), n_first=int(n_first), **self.fixed)

@@ -13,7 +13,7 @@ import ctypes as C
 import torch
 
 from ._lib import Ds4HipError, call, lib
-from .ops import HEAD_DIM, N_NOPE, N_ROT, Fp8KVCache, WindowView, _addr, _check, _on_stream, _ptr, _ready, _stream
+from .ops import HEAD_DIM, N_NOPE, N_ROT, Fp8KVCache, WindowView, _addr, _check, _on_stream, _ptr, _ready, _same_gpu, _stream
 
 MAX_JOBS = 1024    # sequences of one call
 
@@ -38,7 +38,7 @@ class PagePool:
     def __init__(self, codes, sexp, tail, refs, table, rows, page_rows, status=None):
         if codes.dim() != 3 or table.dim() != 2:
             raise Ds4HipError("codes must be [layers, rows, 448] and table [sequences, entries]", -22)
-        if len({t.device for t in (codes, sexp, tail, refs, table, rows)}) > 1:
+        if len({t.device for t in (codes, sexp, tail, refs, table, rows, codes if status is None else status)}) > 1:
             raise Ds4HipError("the pool's tensors must be on one device", -22)
         layers, n_rows = codes.shape[0], codes.shape[1]
         n_pages = refs.numel()
@@ -94,7 +94,7 @@ class PagePool:
             return 0
         if not _ready(ids, torch.int32, self.index):
             _check(ids, torch.int32, None, name)
-            raise Ds4HipError(f"{name}: on {ids.device}, the pool is on {self.device}", -22)
+            _same_gpu(ids, self.index, name)
         k = ids.numel()
         if n is not None and k != n:
             raise Ds4HipError(f"{name}: {n} entries expected, got {k}", -22)
@@ -125,6 +125,7 @@ class PagePool:
             dst_rows = self._empty(n_dst, torch.int64, stream)
         else:
             _check(dst_rows, torch.int64, n_dst, "dst_rows")
+            _same_gpu(dst_rows, self.index, "dst_rows")
         self._call("ds4hip_kv_pages_extend", stream, _addr(seqs), _addr(n_new), n, dst_rows.data_ptr(), int(n_dst))
         return dst_rows
 
@@ -134,6 +135,8 @@ class PagePool:
         n = kv.shape[0]
         _check(kv, torch.float32, n * HEAD_DIM, "kv")
         _check(dst_rows, torch.int64, n, "dst_rows")
+        _same_gpu(kv, self.index, "kv")
+        _same_gpu(dst_rows, self.index, "dst_rows")
         self._call("ds4hip_kv_pages_append", stream, int(layer), kv.data_ptr(), n, dst_rows.data_ptr())
 
     def fork(self, parents, children, n_rows=None, deep=False, stream=None):
@@ -160,6 +163,7 @@ class PagePool:
             n_live = self._empty((), torch.int32, stream)
         else:
             _check(n_live, torch.int32, 1, "n_live")
+            _same_gpu(n_live, self.index, "n_live")
         self._call("ds4hip_kv_pages_compact", stream, n_live.data_ptr(), *self._ws(stream))
         return n_live
 

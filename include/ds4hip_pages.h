@@ -104,12 +104,16 @@ int ds4hip_kv_pages_compact(const ds4hip_kv_pages *p, int32_t *n_live, void *wor
  * and its softmax runs over those rows and, where sinks is not NULL, the
  * head's sink logit (a term of the denominator with no row). It is 0 where it sees
  * nothing; outputs of queries that no entry names are left as they were.
- * n_head: 8, 16, 32, 64 or 128. io_f32 0: q and out are bf16, and P is rounded to one
- * f16 (2^-12 relative); 1: both are fp32, with q and P as f16 hi + lo halves.
- * All arrays are device memory (q, out, codes and tail 16-byte aligned, sexp 8-byte): the lengths are read on
- * the device, so a captured call follows them. No entry outside the table and no row
- * outside [0, n_cache_rows) is read; a query of a sequence that names one is NaN. A
- * row that is not finite reaches only the queries that see it. */
+ * n_head: 8, 16, 32, 64 or 128. io_f32 0: q and out are bf16, and weights are rounded to
+ * one f16 (by up to 2^-11 of the weight, or 2^-17 of the largest where that is more); 1:
+ * both are fp32, with q and weights as f16 hi + lo halves.
+ * All arrays are device memory (q, out, codes, tail and workspace 16-byte aligned, sexp
+ * 8-byte). The lengths are read on the device, so a captured call follows them. No
+ * entry outside the table and no row outside [0, n_cache_rows) is read: queries are NaN
+ * where their sequence is outside the table, has more rows than its table row holds (or
+ * than 2^31 - 256), or where a group of 32 rows from a multiple of 32 on in which they
+ * see one names such a row (with them, up to 63 queries next to them in their sequence).
+ * A row that is not finite reaches only the queries that see it. */
 typedef struct ds4hip_window_attn {
     const void *q;
     void *out;
@@ -126,6 +130,8 @@ typedef struct ds4hip_window_attn {
     const int32_t *seq_ids; /* [n_seqs] or NULL */
     int n_seqs, n_q, n_head, window, n_first;
 } ds4hip_window_attn;
+/* Bytes of workspace; enough also for fewer sequences and fewer queries. Two calls that can
+ * run at the same time need one each. */
 size_t ds4hip_flash_attn_window_fp8_workspace_bytes(int n_seqs, int n_q, int n_head);
 int ds4hip_flash_attn_window_fp8(const ds4hip_window_attn *a, void *workspace, size_t workspace_bytes, void *stream);
 

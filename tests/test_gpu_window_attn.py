@@ -52,7 +52,7 @@ class Batch:
         return row_values(self.cache.codes[a], self.cache.sexp[a], self.cache.tail[a])
 
 
-def check(b, q, out, new, window, first, sinks, seqs=None, near=True):
+def check(b, q, out, new, window, first, sinks, seqs=None):
     """Every query's output against 64 bits; new[i] queries of entry i."""
     f32, a, off, norm = q.dtype == torch.float32, 0, 0.0, 0.0
     for i, n in enumerate(new):
@@ -352,6 +352,48 @@ def test_pages_past_32_bits(gpu):
     check(b, q, run(b, q, [3]), [3], 0, 0, None)
     del b, cache
     torch.cuda.empty_cache()
+
+
+@pytest.mark.parametrize("typ,heads", [("bf16", 64), ("fp32", 64), ("bf16", 8), ("fp32", 8)])
+def test_positions_up_to_2_31(gpu, typ, heads):
+    """A page of 2^20 rows named 2048 times: the last rows of the longest sequence are those
+    of a short one, to the bit; a longer one is NaN."""
+    from ds4cuda_amd import ops
+    n, most = 1 << 20, (1 << 31) - 256
+    g = torch.Generator(gpu).manual_seed(31)
+    codes = torch.randint(0, 0x70, (n, 448), generator=g, device=gpu, dtype=torch.uint8)
+    cache = ops.Fp8KVCache(codes, torch.zeros((n, 8), dtype=torch.int8, device=gpu),
+                           torch.zeros((n, 64), dtype=torch.float16, device=gpu))
+    table = torch.zeros((3, 2048), dtype=torch.int32, device=gpu)
+    rows = i32([most, most % n + n, most + 1], gpu)
+    q = queries(gpu, 1, heads, typ, 32).expand(3, heads, 512).contiguous()
+    out = ops.flash_attn_window_fp8(q, cache, table, rows, page_rows=n, window=100, n_first=3)
+    assert torch.isfinite(out[:2]).all() and torch.equal(out[0], out[1]) and bool(out[0].any())
+    assert torch.isnan(out[2]).all()
+
+
+@pytest.mark.parametrize("typ", ["bf16", "fp32"])
+def test_many_single_tokens_of_a_slice(gpu, typ):
+    """More problems of 16 rows than a workgroup lays out itself, some of them cut."""
+    rows = [2500 if i % 50 == 7 else (37 * i) % 90 for i in range(300)]
+    b = Batch(gpu, rows, 32, 33)
+    q = queries(gpu, len(rows), 16, typ, 34)
+    out = run(b, q, [1] * len(rows))
+    for i, r in enumerate(rows):
+        if r == 0:
+            assert not out[i].any()
+    live = [i for i, r in enumerate(rows) if r]
+    check(b, q[live], out[live], [1] * len(live), 0, 0, None, seqs=live)
+
+
+@pytest.mark.parametrize("typ", ["bf16", "fp32"])
+@pytest.mark.parametrize("heads", [16, 64])
+def test_one_sequence_over_all_workgroups(gpu, heads, typ):
+    """Its rows are joined from more than 64 parts."""
+    b = Batch(gpu, [41003], 64, 35)
+    sinks = torch.linspace(-2, 2, heads, device=gpu)
+    q = queries(gpu, 1, heads, typ, 36)
+    check(b, q, run(b, q, [1], sinks=sinks), [1], 0, 0, sinks)
 
 
 def test_the_pages_and_the_attention_as_they_are_used(gpu):

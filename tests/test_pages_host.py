@@ -95,6 +95,21 @@ def test_attention_workspace():
     assert [size(*a) for a in ((0, 5, 64), (4097, 5, 64), (2, 0, 64), (2, (1 << 24) + 1, 64), (2, 5, 65))] == [0] * 5
 
 
+def test_a_workspace_is_enough_for_smaller_calls():
+    from ds4cuda_amd import lib
+    size = lib().ds4hip_flash_attn_window_fp8_workspace_bytes
+    for heads in (8, 16, 64, 128):
+        for n_seqs in (1, 2, 16, 200):
+            for n_q in (1, 2, 31, 400):
+                need = size(n_seqs, n_q, heads)
+                assert all(size(s, q, heads) <= need for s in (1, n_seqs) for q in (1, (n_q + 1) // 2, n_q))
+
+
+def test_attention_outputs_are_aligned():
+    from ds4cuda_amd import lib
+    assert lib().ds4hip_flash_attn_window_fp8(C.byref(attn(out=X + 8)), X, BIG, None) == -22
+
+
 def test_python_refuses_host_tensors_and_shapes():
     from ds4cuda_amd import Ds4HipError, ops, pages
 
