@@ -37,6 +37,7 @@ constexpr int kMaxWgs = 512;         // workgroups the line of tiles is cut for:
 constexpr int kMinTiles = 4;         // tiles of a part
 constexpr int kWhole = 8;            // tiles of a problem that is never cut
 constexpr int kPart = 12;            // tiles whose time a cut costs: its parts' 256 KB and their merge
+constexpr int kSecond = 4;           // tiles whose time a workgroup's second problem costs
 constexpr int kMaxSeqs = 4096;
 constexpr int kMaxRows = 0x7FFFFF00; // rows of a sequence: a tile's keys stay in 32 bits
 constexpr int kFewProbs = 512, kFewProbs16 = 128;   // problems of 64, 16 rows that a workgroup lays out itself
@@ -323,6 +324,7 @@ struct Line {
 struct Place {
     int n_prob, prob;
     long long t, end;
+    int part;   // > 0: even parts of that many tiles at most
 };
 
 // Few problems: every workgroup lays out the line itself (a launch and a wait less), and
@@ -331,6 +333,7 @@ template <int kFew, int kThreads>
 __device__ inline Place take_place(const WinArgs &A, Line<kFew> &L) {
     const int tid = threadIdx.x, wg = blockIdx.x;
     Place at;
+    at.part = 0;
     if constexpr (kFew != 0) {
         if (tid == 0) L.longest = 0;
         long long tiles;
@@ -340,7 +343,27 @@ __device__ inline Place take_place(const WinArgs &A, Line<kFew> &L) {
         });
         if (tid == 0) L.pre[at.n_prob] = tiles;
         __syncthreads();
-        const Cuts C = cuts_of(tiles, A.n_wg, at.n_prob, L.longest);
+        Cuts C = cuts_of(tiles, A.n_wg, at.n_prob, L.longest);
+        // Even parts: a problem is cut into equal ones and no workgroup has parts of two (the second's
+        // queries and stores take as long as about kSecond tiles); the line then counts a problem as
+        // a whole number of cuts. 16 long sequences: 70 us with parts that pass from one to the
+        // next, 63 with even ones. Where the parts would be much longer for it (one long sequence among
+        // a hundred short ones, whose workgroups are lost to it) they pass.
+        if (C.whole >= 0 && at.n_prob < A.n_wg) {
+            const long long per = max(C.per, (tiles + A.n_wg - at.n_prob - 1) / (A.n_wg - at.n_prob));
+            if (per <= C.per + kSecond) {   // (a sum over problems of tiles / per, rounded up, is at most n_wg)
+                const long long n = tid < at.n_prob ? L.pre[tid + 1] - L.pre[tid] : 0;
+                long long all;
+                const long long before = block_scan<kThreads>((n + per - 1) / per * per, L.sums, &all);
+                if (tid < at.n_prob) L.pre[tid] = before;
+                if (tid == 0) L.pre[at.n_prob] = all;
+                __syncthreads();
+                C.tiles = all;
+                C.per = per;
+                C.whole = 0;
+                at.part = (int)per;
+            }
+        }
         if (wg == 0) {
             for (int i = tid; i <= at.n_prob; i += kThreads) {
                 if (i < at.n_prob) A.prob[i] = L.prob[i];
@@ -376,8 +399,14 @@ __device__ inline bool next_stretch(const WinArgs &A, const Line<kFew> &L, Place
                                   __builtin_amdgcn_readfirstlane(rec.z), __builtin_amdgcn_readfirstlane(rec.w)));
     S.begins = at.t == begin;
     S.ends = end <= at.end;
-    S.i0 = __builtin_amdgcn_readfirstlane((int)(at.t - begin));
-    S.i1 = __builtin_amdgcn_readfirstlane((int)(min(end, at.end) - begin));
+    int i0 = (int)(at.t - begin), i1 = (int)(min(end, at.end) - begin);
+    if (kFew && at.part) {
+        const int parts = (int)(end - begin) / at.part, k = i0 / at.part, n = S.P.tiles / parts, more = S.P.tiles - n * parts;
+        i0 = n * k + min(k, more);
+        i1 = i0 + n + (k < more);
+    }
+    S.i0 = __builtin_amdgcn_readfirstlane(i0);
+    S.i1 = __builtin_amdgcn_readfirstlane(i1);
     at.t = min(end, at.end);
     return true;
 }
