@@ -84,9 +84,11 @@ class PagePool:
     def check(self):
         """Waits for the device; raises Ds4HipError where a call was refused there
         since the last check (-22 or -28), and resets the status."""
+        torch.cuda.synchronize(self.device)   # (whatever stream the calls were made on)
         code = int(self.status.item())
         if code:
             self.status.zero_()
+            torch.cuda.synchronize(self.device)
             raise Ds4HipError("PagePool", code)
 
     def _jobs(self, ids, name, n=None):

@@ -299,3 +299,18 @@ def test_another_stream(gpu):
     s.synchronize()
     model.free([1], None)
     same(pool, model)
+
+
+def test_a_check_waits_for_calls_on_other_streams(gpu):
+    from ds4cuda_amd import Ds4HipError, pages
+    pool = pages.PagePool.empty(4, 16, 2, 64, 1, gpu)
+    seqs, n_new = (torch.tensor([v], dtype=torch.int32, device=gpu) for v in (0, 65))
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        torch.cuda._sleep(20_000_000)   # about 10 ms
+    pool.extend(seqs, n_new, 65, stream=s)
+    with pytest.raises(Ds4HipError) as e:
+        pool.check()
+    assert e.value.code == -28
+    pool.check()
