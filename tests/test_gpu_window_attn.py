@@ -386,6 +386,23 @@ def test_many_single_tokens_of_a_slice(gpu, typ):
     check(b, q[live], out[live], [1] * len(live), 0, 0, None, seqs=live)
 
 
+def test_as_many_sequences_as_a_call_takes(gpu):
+    """4096 sequences, more than 8192 problems, a long one among the last."""
+    new = [1 + (i % 4 == 0) for i in range(4096)]
+    rows = [(7 * i) % 40 + n for i, n in enumerate(new)]
+    rows[4050] = 3100
+    b = Batch(gpu, rows, 16, 37)
+    q = queries(gpu, sum(new), 128, "bf16", 38)
+    out = run(b, q, new, window=2500, first=20)
+    some = [i for i in range(4096) if i % 37 == 0 or i > 4000]
+    start = [0]
+    for n in new:
+        start.append(start[-1] + n)
+    pick = torch.tensor([k for i in some for k in range(start[i], start[i + 1])], device=gpu)
+    check(b, q[pick], out[pick], [new[i] for i in some], 2500, 20, None, seqs=some)
+    assert torch.isfinite(out).all()
+
+
 @pytest.mark.parametrize("typ", ["bf16", "fp32"])
 @pytest.mark.parametrize("heads", [16, 64])
 def test_one_sequence_over_all_workgroups(gpu, heads, typ):
