@@ -16,7 +16,7 @@
 // kernel does.
 //
 // What bounds it. In a tile of 64 rows the matrix instructions (0.4 us at peak, 0.9 at a
-// library product's rate), 228 KB through LDS (0.7) and the weights take turns: 1.4 us, 1.8
+// library product's rate), 150 or 228 KB through LDS (0.5, 0.7) and the weights take turns: 1.4 us, 1.8
 // over a long prompt; lists that come from memory wait for it too (1.9). Calls of a few tiles
 // are launch, the queries, the first rows and the outputs one after the other (about 20 us).
 // (A workgroup's place on the line by XCD, so that neighbours share an L2, changed nothing:
@@ -604,11 +604,9 @@ __device__ inline void store_part(uint8_t *stage, int tid, const Part &R) {
 // gained 7% on lists that come from memory alone and lost on all others. 128 rows a workgroup, which
 // would halve the rows read, spilled.
 //
-// Measured. 4096 queries of 64 heads over windows of 1024 rows (584 GFLOP): 1.05 ms, 0.55
-// PFLOP/s, half of a library f16 product's 1.1 here. 16 single tokens of 64 heads over 105 MB of
-// rows: 62 us, 1.7 TB/s of the 5.1 that a copy reaches; a tile's chain (wait for its rows, to f16, scores,
-// weights, outputs, one barrier) bounds it, 2 us where memory alone would take 0.9. 3 x 501 queries of 16
-// heads over windows of 500 rows in fp32 (13 GFLOP, issued twice): 90 us.
+// Measured. Six prompts of up to 640 queries of 64 heads over windows of 128 rows and 4: 165 us, 11 a
+// problem of six tiles, three of them with masks; the queries and outputs take 3 (212 MB, 1.3
+// TB/s). 3 x 501 queries of 16 heads over windows of 500 rows in fp32 (13 GFLOP, issued twice): 90 us.
 template <bool kF32, bool kInline>
 __global__ __launch_bounds__(kF32 ? 256 : 512, kF32 ? 1 : 2) void window_kernel(const WinArgs A) {
     constexpr int kRT = 4, kRows = 16 * kRT;   // row tiles and rows of a problem
@@ -958,6 +956,371 @@ __global__ __launch_bounds__(kF32 ? 256 : 512, kF32 ? 1 : 2) void window_kernel(
             }
         }
         lds_barrier();   // what is shared is free again
+    }
+}
+
+// A thread's share of the tiles of a stretch: its row of each, and the row's page.
+struct Fetch {
+    Part R;
+    int page;
+    bool bad;   // a page lay outside the pool
+    // (past the last row seen: that row again, masked)
+    __device__ int row_of(const Stretch &T, int i, int tid) const {
+        return min(kTile * tile_at(T.P, min(i, T.i1 - 1)) + (tid >> 4), T.P.pos1);
+    }
+    __device__ int page_of(const WinArgs &A, const Stretch &T, int i, int tid) const {
+        return A.table[(long long)T.P.slot * A.stride + (row_of(T, i, tid) >> A.shift)];
+    }
+    // Tile i (the page after it first: waiting for a page must not wait for the rows). An entry
+    // outside the pool reads row 0.
+    __device__ void tile(const WinArgs &A, const Stretch &T, int i, int tid) {
+        const int after = page_of(A, T, i + 1, tid);
+        if (page < 0 || page >= A.n_pages) {
+            bad = true;
+            page = 0;
+        }
+        load_part(A, ((long long)page << A.shift) + (row_of(T, i, tid) & ((1 << A.shift) - 1)), tid & 15, R);
+        page = after;
+    }
+};
+
+// Whether some query of the problem must not see some row of tile i.
+__device__ inline bool edge_at(const Problem &P, int i) {
+    const int tile = tile_at(P, i);
+    return !(tile < P.whole_c && (tile >= P.whole_b || tile < P.whole_a));
+}
+
+// The stages of tiles i - 1, i, i + 1 (bytes from the first), and the P buffer of tile i.
+struct Ring {
+    int sp = 2 * kStageB, sc = 0, sn = kStageB, buf = 0;
+    __device__ void turn() {
+        buf ^= 1;
+        const int free = sp;
+        sp = sc;
+        sc = sn;
+        sn = free;
+    }
+};
+
+// ---- 64 rows of bf16, long problems --------------------------------------------------
+//
+// Four waves make the scores and weights (two row tiles by one key half each, their queries in
+// 128 registers), four the outputs (128 dims each, in as many): a K fragment read from LDS
+// serves two row tiles, 150 KB a tile and not 228. Iteration i, with one barrier: the first four
+// have scores and P of tile i, the others O += P V of tile i - 1; all dequantize tile i + 1
+// and fetch a later one. P, its marks and the references are the eight equal waves' ones above. Both
+// roles pass the same barriers: one a tile, two more where a tile is marked, which both read
+// from the same words.
+//
+// Measured. 4096 queries of 64 heads over windows of 1024 rows (584 GFLOP): 1.02 ms, 0.57 PFLOP/s,
+// half of a library f16 product's 1.1 here. 16 single tokens of 64 heads over 105 MB of rows: 60
+// us, 1.75 TB/s of the 5.1 that a copy reaches: a tile's chain (wait for its rows, to f16,
+// scores, weights, outputs, one barrier) bounds it, 1.9 us where memory alone would take 0.9.
+template <bool kInline>
+__global__ __launch_bounds__(512, 2) void roles_kernel(const WinArgs A) {
+    constexpr int kRT = 4, kRows = 16 * kRT, kDT = 8;
+    constexpr int kFew = kInline ? kFewProbs : 0;
+    constexpr int kOutB = 2 * kD + 16;   // a bf16 row in LDS
+    __shared__ __attribute__((aligned(16))) uint8_t stages[3][kStageB];
+    __shared__ __attribute__((aligned(16))) half4_t pb[2][kRT][64][2];   // [buffer][row tile][lane][key half]
+    __shared__ float top_s[2][kRows], l_s[2][kRows], m_s[kRows], kq_s[kRows];
+    __shared__ uint32_t odd_s[2][4];   // keys whose scores are not finite, per wave
+    __shared__ __attribute__((aligned(16))) int moved_s[2][4];   // whether a row of the wave's outgrew its reference
+    __shared__ int bad_s;
+    __shared__ Line<kFew> line;
+
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    Place at = take_place<kFew, 512>(A, line);
+    const int lh = log_hpt(A);
+    Stretch S;
+    Fetch F;
+    // (the next problem's first page is looked up before the outputs of this one are stored)
+    auto next = [&]() {
+        if (!next_stretch(A, line, at, S)) return false;
+        F.page = S.P.pos1 < 0 ? -1 : F.page_of(A, S, S.i0, again(tid));
+        return true;
+    };
+    auto marked = [&](int4 f) { return __builtin_amdgcn_readfirstlane(f.x | f.y | f.z | f.w); };
+    // bf16 outputs from LDS, whole rows of 1 KB (eight bytes a lane from the accumulators: 2 us more)
+    auto rows_out = [&](const Problem &P) {
+        lds_barrier();
+        const int lane_e = again(lane);
+        for (int row = w; row < P.n << lh; row += 8) {
+            const size_t to = (((size_t)(P.q0 + (row >> lh)) << A.log_head) + P.head0 + (row & ((1 << lh) - 1))) * kD + 8 * lane_e;
+            *reinterpret_cast<uint4_t *>(static_cast<uint16_t *>(A.out) + to) =
+                *reinterpret_cast<const uint4_t *>(stages[0] + row * kOutB + 16 * lane_e);
+        }
+    };
+    if (w < 4) {
+        const int n16 = lane & 15, g = lane >> 4, rg = w & 1, kh = w >> 1;
+        QRow<false> q[2];   // of the problem to come: no outputs here, so there are registers for them
+        auto load_next = [&]() {
+            if (!next()) {   // (else their last values would be kept for it)
+                q[0] = q[1] = {};
+                return false;
+            }
+            const int lane_q = again(lane);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) load_row<false>(A, S.P, 32 * rg + 16 * j + (lane_q & 15), lane_q >> 4, q[j]);
+            return true;
+        };
+        bool more = load_next();
+        while (more) {
+            const Stretch T = S;
+            const Problem &P = T.P;
+            const bool whole = T.begins && T.ends;
+            const int slot = 2 * blockIdx.x + (T.begins ? 1 : 0), i0 = T.i0, i1 = T.i1;
+            const int n_rt = ((P.n << lh) + 15) >> 4;   // row tiles in use
+            F.bad = P.slot < 0;
+            Ring G;
+            if (tid == 0) bad_s = 0;
+            const bool mine = 2 * rg < n_rt;   // else the wave only shares the rest
+            if (P.pos1 >= 0) {
+                const uint32_t ka = pi_key(16 * kh + n16) * kRowB + 16 * g;
+                F.tile(A, T, i0, tid);
+                half8_t qh[2][16];
+                float kq[2] = {0.0f, 0.0f}, m[2], l[2], ref[2], sum[2];   // ref: m, or 0 while there is none
+                int pos[2];
+                // (not under `mine`: the compiler then spilled 118 registers)
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+                    kq[j] = fragments_of<false>(q[j], qh[j], nullptr) * (kLog2e / 22.62741699796952f);   // 1 / sqrt(512)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const int row = 32 * rg + 16 * j + n16;
+                    pos[j] = P.pos0 + min(row >> lh, P.n - 1);   // (rows past the queries repeat the last one's)
+                    m[j] = -INFINITY;
+                    l[j] = ref[j] = sum[j] = 0.0f;
+                    if (kh == 0 && g == 0) {
+                        m_s[row] = -INFINITY;
+                        kq_s[row] = kq[j];
+                    }
+                }
+                store_part(stages[0], tid, F.R);
+                F.tile(A, T, i0 + 1, tid);
+                float4_t acc[2];   // scores of the tile whose P is the newest
+                auto weights = [&](int b) {
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        half4_t ph;
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) ph[r] = (half_t)__builtin_amdgcn_exp2f(fmaf(acc[j][r] - ref[j], kq[j], kTop<false>));
+                        // of the rounded values: the output stays an average
+                        const half2_t one = {(half_t)1.0f, (half_t)1.0f};
+                        sum[j] = __builtin_amdgcn_fdot2(half2_t{ph[0], ph[1]}, one, 0.0f, false);
+                        sum[j] = __builtin_amdgcn_fdot2(half2_t{ph[2], ph[3]}, one, sum[j], false);
+                        pb[b][2 * rg + j][lane][kh] = ph;
+                    }
+                };
+                auto top_of = [&](int j) { return fmaxf(fmaxf(acc[j][0], acc[j][1]), fmaxf(acc[j][2], acc[j][3])); };
+                for (int i = i0;; ++i) {
+                    const bool live = i < i1;
+                    lds_barrier();
+                    const int4 f = *reinterpret_cast<const int4 *>(&moved_s[G.buf ^ 1][0]);
+                    float4_t a[2][2];   // two chains each
+                    if (live) {
+                        const uint8_t *st = stages[0] + G.sc + ka;
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) a[j][0] = a[j][1] = float4_t{0, 0, 0, 0};
+                        half8_t k[2][2];   // K fragments, read two steps ahead
+#pragma unroll
+                        for (int v = 0; v < 2; ++v) k[0][v] = *reinterpret_cast<const half8_t *>(st + 64 * v);
+#pragma unroll
+                        for (int s0 = 0; s0 < 16; s0 += 2) {
+                            const int now = (s0 / 2) & 1;
+#pragma unroll
+                            for (int v = 0; v < 2; ++v)
+                                if (s0 < 14) k[now ^ 1][v] = *reinterpret_cast<const half8_t *>(st + 64 * (s0 + 2 + v));
+#pragma unroll
+                            for (int v = 0; v < 2; ++v)
+#pragma unroll
+                                for (int j = 0; j < 2; ++j)
+                                    a[j][v] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[now][v], qh[j][s0 + v], a[j][v], 0, 0, 0);
+                            __builtin_amdgcn_sched_barrier(0);
+                        }
+                    }
+                    if (i > i0) {
+                        if (marked(f)) {   // (acc: still the scores of the tile before)
+                            const int lane_r = again(lane), n_r = lane_r & 15;
+#pragma unroll
+                            for (int j = 0; j < 2; ++j) {
+                                const float top = xmax_16_32(top_of(j));   // (all lanes take part)
+                                if (lane_r < 16 && mine) top_s[kh][32 * rg + 16 * j + n_r] = top;
+                            }
+                            lds_barrier();
+                            if (mine) {
+#pragma unroll
+                                for (int j = 0; j < 2; ++j) {
+                                    const int row = 32 * rg + 16 * j + n_r;
+                                    const float top = fmaxf(top_s[0][row], top_s[1][row]);
+                                    if ((top - m[j]) * kq[j] > kLazy<false>) {   // (-inf before the first key seen)
+                                        l[j] *= m[j] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m[j] - top) * kq[j]);
+                                        m[j] = top;
+                                    }
+                                    ref[j] = m[j] == -INFINITY ? 0.0f : m[j];
+                                }
+                                weights(G.buf ^ 1);
+                            }
+                            lds_barrier();
+                            if (mine && kh == 0 && lane_r < 16) {   // (read again after more barriers)
+                                m_s[32 * rg + n_r] = m[0];
+                                m_s[32 * rg + 16 + n_r] = m[1];
+                            }
+                        }
+                        l[0] += sum[0];
+                        l[1] += sum[1];
+                    }
+                    if (!live) break;
+                    store_part(stages[0] + G.sn, tid, F.R);
+                    F.tile(A, T, i + 2, tid);
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) acc[j] = a[j][0] + a[j][1];
+                    if (edge_at(P, i)) {
+                        const int key0 = kTile * tile_at(P, i), lane_r = again(lane), g_r = lane_r >> 4;
+                        uint32_t odd = 0;
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const int k = pi_key(16 * kh + 4 * g_r + r);
+                            bool any = false;
+#pragma unroll
+                            for (int j = 0; j < 2; ++j) {
+                                const bool fine = fabsf(acc[j][r]) < INFINITY;
+                                any = any || fine;
+                                acc[j][r] = !sees(A, pos[j], key0 + k) ? -INFINITY : fine ? acc[j][r] : __builtin_nanf("");
+                            }
+                            if (((__ballot(!any) >> (16 * g_r)) & 0xFFFF) == 0xFFFF) odd |= 1u << k;
+                        }
+                        odd |= __shfl_xor(odd, 16);
+                        odd |= __shfl_xor(odd, 32);
+                        if (lane_r == 0) odd_s[G.buf][w] = mine ? odd : ~0u;
+                    }
+                    const bool moved = mine && __any((top_of(0) - m[0]) * kq[0] > kLazy<false> || (top_of(1) - m[1]) * kq[1] > kLazy<false>);
+                    if (lane == 0) moved_s[G.buf][w] = moved;
+                    if (mine) weights(G.buf);
+                    G.turn();
+                }
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    l[j] = xsum_16_32(l[j]);
+                    if (g == 0 && mine) l_s[kh][32 * rg + 16 * j + n16] = l[j];
+                }
+            } else if (tid < kRows) {
+                m_s[tid] = -INFINITY;
+            }
+            if (__any(F.bad) && lane == 0) bad_s = 1;
+            more = load_next();
+            lds_barrier();
+            if (!whole && tid < kRows) {
+                float *ml = A.part_ml + (size_t)slot * 3 * kRows + tid;
+                ml[0] = m_s[tid];
+                ml[kRows] = l_s[0][tid] + l_s[1][tid] + (bad_s ? __builtin_nanf("") : 0.0f);
+                ml[2 * kRows] = kq_s[tid];
+            }
+            if (whole) rows_out(P);
+            lds_barrier();   // what is shared is free again
+        }
+    } else {
+        bool more = next();
+        while (more) {
+            const Stretch T = S;
+            const Problem &P = T.P;
+            const bool whole = T.begins && T.ends;
+            const int slot = 2 * blockIdx.x + (T.begins ? 1 : 0), i0 = T.i0, i1 = T.i1;
+            const int n_rt = ((P.n << lh) + 15) >> 4;   // row tiles in use
+            F.bad = P.slot < 0;
+            Ring G;
+        float4_t o[kRT][kDT];
+#pragma unroll
+            for (int a = 0; a < kRT; ++a)
+#pragma unroll
+                for (int b = 0; b < kDT; ++b) o[a][b] = float4_t{0, 0, 0, 0};
+            if (P.pos1 >= 0) {
+                uint32_t va[2];
+#pragma unroll
+                for (int kt = 0; kt < 2; ++kt)
+                    va[kt] = lds_addr(stages[0]) + pi_key(16 * kt + 4 * (lane >> 4) + ((lane & 15) >> 2)) * kRowB + 256 * (w - 4) + 8 * (lane & 3);
+                F.tile(A, T, i0, tid);
+                store_part(stages[0], tid, F.R);
+                F.tile(A, T, i0 + 1, tid);
+                for (int i = i0;; ++i) {
+                    lds_barrier();
+                    if (i > i0) {
+                        const int b = G.buf ^ 1;
+                        if (marked(*reinterpret_cast<const int4 *>(&moved_s[b][0]))) {
+                            lds_barrier();
+                            const int n_r = again(lane) & 15;
+#pragma unroll
+                            for (int rt = 0; rt < kRT; ++rt) {
+                                if (rt >= n_rt) break;
+                                const int row = 16 * rt + n_r;
+                                const float old = m_s[row], top = fmaxf(top_s[0][row], top_s[1][row]), scale = kq_s[row];
+                                const float f = (top - old) * scale > kLazy<false>
+                                                    ? old == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((old - top) * scale) : 1.0f;
+#pragma unroll
+                                for (int dt = 0; dt < kDT; ++dt) o[rt][dt] *= f;
+                            }
+                            lds_barrier();
+                        }
+                        if (edge_at(P, i - 1)) {
+                            // a row that is not finite and that some query must not see: zeroed in this wave's own
+                            // dims (0 x inf would reach it). Queries that see it have a P that is not finite.
+                            uint32_t odd = __builtin_amdgcn_readfirstlane((odd_s[b][0] & odd_s[b][1]) | (odd_s[b][2] & odd_s[b][3]));
+                            for (; odd; odd &= odd - 1)
+                                *reinterpret_cast<uint32_t *>(stages[0] + G.sp + __builtin_ctz(odd) * kRowB + 256 * (w - 4) + 4 * lane) = 0;
+                            asm volatile("" ::: "memory");   // before the reads below, which are asm
+                        }
+#pragma unroll
+                        for (int d0 = 0; d0 < kDT; d0 += 4) {
+                            half8_t vb[4];
+                            if (d0 == 0)
+                                read_vt4<0>(va[0] + G.sp, va[1] + G.sp, vb);
+                            else
+                                read_vt4<4>(va[0] + G.sp, va[1] + G.sp, vb);
+#pragma unroll
+                            for (int rt = 0; rt < kRT; ++rt) {
+                                if (rt >= n_rt) break;
+                                const half8_t h = *reinterpret_cast<const half8_t *>(&pb[b][rt][lane][0]);
+#pragma unroll
+                                for (int dt = 0; dt < 4; ++dt)
+                                    o[rt][d0 + dt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vb[dt], h, o[rt][d0 + dt], 0, 0, 0);
+                            }
+                        }
+                    }
+                    if (i >= i1) break;
+                    store_part(stages[0] + G.sn, tid, F.R);
+                    F.tile(A, T, i + 2, tid);
+                    G.turn();
+                }
+            }
+            if (__any(F.bad) && lane == 0) bad_s = 1;
+            more = next();
+            lds_barrier();
+            const int lane_e = again(lane), n_e = lane_e & 15, g_e = lane_e >> 4;
+            // first of the lane's four dims of the wave's dim tile dt
+            auto out_dim = [&](int dt) { return dim_of(16 * (w - 4) + 2 * dt + (g_e >> 1)) + 4 * (g_e & 1); };
+            if (whole) {
+                const float nan = bad_s ? __builtin_nanf("") : 0.0f;
+#pragma unroll
+                for (int rt = 0; rt < kRT; ++rt) {
+                    const int row = 16 * rt + n_e;
+                    if (row >> lh >= P.n) continue;
+                    const float mm = m_s[row], head_sink = sink_term<false>(A, P.head0 + (row & ((1 << lh) - 1)), mm, kq_s[row]);
+                    const float inv = mm == -INFINITY ? nan : 1.0f / (l_s[0][row] + l_s[1][row] + head_sink) + nan;
+#pragma unroll
+                    for (int dt = 0; dt < kDT; ++dt) store_out<false>(stages[0], (row * kOutB) / 2 + out_dim(dt), o[rt][dt] * inv);
+                }
+            } else {
+                float *dst = A.part_o + ((size_t)slot * kRows + n_e) * kD;
+#pragma unroll
+                for (int rt = 0; rt < kRT; ++rt) {
+                    if (rt >= n_rt) break;
+#pragma unroll
+                    for (int dt = 0; dt < kDT; ++dt) *reinterpret_cast<float4_t *>(dst + 16 * rt * kD + out_dim(dt)) = o[rt][dt];
+                }
+            }
+            if (whole) rows_out(P);
+            lds_barrier();   // what is shared is free again
+        }
     }
 }
 
@@ -1392,17 +1755,21 @@ extern "C" int ds4hip_flash_attn_window_fp8(const ds4hip_window_attn *a, void *w
     if (!a->q_start) A.prob_cap = a->n_seqs << (lh - std::min(lh, log_rows));
     const bool f32 = a->io_f32, in = A.prob_cap <= (log_rows == 4 ? kFewProbs16 : kFewProbs);
     if (!in) hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(1024), 0, st, A);
-    auto *main = log_rows == 4 ? f32 ? in ? few_rows_kernel<true, true> : few_rows_kernel<true, false>
-                                     : in ? few_rows_kernel<false, true> : few_rows_kernel<false, false>
-                                 : f32 ? in ? window_kernel<true, true> : window_kernel<true, false>
-                                       : in ? window_kernel<false, true> : window_kernel<false, false>;
-    hipLaunchKernelGGL(main, dim3(A.n_wg), dim3(log_rows < 6 || f32 ? 256 : 512), 0, st, A);
-    // no problem is cut where none can have that many tiles: of rows that the table can name, or of
-    // the window, the queries' own span and the first rows, with their ends inside tiles
+    // tiles that a problem can have: of rows that the table can name, or of the window, the queries'
+    // own span and the first rows, with their ends inside tiles
     const long long held = (long long)a->table_stride << shift;
     const long long span = std::min<long long>(held, (long long)a->window + ((1 << log_rows) >> std::min(lh, log_rows)));
     const long long most = a->window > 0 ? span / kTile + 2 + (std::min<long long>(a->n_first, held) + kTile - 1) / kTile : held / kTile + 1;
-    if (most > kWhole) {
+    // Waves with roles for long problems of bf16 (us, with roles and without: problems of 34 tiles 1045, 1116,
+    // 16 sequences of up to 32768 rows 60, 63; problems of 6 tiles 173, 165; one token over 4000 rows, in
+    // parts of 4 tiles, 24.4, 23.5)
+    auto *main = log_rows == 4 ? f32 ? in ? few_rows_kernel<true, true> : few_rows_kernel<true, false>
+                                     : in ? few_rows_kernel<false, true> : few_rows_kernel<false, false>
+                 : f32         ? in ? window_kernel<true, true> : window_kernel<true, false>
+                 : most > 16   ? in ? roles_kernel<true> : roles_kernel<false>
+                               : in ? window_kernel<false, true> : window_kernel<false, false>;
+    hipLaunchKernelGGL(main, dim3(A.n_wg), dim3(log_rows < 6 || f32 ? 256 : 512), 0, st, A);
+    if (most > kWhole) {   // (else nothing is cut)
         const int n = in ? A.prob_cap : A.n_wg - 1;
         // parts that a problem can have: its share of the workgroups, or as many as `per` leaves. Four rows a
         // workgroup from 17 problems on; a row's parts are shared by four waves, by eight from

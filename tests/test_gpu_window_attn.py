@@ -386,6 +386,34 @@ def test_many_single_tokens_of_a_slice(gpu, typ):
     check(b, q[live], out[live], [1] * len(live), 0, 0, None, seqs=live)
 
 
+@pytest.mark.parametrize("heads", [8, 64, 128])
+@pytest.mark.parametrize("rows,new,page,window,first", [
+    ([1, 2, 3], [1, 2, 3], 16, 0, 0), ([0, 33, 64], [0, 1, 64], 32, 0, 0), ([700, 90, 1], [130, 0, 1], 128, 640, 2),
+    ([1500, 40], [1, 40], 256, 700, 33), ([260, 131], [9, 100], 4, 0, 64), ([2000], [3], 64, 600, 700)])
+def test_tables_for_long_sequences(gpu, rows, new, page, window, first, heads):
+    """Short sequences too, in tables that have room for long ones."""
+    b = Batch(gpu, rows, page, 40, entries=max(-(-r // page) for r in rows) + -(-1024 // page))
+    sinks = torch.linspace(-3, 3, heads, device=gpu)
+    q = queries(gpu, sum(new), heads, "bf16", 41)
+    check(b, q, run(b, q, new, window, first, sinks), new, window, first, sinks)
+
+
+@pytest.mark.parametrize("value", ["nan", "inf"])
+@pytest.mark.parametrize("heads", [8, 64])
+def test_rows_that_are_not_finite_in_long_tables(gpu, heads, value):
+    b = Batch(gpu, [700], 16, 42, entries=100)
+    q = queries(gpu, 60, heads, "bf16", 43)
+    want = run(b, q, [60])
+    at = int(b.at(0)[660])
+    if value == "nan":
+        b.cache.codes[at, 5] = 0x7F
+    else:
+        b.cache.tail[at] = float("inf")
+    got = run(b, q, [60])
+    assert torch.equal(got[:20], want[:20])   # positions 640 .. 659
+    assert not torch.isfinite(got[20:]).all(-1).any()
+
+
 def test_as_many_sequences_as_a_call_takes(gpu):
     """4096 sequences, more than 8192 problems, a long one among the last."""
     new = [1 + (i % 4 == 0) for i in range(4096)]
