@@ -44,13 +44,19 @@ constexpr int kFewProbs = 512, kFewProbs16 = 128;   // problems of 64, 16 rows t
 // P = 2^((s - m) kq + top) with s and the row's reference m as the matrix
 // instructions leave them and kq its scale to log2: their difference is exact where P is
 // large, at any magnitude. The reference moves only where P would pass 2^15 (f16 ends at
-// 2^16). One f16 (bf16 outputs) starts at 2^-8: a row may gain 23 bits before it moves
-// (moving costs half a tile: rows of which 1% are eight times as large moved in 9 of 32 tiles from
-// 2^8 on), and weights under 2^-6 of the largest are off by up to 2^-17 of it. hi + lo (fp32) start at 2^8: 2^-32.
+// 2^16): a row gains 15 - top bits before it moves. An f16 under 2^-14 is off by up to 2^-25. The largest P
+// is 2^top at least, so the small weights of n rows are off by up to n 2^-(25 + top) of it together, in
+// the sum and in the outputs, and many that each are little count. So the start grows with the tiles of
+// a stretch (the parts of a cut problem have references of their own): with one f16 they are off by
+// 2^-16 of the largest together, with hi + lo by 2^-22 (up to 2^18, 2^12 tiles, where it stays at 2^14).
+// Moving costs up to half a tile: 4096 queries over windows of 1024 rows, 1% of them eight times as large, took
+// 1020 us from 2^-8 on, 1090 from the 2^2 that their 34 tiles ask for; 16 tokens of up to 32768 rows 67 and 70.5.
 template <bool kF32>
-constexpr float kTop = kF32 ? 8.0f : -8.0f;
-template <bool kF32>
-constexpr float kLazy = 15.0f - kTop<kF32>;
+__device__ inline float start_of(int tiles) {
+    const int log_up = 32 - __clz(tiles - 1);   // (of one tile: 0)
+    const int top = min(14, kF32 ? max(8, log_up + 2) : max(0, log_up - 4));
+    return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint((float)top)));
+}
 
 struct WinArgs {
     const void *q;
@@ -390,8 +396,9 @@ struct Stretch {
     Problem P;
     bool begins, ends;
     int i0, i1;
+    float top;   // P starts at 2^top
 };
-template <int kFew>
+template <bool kF32, int kFew>
 __device__ inline bool next_stretch(const WinArgs &A, const Line<kFew> &L, Place &at, Stretch &S) {
     if (__builtin_amdgcn_readfirstlane(at.t >= at.end || at.prob >= at.n_prob)) return false;
     const int pi = at.prob++;
@@ -409,6 +416,7 @@ __device__ inline bool next_stretch(const WinArgs &A, const Line<kFew> &L, Place
     }
     S.i0 = __builtin_amdgcn_readfirstlane(i0);
     S.i1 = __builtin_amdgcn_readfirstlane(i1);
+    S.top = start_of<kF32>(S.i1 - S.i0);
     at.t = min(end, at.end);
     return true;
 }
@@ -530,10 +538,9 @@ __device__ inline float fragments_of(const QRow<kF32> &q, half8_t *hi, half8_t *
     }
 }
 
-// The sink's part of a denominator with reference m.
-template <bool kF32>
-__device__ inline float sink_term(const WinArgs &A, int head, float m, float kq) {
-    return A.sinks ? __builtin_amdgcn_exp2f(fmaf(-m, kq, fmaf(A.sinks[head], kLog2e, kTop<kF32>))) : 0.0f;
+// The sink's part of a denominator with reference m, whose weights start at 2^top.
+__device__ inline float sink_term(const WinArgs &A, int head, float m, float kq, float top) {
+    return A.sinks ? __builtin_amdgcn_exp2f(fmaf(-m, kq, fmaf(A.sinks[head], kLog2e, top))) : 0.0f;
 }
 
 // Four outputs, rounded to bf16 unless the call's type is fp32.
@@ -648,7 +655,7 @@ __global__ __launch_bounds__(kF32 ? 256 : 512, kF32 ? 1 : 2) void window_kernel(
     Stretch S;
     int page[kN];
     auto next = [&]() {
-        if (!next_stretch(A, line, at, S)) return false;
+        if (!next_stretch<kF32>(A, line, at, S)) return false;
         const int t = again(tid);
 #pragma unroll
         for (int u = 0; u < kN; ++u) {
@@ -662,6 +669,7 @@ __global__ __launch_bounds__(kF32 ? 256 : 512, kF32 ? 1 : 2) void window_kernel(
         const Problem P = S.P;
         const bool begins = S.begins, ends = S.ends;
         const int i0 = S.i0, i1 = S.i1;
+        const float start = S.top;
         bool bad = P.slot < 0;
         float4_t o[kRT][kDT];
 #pragma unroll
@@ -723,7 +731,7 @@ __global__ __launch_bounds__(kF32 ? 256 : 512, kF32 ? 1 : 2) void window_kernel(
                     float p[4];
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        p[r] = __builtin_amdgcn_exp2f(fmaf(acc[u][r] - ref, kq, kTop<kF32>));
+                        p[r] = __builtin_amdgcn_exp2f(fmaf(acc[u][r] - ref, kq, start));
                         ph[r] = (half_t)p[r];
                         if (kF32) pl[r] = (half_t)(p[r] - (float)ph[r]);
                     }
@@ -758,7 +766,7 @@ __global__ __launch_bounds__(kF32 ? 256 : 512, kF32 ? 1 : 2) void window_kernel(
                     auto renew = [&](int r, float &old, float scale) {
                         const float top = kW == 8 ? fmaxf(top_s[0][r], top_s[1][r]) : top_s[0][r];
                         float f = 1.0f;
-                        if ((top - old) * scale > kLazy<kF32>) {   // (-inf before the first key seen)
+                        if ((top - old) * scale > 15.0f - start) {   // (-inf before the first key seen)
                             f = old == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((old - top) * scale);
                             old = top;
                         }
@@ -769,13 +777,17 @@ __global__ __launch_bounds__(kF32 ? 256 : 512, kF32 ? 1 : 2) void window_kernel(
                         if (rt >= n_rt) break;
                         float old = m_s[16 * rt + n_r];
                         const float f = renew(16 * rt + n_r, old, kq_s[16 * rt + n_r]);
+                        if (!__any(f != 1.0f)) continue;
 #pragma unroll
                         for (int dt = 0; dt < kDT; ++dt) o[rt][dt] *= f;
                     }
                     if (scores_mine) {
-                        l *= renew(row_r, m, kq);
-                        ref = m == -INFINITY ? 0.0f : m;
-                        weights(b);
+                        const float f = renew(row_r, m, kq);
+                        if (__any(f != 1.0f)) {   // (the same in both waves of a row tile)
+                            l *= f;
+                            ref = m == -INFINITY ? 0.0f : m;
+                            weights(b);
+                        }
                     }
                     lds_barrier();
                     if (scores_mine && kh == 0 && lane_r < 16) m_s[row_r] = m;   // (read again after more barriers)
@@ -889,7 +901,7 @@ __global__ __launch_bounds__(kF32 ? 256 : 512, kF32 ? 1 : 2) void window_kernel(
                     odd |= __shfl_xor(odd, 32);
                     if (lane_r == 0) odd_s[buf][w] = scores_mine ? odd : ~0u;
                 }
-                const bool moved = scores_mine && __any((top_of() - m) * kq > kLazy<kF32>);
+                const bool moved = scores_mine && __any((top_of() - m) * kq > 15.0f - start);
                 if (lane == 0) moved_s[buf][w] = moved;
                 if (scores_mine) weights(buf);
                 edge_before = edge;
@@ -921,7 +933,7 @@ __global__ __launch_bounds__(kF32 ? 256 : 512, kF32 ? 1 : 2) void window_kernel(
                 if (qi >= P.n) continue;
                 const float mm = m_s[rr];
                 const float sum = kW == 8 ? l_s[0][rr] + l_s[1][rr] : l_s[0][rr];
-                const float inv = mm == -INFINITY ? nan : 1.0f / (sum + sink_term<kF32>(A, head, mm, kq_s[rr])) + nan;
+                const float inv = mm == -INFINITY ? nan : 1.0f / (sum + sink_term(A, head, mm, kq_s[rr], start)) + nan;
                 const size_t to = (((size_t)(P.q0 + qi) << A.log_head) + head) * kD;
 #pragma unroll
                 for (int dt = 0; dt < kDT; ++dt) {
@@ -940,11 +952,13 @@ __global__ __launch_bounds__(kF32 ? 256 : 512, kF32 ? 1 : 2) void window_kernel(
                 }
             }
         } else {
+            // (as if they had started at 2^0: the parts of a problem need not agree)
+            const float down = ldexpf(1.0f, -(int)start);
             const int slot = 2 * wg + (begins ? 1 : 0);
             if (tid < kRows) {
                 float *ml = A.part_ml + (size_t)slot * 3 * kRows + tid;
                 ml[0] = m_s[tid];
-                ml[kRows] = (kW == 8 ? l_s[0][tid] + l_s[1][tid] : l_s[0][tid]) + nan;
+                ml[kRows] = (kW == 8 ? l_s[0][tid] + l_s[1][tid] : l_s[0][tid]) * down + nan;
                 ml[2 * kRows] = kq_s[tid];
             }
             float *dst = A.part_o + ((size_t)slot * kRows + n_e) * kD;
@@ -952,7 +966,7 @@ __global__ __launch_bounds__(kF32 ? 256 : 512, kF32 ? 1 : 2) void window_kernel(
             for (int rt = 0; rt < kRT; ++rt) {
                 if (16 * rt >= P.n << lh) break;
 #pragma unroll
-                for (int dt = 0; dt < kDT; ++dt) *reinterpret_cast<float4_t *>(dst + 16 * rt * kD + out_dim(dt)) = o[rt][dt];
+                for (int dt = 0; dt < kDT; ++dt) *reinterpret_cast<float4_t *>(dst + 16 * rt * kD + out_dim(dt)) = o[rt][dt] * down;
             }
         }
         lds_barrier();   // what is shared is free again
@@ -1036,7 +1050,7 @@ __global__ __launch_bounds__(512, 2) void roles_kernel(const WinArgs A) {
     Fetch F;
     // (the next problem's first page is looked up before the outputs of this one are stored)
     auto next = [&]() {
-        if (!next_stretch(A, line, at, S)) return false;
+        if (!next_stretch<false>(A, line, at, S)) return false;
         F.page = S.P.pos1 < 0 ? -1 : F.page_of(A, S, S.i0, again(tid));
         return true;
     };
@@ -1104,7 +1118,7 @@ __global__ __launch_bounds__(512, 2) void roles_kernel(const WinArgs A) {
                     for (int j = 0; j < 2; ++j) {
                         half4_t ph;
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) ph[r] = (half_t)__builtin_amdgcn_exp2f(fmaf(acc[j][r] - ref[j], kq[j], kTop<false>));
+                        for (int r = 0; r < 4; ++r) ph[r] = (half_t)__builtin_amdgcn_exp2f(fmaf(acc[j][r] - ref[j], kq[j], T.top));
                         // of the rounded values: the output stays an average
                         const half2_t one = {(half_t)1.0f, (half_t)1.0f};
                         sum[j] = __builtin_amdgcn_fdot2(half2_t{ph[0], ph[1]}, one, 0.0f, false);
@@ -1149,17 +1163,18 @@ __global__ __launch_bounds__(512, 2) void roles_kernel(const WinArgs A) {
                             }
                             lds_barrier();
                             if (mine) {
+                                bool moves = false;
 #pragma unroll
                                 for (int j = 0; j < 2; ++j) {
                                     const int row = 32 * rg + 16 * j + n_r;
                                     const float top = fmaxf(top_s[0][row], top_s[1][row]);
-                                    if ((top - m[j]) * kq[j] > kLazy<false>) {   // (-inf before the first key seen)
+                                    if ((top - m[j]) * kq[j] > 15.0f - T.top) {   // (-inf before the first key seen)
                                         l[j] *= m[j] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m[j] - top) * kq[j]);
-                                        m[j] = top;
+                                        ref[j] = m[j] = top;
+                                        moves = true;
                                     }
-                                    ref[j] = m[j] == -INFINITY ? 0.0f : m[j];
                                 }
-                                weights(G.buf ^ 1);
+                                if (__any(moves)) weights(G.buf ^ 1);   // (the same in both waves of a row tile)
                             }
                             lds_barrier();
                             if (mine && kh == 0 && lane_r < 16) {   // (read again after more barriers)
@@ -1194,7 +1209,7 @@ __global__ __launch_bounds__(512, 2) void roles_kernel(const WinArgs A) {
                         odd |= __shfl_xor(odd, 32);
                         if (lane_r == 0) odd_s[G.buf][w] = mine ? odd : ~0u;
                     }
-                    const bool moved = mine && __any((top_of(0) - m[0]) * kq[0] > kLazy<false> || (top_of(1) - m[1]) * kq[1] > kLazy<false>);
+                    const bool moved = mine && __any((top_of(0) - m[0]) * kq[0] > 15.0f - T.top || (top_of(1) - m[1]) * kq[1] > 15.0f - T.top);
                     if (lane == 0) moved_s[G.buf][w] = moved;
                     if (mine) weights(G.buf);
                     G.turn();
@@ -1213,7 +1228,7 @@ __global__ __launch_bounds__(512, 2) void roles_kernel(const WinArgs A) {
             if (!whole && tid < kRows) {
                 float *ml = A.part_ml + (size_t)slot * 3 * kRows + tid;
                 ml[0] = m_s[tid];
-                ml[kRows] = l_s[0][tid] + l_s[1][tid] + (bad_s ? __builtin_nanf("") : 0.0f);
+                ml[kRows] = (l_s[0][tid] + l_s[1][tid]) * ldexpf(1.0f, -(int)T.top) + (bad_s ? __builtin_nanf("") : 0.0f);
                 ml[2 * kRows] = kq_s[tid];
             }
             if (whole) rows_out(P);
@@ -1254,8 +1269,9 @@ __global__ __launch_bounds__(512, 2) void roles_kernel(const WinArgs A) {
                                 if (rt >= n_rt) break;
                                 const int row = 16 * rt + n_r;
                                 const float old = m_s[row], top = fmaxf(top_s[0][row], top_s[1][row]), scale = kq_s[row];
-                                const float f = (top - old) * scale > kLazy<false>
+                                const float f = (top - old) * scale > 15.0f - T.top
                                                     ? old == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((old - top) * scale) : 1.0f;
+                                if (!__any(f != 1.0f)) continue;
 #pragma unroll
                                 for (int dt = 0; dt < kDT; ++dt) o[rt][dt] *= f;
                             }
@@ -1304,18 +1320,19 @@ __global__ __launch_bounds__(512, 2) void roles_kernel(const WinArgs A) {
                 for (int rt = 0; rt < kRT; ++rt) {
                     const int row = 16 * rt + n_e;
                     if (row >> lh >= P.n) continue;
-                    const float mm = m_s[row], head_sink = sink_term<false>(A, P.head0 + (row & ((1 << lh) - 1)), mm, kq_s[row]);
+                    const float mm = m_s[row], head_sink = sink_term(A, P.head0 + (row & ((1 << lh) - 1)), mm, kq_s[row], T.top);
                     const float inv = mm == -INFINITY ? nan : 1.0f / (l_s[0][row] + l_s[1][row] + head_sink) + nan;
 #pragma unroll
                     for (int dt = 0; dt < kDT; ++dt) store_out<false>(stages[0], (row * kOutB) / 2 + out_dim(dt), o[rt][dt] * inv);
                 }
             } else {
+                const float down = ldexpf(1.0f, -(int)T.top);   // (as if it had started at 2^0)
                 float *dst = A.part_o + ((size_t)slot * kRows + n_e) * kD;
 #pragma unroll
                 for (int rt = 0; rt < kRT; ++rt) {
                     if (rt >= n_rt) break;
 #pragma unroll
-                    for (int dt = 0; dt < kDT; ++dt) *reinterpret_cast<float4_t *>(dst + 16 * rt * kD + out_dim(dt)) = o[rt][dt];
+                    for (int dt = 0; dt < kDT; ++dt) *reinterpret_cast<float4_t *>(dst + 16 * rt * kD + out_dim(dt)) = o[rt][dt] * down;
                 }
             }
             if (whole) rows_out(P);
@@ -1354,7 +1371,7 @@ __global__ __launch_bounds__(256, 2) void few_rows_kernel(const WinArgs A) {
         va[kt] = lds_addr(stages[0]) + pi_key(16 * kt + 4 * g + (n16 >> 2)) * kRowB + 256 * w + 8 * (n16 & 3);
     }
     Stretch S;
-    while (next_stretch(A, line, at, S)) {
+    while (next_stretch<kF32>(A, line, at, S)) {
         const Problem P = S.P;
         const int i0 = S.i0, i1 = S.i1;
         bool bad = P.slot < 0;
@@ -1495,7 +1512,7 @@ __global__ __launch_bounds__(256, 2) void few_rows_kernel(const WinArgs A) {
                     for (int kt = 0; kt < 2; ++kt)
                         top = fmaxf(top, fmaxf(fmaxf(acc[rt][kt][0], acc[rt][kt][1]), fmaxf(acc[rt][kt][2], acc[rt][kt][3])));
                     top = xmax_16_32(top);
-                    const bool moves = (top - m[rt]) * kq[rt] > kLazy<kF32>;   // (m is -inf before the first key seen)
+                    const bool moves = (top - m[rt]) * kq[rt] > 15.0f - S.top;   // (m is -inf before the first key seen)
                     if (__any(moves)) {
                         const float f = !moves ? 1.0f : m[rt] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((m[rt] - top) * kq[rt]);
                         if (moves) m[rt] = top;
@@ -1508,7 +1525,7 @@ __global__ __launch_bounds__(256, 2) void few_rows_kernel(const WinArgs A) {
                     for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
-                            const float p = __builtin_amdgcn_exp2f(fmaf(acc[rt][kt][r] - ref, kq[rt], kTop<kF32>));
+                            const float p = __builtin_amdgcn_exp2f(fmaf(acc[rt][kt][r] - ref, kq[rt], S.top));
                             const half_t h = (half_t)p;
                             ph[rt][4 * kt + r] = h;
                             if (kF32) pl[rt][4 * kt + r] = (half_t)(p - (float)h);
@@ -1545,22 +1562,23 @@ __global__ __launch_bounds__(256, 2) void few_rows_kernel(const WinArgs A) {
             const int row = 16 * rt + n16, qi = row >> lh, head = P.head0 + (row & ((1 << lh) - 1));
             if (qi >= P.n) continue;
             if (S.begins && S.ends) {
-                const float inv = m[rt] == -INFINITY ? nan : 1.0f / (l[rt] + sink_term<kF32>(A, head, m[rt], kq[rt])) + nan;
+                const float inv = m[rt] == -INFINITY ? nan : 1.0f / (l[rt] + sink_term(A, head, m[rt], kq[rt], S.top)) + nan;
                 const size_t to = (((size_t)(P.q0 + qi) << A.log_head) + head) * kD;
 #pragma unroll
                 for (int dt = 0; dt < 8; ++dt)
                     store_out<kF32>(A.out, to + dim_of(16 * w + 2 * dt + (g >> 1)) + 4 * (g & 1), o[rt][dt] * inv);
             } else {
+                const float down = ldexpf(1.0f, -(int)S.top);   // (as if it had started at 2^0)
                 if (w == 0 && g == 0) {
                     float *ml = A.part_ml + (size_t)slot * 3 * kRows + row;
                     ml[0] = m[rt];
-                    ml[kRows] = l[rt] + nan;
+                    ml[kRows] = l[rt] * down + nan;
                     ml[2 * kRows] = kq[rt];
                 }
                 float *to = A.part_o + ((size_t)slot * kRows + row) * kD;
 #pragma unroll
                 for (int dt = 0; dt < 8; ++dt)
-                    *reinterpret_cast<float4_t *>(to + dim_of(16 * w + 2 * dt + (g >> 1)) + 4 * (g & 1)) = o[rt][dt];
+                    *reinterpret_cast<float4_t *>(to + dim_of(16 * w + 2 * dt + (g >> 1)) + 4 * (g & 1)) = o[rt][dt] * down;
             }
         }
         lds_barrier();   // bad_s and the stages are free again
@@ -1640,7 +1658,7 @@ __global__ __launch_bounds__(64 * kWaves) void window_merge_kernel(const WinArgs
         }
     }
     // (a part whose rows could not be read has a NaN sum)
-    const float inv = mx == -INFINITY && den == 0.0f ? 0.0f : 1.0f / (den + sink_term<kF32>(A, head, mx, kq));
+    const float inv = mx == -INFINITY && den == 0.0f ? 0.0f : 1.0f / (den + sink_term(A, head, mx, kq, 0.0f));
     const size_t at = (((size_t)(P.q0 + qi) << A.log_head) + head) * kD + 8 * lane;
     store_out<kF32>(A.out, at, o[0] * inv);
     store_out<kF32>(A.out, at + 4, o[1] * inv);

@@ -105,8 +105,10 @@ int ds4hip_kv_pages_compact(const ds4hip_kv_pages *p, int32_t *n_live, void *wor
  * head's sink logit (a term of the denominator with no row). It is 0 where it sees
  * nothing; outputs of queries that no entry names are left as they were.
  * n_head: 8, 16, 32, 64 or 128. io_f32 0: q and out are bf16, and weights are rounded to
- * one f16 (by up to 2^-11 of the weight, or 2^-17 of the largest where that is more); 1:
- * both are fp32, with q and weights as f16 hi + lo halves.
+ * one f16; 1: both are fp32, with q and weights as f16 hi + lo halves. Beside its own rounding and
+ * that of fp32 sums, an output is off by up to 2^-10 (io_f32 1: 2^-21) of the same average of
+ * |V| and by 2^-15 (2^-21) of the largest weight times the largest |V|, over however many rows (up to
+ * 2^23 in bf16, 2^17 in fp32; over more, by as many times more).
  * All arrays are device memory (q, out, codes, tail and workspace 16-byte aligned, sexp
  * 8-byte). The lengths are read on the device, so a captured call follows them. No
  * entry outside the table and no row outside [0, n_cache_rows) is read: queries are NaN
