@@ -1521,16 +1521,21 @@ __global__ __launch_bounds__(256, 2) void few_rows_kernel(const WinArgs A) {
                         for (int dt = 0; dt < 8; ++dt) o[rt][dt] *= f;
                     }
                     const float ref = m[rt] == -INFINITY ? 0.0f : m[rt];
+                    float sum[2];   // a tile's before l's: one rounding to l's size a tile, not eight
 #pragma unroll
-                    for (int kt = 0; kt < 2; ++kt)
+                    for (int kt = 0; kt < 2; ++kt) {
+                        float p[4];
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
-                            const float p = __builtin_amdgcn_exp2f(fmaf(acc[rt][kt][r] - ref, kq[rt], S.top));
-                            const half_t h = (half_t)p;
+                            p[r] = __builtin_amdgcn_exp2f(fmaf(acc[rt][kt][r] - ref, kq[rt], S.top));
+                            const half_t h = (half_t)p[r];
                             ph[rt][4 * kt + r] = h;
-                            if (kF32) pl[rt][4 * kt + r] = (half_t)(p - (float)h);
-                            l[rt] += kF32 ? p : (float)h;   // (of the rounded values: the output stays an average)
+                            if (kF32) pl[rt][4 * kt + r] = (half_t)(p[r] - (float)h);
+                            else p[r] = (float)h;   // (of the rounded values: the output stays an average)
                         }
+                        sum[kt] = (p[0] + p[1]) + (p[2] + p[3]);
+                    }
+                    l[rt] += sum[0] + sum[1];
                 }
                 const uint32_t v0 = va[0] + cur * kStageB, v1 = va[1] + cur * kStageB;
 #pragma unroll

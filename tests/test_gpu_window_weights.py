@@ -126,3 +126,17 @@ def test_a_kept_row_above_a_window(gpu, window, first, heads, typ):
                                     n_first=first, q_start=i32([0, n_q], gpu))
     some = list(range(0, n_q, 211))
     assert check(peak, q[some], out[some], [n - n_q + i for i in some], typ == "fp32", window, first) > 0.1
+
+
+@pytest.mark.parametrize("typ", ["bf16", "fp32"])
+@pytest.mark.parametrize("heads", [16, 64])
+def test_rows_of_one_score(gpu, heads, typ):
+    """All others alike, so that their roundings do not cancel; the share of weights that f16
+    keeps least of, from far above to far below what counts."""
+    from ds4cuda_amd import ops
+    n, n_seqs = 32768, 512 if heads == 16 else 256
+    peak = Peak(gpu, n, 256, 9, noise=0.0)
+    q = peak.queries(n_seqs, heads, typ, 10, 9.0, 19.0)
+    out = ops.flash_attn_window_fp8(q, peak.cache, peak.table[None].repeat(n_seqs, 1), i32([n] * n_seqs, gpu), page_rows=256)
+    some = list(range(0, n_seqs, n_seqs // 16))
+    assert check(peak, q[some], out[some], [n - 1] * len(some), typ == "fp32") > 0.3
