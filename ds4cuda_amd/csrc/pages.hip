@@ -102,6 +102,7 @@ __device__ inline void start(Plan &S, int n_seqs) {
 __device__ inline bool failed(Plan &S, const ds4hip_kv_pages &P) {
     __syncthreads();
     const int f = S.fail;
+    __syncthreads();   // all have read it before a job of the next check fails: all take the same way
     if (f && threadIdx.x == 0) *P.status = f & 1 ? kEINVAL : kENOSPC;
     return f != 0;
 }
