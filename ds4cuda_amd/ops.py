@@ -305,13 +305,22 @@ def _ready(t, dtype, index):
     return t.dtype is dtype and t.get_device() == index and t.is_contiguous()
 
 
+def _int32(v, name):
+    """v as an int argument (ctypes would cut one past 32 bits to another value)."""
+    v = int(v)
+    if not -(1 << 31) <= v < 1 << 31:
+        raise Ds4HipError(f"{name}: {v} does not fit 32 bits", -22)
+    return v
+
+
 def _same_gpu(t, index, name):
     if t.get_device() != index:
         raise Ds4HipError(f"{name}: on {t.device}, the cache is on GPU {index}", -22)
 
 
 def window_workspace_bytes(n_seqs, n_q, n_head) -> int:
-    return lib().ds4hip_flash_attn_window_fp8_workspace_bytes(n_seqs, n_q, n_head)
+    return lib().ds4hip_flash_attn_window_fp8_workspace_bytes(_int32(n_seqs, "n_seqs"), _int32(n_q, "n_q"),
+                                                              _int32(n_head, "n_head"))
 
 
 class _Here:
@@ -364,7 +373,8 @@ class WindowView:
     def __init__(self, cache: Fp8KVCache, page_table, seq_rows, page_rows):
         if page_table.dim() != 2:
             raise Ds4HipError("page_table must be [slots, entries]", -22)
-        slots, stride = page_table.shape
+        slots, stride = (_int32(n, "page_table") for n in page_table.shape)
+        page_rows = _int32(page_rows, "page_rows")
         _check(page_table, torch.int32, None, "page_table")
         _check(seq_rows, torch.int32, slots, "seq_rows")
         _check(cache.codes, torch.uint8, cache.n_rows * N_NOPE, "codes")
@@ -378,12 +388,13 @@ class WindowView:
         self.keep = (cache, page_table, seq_rows)
         self.fixed = dict(codes=cache.codes.data_ptr(), sexp=cache.sexp.data_ptr(), tail=cache.tail.data_ptr(),
                           n_cache_rows=cache.n_rows, table=page_table.data_ptr(), rows=seq_rows.data_ptr(), n_slots=slots,
-                          table_stride=stride, page_rows=int(page_rows))
+                          table_stride=stride, page_rows=page_rows)
 
     def attend(self, q, *, window=0, n_first=0, sinks=None, q_start=None, seq_ids=None, out=None, workspace=None, stream=None):
         if q.dim() != 3 or q.shape[2] != HEAD_DIM or q.dtype not in (torch.bfloat16, torch.float32):
             raise Ds4HipError("q must be bf16 or fp32 [n_q, n_head, 512]", -22)
         n_q, n_head = q.shape[0], q.shape[1]
+        window, n_first = _int32(window, "window"), _int32(n_first, "n_first")
         for t, dtype, n, name in ((q, q.dtype, None, "q"), (sinks, torch.float32, n_head, "sinks"),
                                   (q_start, torch.int32, 1, "q_start"), (seq_ids, torch.int32, None, "seq_ids")):
             if t is not None and (not _ready(t, dtype, self.index) or (n and t.numel() < n)):
@@ -408,7 +419,7 @@ class WindowView:
                 _same_gpu(workspace, self.index, "workspace")
             a = WindowAttn(q=q.data_ptr(), out=out.data_ptr(), io_f32=q.dtype == torch.float32, sinks=_addr(sinks),
                            q_start=_addr(q_start), seq_ids=_addr(seq_ids), n_seqs=n_seqs, n_q=n_q, n_head=n_head,
-                           window=int(window), n_first=int(n_first), **self.fixed)
+                           window=window, n_first=n_first, **self.fixed)
             call("ds4hip_flash_attn_window_fp8", C.byref(a), workspace.data_ptr(),
                  workspace.numel() * workspace.element_size(), _stream(stream))
         return out

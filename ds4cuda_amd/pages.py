@@ -13,7 +13,8 @@ import ctypes as C
 import torch
 
 from ._lib import Ds4HipError, call, lib
-from .ops import HEAD_DIM, N_NOPE, N_ROT, Fp8KVCache, WindowView, _addr, _check, _on_stream, _ptr, _ready, _same_gpu, _stream
+from .ops import (HEAD_DIM, N_NOPE, N_ROT, Fp8KVCache, WindowView, _addr, _check, _int32, _on_stream, _ptr, _ready, _same_gpu,
+                  _stream)
 
 MAX_JOBS = 1024    # sequences of one call
 
@@ -57,6 +58,9 @@ class PagePool:
         self.refs, self.table, self.rows = refs, table, rows
         self.page_rows, self.n_layers, self.n_pages, self.n_seqs = int(page_rows), layers, n_pages, table.shape[0]
         self.device, self.index = codes.device, codes.device.index
+        for n, name in ((layers, "codes"), (n_pages, "refs"), (self.page_rows, "page_rows"), (table.shape[1], "table"),
+                        (self.n_seqs, "table")):
+            _int32(n, name)
         self.c = KvPages(_ptr(codes), _ptr(sexp), _ptr(tail), n_rows, layers, n_pages, self.page_rows, table.shape[1],
                          self.n_seqs, _ptr(refs), _ptr(table), _ptr(rows), _ptr(self.status))
         self._c = C.byref(self.c)
@@ -123,23 +127,24 @@ class PagePool:
         (-1 past the last job's rows, or everywhere where the call is refused)."""
         n = self._jobs(seqs, "seqs")
         self._jobs(n_new, "n_new", n)
+        n_dst = _int32(n_dst, "n_dst")
         if dst_rows is None:
             dst_rows = self._empty(n_dst, torch.int64, stream)
         else:
             _check(dst_rows, torch.int64, n_dst, "dst_rows")
             _same_gpu(dst_rows, self.index, "dst_rows")
-        self._call("ds4hip_kv_pages_extend", stream, _addr(seqs), _addr(n_new), n, dst_rows.data_ptr(), int(n_dst))
+        self._call("ds4hip_kv_pages_extend", stream, _addr(seqs), _addr(n_new), n, dst_rows.data_ptr(), n_dst)
         return dst_rows
 
     def append(self, kv, dst_rows, layer=0, stream=None):
         """Quantizes fp32 rows kv [n, 512] into the layer at dst_rows (extend's); a row
         whose place is -1 is skipped."""
-        n = kv.shape[0]
+        n, layer = _int32(kv.shape[0], "kv"), _int32(layer, "layer")
         _check(kv, torch.float32, n * HEAD_DIM, "kv")
         _check(dst_rows, torch.int64, n, "dst_rows")
         _same_gpu(kv, self.index, "kv")
         _same_gpu(dst_rows, self.index, "dst_rows")
-        self._call("ds4hip_kv_pages_append", stream, int(layer), kv.data_ptr(), n, dst_rows.data_ptr())
+        self._call("ds4hip_kv_pages_append", stream, layer, kv.data_ptr(), n, dst_rows.data_ptr())
 
     def fork(self, parents, children, n_rows=None, deep=False, stream=None):
         """children[j] (empty sequences) become copies of the first n_rows[j] rows (None
