@@ -104,6 +104,8 @@ class PagePool:
         k = ids.numel()
         if n is not None and k != n:
             raise Ds4HipError(f"{name}: {n} entries expected, got {k}", -22)
+        if k > MAX_JOBS:
+            raise Ds4HipError(f"{name}: a call takes {MAX_JOBS} sequences at most, got {k}", -22)
         return k
 
     def _call(self, name, stream, *args):

@@ -39,3 +39,17 @@ def test_one_bad_table_among_many_jobs(gpu, n):
     pool.free(kids)
     pool.check()
     assert not pool.refs.any() and not pool.rows.any()
+
+
+def test_more_jobs_than_a_call_takes(gpu):
+    from ds4cuda_amd import Ds4HipError, pages
+    n = pages.MAX_JOBS + 1
+    pool = pages.PagePool.empty(8, 4, 2 * n, 40, 1, gpu)
+    seqs, kids = i32(range(n), gpu), i32(range(n - 1, 2 * n - 1), gpu)
+    for call in (lambda: pool.extend(seqs, seqs, 4), lambda: pool.fork(seqs, kids), lambda: pool.free(seqs)):
+        with pytest.raises(Ds4HipError, match="1024 sequences at most") as e:
+            call()
+        assert e.value.code == -22
+    pool.check()
+    pool.free(seqs[:-1])
+    pool.check()
