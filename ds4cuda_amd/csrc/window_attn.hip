@@ -1244,7 +1244,7 @@ __global__ __launch_bounds__(512, 2) void roles_kernel(const WinArgs A) {
             const int n_rt = ((P.n << lh) + 15) >> 4;   // row tiles in use
             F.bad = P.slot < 0;
             Ring G;
-        float4_t o[kRT][kDT];
+            float4_t o[kRT][kDT];
 #pragma unroll
             for (int a = 0; a < kRT; ++a)
 #pragma unroll

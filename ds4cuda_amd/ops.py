@@ -359,7 +359,8 @@ def flash_attn_window_fp8(q, cache: Fp8KVCache, page_table, seq_rows, *, page_ro
     q_start[s + 1] - 1 (int32 [entries + 1]), or one query each where q_start is
     None. The query at position p sees row k where k <= p and (window == 0 or k >
     p - window or k < n_first); sinks [n_head] fp32: a sink logit per head.
-    All lengths are read on the device: a captured call follows them.
+    All lengths are read on the device: a captured call follows them. Queries that no
+    entry names keep what out held: without out, whatever the new tensor's memory did.
     """
     view = WindowView(cache, page_table, seq_rows, page_rows)
     return view.attend(q, window=window, n_first=n_first, sinks=sinks, q_start=q_start, seq_ids=seq_ids, out=out,

@@ -179,7 +179,8 @@ class PagePool:
     def attend(self, q, *, seqs=None, q_start=None, window=0, n_first=0, sinks=None, layer=0, out=None, workspace=None,
                stream=None):
         """ops.flash_attn_window_fp8 over this pool's pages of one layer: the sequences
-        seqs (None: slots 0, 1, ..)."""
+        seqs (None: slots 0, 1, ..). Queries that q_start names for none of them are left
+        as they were in out, and undefined without out."""
         view = self._views.get(layer)
         if view is None:
             view = self._views[layer] = WindowView(self.layer(layer), self.table, self.rows, self.page_rows)

@@ -114,7 +114,8 @@ int ds4hip_kv_pages_compact(const ds4hip_kv_pages *p, int32_t *n_live, void *wor
  * entry outside the table and no row outside [0, n_cache_rows) is read: queries are NaN
  * where their sequence is outside the table, has more rows than its table row holds (or
  * than 2^31 - 256), or where a group of 32 rows from a multiple of 32 on in which they
- * see one names such a row (with them, up to 63 queries next to them in their sequence).
+ * see one names such a row (with them, up to 64 / n_head - 1 queries next to them in their
+ * sequence: 7 of 8 heads, none of 64 or more).
  * A row that is not finite reaches only the queries that see it. */
 typedef struct ds4hip_window_attn {
     const void *q;

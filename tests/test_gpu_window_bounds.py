@@ -51,3 +51,34 @@ def test_starts_outside_the_batch(gpu, n_q, rows, start, window, heads, typ):
     assert (out[rest] == 7.0).all()
     if sum(max(b - a, 0) for a, b in zip(clamped, clamped[1:])) == len(named):   # (no two entries name one query)
         assert torch.isfinite(out).all() and all(bool((out[i] != 7.0).any()) for i in named)
+
+
+@pytest.mark.parametrize("typ", ["bf16", "fp32"])
+@pytest.mark.parametrize("heads", [8, 16, 64, 128])
+@pytest.mark.parametrize("n,window,first,bad", [(400, 40, 3, 5), (400, 0, 0, 9), (700, 600, 0, 2), (400, 40, 70, 1), (2000, 100, 0, 40)])
+def test_a_bad_entry_reaches_few_neighbours(gpu, n, window, first, bad, heads, typ):
+    """NaN where a query sees a row of the 32 that the entry stands for, with up to 64 / heads - 1 queries
+    next to it; all others as without it."""
+    from ds4cuda_amd import ops
+    page = 32
+    per = -(-n // page)
+    cache = ops.Fp8KVCache(*quantized_rows(per * page, 2, gpu))
+    table = torch.arange(per, dtype=torch.int32, device=gpu)[None]
+    dtype = {"bf16": torch.bfloat16, "fp32": torch.float32}[typ]
+    n_q = n // 2
+    q = torch.randn((n_q, heads, 512), device=gpu).to(dtype)
+    call = lambda: ops.flash_attn_window_fp8(q, cache, table, i32([n], gpu), page_rows=page, window=window, n_first=first,
+                                             q_start=i32([0, n_q], gpu))
+    want = call()
+    table[0, bad] = per
+    got = call()
+    lost = torch.isnan(got).flatten(1)
+    hit = [any(k <= p and (window == 0 or k > p - window or k < first) for k in range(page * bad, page * bad + page))
+           for p in range(n - n_q, n)]
+    near = max(64 // heads - 1, 0)
+    assert torch.isfinite(want).all() and any(hit)
+    for i in range(n_q):
+        if hit[i]:
+            assert lost[i].all(), i
+        elif not any(hit[max(0, i - near):i + near + 1]):
+            assert not lost[i].any() and torch.equal(got[i], want[i]), i
