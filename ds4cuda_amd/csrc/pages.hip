@@ -9,9 +9,9 @@
 // plan's list: 584 bytes a row and layer, read and written once.
 //
 // What bounds them. A plan is a chain of loads that wait for each other (jobs, rows, table
-// entries, counts) and of barriers: 3.9 us to extend 6 sequences, 8.0 to fork 6, 3.2 to free
-// them, 7.2 to compact a pool of 352 pages. The moves run at memory speed: deep copies of four
-// sequences of 7001 rows in 43 layers (647 MB read and written) 139 us, 4.7 TB/s of the 5.1 that
+// entries, counts) and of barriers: 4.0 us to extend 6 sequences, 8.2 to fork 6, 3.4 to free
+// them, 7.4 to compact a pool of 352 pages. The moves run at memory speed: deep copies of four
+// sequences of 7001 rows in 43 layers (647 MB read and written) 140 us, 4.6 TB/s of the 5.1 that
 // a large copy reaches.
 
 #include "ds4hip_common.h"

@@ -16,9 +16,10 @@
 // kernel does.
 //
 // What bounds it. In a tile of 64 rows the matrix instructions (0.4 us at peak, 0.9 at a
-// library product's rate), 150 or 228 KB through LDS (0.5, 0.7) and the weights take turns: 1.4 us, 1.8
-// over a long prompt; lists that come from memory wait for it too (1.9). Calls of a few tiles
-// are launch, the queries, the first rows and the outputs one after the other (about 20 us).
+// library product's rate), 150 or 228 KB through LDS (0.5, 0.7) and the weights take turns: 1.4 us, 1.9
+// over a long prompt whose references move, where counters have the matrix units busy for 22% of the cycles and
+// the LDS for 23% (8% of those bank conflicts); lists that come from memory wait for it too (2.0: 14%, 15%). Calls
+// of a few tiles are launch, the queries, the first rows and the outputs one after the other (about 20 us).
 // (A workgroup's place on the line by XCD, so that neighbours share an L2, changed nothing:
 // the rows come from there already.)
 
@@ -50,7 +51,7 @@ constexpr int kFewProbs = 512, kFewProbs16 = 128;   // problems of 64, 16 rows t
 // a stretch (the parts of a cut problem have references of their own): with one f16 they are off by
 // 2^-16 of the largest together, with hi + lo by 2^-22 (up to 2^18, 2^12 tiles, where it stays at 2^14).
 // Moving costs up to half a tile: 4096 queries over windows of 1024 rows, 1% of them eight times as large, took
-// 1020 us from 2^-8 on, 1090 from the 2^2 that their 34 tiles ask for; 16 tokens of up to 32768 rows 67 and 70.5.
+// 1017 us from 2^-8 on, 1083 from the 2^2 that their 34 tiles ask for; 16 tokens of up to 32768 rows 67 and 69.5.
 template <bool kF32>
 __device__ inline float start_of(int tiles) {
     const int log_up = 32 - __clz(tiles - 1);   // (of one tile: 0)
@@ -1026,10 +1027,11 @@ struct Ring {
 // roles pass the same barriers: one a tile, two more where a tile is marked, which both read
 // from the same words.
 //
-// Measured. 4096 queries of 64 heads over windows of 1024 rows (584 GFLOP): 1.02 ms, 0.57 PFLOP/s,
-// half of a library f16 product's 1.1 here. 16 single tokens of 64 heads over 105 MB of rows: 60
-// us, 1.75 TB/s of the 5.1 that a copy reaches: a tile's chain (wait for its rows, to f16,
-// scores, weights, outputs, one barrier) bounds it, 1.9 us where memory alone would take 0.9.
+// Measured. 4096 queries of 64 heads over windows of 1024 rows (584 GFLOP): 1.08 ms, 0.54 PFLOP/s,
+// half of a library f16 product's 1.1 here. 4096 queries over 32768 rows and their own (18.7 TFLOP):
+// 22.7 ms, 0.82 PFLOP/s. 16 single tokens of 64 heads over 105 MB of rows: 63
+// us, 1.7 TB/s of the 5.1 that a copy reaches: a tile's chain (wait for its rows, to f16,
+// scores, weights, outputs, one barrier) bounds it, 2 us where memory alone would take 0.9.
 template <bool kInline>
 __global__ __launch_bounds__(512, 2) void roles_kernel(const WinArgs A) {
     constexpr int kRT = 4, kRows = 16 * kRT, kDT = 8;
@@ -1783,9 +1785,9 @@ extern "C" int ds4hip_flash_attn_window_fp8(const ds4hip_window_attn *a, void *w
     const long long held = (long long)a->table_stride << shift;
     const long long span = std::min<long long>(held, (long long)a->window + ((1 << log_rows) >> std::min(lh, log_rows)));
     const long long most = a->window > 0 ? span / kTile + 2 + (std::min<long long>(a->n_first, held) + kTile - 1) / kTile : held / kTile + 1;
-    // Waves with roles for long problems of bf16 (us, with roles and without: problems of 34 tiles 1045, 1116,
-    // 16 sequences of up to 32768 rows 60, 63; problems of 6 tiles 173, 165; one token over 4000 rows, in
-    // parts of 4 tiles, 24.4, 23.5)
+    // Waves with roles for long problems of bf16 (us a call, with roles and without: problems of 34 tiles 1083, 1122,
+    // of 1025 to 1152 22700, 24800, 16 sequences of up to 32768 rows 69.5, 72; problems of 6 tiles 176, 166; one
+    // token over 4000 rows, in parts of 4 tiles, 30.5, 29.1)
     auto *main = log_rows == 4 ? f32 ? in ? few_rows_kernel<true, true> : few_rows_kernel<true, false>
                                      : in ? few_rows_kernel<false, true> : few_rows_kernel<false, false>
                  : f32         ? in ? window_kernel<true, true> : window_kernel<true, false>
