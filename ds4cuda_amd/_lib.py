@@ -112,6 +112,11 @@ SIGNATURES: dict[str, list] = {
     "ds4hip_kv_pages_fork": [_vp, _vp, _vp, _vp, _i, _i, _vp, _sz, _vp],
     "ds4hip_kv_pages_free": [_vp, _vp, _vp, _i, _vp],
     "ds4hip_kv_pages_compact": [_vp, _vp, _vp, _sz, _vp],
+    "ds4hip_kv_pages_keep": [_vp, _vp, _vp, _i, _vp, _i, _vp, _vp, _sz, _vp],
+    "ds4hip_kv_pages_accept": [_vp, _vp, _vp, _i, _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _sz, _vp],
+    "ds4hip_flash_attn_tree_fp8": [_vp, _vp, _vp, _sz, _vp],
+    "ds4hip_sample_workspace_bytes": [_i, _i],
+    "ds4hip_sample_tokens": [_vp, _vp, _sz, _vp],
     "ds4hip_flash_attn_window_fp8_workspace_bytes": [_i, _i, _i],
     "ds4hip_flash_attn_window_fp8": [_vp, _vp, _sz, _vp],
     "ds4hip_ds4cudak_probe": [C.c_char_p, _vp],
@@ -126,6 +131,7 @@ RESTYPES = {"ds4hip_indexer_select_scratch_bytes": C.c_size_t,
             "ds4hip_session_state_arena_bytes": C.c_size_t,
             "ds4hip_kv_pages_workspace_bytes": C.c_size_t,
             "ds4hip_flash_attn_window_fp8_workspace_bytes": C.c_size_t,
+            "ds4hip_sample_workspace_bytes": C.c_size_t,
             "ds4hip_session_chunk_step_workspace_bytes": C.c_size_t,
             "ds4hip_mul_mm_workspace_bytes": C.c_size_t,
             "ds4hip_compressor_batch_scratch_bytes": C.c_size_t,

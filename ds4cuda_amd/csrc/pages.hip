@@ -37,13 +37,15 @@ struct Moves {
     int *n_live;   // held pages (compact)
     int *src, *dst, *count;   // [n_pages] pages, and the rows of each
     int *now;      // [n_pages] where a page went (compact)
+    int *base;     // [kJobs] a sequence's rows before its drafts (keep)
 };
 
-size_t moves_bytes(int n_pages) { return sizeof(int) * (64 + 4 * (size_t)n_pages); }
+size_t moves_bytes(int n_pages) { return sizeof(int) * (64 + 4 * (size_t)n_pages + kJobs); }
 
 Moves moves_at(void *ws, int n_pages) {
     int *p = static_cast<int *>(ws);
-    return {p, p + 1, p + 64, p + 64 + (size_t)n_pages, p + 64 + 2 * (size_t)n_pages, p + 64 + 3 * (size_t)n_pages};
+    return {p, p + 1, p + 64, p + 64 + (size_t)n_pages, p + 64 + 2 * (size_t)n_pages, p + 64 + 3 * (size_t)n_pages,
+            p + 64 + 4 * (size_t)n_pages};
 }
 
 struct Plan {
@@ -463,6 +465,186 @@ __global__ __launch_bounds__(256) void move_kernel(const ds4hip_kv_pages P, cons
     }
 }
 
+// ---- drafted trees ---------------------------------------------------------------
+
+constexpr int kNodes = DS4HIP_TREE_MAX_NODES;
+
+// One wave a tree: from node 0 to the first child whose token is its parent's target, and so on. The tree lies
+// in LDS; a step is a look at 64 nodes at a time behind the last one (children follow their parents).
+__global__ __launch_bounds__(64) void walk_kernel(const int32_t *q_start, int n_jobs, const int32_t *parents, const int32_t *tokens,
+                                                  const int32_t *targets, int n_nodes, int32_t *path, int32_t *n_path,
+                                                  int32_t *next) {
+    __shared__ int parent_s[kNodes], token_s[kNodes], target_s[kNodes];
+    const int j = blockIdx.x, lane = threadIdx.x;
+    const int a = q_start[j], b = q_start[j + 1], n = b - a;
+    // nodes that no job names
+    if (j == 0)
+        for (int i = lane; i < min(a, n_nodes); i += 64) path[i] = -1;
+    if (j == n_jobs - 1)
+        for (int i = max(b, 0) + lane; i < n_nodes; i += 64) path[i] = -1;
+    if (a < 0 || b > n_nodes || n <= 0 || n > kNodes) {   // (the plan refuses what is not 0 nodes)
+        if (lane == 0) n_path[j] = 0, next[j] = -1;
+        return;
+    }
+    for (int i = lane; i < n; i += 64) {
+        parent_s[i] = parents[a + i];
+        token_s[i] = tokens[a + i];
+        target_s[i] = targets[a + i];
+    }
+    __syncthreads();
+    int at = 0, length = 0, says;
+    while (true) {
+        if (lane == 0) path[a + length] = at;
+        ++length;
+        says = target_s[at];
+        int child = -1;
+        for (int c0 = at + 1; says >= 0 && c0 < n; c0 += 64) {
+            const int c = c0 + lane;
+            const uint64_t fits = __ballot(c < n && parent_s[min(c, n - 1)] == at && token_s[min(c, n - 1)] == says);
+            if (fits) {
+                child = c0 + __builtin_ctzll(fits);
+                break;
+            }
+        }
+        if (child < 0) break;
+        at = child;
+    }
+    for (int i = length + lane; i < n; i += 64) path[a + i] = -1;
+    if (lane == 0) {
+        n_path[j] = length;
+        next[j] = says;
+    }
+}
+
+// Checks the jobs' paths, cuts their sequences and releases the pages behind them. kAccept: a refused call
+// takes back what the walk wrote.
+template <bool kAccept>
+__global__ __launch_bounds__(kThreads) void keep_kernel(const ds4hip_kv_pages P, const int32_t *seqs, const int32_t *q_start,
+                                                        int n_jobs, int n_nodes, int32_t *path, int32_t *n_path, int32_t *next,
+                                                        const Moves M) {
+    __shared__ Plan S;
+    __shared__ int kept_s[kJobs], nodes_s[kJobs];
+    const int tid = threadIdx.x, shift = __builtin_ctz(P.page_rows);
+    start(S, P.n_seqs);
+    int seq = -1, base = -1, n = 0, kept = 0, held_pages = 0;
+    if (tid < n_jobs) {
+        const int a = q_start[tid], b = q_start[tid + 1];
+        seq = seqs[tid];
+        kept = n_path[tid];
+        const long long count = (long long)b - a;
+        if (a < 0 || count < 0 || b > n_nodes || seq < 0 || seq >= P.n_seqs || !first_named(S, seq) || kept < 0 || kept > count ||
+            count > P.rows[seq] || (kAccept && count > kNodes) || pages_of(P, P.rows[seq]) > P.table_stride) {
+            fail(S, kEINVAL);
+        } else {
+            n = (int)count;
+            base = P.rows[seq] - n;
+            if (n > 0) held_pages = pages_of(P, P.rows[seq]) - (base >> shift);
+        }
+        S.at[tid] = seq;
+        nodes_s[tid] = a;
+        kept_s[tid] = kept;
+    }
+    scan_jobs(S, held_pages, S.base, n_jobs);   // pages with drafts in them
+    scan_jobs(S, n > 0 ? kept : 0, S.more, n_jobs);
+    if (failed(S, P)) {
+        if (kAccept) goto refuse;
+        if (tid == 0) *M.n = 0;
+        return;
+    }
+    {
+        const int pages = S.base[n_jobs], rows = S.more[n_jobs];
+        // this sequence's alone: its rows move, or are cut
+        for (int i = tid; i < pages; i += kThreads) {
+            const int j = job_of(S.base, n_jobs, i), s = S.at[j];
+            const int page = *entry(P, s, pages_of(P, P.rows[s]) - (S.base[j + 1] - i));
+            if (!held(P, page) || P.refs[page] != 1) fail(S, kEINVAL);
+        }
+        if (!kAccept)
+            for (int i = tid; i < rows; i += kThreads) {   // nodes in order
+                const int j = job_of(S.more, n_jobs, i), k = i - S.more[j];
+                const int v = path[nodes_s[j] + k], before = k ? path[nodes_s[j] + k - 1] : -1;
+                if (v <= before || v >= q_start[j + 1] - nodes_s[j]) fail(S, kEINVAL);
+            }
+        if (failed(S, P)) {
+            if (kAccept) goto refuse;
+            if (tid == 0) *M.n = 0;
+            return;
+        }
+        for (int i = tid; i < pages; i += kThreads) {
+            const int j = job_of(S.base, n_jobs, i), s = S.at[j];
+            const int had = pages_of(P, P.rows[s]), k = had - (S.base[j + 1] - i);
+            // (its rows are still those before the call)
+            const int now = P.rows[s] - (q_start[j + 1] - nodes_s[j]) + kept_s[j];
+            if (k >= pages_of(P, now)) P.refs[*entry(P, s, k)] = 0;
+        }
+        __syncthreads();
+        if (tid < n_jobs) {
+            P.rows[seq] = base + kept;
+            M.base[tid] = base;
+        }
+        if (tid == 0) *M.n = n_jobs;
+        return;
+    }
+refuse:
+    if (tid == 0) *M.n = 0;
+    for (int i = tid; i < n_nodes; i += kThreads) path[i] = -1;
+    if (tid < n_jobs) n_path[tid] = 0, next[tid] = -1;
+}
+
+// The paths' rows, a workgroup a job and layer: row path[i] of the drafts becomes row i, 64 at a time in order
+// (path[i] >= i: a row that is read later lies behind those already written), every load before the first store.
+__global__ __launch_bounds__(256) void keep_rows_kernel(const ds4hip_kv_pages P, const int32_t *seqs, const int32_t *q_start,
+                                                        const int32_t *path, const int32_t *n_path, const Moves M) {
+    constexpr int kRows = 64;
+    __shared__ long long from_s[kRows], to_s[kRows];
+    const int tid = threadIdx.x, n_jobs = *M.n, shift = __builtin_ctz(P.page_rows);   // (0 jobs: refused)
+    for (long long unit = blockIdx.x; unit < (long long)n_jobs * P.n_layers; unit += gridDim.x) {
+        const int j = (int)(unit / P.n_layers), kept = n_path[j], seq = seqs[j], base = M.base[j], a = q_start[j];
+        const long long first = (unit - (long long)j * P.n_layers) * P.layer_rows;
+        for (int i0 = 0; i0 < kept; i0 += kRows) {
+            const int rows = min(kRows, kept - i0);
+            __syncthreads();   // (the places before are read)
+            bool moves = false;
+            if (tid < rows) {
+                const int f = base + path[a + i0 + tid], t = base + i0 + tid;
+                moves = f != t;
+                from_s[tid] = first + ((long long)*entry(P, seq, f >> shift) << shift) + (f & (P.page_rows - 1));
+                to_s[tid] = first + ((long long)*entry(P, seq, t >> shift) << shift) + (t & (P.page_rows - 1));
+            }
+            if (!__syncthreads_or(moves)) continue;
+            constexpr int kUnits = 36, kEach = kRows * kUnits / 256;   // 16 bytes each: 28 of codes, 8 of the tail
+            uint4_t v[kEach];
+            uint2_t e = {0, 0};
+#pragma unroll
+            for (int u = 0; u < kEach; ++u) {
+                const int i = tid + 256 * u, row = i / kUnits, k = i - row * kUnits;
+                if (row < rows)
+                    v[u] = k < 28 ? reinterpret_cast<const uint4_t *>(P.codes + from_s[row] * kCodes)[k]
+                                  : reinterpret_cast<const uint4_t *>(P.tail + from_s[row] * kRotD)[k - 28];
+            }
+            if (tid < rows) e = *reinterpret_cast<const uint2_t *>(P.sexp + from_s[tid] * 8);
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // no other wave's store overtakes a load
+            __syncthreads();
+#pragma unroll
+            for (int u = 0; u < kEach; ++u) {
+                const int i = tid + 256 * u, row = i / kUnits, k = i - row * kUnits;
+                if (row < rows) {
+                    if (k < 28)
+                        reinterpret_cast<uint4_t *>(P.codes + to_s[row] * kCodes)[k] = v[u];
+                    else
+                        reinterpret_cast<uint4_t *>(P.tail + to_s[row] * kRotD)[k - 28] = v[u];
+                }
+            }
+            if (tid < rows) *reinterpret_cast<uint2_t *>(P.sexp + to_s[tid] * 8) = e;
+        }
+    }
+}
+
+// Workgroups for n jobs' rows: whole rounds of the chip at most.
+unsigned keep_grid(const ds4hip_kv_pages *p, int n_jobs) {
+    return (unsigned)std::min<long long>((long long)n_jobs * p->n_layers, 256 * 16);
+}
+
 bool aligned(const void *p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
 bool pool_ok(const ds4hip_kv_pages *p) {
@@ -543,5 +725,42 @@ extern "C" int ds4hip_kv_pages_compact(const ds4hip_kv_pages *p, int32_t *n_live
     const hipStream_t st = (hipStream_t)stream;
     hipLaunchKernelGGL(compact_kernel, dim3(1), dim3(kThreads), 0, st, *p, M, n_live);
     hipLaunchKernelGGL(move_kernel<true>, dim3(256 * 8), dim3(256), 0, st, *p, M);
+    return ds4hip_set_last_error(hip_status(hipGetLastError()));
+}
+
+extern "C" int ds4hip_kv_pages_keep(const ds4hip_kv_pages *p, const int32_t *seqs, const int32_t *q_start, int n_jobs,
+                                    const int32_t *path, int n_nodes, const int32_t *n_path, void *workspace,
+                                    size_t workspace_bytes, void *stream) {
+    if (!pool_ok(p) || n_jobs < 0 || n_jobs > kJobs || n_nodes < 0 || n_nodes > (1 << 24) ||
+        (n_jobs && (!seqs || !q_start || !n_path || (n_nodes && !path) || !workspace || !aligned(workspace, 8) ||
+                    workspace_bytes < moves_bytes(p->n_pages))))
+        return ds4hip_set_last_error(kEINVAL);
+    if (n_jobs == 0) return 0;
+    const Moves M = moves_at(workspace, p->n_pages);
+    const hipStream_t st = (hipStream_t)stream;
+    // (only read)
+    int32_t *nodes = const_cast<int32_t *>(path), *counts = const_cast<int32_t *>(n_path);
+    hipLaunchKernelGGL(keep_kernel<false>, dim3(1), dim3(kThreads), 0, st, *p, seqs, q_start, n_jobs, n_nodes, nodes, counts,
+                       nullptr, M);
+    hipLaunchKernelGGL(keep_rows_kernel, dim3(keep_grid(p, n_jobs)), dim3(256), 0, st, *p, seqs, q_start, path, n_path, M);
+    return ds4hip_set_last_error(hip_status(hipGetLastError()));
+}
+
+extern "C" int ds4hip_kv_pages_accept(const ds4hip_kv_pages *p, const int32_t *seqs, const int32_t *q_start, int n_jobs,
+                                      const int32_t *parents, const int32_t *tokens, const int32_t *targets, int n_nodes,
+                                      int32_t *path, int32_t *n_path, int32_t *next, void *workspace, size_t workspace_bytes,
+                                      void *stream) {
+    if (!pool_ok(p) || n_jobs < 0 || n_jobs > kJobs || n_nodes < 0 || n_nodes > (1 << 24) ||
+        (n_jobs && (!seqs || !q_start || !n_path || !next || (n_nodes && (!parents || !tokens || !targets || !path)) ||
+                    !workspace || !aligned(workspace, 8) || workspace_bytes < moves_bytes(p->n_pages))))
+        return ds4hip_set_last_error(kEINVAL);
+    if (n_jobs == 0) return 0;
+    const Moves M = moves_at(workspace, p->n_pages);
+    const hipStream_t st = (hipStream_t)stream;
+    hipLaunchKernelGGL(walk_kernel, dim3(n_jobs), dim3(64), 0, st, q_start, n_jobs, parents, tokens, targets, n_nodes, path,
+                       n_path, next);
+    hipLaunchKernelGGL(keep_kernel<true>, dim3(1), dim3(kThreads), 0, st, *p, seqs, q_start, n_jobs, n_nodes, path, n_path, next,
+                       M);
+    hipLaunchKernelGGL(keep_rows_kernel, dim3(keep_grid(p, n_jobs)), dim3(256), 0, st, *p, seqs, q_start, path, n_path, M);
     return ds4hip_set_last_error(hip_status(hipGetLastError()));
 }

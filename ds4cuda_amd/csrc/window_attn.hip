@@ -42,6 +42,7 @@ constexpr int kSecond = 4;           // tiles whose time a workgroup's second pr
 constexpr int kMaxSeqs = 4096;
 constexpr int kMaxRows = 0x7FFFFF00; // rows of a sequence: a tile's keys stay in 32 bits
 constexpr int kFewProbs = 512, kFewProbs16 = 128;   // problems of 64, 16 rows that a workgroup lays out itself
+constexpr int kMaxNodes = DS4HIP_TREE_MAX_NODES;     // drafted nodes of a tree
 // P = 2^((s - m) kq + top) with s and the row's reference m as the matrix
 // instructions leave them and kq its scale to log2: their difference is exact where P is
 // large, at any magnitude. The reference moves only where P would pass 2^15 (f16 ends at
@@ -67,6 +68,7 @@ struct WinArgs {
     const int8_t *sexp;
     const uint16_t *tail;
     const int32_t *table, *rows, *q_start, *seq_ids;
+    const int32_t *parents;  // of the queries' nodes (trees)
     int n_seqs, n_slots, n_q, log_head, window, first, stride, shift, n_pages;
     int log_rows;            // a problem has 2^log_rows rows (queries x heads)
     int n_wg;                // workgroups that the line is cut for
@@ -95,15 +97,20 @@ __device__ inline int log_hpt(const WinArgs &A) { return min(A.log_head, A.log_r
 
 // Problem `tile` of sequence s as the plan keeps it: its table row (-1: not a sequence of
 // the table, or one with more rows than its table row holds), first packed query, number of
-// queries and first head (times 256), position of its first query.
+// queries, first head (times 256) and, of a tree, first node (times 65536; also -1: more nodes than
+// a tree may have, or than the sequence has rows), position (of a tree: row) of its first query.
+template <bool kTree>
 __device__ inline int4 record_of(const WinArgs &A, int s, int tile) {
     const int lh = log_hpt(A), lg = A.log_head - lh, qpt = (1 << A.log_rows) >> lh;
     const int2 qs = queries_of(A, s);
     const int q = (tile >> lg) * qpt, slot = A.seq_ids ? A.seq_ids[s] : s;
     const bool in = slot >= 0 && slot < A.n_slots;
     const int rows = in ? max(A.rows[slot], 0) : 0;
-    return make_int4(in && rows <= kMaxRows && ((rows - 1) >> A.shift) < A.stride ? slot : -1, qs.x + q,
-                     min(qpt, qs.y - q) | ((tile & ((1 << lg) - 1)) << lh) << 8, rows - qs.y + q);
+    const bool fits = in && rows <= kMaxRows && ((rows - 1) >> A.shift) < A.stride &&
+                      (!kTree || (qs.y <= kMaxNodes && qs.y <= rows));
+    return make_int4(fits ? slot : -1, qs.x + q,
+                     min(qpt, qs.y - q) | ((tile & ((1 << lg) - 1)) << lh) << 8 | (kTree && fits ? q << 16 : 0),
+                     rows - qs.y + q);
 }
 
 struct Problem {
@@ -113,30 +120,36 @@ struct Problem {
     int pos0, pos1; // positions of the first and the last query; pos1 < 0: it sees nothing
     int n_first, t_window, tiles;   // tiles of the first rows, first tile of the window, all tiles
     int whole_a, whole_b, whole_c;  // tiles t < a, or b <= t, of those t < c, are seen whole by every query
+    int node0, base;   // of a tree: the first query's node, the rows before the tree's
 };
 
+// A tree's node sees rows before the tree's from its position on backwards, which is base at least and
+// no more than its own row's place; rows of the tree as its ancestors are (so no tile of them is whole).
+template <bool kTree>
 __device__ inline Problem problem_of(const WinArgs &A, int4 rec) {
     Problem P;
     P.slot = rec.x;
     P.q0 = rec.y;
     P.n = rec.z & 255;
-    P.head0 = rec.z >> 8;
+    P.head0 = rec.z >> 8 & 255;
+    P.node0 = kTree ? rec.z >> 16 : 0;
     P.pos0 = rec.w;
     P.pos1 = P.pos0 + P.n - 1;
+    P.base = P.pos0 - P.node0;
     P.n_first = P.t_window = P.whole_a = P.whole_b = P.whole_c = 0;
     if (P.slot < 0 || P.pos1 < 0) {   // one tile that sees nothing
         P.pos1 = -1;
         P.tiles = 1;
         return P;
     }
-    const int lo = A.window > 0 ? max(0, max(P.pos0, 0) - A.window + 1) : 0;
+    const int lo = A.window > 0 ? max(0, max(kTree ? P.base : P.pos0, 0) - A.window + 1) : 0;
     P.n_first = (min(A.first, lo) + kTile - 1) / kTile;
     P.t_window = lo / kTile;
     if (P.n_first >= P.t_window) P.n_first = P.t_window = 0;   // they meet: one run of tiles from row 0
     P.tiles = P.n_first + P.pos1 / kTile - P.t_window + 1;
     P.whole_a = A.first / kTile;
     P.whole_b = A.window > 0 && P.pos1 >= A.window ? (P.pos1 - A.window) / kTile + 1 : 0;
-    P.whole_c = max(P.pos0 + 1, 0) / kTile;
+    P.whole_c = kTree ? P.base / kTile : max(P.pos0 + 1, 0) / kTile;
     return P;
 }
 
@@ -146,6 +159,80 @@ __device__ inline int tile_at(const Problem &P, int i) { return i < P.n_first ? 
 __device__ inline bool sees(const WinArgs &A, int pos, int key) {
     return key <= pos && (A.window <= 0 || key > pos - A.window || key < A.first);
 }
+
+// ---- trees -----------------------------------------------------------------------
+
+// What the queries of a problem see of their tree: each one's position (the rows before the tree's
+// and its depth), and a bit for each node that is its own or an ancestor's and lies in the window or
+// among the first rows.
+template <bool kTree, int kRows>
+struct Tree {};
+template <int kRows>
+struct Tree<true, kRows> {
+    static constexpr int kWords = kMaxNodes / 32 + 2;
+    uint32_t mask[kRows / 8][kWords];   // (8 heads at least) words 1 ..; a word of zeros at each end
+    int pos[kRows / 8], base;
+};
+
+// All threads of the workgroup, between barriers of it; false in the threads whose query has an ancestor
+// whose parent is none. A thread walks one query's line to the root in LDS (twice: its depth first), 64 cycles
+// a step; parents come before their children, so every walk ends. parent: LDS that nothing else uses up to
+// the second barrier from here (the stage of a later tile).
+template <int kThreads, int kRows>
+__device__ inline bool plant(const WinArgs &A, const Problem &P, Tree<true, kRows> &T, uint8_t *stage) {
+    static_assert(2 * kMaxNodes <= kStageB, "a node's parent takes two bytes");
+    const int tid = threadIdx.x, n = P.node0 + P.n;
+    short *parent = reinterpret_cast<short *>(stage);   // -1: a child of the last row before the tree's; -2: not a parent
+    const int32_t *parents = A.parents + (P.q0 - P.node0);
+    for (int i = tid; i < n; i += kThreads) {
+        const int p = parents[i];
+        parent[i] = (short)(p >= -1 && p < i ? p : -2);
+    }
+    for (int i = tid; i < P.n * T.kWords; i += kThreads) T.mask[0][i] = 0;
+    if (tid == 0) T.base = P.base;
+    lds_barrier();
+    if (tid >= P.n) return true;
+    int depth = 0, v = parent[P.node0 + tid];
+    for (; v >= 0; v = parent[v]) ++depth;
+    const bool good = v == -1;
+    const int pos = P.base + depth;
+    T.pos[tid] = pos;
+    v = P.node0 + tid;
+    for (int at = pos; v >= 0; v = parent[v], --at)
+        if (A.window <= 0 || at > pos - A.window || at < A.first) T.mask[tid][1 + (v >> 5)] |= 1u << (v & 31);
+    return good;
+}
+
+// Whether the stretch of tiles up to i1 has any that the masks and positions are needed for.
+__device__ inline bool needs_tree(const WinArgs &A, const Problem &P, int i1) {
+    return A.window > 0 || tile_at(P, i1 - 1) >= P.whole_c;
+}
+
+// What a query sees of a tile, for its rows k = 0 .. 31.
+struct TreeSight {
+    int pos, base;
+    uint32_t bits;   // of the tree's rows in it
+    __device__ bool operator()(const WinArgs &A, int key0, int k) const {
+        const int key = key0 + k;
+        return key < base ? A.window <= 0 || key > pos - A.window || key < A.first : bits >> k & 1;
+    }
+};
+struct RowSight {
+    int pos;
+    __device__ bool operator()(const WinArgs &A, int key0, int k) const { return sees(A, pos, key0 + k); }
+};
+template <int kRows>
+__device__ inline TreeSight sight_of(const Tree<true, kRows> &T, int, int qi, int key0) {
+    TreeSight v{T.pos[qi], T.base, 0};
+    const int at = key0 - v.base;
+    if (at > -32) {
+        const uint32_t *m = &T.mask[qi][1 + (at >> 5)];
+        v.bits = (uint32_t)((((uint64_t)m[1] << 32) | m[0]) >> (at & 31));
+    }
+    return v;
+}
+template <int kRows>
+__device__ inline RowSight sight_of(const Tree<false, kRows> &, int pos, int, int) { return {pos}; }
 
 // ---- plan ------------------------------------------------------------------------
 
@@ -175,7 +262,7 @@ __device__ inline long long block_scan(long long v, long long *sums, long long *
 
 // put(i, record, tiles before) for every problem; returns their number, *tiles and, in
 // *longest (shared, 0 before), the most of one. All threads of the workgroup; first_s: [n_seqs].
-template <int kThreads, int kEach, typename Put>
+template <bool kTree, int kThreads, int kEach, typename Put>
 __device__ inline int lay_line(const WinArgs &A, int *first_s, long long *sums, int *longest, long long *tiles, Put put) {
     const int tid = threadIdx.x;
     const int lh = log_hpt(A), lg = A.log_head - lh, qpt = (1 << A.log_rows) >> lh;
@@ -212,13 +299,13 @@ __device__ inline int lay_line(const WinArgs &A, int *first_s, long long *sums, 
                     }
                     first = first_s[s];
                 }
-                rec[u] = record_of(A, s, i - first);
+                rec[u] = record_of<kTree>(A, s, i - first);
             }
         }
 #pragma unroll
         for (int u = 0; u < kEach; ++u)
             if (i0 + kEach * tid + u < n_prob) {
-                n[u] = problem_of(A, rec[u]).tiles;
+                n[u] = problem_of<kTree>(A, rec[u]).tiles;
                 sum += n[u];   // (four problems have under 2^30)
                 most = max(most, n[u]);
             }
@@ -293,6 +380,7 @@ __device__ inline void leave(const WinArgs &A, const Cuts &C, int n_prob) {
 
 // One workgroup, for lines of many problems: latency of a few loads, scans and a search in LDS,
 // 10 us for 3840 problems and 12 for 4096 of one sequence.
+template <bool kTree>
 __global__ __launch_bounds__(1024) void plan_kernel(const WinArgs A) {
     __shared__ int first_s[kMaxSeqs];   // problems before each sequence
     __shared__ long long sums[16];
@@ -302,7 +390,7 @@ __global__ __launch_bounds__(1024) void plan_kernel(const WinArgs A) {
     constexpr int kHeld = 8192;   // (64 KB; the search below took half the kernel's time in memory)
     __shared__ long long pre_s[kHeld];
     // four problems a thread: their loads and one sum for 4096 (12 us; with one a thread 17)
-    const int n_prob = lay_line<1024, 4>(A, first_s, sums, &longest, &tiles, [&](int i, int4 rec, long long before) {
+    const int n_prob = lay_line<kTree, 1024, 4>(A, first_s, sums, &longest, &tiles, [&](int i, int4 rec, long long before) {
         A.prob[i] = rec;
         A.pre[i] = before;
         if (i < kHeld) pre_s[i] = before;
@@ -338,7 +426,7 @@ struct Place {
 
 // Few problems: every workgroup lays out the line itself (a launch and a wait less), and
 // the first one leaves it to the merge; else the plan kernel did.
-template <int kFew, int kThreads>
+template <bool kTree, int kFew, int kThreads>
 __device__ inline Place take_place(const WinArgs &A, Line<kFew> &L) {
     const int tid = threadIdx.x, wg = blockIdx.x;
     Place at;
@@ -346,7 +434,7 @@ __device__ inline Place take_place(const WinArgs &A, Line<kFew> &L) {
     if constexpr (kFew != 0) {
         if (tid == 0) L.longest = 0;
         long long tiles;
-        at.n_prob = lay_line<kThreads, 1>(A, L.first, L.sums, &L.longest, &tiles, [&](int i, int4 rec, long long before) {
+        at.n_prob = lay_line<kTree, kThreads, 1>(A, L.first, L.sums, &L.longest, &tiles, [&](int i, int4 rec, long long before) {
             L.prob[i] = rec;
             L.pre[i] = before;
         });
@@ -399,13 +487,13 @@ struct Stretch {
     int i0, i1;
     float top;   // P starts at 2^top
 };
-template <bool kF32, int kFew>
+template <bool kTree, bool kF32, int kFew>
 __device__ inline bool next_stretch(const WinArgs &A, const Line<kFew> &L, Place &at, Stretch &S) {
     if (__builtin_amdgcn_readfirstlane(at.t >= at.end || at.prob >= at.n_prob)) return false;
     const int pi = at.prob++;
     const long long begin = kFew ? L.pre[kFew ? pi : 0] : A.pre[pi], end = kFew ? L.pre[kFew ? pi + 1 : 0] : A.pre[pi + 1];
     const int4 rec = kFew ? L.prob[kFew ? pi : 0] : A.prob[pi];
-    S.P = problem_of(A, make_int4(__builtin_amdgcn_readfirstlane(rec.x), __builtin_amdgcn_readfirstlane(rec.y),
+    S.P = problem_of<kTree>(A, make_int4(__builtin_amdgcn_readfirstlane(rec.x), __builtin_amdgcn_readfirstlane(rec.y),
                                   __builtin_amdgcn_readfirstlane(rec.z), __builtin_amdgcn_readfirstlane(rec.w)));
     S.begins = at.t == begin;
     S.ends = end <= at.end;
@@ -615,7 +703,7 @@ __device__ inline void store_part(uint8_t *stage, int tid, const Part &R) {
 // Measured. Six prompts of up to 640 queries of 64 heads over windows of 128 rows and 4: 165 us, 11 a
 // problem of six tiles, three of them with masks; the queries and outputs take 3 (212 MB, 1.3
 // TB/s). 3 x 501 queries of 16 heads over windows of 500 rows in fp32 (13 GFLOP, issued twice): 90 us.
-template <bool kF32, bool kInline>
+template <bool kTree, bool kF32, bool kInline>
 __global__ __launch_bounds__(kF32 ? 256 : 512, kF32 ? 1 : 2) void window_kernel(const WinArgs A) {
     constexpr int kRT = 4, kRows = 16 * kRT;   // row tiles and rows of a problem
     constexpr int kW = kF32 ? 4 : 8;     // waves
@@ -635,7 +723,8 @@ __global__ __launch_bounds__(kF32 ? 256 : 512, kF32 ? 1 : 2) void window_kernel(
     const int wg = blockIdx.x;
     constexpr int kFew = kInline ? kFewProbs : 0;
     __shared__ Line<kFew> line;
-    Place at = take_place<kFew, 64 * kW>(A, line);
+    __shared__ Tree<kTree, kRows> tree;
+    Place at = take_place<kTree, kFew, 64 * kW>(A, line);
     const int lh = log_hpt(A);
     uint32_t ka[kN], va[2];
     {
@@ -656,7 +745,7 @@ __global__ __launch_bounds__(kF32 ? 256 : 512, kF32 ? 1 : 2) void window_kernel(
     Stretch S;
     int page[kN];
     auto next = [&]() {
-        if (!next_stretch<kF32>(A, line, at, S)) return false;
+        if (!next_stretch<kTree, kF32>(A, line, at, S)) return false;
         const int t = again(tid);
 #pragma unroll
         for (int u = 0; u < kN; ++u) {
@@ -679,6 +768,8 @@ __global__ __launch_bounds__(kF32 ? 256 : 512, kF32 ? 1 : 2) void window_kernel(
             for (int b = 0; b < kDT; ++b) o[a][b] = float4_t{0, 0, 0, 0};
         if (tid == 0) bad_s = 0;
         if (P.pos1 >= 0) {   // else its one tile sees nothing
+            if constexpr (kTree)
+                if (needs_tree(A, P, i1)) bad |= !plant<64 * kW>(A, P, tree, stages[2]);   // (read after the tiles' first barrier)
             // row tiles in use; the waves of the others only share the rest
             const int n_rt = ((P.n << lh) + 15) >> 4;
             const bool scores_mine = (w & 3) < n_rt;
@@ -889,6 +980,7 @@ __global__ __launch_bounds__(kF32 ? 256 : 512, kF32 ? 1 : 2) void window_kernel(
                 if (edge) {
                     uint32_t odd = 0;
                     const int lane_r = again(lane), g_r = lane_r >> 4;
+                    const auto sight = sight_of(tree, pos, min((16 * (w & 3) + (lane_r & 15)) >> lh, P.n - 1), key0);
 #pragma unroll
                     for (int u = 0; u < kN; ++u)
 #pragma unroll
@@ -896,7 +988,7 @@ __global__ __launch_bounds__(kF32 ? 256 : 512, kF32 ? 1 : 2) void window_kernel(
                             const int k = pi_key(16 * (kh + u) + 4 * g_r + r);
                             const bool fine = fabsf(acc[u][r]) < INFINITY;
                             if (((__ballot(!fine) >> (16 * g_r)) & 0xFFFF) == 0xFFFF) odd |= 1u << k;
-                            acc[u][r] = !sees(A, pos, key0 + k) ? -INFINITY : fine ? acc[u][r] : __builtin_nanf("");
+                            acc[u][r] = !sight(A, key0, k) ? -INFINITY : fine ? acc[u][r] : __builtin_nanf("");
                         }
                     odd |= __shfl_xor(odd, 16);
                     odd |= __shfl_xor(odd, 32);
@@ -1032,7 +1124,7 @@ struct Ring {
 // 22.7 ms, 0.82 PFLOP/s. 16 single tokens of 64 heads over 105 MB of rows: 63
 // us, 1.7 TB/s of the 5.1 that a copy reaches: a tile's chain (wait for its rows, to f16,
 // scores, weights, outputs, one barrier) bounds it, 2 us where memory alone would take 0.9.
-template <bool kInline>
+template <bool kTree, bool kInline>
 __global__ __launch_bounds__(512, 2) void roles_kernel(const WinArgs A) {
     constexpr int kRT = 4, kRows = 16 * kRT, kDT = 8;
     constexpr int kFew = kInline ? kFewProbs : 0;
@@ -1044,15 +1136,16 @@ __global__ __launch_bounds__(512, 2) void roles_kernel(const WinArgs A) {
     __shared__ __attribute__((aligned(16))) int moved_s[2][4];   // whether a row of the wave's outgrew its reference
     __shared__ int bad_s;
     __shared__ Line<kFew> line;
+    __shared__ Tree<kTree, kRows> tree;
 
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
-    Place at = take_place<kFew, 512>(A, line);
+    Place at = take_place<kTree, kFew, 512>(A, line);
     const int lh = log_hpt(A);
     Stretch S;
     Fetch F;
     // (the next problem's first page is looked up before the outputs of this one are stored)
     auto next = [&]() {
-        if (!next_stretch<false>(A, line, at, S)) return false;
+        if (!next_stretch<kTree, false>(A, line, at, S)) return false;
         F.page = S.P.pos1 < 0 ? -1 : F.page_of(A, S, S.i0, again(tid));
         return true;
     };
@@ -1092,6 +1185,8 @@ __global__ __launch_bounds__(512, 2) void roles_kernel(const WinArgs A) {
             if (tid == 0) bad_s = 0;
             const bool mine = 2 * rg < n_rt;   // else the wave only shares the rest
             if (P.pos1 >= 0) {
+                if constexpr (kTree)
+                    if (needs_tree(A, P, i1)) F.bad |= !plant<512>(A, P, tree, stages[2]);   // (with the other role's waves)
                 const uint32_t ka = pi_key(16 * kh + n16) * kRowB + 16 * g;
                 F.tile(A, T, i0, tid);
                 half8_t qh[2][16];
@@ -1195,6 +1290,9 @@ __global__ __launch_bounds__(512, 2) void roles_kernel(const WinArgs A) {
                     if (edge_at(P, i)) {
                         const int key0 = kTile * tile_at(P, i), lane_r = again(lane), g_r = lane_r >> 4;
                         uint32_t odd = 0;
+                        const decltype(sight_of(tree, 0, 0, 0)) sight[2] = {
+                            sight_of(tree, pos[0], min((32 * rg + (lane_r & 15)) >> lh, P.n - 1), key0),
+                            sight_of(tree, pos[1], min((32 * rg + 16 + (lane_r & 15)) >> lh, P.n - 1), key0)};
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
                             const int k = pi_key(16 * kh + 4 * g_r + r);
@@ -1203,7 +1301,7 @@ __global__ __launch_bounds__(512, 2) void roles_kernel(const WinArgs A) {
                             for (int j = 0; j < 2; ++j) {
                                 const bool fine = fabsf(acc[j][r]) < INFINITY;
                                 any = any || fine;
-                                acc[j][r] = !sees(A, pos[j], key0 + k) ? -INFINITY : fine ? acc[j][r] : __builtin_nanf("");
+                                acc[j][r] = !sight[j](A, key0, k) ? -INFINITY : fine ? acc[j][r] : __builtin_nanf("");
                             }
                             if (((__ballot(!any) >> (16 * g_r)) & 0xFFFF) == 0xFFFF) odd |= 1u << k;
                         }
@@ -1252,6 +1350,8 @@ __global__ __launch_bounds__(512, 2) void roles_kernel(const WinArgs A) {
 #pragma unroll
                 for (int b = 0; b < kDT; ++b) o[a][b] = float4_t{0, 0, 0, 0};
             if (P.pos1 >= 0) {
+                if constexpr (kTree)
+                    if (needs_tree(A, P, i1)) F.bad |= !plant<512>(A, P, tree, stages[2]);
                 uint32_t va[2];
 #pragma unroll
                 for (int kt = 0; kt < 2; ++kt)
@@ -1353,7 +1453,7 @@ __global__ __launch_bounds__(512, 2) void roles_kernel(const WinArgs A) {
 //
 // Measured: 4 tokens of 16 heads over 112 MB of rows, fp32: 44 us, 2.5 TB/s (101 us on 64-row
 // problems). The same chain bounds it, two of them a CU.
-template <bool kF32, bool kInline>
+template <bool kTree, bool kF32, bool kInline>
 __global__ __launch_bounds__(256, 2) void few_rows_kernel(const WinArgs A) {
     constexpr int kRT = 1, kRows = 16 * kRT;
     constexpr int kFew = kInline ? kFewProbs16 : 0;
@@ -1362,9 +1462,10 @@ __global__ __launch_bounds__(256, 2) void few_rows_kernel(const WinArgs A) {
     __shared__ uint32_t top_s[4][kRows];   // bits of the largest query value
     __shared__ int bad_s;
     __shared__ Line<kFew> line;
+    __shared__ Tree<kTree, kRows> tree;
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
     const int n16 = lane & 15, g = lane >> 4;
-    Place at = take_place<kFew, 256>(A, line);
+    Place at = take_place<kTree, kFew, 256>(A, line);
     const int lh = log_hpt(A);
     uint32_t ka[2], va[2];
 #pragma unroll
@@ -1373,7 +1474,7 @@ __global__ __launch_bounds__(256, 2) void few_rows_kernel(const WinArgs A) {
         va[kt] = lds_addr(stages[0]) + pi_key(16 * kt + 4 * g + (n16 >> 2)) * kRowB + 256 * w + 8 * (n16 & 3);
     }
     Stretch S;
-    while (next_stretch<kF32>(A, line, at, S)) {
+    while (next_stretch<kTree, kF32>(A, line, at, S)) {
         const Problem P = S.P;
         const int i0 = S.i0, i1 = S.i1;
         bool bad = P.slot < 0;
@@ -1387,6 +1488,8 @@ __global__ __launch_bounds__(256, 2) void few_rows_kernel(const WinArgs A) {
         for (int rt = 0; rt < kRT; ++rt) m[rt] = -INFINITY, l[rt] = kq[rt] = 0.0f;
         if (tid == 0) bad_s = 0;
         if (P.pos1 >= 0) {   // else its one tile sees nothing
+            if constexpr (kTree)
+                if (needs_tree(A, P, i1)) bad |= !plant<256>(A, P, tree, stages[1]);   // (read after the tiles' first barrier)
             // the thread's u-th row of tile i (past the last row seen: that row again, masked), and its page
             auto row_of = [&](int i, int u) { return min(kTile * tile_at(P, min(i, i1 - 1)) + (tid >> 4) + 16 * u, P.pos1); };
             auto page_of = [&](int i, int u) { return A.table[(long long)P.slot * A.stride + (row_of(i, u) >> A.shift)]; };
@@ -1482,7 +1585,11 @@ __global__ __launch_bounds__(256, 2) void few_rows_kernel(const WinArgs A) {
                 const int tile = tile_at(P, i), key0 = kTile * tile;
                 if (!(tile < P.whole_c && (tile >= P.whole_b || tile < P.whole_a))) {
                     uint32_t odd = 0;   // keys whose scores are not finite in any row
-                    const int g_r = again(lane) >> 4;
+                    const int lane_r = again(lane), g_r = lane_r >> 4;
+                    decltype(sight_of(tree, 0, 0, 0)) sight[kRT];
+#pragma unroll
+                    for (int rt = 0; rt < kRT; ++rt)
+                        sight[rt] = sight_of(tree, pos[rt], min((16 * rt + (lane_r & 15)) >> lh, P.n - 1), key0);
 #pragma unroll
                     for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
@@ -1493,7 +1600,7 @@ __global__ __launch_bounds__(256, 2) void few_rows_kernel(const WinArgs A) {
                             for (int rt = 0; rt < kRT; ++rt) {
                                 const bool fine = fabsf(acc[rt][kt][r]) < INFINITY;
                                 all = all && !fine;
-                                acc[rt][kt][r] = !sees(A, pos[rt], key0 + k) ? -INFINITY : fine ? acc[rt][kt][r] : __builtin_nanf("");
+                                acc[rt][kt][r] = !sight[rt](A, key0, k) ? -INFINITY : fine ? acc[rt][kt][r] : __builtin_nanf("");
                             }
                             if (((__ballot(all) >> (16 * g_r)) & 0xFFFF) == 0xFFFF) odd |= 1u << k;
                         }
@@ -1613,7 +1720,7 @@ __global__ __launch_bounds__(64 * kWaves) void window_merge_kernel(const WinArgs
     const long long b0 = begin / per;   // the workgroup of its first tile; the first cut is the next one's
     if (end - begin <= whole || (b0 + 1) * per >= end) return;
     if (!kInline && b0 != blockIdx.x / wgs) return;
-    const Problem P = problem_of(A, A.prob[pi]);
+    const Problem P = problem_of<false>(A, A.prob[pi]);   // (its queries and heads)
     const int lh = log_hpt(A), qi = row >> lh, head = P.head0 + (row & ((1 << lh) - 1));
     if (qi >= P.n) return;   // (of four rows, whole waves; one row's waves leave together)
     const int parts = (int)((end - 1) / per - b0) + 1;
@@ -1737,8 +1844,9 @@ extern "C" size_t ds4hip_flash_attn_window_fp8_workspace_bytes(int n_seqs, int n
     return most;
 }
 
-extern "C" int ds4hip_flash_attn_window_fp8(const ds4hip_window_attn *a, void *workspace, size_t workspace_bytes,
-                                            void *stream) {
+// Trees: the queries are the nodes of their sequences' trees.
+template <bool kTree>
+static int attend(const ds4hip_window_attn *a, const int32_t *parents, void *workspace, size_t workspace_bytes, void *stream) {
     if (!a) return ds4hip_set_last_error(kEINVAL);
     const int lh = log2_heads(a->n_head);
     const int shift = a->page_rows > 0 ? __builtin_ctz(a->page_rows) : 0;
@@ -1748,7 +1856,7 @@ extern "C" int ds4hip_flash_attn_window_fp8(const ds4hip_window_attn *a, void *w
     if (a->n_seqs == 0 || a->n_q == 0) return 0;
     if (!a->q || !a->out || !a->codes || !a->sexp || !a->tail || !a->table || !a->rows || a->table_stride <= 0 ||
         a->n_slots <= 0 || a->n_cache_rows < a->page_rows || (a->n_cache_rows >> shift) > 0x7FFFFFFF || !workspace ||
-        (!a->q_start && a->n_q < a->n_seqs) || (!a->seq_ids && a->n_slots < a->n_seqs) || !aligned(a->q, 16) ||
+        (!a->q_start && a->n_q < a->n_seqs) || (kTree && !parents) || (!a->seq_ids && a->n_slots < a->n_seqs) || !aligned(a->q, 16) ||
         !aligned(a->out, 16) || !aligned(a->codes, 16) || !aligned(a->sexp, 8) || !aligned(a->tail, 16) ||
         !aligned(workspace, 16))
         return ds4hip_set_last_error(kEINVAL);
@@ -1766,6 +1874,7 @@ extern "C" int ds4hip_flash_attn_window_fp8(const ds4hip_window_attn *a, void *w
     A.rows = a->rows;
     A.q_start = a->q_start;
     A.seq_ids = a->seq_ids;
+    A.parents = parents;
     A.n_seqs = a->n_seqs;
     A.n_slots = a->n_slots;
     A.n_q = a->n_q;
@@ -1779,20 +1888,20 @@ extern "C" int ds4hip_flash_attn_window_fp8(const ds4hip_window_attn *a, void *w
     // (one query each: exactly as many problems)
     if (!a->q_start) A.prob_cap = a->n_seqs << (lh - std::min(lh, log_rows));
     const bool f32 = a->io_f32, in = A.prob_cap <= (log_rows == 4 ? kFewProbs16 : kFewProbs);
-    if (!in) hipLaunchKernelGGL(plan_kernel, dim3(1), dim3(1024), 0, st, A);
+    if (!in) hipLaunchKernelGGL(plan_kernel<kTree>, dim3(1), dim3(1024), 0, st, A);
     // tiles that a problem can have: of rows that the table can name, or of the window, the queries'
     // own span and the first rows, with their ends inside tiles
     const long long held = (long long)a->table_stride << shift;
-    const long long span = std::min<long long>(held, (long long)a->window + ((1 << log_rows) >> std::min(lh, log_rows)));
+    const long long span = std::min<long long>(held, (long long)a->window + (kTree ? kMaxNodes : (1 << log_rows) >> std::min(lh, log_rows)));
     const long long most = a->window > 0 ? span / kTile + 2 + (std::min<long long>(a->n_first, held) + kTile - 1) / kTile : held / kTile + 1;
     // Waves with roles for long problems of bf16 (us a call, with roles and without: problems of 34 tiles 1083, 1122,
     // of 1025 to 1152 22700, 24800, 16 sequences of up to 32768 rows 69.5, 72; problems of 6 tiles 176, 166; one
     // token over 4000 rows, in parts of 4 tiles, 30.5, 29.1)
-    auto *main = log_rows == 4 ? f32 ? in ? few_rows_kernel<true, true> : few_rows_kernel<true, false>
-                                     : in ? few_rows_kernel<false, true> : few_rows_kernel<false, false>
-                 : f32         ? in ? window_kernel<true, true> : window_kernel<true, false>
-                 : most > 16   ? in ? roles_kernel<true> : roles_kernel<false>
-                               : in ? window_kernel<false, true> : window_kernel<false, false>;
+    auto *main = log_rows == 4 ? f32 ? in ? few_rows_kernel<kTree, true, true> : few_rows_kernel<kTree, true, false>
+                                     : in ? few_rows_kernel<kTree, false, true> : few_rows_kernel<kTree, false, false>
+                 : f32         ? in ? window_kernel<kTree, true, true> : window_kernel<kTree, true, false>
+                 : most > 16   ? in ? roles_kernel<kTree, true> : roles_kernel<kTree, false>
+                               : in ? window_kernel<kTree, false, true> : window_kernel<kTree, false, false>;
     hipLaunchKernelGGL(main, dim3(A.n_wg), dim3(log_rows < 6 || f32 ? 256 : 512), 0, st, A);
     if (most > kWhole) {   // (else nothing is cut)
         const int n = in ? A.prob_cap : A.n_wg - 1;
@@ -1808,4 +1917,14 @@ extern "C" int ds4hip_flash_attn_window_fp8(const ds4hip_window_attn *a, void *w
         hipLaunchKernelGGL(merge, dim3(n << (shared ? log_rows : log_rows - 2)), dim3(eight ? 512 : 256), 0, st, A);
     }
     return ds4hip_set_last_error(hip_status(hipGetLastError()));
+}
+
+extern "C" int ds4hip_flash_attn_window_fp8(const ds4hip_window_attn *a, void *workspace, size_t workspace_bytes,
+                                            void *stream) {
+    return attend<false>(a, nullptr, workspace, workspace_bytes, stream);
+}
+
+extern "C" int ds4hip_flash_attn_tree_fp8(const ds4hip_window_attn *a, const int32_t *parents, void *workspace,
+                                          size_t workspace_bytes, void *stream) {
+    return attend<true>(a, parents, workspace, workspace_bytes, stream);
 }

@@ -367,9 +367,21 @@ def flash_attn_window_fp8(q, cache: Fp8KVCache, page_table, seq_rows, *, page_ro
                        workspace=workspace, stream=stream)
 
 
+def flash_attn_tree_fp8(q, parents, cache: Fp8KVCache, page_table, seq_rows, *, page_rows, window=0, n_first=0,
+                        sinks=None, q_start=None, seq_ids=None, out=None, workspace=None, stream=None):
+    """flash_attn_window_fp8 of trees of drafted tokens: a sequence's queries are its tree's nodes (at most 1024), whose
+    rows are its last ones. parents int32 [n_q]: each node's parent, a smaller number of its own tree, or -1. A node's
+    position is the number of rows before the tree's and of its ancestors; it sees those rows as a query there does, and
+    of the tree itself and its ancestors, by their positions. NaN where a parent is none of these.
+    """
+    view = WindowView(cache, page_table, seq_rows, page_rows)
+    return view.attend(q, parents=parents, window=window, n_first=n_first, sinks=sinks, q_start=q_start, seq_ids=seq_ids,
+                       out=out, workspace=workspace, stream=stream)
+
+
 class WindowView:
-    """The checked arguments of flash_attn_window_fp8 that stay the same from call to call:
-    a cache, its page table and its sequences' rows."""
+    """The checked arguments of flash_attn_window_fp8 and flash_attn_tree_fp8 that stay the same from call to
+    call: a cache, its page table and its sequences' rows."""
 
     def __init__(self, cache: Fp8KVCache, page_table, seq_rows, page_rows):
         if page_table.dim() != 2:
@@ -391,13 +403,15 @@ class WindowView:
                           n_cache_rows=cache.n_rows, table=page_table.data_ptr(), rows=seq_rows.data_ptr(), n_slots=slots,
                           table_stride=stride, page_rows=page_rows)
 
-    def attend(self, q, *, window=0, n_first=0, sinks=None, q_start=None, seq_ids=None, out=None, workspace=None, stream=None):
+    def attend(self, q, *, parents=None, window=0, n_first=0, sinks=None, q_start=None, seq_ids=None, out=None, workspace=None,
+               stream=None):
         if q.dim() != 3 or q.shape[2] != HEAD_DIM or q.dtype not in (torch.bfloat16, torch.float32):
             raise Ds4HipError("q must be bf16 or fp32 [n_q, n_head, 512]", -22)
         n_q, n_head = q.shape[0], q.shape[1]
         window, n_first = _int32(window, "window"), _int32(n_first, "n_first")
         for t, dtype, n, name in ((q, q.dtype, None, "q"), (sinks, torch.float32, n_head, "sinks"),
-                                  (q_start, torch.int32, 1, "q_start"), (seq_ids, torch.int32, None, "seq_ids")):
+                                  (q_start, torch.int32, 1, "q_start"), (seq_ids, torch.int32, None, "seq_ids"),
+                                  (parents, torch.int32, n_q, "parents")):
             if t is not None and (not _ready(t, dtype, self.index) or (n and t.numel() < n)):
                 _check(t, dtype, n, name)
                 _same_gpu(t, self.index, name)
@@ -421,9 +435,79 @@ class WindowView:
             a = WindowAttn(q=q.data_ptr(), out=out.data_ptr(), io_f32=q.dtype == torch.float32, sinks=_addr(sinks),
                            q_start=_addr(q_start), seq_ids=_addr(seq_ids), n_seqs=n_seqs, n_q=n_q, n_head=n_head,
                            window=window, n_first=n_first, **self.fixed)
-            call("ds4hip_flash_attn_window_fp8", C.byref(a), workspace.data_ptr(),
-                 workspace.numel() * workspace.element_size(), _stream(stream))
+            size = workspace.numel() * workspace.element_size()
+            if parents is None:
+                call("ds4hip_flash_attn_window_fp8", C.byref(a), workspace.data_ptr(), size, _stream(stream))
+            else:
+                call("ds4hip_flash_attn_tree_fp8", C.byref(a), parents.data_ptr(), workspace.data_ptr(), size, _stream(stream))
         return out
+
+
+# ---- sampling ------------------------------------------------------------------------------
+
+class Sample(C.Structure):
+    """ds4hip_sample (include/ds4hip.h)."""
+    _fields_ = [("logits", C.c_void_p), ("logits_f32", C.c_int), ("row_stride", C.c_longlong), ("n_rows", C.c_int),
+                ("n_vocab", C.c_int), ("u", C.c_void_p), ("temperature", C.c_void_p), ("top_k", C.c_void_p),
+                ("top_p", C.c_void_p), ("min_p", C.c_void_p), ("all_temperature", C.c_float), ("all_top_k", C.c_int),
+                ("all_top_p", C.c_float), ("all_min_p", C.c_float), ("tokens", C.c_void_p), ("probs", C.c_void_p)]
+
+
+def sample_workspace_bytes(n_rows, n_vocab) -> int:
+    return lib().ds4hip_sample_workspace_bytes(_int32(n_rows, "n_rows"), _int32(n_vocab, "n_vocab"))
+
+
+def sample_tokens(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, tokens=None, probs=None, workspace=None,
+                  stream=None):
+    """One token of each row of logits [n, vocab] (bf16 or fp32, rows of consecutive values), by its random number u
+    [n] fp32 in [0, 1); returns (tokens int32 [n], probs fp32 [n]).
+
+    temperature, top_k, top_p, min_p: one value for all rows, or a tensor of one a row (int32 for top_k, else
+    fp32). Of the tokens in the order of their logits (equal ones: lower index first), with weights exp((logit -
+    largest) / temperature), those stay that are among the first top_k (<= 0: all), before which the weights' sum is
+    under top_p of the first top_k's (>= 1: all), and whose weight is min_p at least; the first one always. The token
+    is the first in the vocabulary's order at which the sum of the weights that stay passes u of all of it, and its
+    probability its share. Temperature 0: the first token of that order, probability 1. A row with a NaN or +inf, with no
+    logit above -inf, or with a parameter or u outside its range gives -1 and NaN.
+    """
+    if logits.dim() != 2 or logits.dtype not in (torch.bfloat16, torch.float32) or logits.device.type != "cuda":
+        raise Ds4HipError("logits must be bf16 or fp32 [n, vocab] on the GPU", -22)
+    n, vocab = (_int32(x, "logits") for x in logits.shape)
+    stride = logits.stride(0) if n > 1 else max(vocab, 1)
+    if vocab > 1 and logits.stride(1) != 1 or stride < vocab:
+        raise Ds4HipError("logits: a row's values must be consecutive, and rows must not overlap", -22)
+    index = logits.get_device()
+    a = Sample(logits=logits.data_ptr(), logits_f32=logits.dtype == torch.float32, row_stride=stride, n_rows=n, n_vocab=vocab)
+    for t, dtype, name in ((temperature, torch.float32, "temperature"), (top_k, torch.int32, "top_k"),
+                           (top_p, torch.float32, "top_p"), (min_p, torch.float32, "min_p"), (u, torch.float32, "u")):
+        if isinstance(t, torch.Tensor) or name == "u":
+            if not _ready(t, dtype, index) or t.numel() != n:
+                _check(t, dtype, n, name)
+                _same_gpu(t, index, name)
+                raise Ds4HipError(f"{name}: {n} entries expected, got {t.numel()}", -22)
+            setattr(a, name, t.data_ptr())
+        else:
+            setattr(a, "all_" + name, _int32(t, name) if dtype is torch.int32 else t)
+    with _on_stream(stream, logits.device):
+        if tokens is None:
+            tokens = torch.empty(n, dtype=torch.int32, device=logits.device)
+        if probs is None:
+            probs = torch.empty(n, dtype=torch.float32, device=logits.device)
+        for t, dtype, name in ((tokens, torch.int32, "tokens"), (probs, torch.float32, "probs")):
+            _check(t, dtype, n, name)
+            _same_gpu(t, index, name)
+        if n == 0:
+            return tokens, probs
+        need = sample_workspace_bytes(n, vocab)
+        if workspace is None:
+            workspace = torch.empty(need, dtype=torch.uint8, device=logits.device)
+        else:
+            _dev(workspace, "workspace", need)
+            _same_gpu(workspace, index, "workspace")
+        a.tokens, a.probs = tokens.data_ptr(), probs.data_ptr()
+        call("ds4hip_sample_tokens", C.byref(a), workspace.data_ptr(), workspace.numel() * workspace.element_size(),
+             _stream(stream))
+    return tokens, probs
 
 
 # ---- tail RoPE (cuda/rope.cuh:51, cuda/attn_out.cuh:52) ----------------------------------

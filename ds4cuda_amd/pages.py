@@ -165,6 +165,47 @@ class PagePool:
         self._jobs(keep, "keep", n)
         self._call("ds4hip_kv_pages_free", stream, _addr(seqs), _addr(keep), n)
 
+    def _nodes(self, q_start, n_jobs, tensors):
+        """Checks packed nodes: q_start of n_jobs trees and tensors of one int32 a node; their number."""
+        n = tensors[0][0].numel()
+        for t, want, name in ((q_start, n_jobs + 1, "q_start"), *((t, n, name) for t, name in tensors)):
+            if not _ready(t, torch.int32, self.index) or t.numel() != want:
+                _check(t, torch.int32, None, name)
+                _same_gpu(t, self.index, name)
+                raise Ds4HipError(f"{name}: {want} entries expected, got {t.numel()}", -22)
+        return _int32(n, "nodes")
+
+    def keep(self, seqs, q_start, path, n_path, stream=None):
+        """Of the drafted nodes q_start[j] .. q_start[j + 1] - 1, the last rows of sequence seqs[j],
+        the n_path[j] ones path[q_start[j]], .. (ascending, counted from the tree's first) stay: their rows move to the
+        front of the tree's in all layers, and the sequence is cut behind them. (int32 device
+        tensors; path has an entry for every node.)"""
+        k = self._jobs(seqs, "seqs")
+        self._jobs(n_path, "n_path", k)
+        n = self._nodes(q_start, k, ((path, "path"),))
+        self._call("ds4hip_kv_pages_keep", stream, _addr(seqs), _addr(q_start), k, _addr(path), n, _addr(n_path),
+                   *self._ws(stream))
+
+    def accept(self, seqs, q_start, parents, tokens, targets, path=None, n_path=None, next=None, stream=None):
+        """Accepts of each tree of drafted nodes the path that the model agrees with, and keeps its rows
+        (keep). parents, tokens, targets int32 [nodes]: each node's parent in its tree (-1: none), its
+        drafted token, and the token sampled behind it. From a tree's first node the path goes on to the first
+        child whose token is the target of its parent. Returns (path [nodes], the accepted nodes packed as
+        q_start has them and -1 behind; n_path [jobs]; next [jobs], the last ones' targets)."""
+        k = self._jobs(seqs, "seqs")
+        n = self._nodes(q_start, k, ((parents, "parents"), (tokens, "tokens"), (targets, "targets")))
+        outs = []
+        for t, size, name in ((path, n, "path"), (n_path, k, "n_path"), (next, k, "next")):
+            if t is None:
+                t = self._empty(size, torch.int32, stream)
+            else:
+                _check(t, torch.int32, size, name)
+                _same_gpu(t, self.index, name)
+            outs.append(t)
+        self._call("ds4hip_kv_pages_accept", stream, _addr(seqs), _addr(q_start), k, _addr(parents), _addr(tokens),
+                   _addr(targets), n, *(t.data_ptr() for t in outs), *self._ws(stream))
+        return tuple(outs)
+
     def compact(self, n_live=None, stream=None):
         """Moves the held pages to the front of the pool; returns their number, an int32
         device scalar."""
@@ -181,8 +222,18 @@ class PagePool:
         """ops.flash_attn_window_fp8 over this pool's pages of one layer: the sequences
         seqs (None: slots 0, 1, ..). Queries that q_start names for none of them are left
         as they were in out, and undefined without out."""
+        return self._view(layer).attend(q, window=window, n_first=n_first, sinks=sinks, q_start=q_start, seq_ids=seqs, out=out,
+                                        workspace=workspace, stream=stream)
+
+    def attend_tree(self, q, parents, *, seqs=None, q_start=None, window=0, n_first=0, sinks=None, layer=0, out=None,
+                    workspace=None, stream=None):
+        """ops.flash_attn_tree_fp8 over this pool's pages of one layer: attend, for queries that are the
+        nodes of trees of drafted tokens."""
+        return self._view(layer).attend(q, parents=parents, window=window, n_first=n_first, sinks=sinks, q_start=q_start,
+                                        seq_ids=seqs, out=out, workspace=workspace, stream=stream)
+
+    def _view(self, layer):
         view = self._views.get(layer)
         if view is None:
             view = self._views[layer] = WindowView(self.layer(layer), self.table, self.rows, self.page_rows)
-        return view.attend(q, window=window, n_first=n_first, sinks=sinks, q_start=q_start, seq_ids=seqs, out=out,
-                           workspace=workspace, stream=stream)
+        return view

@@ -495,6 +495,39 @@ int ds4hip_indexer_topk_positions_batch(const float *q, const float *weights, co
                                         float *scratch_scores, int32_t *positions_out,
                                         int pos_stride, void *stream);
 
+/* ---- sampling ---------------------------------------------------------------------------- */
+
+/* One token of each row of logits, by a given random number (additive: the reference takes the largest logit,
+ * cuda/argmax.cu). Of row r, logits l [n_vocab] at logits + r * row_stride (bf16, or fp32 where logits_f32 is 1), with
+ * its temperature T, top_k k, top_p p, min_p m and u (device arrays [n_rows]; a NULL one: all_.. for every row):
+ * the tokens are ordered by logit, equal ones by index, and have the weights exp((l - max l) / T). Those stay that
+ *   are among the first k (k <= 0: all),
+ *   have a sum of the weights before them under p of the sum of those first k (p >= 1: all), and
+ *   have a weight of m at least;
+ * the first one always does. tokens [n_rows] receives the first one, by index, at which the running sum of
+ * the weights that stay passes u of all of it, and probs its share of it. T 0: the first of the order, share 1. Sums are
+ * held in 64 bits; weights under 2^-46 of the largest may count as none.
+ * Token -1 and share NaN: a row with a NaN or +inf, or with no logit over -inf; a T that is negative or not
+ * finite, a p or m that is NaN, a u outside [0, 1). n_rows up to 65536, n_vocab up to 262144. */
+typedef struct ds4hip_sample {
+    const void *logits;
+    int logits_f32;
+    long long row_stride;   /* elements, n_vocab at least (of one row: any) */
+    int n_rows, n_vocab;
+    const float *u;
+    const float *temperature;
+    const int32_t *top_k;
+    const float *top_p, *min_p;
+    float all_temperature;
+    int all_top_k;
+    float all_top_p, all_min_p;
+    int32_t *tokens;
+    float *probs;
+} ds4hip_sample;
+/* Bytes of workspace (8-byte aligned; calls that can run at the same time need one each). */
+size_t ds4hip_sample_workspace_bytes(int n_rows, int n_vocab);
+int ds4hip_sample_tokens(const ds4hip_sample *a, void *workspace, size_t workspace_bytes, void *stream);
+
 /* ---- compressor ------------------------------------------------------------------------ */
 
 /* Replaces ds4cuda::launch_compressor_decode_step_f32_prealloc

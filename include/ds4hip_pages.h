@@ -51,7 +51,7 @@ typedef struct ds4hip_kv_pages {
 /* An empty pool: refs, rows and status 0, table -1. */
 int ds4hip_kv_pages_init(const ds4hip_kv_pages *p, void *stream);
 
-/* Bytes of workspace for fork and compact on this pool (8-byte aligned; calls
+/* Bytes of workspace for fork, compact, keep and accept on this pool (8-byte aligned; calls
  * that share one are ordered on one stream). */
 size_t ds4hip_kv_pages_workspace_bytes(const ds4hip_kv_pages *p);
 
@@ -91,6 +91,32 @@ int ds4hip_kv_pages_free(const ds4hip_kv_pages *p, const int32_t *seqs, const in
  * name them there. *n_live (device) receives n. */
 int ds4hip_kv_pages_compact(const ds4hip_kv_pages *p, int32_t *n_live, void *workspace, size_t workspace_bytes,
                             void *stream);
+
+/* ---- drafted trees ------------------------------------------------------------------ */
+
+#define DS4HIP_TREE_MAX_NODES 1024   /* drafted nodes of one sequence */
+
+/* After a step over drafted tokens: of job j's tree, whose q_start[j + 1] - q_start[j] nodes (device int32
+ * [n_jobs + 1], ascending, 0 <= .. <= n_nodes) are the last rows of sequence seqs[j], the n_path[j] nodes path[q_start[j]], ..
+ * stay (ascending, each a node of its own tree): the row of the i-th becomes the i-th row behind
+ * those before the tree's, in all layers, and the sequence ends there; pages past it are
+ * released. No sequence twice. -22: also a path that is not such nodes, more nodes than the
+ * sequence has rows, or a page with rows of the tree's in it that another sequence holds too. */
+int ds4hip_kv_pages_keep(const ds4hip_kv_pages *p, const int32_t *seqs, const int32_t *q_start, int n_jobs,
+                         const int32_t *path, int n_nodes, const int32_t *n_path, void *workspace, size_t workspace_bytes,
+                         void *stream);
+
+/* The same with the paths found here, by what the model says after each node. parents, tokens and targets (device int32
+ * [n_nodes], as ds4hip_flash_attn_tree_fp8 takes the nodes): each node's parent, its drafted token, and
+ * the token that follows it (sampled; < 0 agrees with no draft). A path begins with node 0 and goes on with the first
+ * node that has its last one as parent and that one's target as token, until there is none. path receives the
+ * nodes (-1 behind them and where no job has nodes), n_path their numbers and next [n_jobs] the target of
+ * each last one: the token that the step adds behind the drafts (no nodes: 0 and -1). Where the call is
+ * refused, path and next are -1 and n_path 0. -22: also more than DS4HIP_TREE_MAX_NODES nodes. */
+int ds4hip_kv_pages_accept(const ds4hip_kv_pages *p, const int32_t *seqs, const int32_t *q_start, int n_jobs,
+                           const int32_t *parents, const int32_t *tokens, const int32_t *targets, int n_nodes,
+                           int32_t *path, int32_t *n_path, int32_t *next, void *workspace, size_t workspace_bytes,
+                           void *stream);
 
 /* ---- attention over pages --------------------------------------------------------- */
 
@@ -137,6 +163,19 @@ typedef struct ds4hip_window_attn {
  * run at the same time need one each. */
 size_t ds4hip_flash_attn_window_fp8_workspace_bytes(int n_seqs, int n_q, int n_head);
 int ds4hip_flash_attn_window_fp8(const ds4hip_window_attn *a, void *workspace, size_t workspace_bytes, void *stream);
+
+/* The same attention of trees of drafted tokens. A sequence's queries are the nodes of its tree
+ * (n of them, DS4HIP_TREE_MAX_NODES at most), in the order of their rows, its last n: node i is row
+ * rows - n + i. parents (device int32 [n_q]) has each node's parent as a node of its own tree, -1 <= parent < i;
+ * -1: the node follows the rows before the tree's (at least one such node, the first one). A node's
+ * position is rows - n plus the number of its ancestors. It sees the rows before the tree's as a query at its
+ * position does, and of the tree its own row and its ancestors', by their positions (p - window < position, or
+ * position < n_first); no others. (Chains of parents i - 1 give what ds4hip_flash_attn_window_fp8 gives.) Queries are also
+ * NaN where their sequence has more nodes than that or than rows, or where a parent of
+ * theirs or of an ancestor's is outside [-1, i) (with the queries next to them, as above).
+ * The workspace is ds4hip_flash_attn_window_fp8_workspace_bytes(). */
+int ds4hip_flash_attn_tree_fp8(const ds4hip_window_attn *a, const int32_t *parents, void *workspace,
+                               size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }
