@@ -12,9 +12,12 @@
 // that part again. Else it finds a border from the groups' maxima alone: k groups above it hold k tokens
 // above it, and the weights of groups' maxima that sum to p of all do as well. The few groups above
 // the border are read again; their tokens above it hold all that is kept. Where that is too many (a flat
-// distribution, most of the vocabulary), the row is read again, in four or more passes.
+// distribution, most of the vocabulary), the whole row takes their place.
 //
-// Precision. Weights are fp64 (a table of 64 and a polynomial: off by 2^-51), since the index of a running
+// A cut is found in bins of the weight, among the candidates or the whole row: the one that reaches k, or p, is
+// known by the sums of the bins, and the few tokens in it are compared with each other.
+//
+// Precision. Weights are fp64 (a table of 64 and a polynomial: off by 2^-44), since the index of a running
 // sum over a vocabulary is compared with a given border. Sums are fp64 in a fixed order, or, where
 // histograms add in any order, whole numbers in steps of 2^-45 of the largest weight.
 
@@ -30,11 +33,12 @@ namespace {
 constexpr int kPart = 8192, kGroup = 32;   // logits of a workgroup, of a group
 constexpr int kMaxVocab = 1 << 18;         // (sums of 2^45 stay in 64 bits)
 constexpr int kScanThreads = 256;
-constexpr int kThreads = 1024, kWaves = kThreads / 64;
+constexpr int kThreads = 512, kWaves = kThreads / 64;
 constexpr int kBins = 2048;
 constexpr int kList = 4096;      // candidates in LDS
-constexpr int kRanked = 512;     // candidates that are put in order by counting
-constexpr double kLog2e64 = 1.4426950408889634074;
+constexpr int kFew = 256;        // candidates that are all compared with each other
+constexpr int kNear = 512;       // tokens of a bin that are compared with each other
+constexpr double kLog2e = 1.4426950408889634074;
 
 struct Args {
     const void *logits;
@@ -54,7 +58,7 @@ struct Args {
 
 // A row's parameters.
 struct Row {
-    double c;        // log2(e) / T; 0: the largest logit
+    double c;        // 64 log2(e) / T; 0: the largest logit
     int k;           // 0: all
     double p, m, u;
     bool valid;
@@ -67,7 +71,7 @@ __device__ inline Row row_of(const Args &A, int row) {
     const int k = A.top_k ? A.top_k[row] : A.all_top_k;
     const float u = A.u[row];
     R.valid = t >= 0.0f && t < INFINITY && p == p && m == m && u >= 0.0f && u < 1.0f;
-    R.c = t > 0.0f ? kLog2e64 / t : 0.0;
+    R.c = t > 0.0f ? 64.0 * kLog2e / t : 0.0;
     R.k = m > 1.0f ? 1 : k > 0 && k < A.n_vocab ? k : 0;   // (a weight over 1: the first one alone)
     R.p = p > 0.0f ? p : 0.0;
     R.m = m > 1.0f ? 0.0 : m;
@@ -80,28 +84,35 @@ __device__ inline bool cuts_m(const Row &R) { return R.m > 0.0; }
 // Whether the sum of all weights is needed.
 __device__ inline bool needs_sum(const Row &R) { return R.c > 0.0 && R.k == 0 && (cuts_p(R) || !cuts_m(R)); }
 
-// 2^t for t <= 0, from 2^(j/64) in LDS and the Taylor series of 2^r, |r| <= 2^-7, up to r^5.
+// 2^(t / 64) for t <= 0 (2^-1000 for all under -64000), from 2^(j/64) in LDS and the Taylor series of
+// 2^(r/64), |r| <= 1/2, up to r^4. Adding 1.5 x 2^52 rounds t to a whole number and leaves it in the low bits: 18
+// instructions, eight or more of them side by side (26 with the rounding and conversion instructions and a test).
 __device__ inline double pow2(double t, const double *table) {
-    if (!(t > -1000.0)) return 0.0;
-    const double n = rint(t * 64.0), r = fma(n, -1.0 / 64.0, t);
-    const int i = (int)n;
-    constexpr double l = 0.69314718055994530942;
-    double y = l * l * l * l * l / 120.0;
-    y = fma(y, r, l * l * l * l / 24.0);
+    constexpr double round = 6755399441055744.0, l = 0.69314718055994530942 / 64.0;
+    t = fmax(t, -64000.0);
+    const double s = t + round, r = t - (s - round);
+    const int n = (int)(uint32_t)__double_as_longlong(s);
+    double y = l * l * l * l / 24.0;
     y = fma(y, r, l * l * l / 6.0);
     y = fma(y, r, l * l / 2.0);
     y = fma(y, r, l);
     y = fma(y, r, 1.0);
-    return __longlong_as_double(__double_as_longlong(table[i & 63] * y) + ((long long)(i >> 6) << 52));
+    uint2_t x = __builtin_bit_cast(uint2_t, table[n & 63] * y);
+    x[1] += (uint32_t)(n >> 6) << 20;
+    return __builtin_bit_cast(double, x);
 }
 
 __device__ inline void fill_table(double *table) {
     if (threadIdx.x < 64) table[threadIdx.x] = exp2((double)threadIdx.x / 64.0);
 }
 
-// Weight of logit x where the row's largest is `top`.
-__device__ inline double weight(float x, float top, double c, const double *table) {
+// Weight of logit x where the row's largest is `top`; some_weight: 2^-1000 at least, also for -inf.
+__device__ inline double some_weight(float x, float top, double c, const double *table) {
     return pow2(((double)x - (double)top) * c, table);
+}
+__device__ inline double weight(float x, float top, double c, const double *table) {
+    const double w = some_weight(x, top, c, table);
+    return w > 0x1p-999 ? w : 0.0;
 }
 
 // Order of the logits as whole numbers (-0 is 0).
@@ -111,30 +122,35 @@ __device__ inline uint32_t key_of(float x) {
 }
 __device__ inline float value_of(uint32_t k) { return __uint_as_float(k >> 31 ? k & 0x7FFFFFFFu : ~k); }
 
-// Eight logits of a row from e on (-inf past its end). Rows start at any multiple of a logit's size.
+// Eight logits of a row from e on (-inf past its end), as they lie in memory. Rows start at any multiple of
+// a logit's size.
 template <bool kF32>
-__device__ inline void load_eight(const Args &A, int row, int e, float *x) {
-    if (kF32) {
-        const float *src = static_cast<const float *>(A.logits) + row * A.stride + e;
-        if (e + 8 <= A.n_vocab) {
-            __builtin_memcpy(x, src, 32);
+struct Eight {
+    uint4_t v[kF32 ? 2 : 1];
+    __device__ void load(const Args &A, int row, int e) {
+        if (kF32) {
+            const float *src = static_cast<const float *>(A.logits) + row * A.stride + e;
+            if (e + 8 <= A.n_vocab) {
+                __builtin_memcpy(v, src, 32);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[kF32 ? i >> 2 : 0][i & 3] = e + i < A.n_vocab ? __float_as_uint(src[i]) : 0xFF800000u;
+            }
         } else {
+            const uint16_t *src = static_cast<const uint16_t *>(A.logits) + row * A.stride + e;
+            if (e + 8 <= A.n_vocab) {
+                __builtin_memcpy(v, src, 16);
+            } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = e + i < A.n_vocab ? src[i] : -INFINITY;
-        }
-    } else {
-        const uint16_t *src = static_cast<const uint16_t *>(A.logits) + row * A.stride + e;
-        if (e + 8 <= A.n_vocab) {
-            uint4_t v;
-            __builtin_memcpy(&v, src, 16);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x[2 * i] = __uint_as_float(v[i] << 16), x[2 * i + 1] = __uint_as_float(v[i] & 0xFFFF0000u);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = e + i < A.n_vocab ? bf16_to_f32(src[i]) : -INFINITY;
+                for (int i = 0; i < 4; ++i)
+                    v[0][i] = (e + 2 * i < A.n_vocab ? src[2 * i] : 0xFF80u) | (e + 2 * i + 1 < A.n_vocab ? src[2 * i + 1] : 0xFF80u) << 16;
+            }
         }
     }
-}
+    __device__ float operator[](int i) const {
+        return __uint_as_float(kF32 ? v[kF32 ? i >> 2 : 0][i & 3] : i & 1 ? v[0][i >> 1] & 0xFFFF0000u : v[0][i >> 1] << 16);
+    }
+};
 
 template <bool kF32>
 __device__ inline float load_one(const Args &A, int row, int e) {
@@ -154,9 +170,10 @@ __global__ __launch_bounds__(kScanThreads) void scan_kernel(const Args A) {
     __shared__ float max_s[kScanThreads / 64];
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
     const int row = blockIdx.x / A.parts, part = blockIdx.x - row * A.parts;
-    float x[4][8], top = -INFINITY;
+    Eight<kF32> x[4];
+    float top = -INFINITY;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) load_eight<kF32>(A, row, part * kPart + j * 2048 + tid * 8, x[j]);
+    for (int j = 0; j < 4; ++j) x[j].load(A, row, min(part * kPart + j * 2048 + tid * 8, A.n_vocab));
     fill_table(table);
     const Row R = row_of(A, row);
     bool odd = false;
@@ -193,7 +210,7 @@ __global__ __launch_bounds__(kScanThreads) void scan_kernel(const Args A) {
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sum += weight(x[j][i], top, R.c, table);
+            for (int i = 0; i < 8; ++i) sum += some_weight(x[j][i], top, R.c, table);
     }
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off);
@@ -211,256 +228,396 @@ __global__ __launch_bounds__(kScanThreads) void scan_kernel(const Args A) {
 struct Pick {
     double table[64];
     double sums[kWaves];
+    unsigned long long scans[kWaves];
     int counts[kWaves];
-    // the border's and the radix search's histogram
-    uint32_t bin_n[kBins];
-    unsigned long long bin_w[kBins];
-    uint16_t groups[kMaxVocab / kGroup];   // those above the border, by index
-    // the candidates, by index
-    uint32_t key[kList], index[kList];
-    unsigned long long order[kRanked];     // in order of their keys (equal ones by index)
-    int found, found_n;
-    unsigned long long found_w;
-    float top;
+    unsigned long long bins[kBins];        // weights, or numbers, of tokens
+    uint16_t groups[kMaxVocab / kGroup];   // those with a candidate, by index
+    uint32_t key[kList], index[kList];     // the candidates, by index
+    unsigned long long near[kNear], near_w[kNear];   // the places and weights in a cut's bin
+    double wave_sum[kMaxVocab / 512];      // of 512 tokens of the row each
+    int n_near, found;
+    unsigned long long found_above, place;
+    double before;
 };
 
-// Inclusive sum over the workgroup's threads, in their order; *total: of all.
+// A token's place in the order of logits, as a whole number: the highest first, equal logits by index.
+__device__ inline unsigned long long place_of(uint32_t key, uint32_t index) { return (unsigned long long)key << 32 | ~index; }
+
+template <int kCtrl, int kRowMask, typename T>
+__device__ inline T dpp_or_0(T v) {
+    if constexpr (sizeof(T) == 4) {
+        return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), kCtrl, kRowMask, 0xF, false));
+    } else {
+        uint2_t x = __builtin_bit_cast(uint2_t, v);
+        x[0] = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x[0], kCtrl, kRowMask, 0xF, false);
+        x[1] = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x[1], kCtrl, kRowMask, 0xF, false);
+        return __builtin_bit_cast(T, x);
+    }
+}
+
+// Inclusive sum over the wave's lanes: in rows of 16, then the last lanes of the rows before.
+template <typename T>
+__device__ inline T wave_scan(T x) {
+    x += dpp_or_0<0x111, 0xF>(x);   // the lane 1, 2, 4, 8 before
+    x += dpp_or_0<0x112, 0xF>(x);
+    x += dpp_or_0<0x114, 0xF>(x);
+    x += dpp_or_0<0x118, 0xF>(x);
+    x += dpp_or_0<0x142, 0xA>(x);   // lane 15 of the row before, to rows 1 and 3
+    x += dpp_or_0<0x143, 0xC>(x);   // lane 31, to rows 2 and 3
+    return x;
+}
+
+template <typename T>
+__device__ inline T lane_of(T v, int lane) {
+    if constexpr (sizeof(T) == 4) {
+        return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
+    } else {
+        uint2_t x = __builtin_bit_cast(uint2_t, v);
+        x[0] = (uint32_t)__builtin_amdgcn_readlane((int)x[0], lane);
+        x[1] = (uint32_t)__builtin_amdgcn_readlane((int)x[1], lane);
+        return __builtin_bit_cast(T, x);
+    }
+}
+
+// Inclusive sum over the workgroup's threads, in their order; *total: of all. (Every wave sums the
+// waves' sums in its own lanes: with each thread adding them up, a sum took half a microsecond.)
 template <typename T>
 __device__ inline T block_scan(T v, T *sums, T *total) {
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    T x = v;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const T y = __shfl_up(x, off);
-        if (lane >= off) x += y;
-    }
+    static_assert(kWaves <= 16, "the waves' sums lie in a row of lanes");
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const T x = wave_scan(v);
     __syncthreads();
     if (lane == 63) sums[w] = x;
     __syncthreads();
-    T before = 0, all = 0;
-#pragma unroll
-    for (int i = 0; i < kWaves; ++i) {
-        before += i < w ? sums[i] : 0;
-        all += sums[i];
-    }
-    *total = all;
-    return before + x;
+    T y = sums[lane & (kWaves - 1)];
+    y += dpp_or_0<0x111, 0xF>(y);
+    y += dpp_or_0<0x112, 0xF>(y);
+    y += dpp_or_0<0x114, 0xF>(y);
+    if (kWaves > 8) y += dpp_or_0<0x118, 0xF>(y);
+    *total = lane_of(y, kWaves - 1);
+    return w ? lane_of(y, w - 1) + x : x;
 }
 
-__device__ inline void give(const Args &A, int row, int token, float prob) {
+__device__ inline void give(const Args &A, int row, int token, double share) {
     A.tokens[row] = token;
-    A.probs[row] = prob;
+    A.probs[row] = (float)share;
 }
 
-// What is kept, in the order of logits: keys over `key`, and the first `ties` of equal ones.
-struct Cut {
-    uint32_t key;
-    int ties;
-};
-
-// A source of tokens in the order of their indexes: item(i, key, index) for i < n.
+// Tokens in the order of their indexes: the keys of kEach from the i-th on (0 past the last: no logit's), and
+// a token's index.
 struct ListSource {
     const Pick &S;
     int n;
-    __device__ void eight(int i, uint32_t *key) const {
+    static constexpr int kDeep = 1;
+    template <int kEach>
+    struct Some {
+        uint32_t key[kEach];
+        __device__ void load(const ListSource &L, int i) {
 #pragma unroll
-        for (int u = 0; u < 8; ++u) key[u] = i + u < n ? S.key[i + u] : 0;
-    }
+            for (int u = 0; u < kEach; ++u) key[u] = i + u < L.n ? L.S.key[i + u] : 0;
+        }
+        __device__ uint32_t operator()(const ListSource &, int, int u) const { return key[u]; }
+    };
     __device__ int index(int i) const { return S.index[i]; }
 };
 template <bool kF32>
 struct RowSource {
     const Args &A;
-    int row, n;
-    __device__ void eight(int i, uint32_t *key) const {
-        float x[8];
-        load_eight<kF32>(A, row, i, x);
-#pragma unroll
-        for (int u = 0; u < 8; ++u) key[u] = i + u < n ? key_of(x[u]) : 0;   // (0 is no logit's)
-    }
-    __device__ int index(int i) const { return i; }
+    int row, first, n;   // logits first .. first + n - 1 of the row
+    static constexpr int kDeep = 4;
+    template <int kEach>
+    struct Some {
+        static_assert(kEach == 8, "as the loads are");
+        Eight<kF32> x;
+        __device__ void load(const RowSource &L, int i) { x.load(L.A, L.row, min(L.first + i, L.A.n_vocab)); }   // (past the end: nothing is read)
+        __device__ uint32_t operator()(const RowSource &L, int i, int u) const { return i + u < L.n ? key_of(x[u]) : 0; }
+    };
+    __device__ int index(int i) const { return first + i; }
 };
 
-// The token: the first by index at which the kept weights' sum passes u of their total. Two passes
-// of 8192 items at a time; all threads.
-template <typename Source>
-__device__ inline void draw(const Args &A, Pick &S, const Source &src, const Row &R, int row, Cut cut) {
-    const int tid = threadIdx.x;
-    const float top = S.top;
-    double total = 0.0, target = 0.0;
-    for (int pass = 0; pass < 2; ++pass) {
-        if (pass == 1) {
-            target = R.u * total;
-            if (tid == 0) S.found = 0x7FFFFFFF;
-            __syncthreads();
-        }
-        double sum = 0.0;
-        int ties = 0, last = -1;      // last: an item of this thread that is kept
-        double last_w = 0.0;
-        for (int i0 = 0; i0 < src.n; i0 += 8 * kThreads) {
-            const int i = i0 + 8 * tid;
-            uint32_t key[8];
-            if (i < src.n) {
-                src.eight(i, key);
-            } else {
+// use(i, keys) for all of a source, kEach * kThreads at a time. kDeep of them are loaded while those before
+// are used (memory is 2 us away: with one of them ahead, converted as it came, a pass of 65536 took 28 us).
+template <int kEach, typename Source, typename Use>
+__device__ inline void each_tile(const Source &src, Use use) {
+    constexpr int kStep = kEach * kThreads, kDeep = Source::kDeep;
+    typename Source::template Some<kEach> next[kDeep];
+    int i = kEach * threadIdx.x;
 #pragma unroll
-                for (int u = 0; u < 8; ++u) key[u] = 0;
-            }
-            int equal = 0, all_equal = 0;
+    for (int d = 0; d < kDeep; ++d) next[d].load(src, i + d * kStep);
+    for (int i0 = 0; i0 < src.n; i0 += kDeep * kStep, i += kDeep * kStep) {
+        typename Source::template Some<kEach> now[kDeep];
 #pragma unroll
-            for (int u = 0; u < 8; ++u) equal += key[u] == cut.key;
-            const int upto = block_scan(equal, S.counts, &all_equal);
-            int tie = ties + upto - equal;
-            double w[8], mine = 0.0, all;
+        for (int d = 0; d < kDeep; ++d) now[d] = next[d];
+        if (i0 + kDeep * kStep < src.n)
 #pragma unroll
-            for (int u = 0; u < 8; ++u) {
-                bool in = key[u] > cut.key || (key[u] == cut.key && tie < cut.ties);
-                tie += key[u] == cut.key;
-                w[u] = 0.0;
-                if (in) {
-                    const double x = weight(value_of(key[u]), top, R.c, S.table);
-                    w[u] = x >= R.m ? x : 0.0;
-                }
-                mine += w[u];
-            }
-            const double incl = sum + block_scan(mine, S.sums, &all);
-            if (pass == 1) {
-                double at = incl - mine;
-                int hit = -1;
-                double hit_w = 0.0;
+            for (int d = 0; d < kDeep; ++d) next[d].load(src, i + (kDeep + d) * kStep);
+        __builtin_amdgcn_sched_barrier(0);   // (in flight before the others are used)
 #pragma unroll
-                for (int u = 0; u < 8; ++u) {
-                    at += w[u];
-                    if (w[u] > 0.0) {
-                        last = i + u;
-                        last_w = w[u];
-                        if (hit < 0 && at > target) {
-                            hit = i + u;
-                            hit_w = w[u];
-                        }
-                    }
-                }
-                if (hit >= 0) atomicMin(&S.found, hit);
-                __syncthreads();
-                const int found = S.found;
-                if (found < 0x7FFFFFFF) {
-                    if (hit == found) give(A, row, src.index(hit), (float)(hit_w / total));
-                    return;
-                }
-            }
-            sum += all;
-            ties += all_equal;
-        }
-        total = sum;
-        if (pass == 1) {   // (a rounding of the last sum: the last kept one)
-            __syncthreads();
-            if (tid == 0) S.found = -1;
-            __syncthreads();
-            if (last >= 0) atomicMax(&S.found, last);
-            __syncthreads();
-            if (last >= 0 && last == S.found) give(A, row, src.index(last), (float)(last_w / total));
+        for (int d = 0; d < kDeep; ++d) {
+            if (i0 + d * kStep >= src.n) break;
+            uint32_t key[kEach];
+#pragma unroll
+            for (int u = 0; u < kEach; ++u) key[u] = now[d](src, i + d * kStep, u);
+            use(i + d * kStep, key);
         }
     }
-}
-
-// Of the bins, from the highest key on, the first at which `need` is reached (by counts, or by weights);
-// S.found: the bin (-1: none), S.found_n and S.found_w: what lies above it. Two bins a thread.
-__device__ inline void find_bin(Pick &S, bool by_weight, unsigned long long need) {
-    const int tid = threadIdx.x, hi = kBins - 1 - 2 * tid;
-    const unsigned long long n0 = S.bin_n[hi], n1 = S.bin_n[hi - 1], w0 = S.bin_w[hi], w1 = S.bin_w[hi - 1];
-    unsigned long long all_n, all_w;
-    __shared__ unsigned long long scratch[kWaves];
-    const unsigned long long upto_n = block_scan(n0 + n1, scratch, &all_n);
-    const unsigned long long upto_w = block_scan(w0 + w1, scratch, &all_w);
-    if (tid == 0) S.found = -1;
-    __syncthreads();
-    const unsigned long long a = by_weight ? upto_w - w0 - w1 : upto_n - n0 - n1, x0 = by_weight ? w0 : n0,
-                             x1 = by_weight ? w1 : n1;
-    if (a < need && a + x0 + x1 >= need) {
-        const bool first = a + x0 >= need;
-        S.found = first ? hi : hi - 1;
-        S.found_n = (int)(upto_n - n0 - n1 + (first ? 0 : n0));
-        S.found_w = upto_w - w0 - w1 + (first ? 0 : w0);
-    }
-    __syncthreads();
 }
 
 constexpr double kUnit = 35184372088832.0;   // 2^45
 __device__ inline unsigned long long units(double w) { return (unsigned long long)rint(w * kUnit); }
 
-// The cut of the first k items (by_weight: of the items whose weights before them are under the share
-// R.p of `all`, or where that is 0 of all that `within` keeps), by the digits of the keys, highest first.
-template <typename Source>
-__device__ inline Cut radix(Pick &S, const Source &src, const Row &R, bool by_weight, int k, Cut within, double all) {
-    const int tid = threadIdx.x;
-    const float top = S.top;
-    uint32_t prefix = 0;   // the digits found
-    unsigned long long need = k;
-    const unsigned long long tie_w = by_weight ? units(weight(value_of(within.key), top, R.c, S.table)) : 0;
-    const bool bounded = by_weight && within.key;
-    constexpr int kBits[3] = {11, 11, 10};
-    int shift = 32;
-#pragma unroll 1
-    for (int level = 0; level < 3; ++level) {
-        const int bits = kBits[level], below = shift;
-        shift -= bits;
-        for (int i = tid; i < kBins; i += kThreads) S.bin_n[i] = 0, S.bin_w[i] = 0;
-        __syncthreads();
-        for (int i0 = 0; i0 < src.n; i0 += 8 * kThreads) {
-            const int i = i0 + 8 * tid;
-            if (i >= src.n) break;
-            uint32_t key[8];
-            src.eight(i, key);
+// A row's bins, 32 for each halving of the weight: kBins - 1 has the largest logit, 0 all whose weight is under
+// 2^-63.9. What is rounded on the way grows with the distance, so the bins keep the order of logits.
+struct Bins {
+    float top, scale;
+    __device__ float steps(float x) const { return fminf((top - x) * scale, (float)(kBins - 1)); }
+    __device__ int operator()(float x) const { return kBins - 1 - (int)steps(x); }
+    // of x in its bin: the part of kBins that it lies in
+    __device__ int part(float x) const {
+        const float d = steps(x);
+        return kBins - 1 - (int)((d - floorf(d)) * (float)kBins);
+    }
+};
+
+__device__ inline void clear_bins(Pick &S) {
 #pragma unroll
-            for (int u = 0; u < 8; ++u) {
-                if (key[u] == 0 || (level && key[u] >> below != prefix)) continue;
-                if (bounded && key[u] <= within.key) continue;   // (equal ones: below)
-                const uint32_t bin = key[u] >> shift & ((1u << bits) - 1);
-                atomicAdd(&S.bin_n[bin], 1u);
-                if (by_weight) {
-                    const unsigned long long w = units(weight(value_of(key[u]), top, R.c, S.table));
-                    if (w) atomicAdd(&S.bin_w[bin], w);
-                }
-            }
-        }
-        if (bounded && tid == 0 && (!level || within.key >> below == prefix)) {
-            const uint32_t bin = within.key >> shift & ((1u << bits) - 1);
-            atomicAdd(&S.bin_n[bin], (uint32_t)within.ties);
-            atomicAdd(&S.bin_w[bin], within.ties * tie_w);
-        }
-        __syncthreads();
-        if (by_weight && level == 0) {   // the total is known now
-            unsigned long long here;
-            __shared__ unsigned long long scratch[kWaves];
-            block_scan(S.bin_w[2 * tid] + S.bin_w[2 * tid + 1], scratch, &here);
-            need = (unsigned long long)ceil(R.p * (all > 0.0 ? all * kUnit : (double)here));
-            need = need < 1 ? 1 : need > here ? here : need;
-        }
-        find_bin(S, by_weight, need);
-        prefix = prefix << bits | (uint32_t)S.found;
-        need -= by_weight ? S.found_w : S.found_n;
-        __syncthreads();
-    }
-    // all in the last bin are equal: as many of them as are needed
-    Cut cut;
-    cut.key = prefix;
-    if (by_weight) {
-        const unsigned long long w = units(weight(value_of(prefix), top, R.c, S.table));
-        cut.ties = (int)((need + w - 1) / w);   // (w > 0: its bin reached what was needed)
-        if (bounded && prefix == within.key) cut.ties = min(cut.ties, within.ties);
-    } else {
-        cut.ties = (int)need;
-    }
-    return cut;
+    for (int i = 0; i < kBins; i += kThreads) S.bins[i + threadIdx.x] = 0;
+    __syncthreads();
 }
 
-// Any number of items; all: the sum of the row's weights, where its share is asked for.
-template <typename Source>
-__device__ inline void pick_radix(const Args &A, Pick &S, const Source &src, const Row &R, int row, double all) {
-    Cut cut = {0, 0};   // all
-    if (R.k) cut = radix(S, src, R, false, min(R.k, src.n), cut, 0.0);
-    if (cuts_p(R)) cut = radix(S, src, R, true, 0, cut, all);
-    draw(A, S, src, R, row, cut);
+// After a barrier: the first bin, from the highest down, at which the bins' sum reaches need (-1: none), and in
+// S.found_above the sum of those above it. share: need is that of the bins' sum instead.
+__device__ inline int find_bin(Pick &S, unsigned long long *need, double share = 0.0) {
+    constexpr int kEach = kBins / kThreads;
+    const int hi = kBins - 1 - kEach * (int)threadIdx.x;
+    unsigned long long x[kEach], sum = 0, all;
+#pragma unroll
+    for (int u = 0; u < kEach; ++u) sum += x[u] = S.bins[hi - u];
+    const unsigned long long upto = block_scan(sum, S.scans, &all);
+    if (share > 0.0) *need = max((unsigned long long)ceil(share * (double)all), 1ull);
+    if (all < *need) return -1;
+    unsigned long long above = upto - sum;
+    if (above < *need && upto >= *need) {   // one thread's
+        int u = 0;
+#pragma unroll
+        for (int v = 0; v < kEach - 1; ++v)
+            if (u == v && above + x[v] < *need) {
+                above += x[v];
+                u = v + 1;
+            }
+        S.found = hi - u;
+        S.found_above = above;
+    }
+    __syncthreads();
+    return S.found;
+}
+
+// The place of the last of the first k tokens from place `within` up (kWeigh: of those before which their weights' sum
+// is under the share p of `all` units; all 0: of their sum). 0: all of them. Bins of the weight first; where more
+// than kNear tokens are in the one that is found, its parts; then digits of the places, which all differ.
+template <bool kWeigh, int kEach, typename Source>
+__device__ inline unsigned long long cut_at(Pick &S, const Source &src, const Row &R, const Bins &bins, int k,
+                                            unsigned long long within, double all) {
+    const int tid = threadIdx.x;
+    unsigned long long need = kWeigh ? max((unsigned long long)ceil(R.p * all), 1ull) : k, prefix = 0;
+    int level = 0, below = 64, bin[2] = {0, 0};
+    // whether a token lies in the bins of the levels before this one
+    auto inside = [&](uint32_t key, int i, int levels) {
+        if (key == 0) return false;
+        const float x = value_of(key);
+        const int b = bins(x);
+        if (b == 0 || (levels > 0 && b != bin[0]) || (levels > 1 && bins.part(x) != bin[1])) return false;
+        if (!within && below == 64) return true;
+        const unsigned long long place = place_of(key, src.index(i));
+        return place >= within && (below == 64 || place >> below == prefix);
+    };
+    // use(item, key) for those inside, one of a lane at a time: they are few, and in different lanes
+    auto each_inside = [&](int i, const uint32_t *key, auto use) {
+        uint32_t mine = 0;
+#pragma unroll
+        for (int u = 0; u < kEach; ++u) mine |= inside(key[u], i + u, level) ? 1u << u : 0;
+        while (__any(mine != 0)) {
+            const int u = mine ? __builtin_ctz(mine) : 0;
+            uint32_t k = key[0];
+#pragma unroll
+            for (int v = 1; v < kEach; ++v) k = u == v ? key[v] : k;
+            if (mine) use(i + u, k);
+            mine &= mine - 1;
+        }
+    };
+    auto bin_of = [&](uint32_t key, int i) {   // (from the second level on)
+        if (level == 1) return bins.part(value_of(key));
+        const int shift = below - min(below, 11);
+        return (int)(place_of(key, src.index(i)) >> shift & ((1ull << (below - shift)) - 1));
+    };
+    while (true) {
+        clear_bins(S);
+        if (tid == 0) S.n_near = 0;
+        each_tile<kEach>(src, [&](int i, const uint32_t *key) {
+            if (level == 0) {   // most of them
+                unsigned long long x[kEach];
+#pragma unroll
+                for (int u = 0; u < kEach; ++u)
+                    x[u] = !inside(key[u], i + u, 0) ? 0 : kWeigh ? units(weight(value_of(key[u]), bins.top, R.c, S.table)) : 1;
+#pragma unroll
+                for (int u = 0; u < kEach; ++u)
+                    if (x[u]) atomicAdd(&S.bins[bins(value_of(key[u]))], x[u]);
+            } else {
+                each_inside(i, key, [&](int at, uint32_t k) {
+                    atomicAdd(&S.bins[bin_of(k, at)], kWeigh ? units(weight(value_of(k), bins.top, R.c, S.table)) : 1);
+                });
+            }
+        });
+        __syncthreads();
+        const int found = find_bin(S, &need, kWeigh && level == 0 && !(all > 0.0) ? fmax(R.p, 1e-300) : 0.0);
+        if (found < 0) return 0;
+        need -= S.found_above;
+        if (level < 2) {
+            bin[level] = found;
+        } else {
+            const int shift = below - min(below, 11);
+            prefix = prefix << (below - shift) | (unsigned)found;
+            below = shift;
+        }
+        // the tokens in it
+        ++level;
+        each_tile<kEach>(src, [&](int i, const uint32_t *key) {
+            each_inside(i, key, [&](int at, uint32_t k) {
+                const int to = atomicAdd(&S.n_near, 1);
+                if (to < kNear) S.near[to] = place_of(k, src.index(at));
+            });
+        });
+        __syncthreads();
+        const int n = S.n_near;
+        if (n <= kNear) {
+            if (kWeigh) {
+                if (tid < n) S.near_w[tid] = units(weight(value_of((uint32_t)(S.near[tid] >> 32)), bins.top, R.c, S.table));
+                __syncthreads();
+            }
+            if (tid < n) {   // what lies before each of them
+                const unsigned long long mine = S.near[tid];
+                unsigned long long before = 0;
+#pragma unroll 4
+                for (int j = 0; j < n; ++j) before += S.near[j] > mine ? kWeigh ? S.near_w[j] : 1 : 0;
+                if (before < need && before + (kWeigh ? S.near_w[tid] : 1) >= need) S.place = mine;
+            }
+            __syncthreads();
+            return S.place;
+        }
+    }
+}
+
+// Gives the token: the first by index at which the sum of the weights that are kept (from place `cut` up, R.m
+// at least) passes the target, u of their sum, or the one given with the sum of all. A wave's kEach * 64 tokens
+// are summed together; the wave in which the target lies is looked through again.
+template <int kEach, typename Source>
+__device__ inline void draw(const Args &A, Pick &S, const Source &src, const Row &R, int row, float top, unsigned long long cut,
+                            double target, double all) {
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    const uint32_t cut_key = (uint32_t)(cut >> 32);
+    const int cut_index = (int)~(uint32_t)cut;
+    auto weights = [&](int i, const uint32_t *key, double *x) {
+        double sum = 0.0;
+#pragma unroll
+        for (int u = 0; u < kEach; ++u) {
+            const bool in = key[u] != 0 && (key[u] > cut_key || (key[u] == cut_key && src.index(i + u) <= cut_index));
+            const double y = weight(value_of(key[u]), top, R.c, S.table);
+            x[u] = in && y >= R.m ? y : 0.0;
+            sum += x[u];
+        }
+        return sum;
+    };
+    double x[kEach];
+    int n_sums = 0;
+    each_tile<kEach>(src, [&](int i, const uint32_t *key) {
+        const double sum = wave_scan(weights(i, key, x));
+        if (lane == 63) S.wave_sum[n_sums + w] = sum;
+        n_sums += kWaves;
+    });
+    if (tid == 0) S.found = 0x7FFFFFFF, S.n_near = -1;
+    __syncthreads();
+    const double mine = tid < n_sums ? S.wave_sum[tid] : 0.0;
+    double total;
+    const double upto = block_scan(mine, S.sums, &total);
+    if (!(all > 0.0)) {
+        all = total;
+        target = R.u * total;
+    }
+    if (mine > 0.0) {
+        if (upto > target) atomicMin(&S.found, tid);
+        atomicMax(&S.n_near, tid);
+    }
+    __syncthreads();
+    // (none: sums that were rounded otherwise; then the last that is kept)
+    const int at = S.found < 0x7FFFFFFF ? S.found : max(S.n_near, 0);   // (the largest logit is always kept)
+    if (tid == at) S.before = upto - mine;
+    __syncthreads();
+    if (w != 0) return;
+    const int i = (at / kWaves * kThreads + (at % kWaves) * 64 + lane) * kEach;
+    typename Source::template Some<kEach> again;
+    again.load(src, i);
+    uint32_t key[kEach];
+#pragma unroll
+    for (int u = 0; u < kEach; ++u) key[u] = again(src, i, u);
+    const double sum = weights(i, key, x), incl = S.before + wave_scan(sum);
+    const uint64_t over = __ballot(sum > 0.0 && incl > target), any = __ballot(sum > 0.0);
+    if (lane != (over ? __builtin_ctzll(over) : 63 - __builtin_clzll(any))) return;
+    double run = incl - sum, share = 0.0;
+    int hit = -1;
+    bool done = false;
+#pragma unroll
+    for (int u = 0; u < kEach; ++u) {
+        run += x[u];
+        if (x[u] > 0.0 && !done) {
+            hit = i + u;
+            share = x[u];
+            done = run > target;
+        }
+    }
+    give(A, row, src.index(hit), share / all);
+}
+
+// The same and the cuts for a list of at most kFew candidates: each is compared with all others, by as many threads
+// side by side as there are for it, which gives its rank and the weights before it at once. All sums are units.
+__device__ inline void pick_few(const Args &A, Pick &S, int n, const Row &R, int row, float top, double all) {
+    const int tid = threadIdx.x;
+    if (tid < n) {
+        S.near[tid] = place_of(S.key[tid], S.index[tid]);
+        S.near_w[tid] = units(weight(value_of(S.key[tid]), top, R.c, S.table));
+    }
+    __syncthreads();
+    const int log_n = n > 1 ? 32 - __clz(n - 1) : 0, log_parts = min(31 - __clz(kThreads) - log_n, 4), parts = 1 << log_parts;
+    const int i = tid >> log_parts, part = tid & (parts - 1);
+    const unsigned long long mine = i < n ? S.near[i] : 0, w = i < n ? S.near_w[i] : 0;
+    int rank = 0;
+    unsigned long long before = 0;
+    if (R.k || cuts_p(R)) {
+#pragma unroll 4
+        for (int j = part; j < n; j += parts) {
+            const bool is = S.near[j] > mine;
+            rank += is;
+            before += is ? S.near_w[j] : 0;
+        }
+        for (int off = 1; off < parts; off <<= 1) {
+            rank += __shfl_xor(rank, off);
+            before += __shfl_xor(before, off);
+        }
+    }
+    bool in = part == 0 && i < n && (!R.k || rank < R.k);
+    unsigned long long total;
+    if (cuts_p(R)) {
+        double sum = all * kUnit;
+        if (R.k) {
+            block_scan(in ? w : 0, S.scans, &total);
+            sum = (double)total;
+        }
+        in = in && before < max((unsigned long long)ceil(R.p * sum), 1ull);
+    }
+    // (min-p as a share of the largest weight, in doubles as everywhere)
+    if (cuts_m(R)) in = in && (rank == 0 && (R.k || cuts_p(R)) ? true : weight(value_of((uint32_t)(mine >> 32)), top, R.c, S.table) >= R.m);
+    const unsigned long long upto = block_scan(in ? w : 0, S.scans, &total);
+    const unsigned long long target = (unsigned long long)(R.u * (double)total);   // the sum passes it: at least one more
+    if (in && upto > target && upto - w <= target) give(A, row, (int)~(uint32_t)mine, (double)w / (double)total);
 }
 
 template <bool kF32>
@@ -468,200 +625,129 @@ __global__ __launch_bounds__(kThreads) void pick_kernel(const Args A) {
     __shared__ Pick S;
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, row = blockIdx.x;
     const Row R = row_of(A, row);
-    fill_table(S.table);
-    const float *part_max = A.part_max + (size_t)row * A.parts;
-    const double *part_sum = A.part_sum + (size_t)row * A.parts;
+    // the thread's groups: `each` next to each other, a multiple of four as a row's are
+    constexpr int kMost = kMaxVocab / kGroup / kThreads;
+    const int each = (A.groups / 4 + kThreads - 1) / kThreads * 4, g0 = each * tid;
     const float *group_max = A.group_max + (size_t)row * A.groups;
+    float g[kMost];
+#pragma unroll
+    for (int u = 0; u < kMost; ++u) g[u] = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < kMost; u += 4)
+        if (u < each && g0 + u < A.groups) __builtin_memcpy(g + u, group_max + g0 + u, 16);
     // (every wave for itself; at most 32 parts)
-    const float pm = lane < A.parts ? part_max[lane] : -INFINITY;
+    const float pm = lane < A.parts ? A.part_max[(size_t)row * A.parts + lane] : -INFINITY;
     const float top = wave_max(pm);
     if (__any(pm != pm) || !(top > -INFINITY) || !R.valid) {
-        if (tid == 0) give(A, row, -1, __builtin_nanf(""));
+        if (tid == 0) give(A, row, -1, __builtin_nan(""));
         return;
     }
-    if (tid == 0) S.top = top, S.found = 0x7FFFFFFF;
-    __syncthreads();
+    fill_table(S.table);
+    if (tid == 0) S.found = 0x7FFFFFFF;
+    clear_bins(S);
     if (R.c == 0.0) {   // the first group that has the largest, the first of its logits that is it
-        for (int i = tid; i < A.groups; i += kThreads)
-            if (group_max[i] == top) {
-                atomicMin(&S.found, i);
-                break;
-            }
+#pragma unroll
+        for (int u = 0; u < kMost; ++u)
+            if (u < each && g[u] == top) atomicMin(&S.found, g0 + u);
         __syncthreads();
         if (w == 0) {
             const int e = S.found * kGroup + lane;
             const uint64_t is = __ballot(lane < kGroup && e < A.n_vocab && load_one<kF32>(A, row, min(e, A.n_vocab - 1)) == top);
-            if (lane == 0) give(A, row, S.found * kGroup + __builtin_ctzll(is), 1.0f);
+            if (lane == 0) give(A, row, S.found * kGroup + __builtin_ctzll(is), 1.0);
         }
         return;
     }
     double all = 0.0;   // of all weights
     if (needs_sum(R)) {
-        const double mine = lane < A.parts && pm > -INFINITY ? part_sum[lane] * weight(pm, top, R.c, S.table) : 0.0;
-        double upto = mine;
-#pragma unroll
-        for (int off = 1; off < 64; off <<= 1) {
-            const double y = __shfl_up(upto, off);
-            if (lane >= off) upto += y;
-        }
+        const double mine = lane < A.parts && pm > -INFINITY ? A.part_sum[(size_t)row * A.parts + lane] * weight(pm, top, R.c, S.table) : 0.0;
+        const double upto = wave_scan(mine);
         all = __shfl(upto, 63);
         if (!cuts_p(R) && !cuts_m(R)) {   // nothing is cut off
             const double target = R.u * all;
             const uint64_t over = __ballot(mine > 0.0 && upto > target), any = __ballot(mine > 0.0);
             const int part = over ? __builtin_ctzll(over) : 63 - __builtin_clzll(any);
             const double before = __shfl(upto - mine, part);
-            float x[8];
-            const int e = part * kPart + 8 * tid;
-            load_eight<kF32>(A, row, min(e, A.n_vocab), x);   // (past the end: -inf, nothing is read)
-            double wt[8], sum = 0.0, ignored;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                wt[i] = weight(x[i], top, R.c, S.table);
-                sum += wt[i];
-            }
-            double at = before + block_scan(sum, S.sums, &ignored) - sum;
-            int hit = -1, last = -1;
-            double hit_w = 0.0, last_w = 0.0;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                at += wt[i];
-                if (wt[i] > 0.0) {
-                    last = e + i;
-                    last_w = wt[i];
-                    if (hit < 0 && at > target) {
-                        hit = e + i;
-                        hit_w = wt[i];
-                    }
-                }
-            }
-            if (hit >= 0) atomicMin(&S.found, hit);
-            __syncthreads();
-            const int found = S.found;
-            if (found < 0x7FFFFFFF) {
-                if (hit == found) give(A, row, hit, (float)(hit_w / all));
-                return;
-            }
-            __syncthreads();   // (a rounding of the part's sum: its last one)
-            if (tid == 0) S.found = -1;
-            __syncthreads();
-            if (last >= 0) atomicMax(&S.found, last);
-            __syncthreads();
-            if (last >= 0 && last == S.found) give(A, row, last, (float)(last_w / all));
+            draw<8>(A, S, RowSource<kF32>{A, row, part * kPart, min(kPart, A.n_vocab - part * kPart)}, R, row, top, 0, target - before, all);
             return;
         }
     }
 
-    // The border, as a bin of the distance from the largest logit: `scale` bins per unit, up to the lowest
-    // group's maximum. Bins grow with the distance for logits and groups alike, whatever is rounded.
-    constexpr int kSteps = kMaxVocab / kGroup / kThreads;
-    float g[kSteps], low = INFINITY;
-#pragma unroll
-    for (int u = 0; u < kSteps; ++u) {
-        const int i = u * kThreads + tid;
-        g[u] = i < A.groups ? group_max[i] : -INFINITY;
-        if (g[u] > -INFINITY) low = fminf(low, g[u]);
-    }
-    for (int i = tid; i < kBins; i += kThreads) S.bin_n[i] = 0, S.bin_w[i] = 0;
-    __shared__ float low_s[kWaves];
-    low = -wave_max(-low);
-    if (lane == 0) low_s[w] = low;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kWaves; ++i) low = fminf(low, low_s[i]);
-    const float span = top - low, scale = span > 0.0f && span < INFINITY ? (kBins - 1) / span : 0.0f;
-    auto bin_of = [&](float x) {   // kBins - 1: the largest
-        const float d = (top - x) * scale;
-        return x > -INFINITY ? kBins - 1 - min((int)fminf(d, (float)kBins), kBins - 1) : -1;
-    };
-    int border = 0;   // lowest bin of the candidates
-    bool enough = true;
+    // The border: a bin that holds, with those above it, k groups' maxima, or p of all in their weights
+    // (and a unit for each group's rounding). All that is kept lies in it or above it.
+    const Bins bins{top, (float)fmin(R.c * 0.5, 1e30)};
+    int border = 1;
     if (R.k || cuts_p(R)) {
 #pragma unroll
-        for (int u = 0; u < kSteps; ++u) {
-            const int b = bin_of(g[u]);
-            if (b < 0) continue;
-            atomicAdd(&S.bin_n[b], 1u);
-            if (!R.k) {
-                const unsigned long long x = units(weight(g[u], top, R.c, S.table));
-                if (x) atomicAdd(&S.bin_w[b], x);
+        for (int j = 0; j < kMost; j += 4)
+            if (j < each) {
+                unsigned long long x[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) x[u] = bins(g[j + u]) == 0 ? 0 : R.k ? 1 : units(weight(g[j + u], top, R.c, S.table));
+#pragma unroll
+                for (int u = 0; u < 4; ++u)
+                    if (x[u]) atomicAdd(&S.bins[bins(g[j + u])], x[u]);
             }
-        }
         __syncthreads();
-        // (a step of 2^-44 more for each group than the share asks for: the groups' roundings)
-        const unsigned long long need = R.k ? R.k : (unsigned long long)(R.p * all * kUnit) + 2 * A.groups;
-        find_bin(S, !R.k, need < 1 ? 1 : need);
-        border = S.found;
-        enough = border >= 0;
+        unsigned long long need = R.k ? R.k : (unsigned long long)(R.p * all * kUnit) + A.groups;
+        border = max(find_bin(S, &need), 1);
     }
-    int n = 0;
-    if (enough) {
-        // min-p alone gives a border too; exact tests follow
-        const float floor_m = cuts_m(R) ? top + (float)(log2(R.m) / R.c) : -INFINITY;
-        const float slack = 1e-5f * (fabsf(top) + fabsf(floor_m) + 1e-30f);
-        // (not where top-p asks for the sum of the first k, those under the floor among them)
-        const float least = floor_m > -INFINITY && !(R.k && cuts_p(R)) ? fminf(floor_m - slack, top) : -INFINITY;
-        auto in = [&](float x) { return bin_of(x) >= border && x >= least && x > -INFINITY; };
-        // the groups that have a candidate, by index: a thread takes kSteps next to each other
-        int n_groups = 0, mine = 0, taken;
-        float h[kSteps];
-#pragma unroll
-        for (int u = 0; u < kSteps; ++u) {
-            const int i = tid * kSteps + u;
-            h[u] = i < A.groups ? group_max[i] : -INFINITY;
-            mine += in(h[u]);
-        }
-        taken = block_scan(mine, S.counts, &n_groups) - mine;
-#pragma unroll
-        for (int u = 0; u < kSteps; ++u)
-            if (in(h[u])) S.groups[taken++] = (uint16_t)(tid * kSteps + u);
-        __syncthreads();
-        // their candidates, by index
-        for (int i0 = 0; i0 < n_groups * kGroup && n <= kList; i0 += kThreads) {
-            const int i = i0 + tid;
-            const int e = i < n_groups * kGroup ? S.groups[i >> 5] * kGroup + (i & 31) : A.n_vocab;
-            const float x = e < A.n_vocab ? load_one<kF32>(A, row, e) : -INFINITY;
-            const bool is = in(x);
-            int found;
-            const int at = n + block_scan((int)is, S.counts, &found) - 1;
-            if (is && at < kList) S.key[at] = key_of(x), S.index[at] = e;
-            n += found;
-        }
-        __syncthreads();
-    }
-    if (!enough || n > kList) {
-        pick_radix(A, S, RowSource<kF32>{A, row, A.n_vocab}, R, row, all);
-        return;
-    }
-    const ListSource list{S, n};
-    if (n > kRanked) {
-        pick_radix(A, S, list, R, row, all);
-        return;
-    }
-    // Each one's place in the order: how many come before it. Two threads count for one.
+    // min-p is a border too (the exact test comes later), but for those that top-p counts among the first k
+    const float floor_m = cuts_m(R) ? top + (float)(64.0 * log2(R.m) / R.c) : -INFINITY;
+    const float least = floor_m > -INFINITY && !(R.k && cuts_p(R)) ? fminf(floor_m - 1e-5f * (fabsf(top) + fabsf(floor_m) + 1e-30f), top) : -INFINITY;
+    // (as one logit, with room for what is rounded: more candidates do no harm)
+    const float reach = (float)(kBins - border) / bins.scale;
+    const float from = fmaxf(least, top - reach - 1e-6f * (fabsf(top) + reach));
+    auto in = [&](float x) { return x >= from && x > -INFINITY; };
+    // the groups that have a candidate, by index
+    int n_groups = 0;
     {
-        const int i = tid >> 1, half = tid & 1;
-        const unsigned long long mine = i < n ? (unsigned long long)S.key[i] << 32 | ~S.index[i] : 0;
-        int rank = 0;
-        if (i < n)
-            for (int j = half; j < n; j += 2) rank += ((unsigned long long)S.key[j] << 32 | ~S.index[j]) > mine;
-        rank += __shfl_xor(rank, 1);
-        if (i < n && half == 0) S.order[rank] = mine;
+        int mine = 0;
+#pragma unroll
+        for (int u = 0; u < kMost; ++u) mine += u < each && in(g[u]) ? 1 << u : 0;
+        int at = block_scan((int)__popc(mine), S.counts, &n_groups) - __popc(mine);
+        for (; mine; mine &= mine - 1) S.groups[at++] = (uint16_t)(g0 + __builtin_ctz(mine));
+        __syncthreads();
+    }
+    // their candidates, by index: a thread a group
+    int n = 0;
+    for (int i0 = 0; i0 < n_groups && n <= kList; i0 += kThreads) {
+        Eight<kF32> x[kGroup / 8];
+        uint32_t mine = 0;
+        int e = 0, found;
+        if (i0 + 64 * w < n_groups) {   // (waves without a group skip the work)
+            e = i0 + tid < n_groups ? S.groups[i0 + tid] * kGroup : A.n_vocab;
+#pragma unroll
+            for (int j = 0; j < kGroup / 8; ++j) x[j].load(A, row, min(e + 8 * j, A.n_vocab));
+#pragma unroll
+            for (int u = 0; u < kGroup; ++u) mine |= in(x[u >> 3][u & 7]) ? 1u << u : 0;
+        }
+        int at = n + block_scan((int)__popc(mine), S.counts, &found) - __popc(mine);
+        if (__any(mine != 0)) {
+#pragma unroll
+            for (int u = 0; u < kGroup; ++u)
+                if (mine >> u & 1) {
+                    if (at < kList) S.key[at] = key_of(x[u >> 3][u & 7]), S.index[at] = e + u;
+                    ++at;
+                }
+        }
+        n += found;
     }
     __syncthreads();
-    const uint32_t my_key = tid < n ? (uint32_t)(S.order[tid] >> 32) : 0;
-    const double mine = tid < n ? weight(value_of(my_key), top, R.c, S.table) : 0.0;
-    double total;
-    const bool among = tid < n && (!R.k || tid < R.k);
-    const double upto = block_scan(among ? mine : 0.0, S.sums, &total);
-    if (R.k) all = total;
-    const bool stays = among && (tid == 0 || ((!cuts_p(R) || upto - mine < R.p * all) && mine >= R.m));
-    int kept;
-    block_scan((int)stays, S.counts, &kept);
-    // equal ones of the last that stays, among those that do
-    const uint32_t last_key = (uint32_t)(S.order[kept - 1] >> 32);
-    int ties;
-    block_scan((int)(stays && my_key == last_key), S.counts, &ties);
-    draw(A, S, list, R, row, Cut{last_key, ties});
+    if (n <= kFew) {
+        pick_few(A, S, n, R, row, top, all);
+    } else if (n <= kList) {
+        const ListSource src{S, n};
+        unsigned long long cut = 0;
+        if (R.k) cut = cut_at<false, 1>(S, src, R, bins, R.k, 0, 0.0);
+        if (cuts_p(R)) cut = cut_at<true, 1>(S, src, R, bins, 0, cut, all * kUnit);
+        draw<1>(A, S, src, R, row, top, cut, 0.0, 0.0);
+    } else {
+        const RowSource<kF32> src{A, row, 0, A.n_vocab};
+        unsigned long long cut = 0;
+        if (R.k) cut = cut_at<false, 8>(S, src, R, bins, R.k, 0, 0.0);
+        if (cuts_p(R)) cut = cut_at<true, 8>(S, src, R, bins, 0, cut, all * kUnit);
+        draw<8>(A, S, src, R, row, top, cut, 0.0, 0.0);
+    }
 }
 
 size_t up256(size_t b) { return (b + 255) & ~(size_t)255; }
