@@ -6,7 +6,7 @@
 // under p of all of the k's; of them those with w >= m. Each of the three keeps a head of that order. The token
 // is the first one, by index, at which the running sum of the kept w passes u of their total.
 //
-// Split. scan_kernel reads the logits once: a workgroup takes 8192 of a row into registers and leaves
+// Split. scan_kernel reads the logits once: a wave takes a part of 2048 of a row into registers and leaves
 // their maximum, the sum of their weights (where it will be needed) and the maximum of every 32 (a group).
 // pick_kernel has a workgroup a row. Where nothing is cut off, it finds the part by the parts' sums and reads
 // that part again. Else it finds a border from the groups' maxima alone: k groups above it hold k tokens
@@ -30,20 +30,20 @@ using namespace ds4hip;
 
 namespace {
 
-constexpr int kPart = 8192, kGroup = 32;   // logits of a workgroup, of a group
+constexpr int kPart = 2048, kGroup = 32;   // logits of a part (a wave's), of a group
 constexpr int kMaxVocab = 1 << 18;         // (sums of 2^45 stay in 64 bits)
-constexpr int kScanThreads = 256;
+constexpr int kScanThreads = 256, kScanParts = kScanThreads / 64;
 constexpr int kThreads = 512, kWaves = kThreads / 64;
 constexpr int kBins = 2048;
 constexpr int kList = 4096;      // candidates in LDS
-constexpr int kFew = 256;        // candidates that are all compared with each other
+constexpr int kFew = 512;        // candidates that are all compared with each other
 constexpr int kNear = 512;       // tokens of a bin that are compared with each other
 constexpr double kLog2e = 1.4426950408889634074;
 
 struct Args {
     const void *logits;
     long long stride;
-    int n_rows, n_vocab, parts, groups;   // groups of all parts of a row
+    int n_rows, n_vocab, parts, groups;   // of a row, whole workgroups of the scan
     const float *temperature, *top_p, *min_p, *u;
     const int32_t *top_k;
     float all_temperature, all_top_p, all_min_p;
@@ -102,9 +102,19 @@ __device__ inline double pow2(double t, const double *table) {
     return __builtin_bit_cast(double, x);
 }
 
-__device__ inline void fill_table(double *table) {
-    if (threadIdx.x < 64) table[threadIdx.x] = exp2((double)threadIdx.x / 64.0);
-}
+// 2^(j/64), by the exponential series.
+struct Table {
+    double v[64];
+    constexpr Table() : v{} {
+        for (int j = 0; j < 64; ++j) {
+            const double x = j * (0.69314718055994530942 / 64.0);
+            double sum = 0.0;
+            for (int k = 24; k > 0; --k) sum = (sum + 1.0) * x / k;
+            v[j] = 1.0 + sum;
+        }
+    }
+};
+__constant__ const Table kTable = Table();
 
 // Weight of logit x where the row's largest is `top`; some_weight: 2^-1000 at least, also for -inf.
 __device__ inline double some_weight(float x, float top, double c, const double *table) {
@@ -164,20 +174,21 @@ __device__ inline float wave_max(float v) {
     return v;
 }
 
+// Waves on their own: four times 512 logits of a part each.
 template <bool kF32>
 __global__ __launch_bounds__(kScanThreads) void scan_kernel(const Args A) {
-    __shared__ double table[64], sum_s[kScanThreads / 64];
-    __shared__ float max_s[kScanThreads / 64];
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-    const int row = blockIdx.x / A.parts, part = blockIdx.x - row * A.parts;
+    __shared__ double tables[kScanParts][64];
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wgs = A.parts / kScanParts, row = blockIdx.x / wgs, part = (blockIdx.x - row * wgs) * kScanParts + w;
+    const size_t at = (size_t)row * A.parts + part;
+    double *table = tables[w];
+    const double entry = kTable.v[lane];
     Eight<kF32> x[4];
-    float top = -INFINITY;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) x[j].load(A, row, min(part * kPart + j * 2048 + tid * 8, A.n_vocab));
-    fill_table(table);
+    for (int j = 0; j < 4; ++j) x[j].load(A, row, min(part * kPart + j * 512 + lane * 8, A.n_vocab));
     const Row R = row_of(A, row);
     bool odd = false;
-    float *group_max = A.group_max + (size_t)row * A.groups + part * (kPart / kGroup);
+    float top = -INFINITY, *group_max = A.group_max + at * (kPart / kGroup);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         float m = -INFINITY;
@@ -189,22 +200,14 @@ __global__ __launch_bounds__(kScanThreads) void scan_kernel(const Args A) {
         top = fmaxf(top, m);
         m = fmaxf(m, __shfl_xor(m, 1));
         m = fmaxf(m, __shfl_xor(m, 2));
-        if ((lane & 3) == 0) group_max[64 * j + (tid >> 2)] = m;
+        if ((lane & 3) == 0) group_max[16 * j + (lane >> 2)] = m;
     }
     top = wave_max(top);
-    if (__any(odd)) top = __builtin_nanf("");
-    if (lane == 0) max_s[w] = top;
-    __syncthreads();
-    top = max_s[0];
-    odd = top != top;
-#pragma unroll
-    for (int i = 1; i < kScanThreads / 64; ++i) {
-        odd = odd || max_s[i] != max_s[i];
-        top = fmaxf(top, max_s[i]);
-    }
-    if (odd) top = __builtin_nanf("");
-    if (tid == 0) A.part_max[(size_t)row * A.parts + part] = top;
+    odd = __any(odd);   // (all lanes take part)
+    if (lane == 0) A.part_max[at] = odd ? __builtin_nanf("") : top;
     if (!needs_sum(R)) return;
+    table[lane] = entry;   // (a wave's LDS accesses are in order)
+    __builtin_amdgcn_wave_barrier();
     double sum = 0.0;
     if (top > -INFINITY) {
 #pragma unroll
@@ -214,13 +217,7 @@ __global__ __launch_bounds__(kScanThreads) void scan_kernel(const Args A) {
     }
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off);
-    if (lane == 0) sum_s[w] = sum;
-    __syncthreads();
-    if (tid == 0) {
-#pragma unroll
-        for (int i = 1; i < kScanThreads / 64; ++i) sum += sum_s[i];
-        A.part_sum[(size_t)row * A.parts + part] = sum;
-    }
+    if (lane == 0) A.part_sum[at] = sum;
 }
 
 // ---- pick ------------------------------------------------------------------------
@@ -232,10 +229,11 @@ struct Pick {
     int counts[kWaves];
     unsigned long long bins[kBins];        // weights, or numbers, of tokens
     uint16_t groups[kMaxVocab / kGroup];   // those with a candidate, by index
-    uint32_t key[kList], index[kList];     // the candidates, by index
+    float logit[kList];                    // the candidates, by index
+    uint32_t index[kList];
     unsigned long long near[kNear], near_w[kNear];   // the places and weights in a cut's bin
     double wave_sum[kMaxVocab / 512];      // of 512 tokens of the row each
-    int n_near, found;
+    int n_near, n_list, found;
     unsigned long long found_above, place;
     double before;
 };
@@ -303,39 +301,41 @@ __device__ inline void give(const Args &A, int row, int token, double share) {
     A.probs[row] = (float)share;
 }
 
-// Tokens in the order of their indexes: the keys of kEach from the i-th on (0 past the last: no logit's), and
-// a token's index.
+// Tokens in the order of their indexes: the logits of kEach from the i-th on (-inf past the last), and a
+// token's index.
 struct ListSource {
     const Pick &S;
     int n;
     static constexpr int kDeep = 1;
+    static constexpr bool kList = true;
     template <int kEach>
     struct Some {
-        uint32_t key[kEach];
+        float x[kEach];
         __device__ void load(const ListSource &L, int i) {
 #pragma unroll
-            for (int u = 0; u < kEach; ++u) key[u] = i + u < L.n ? L.S.key[i + u] : 0;
+            for (int u = 0; u < kEach; ++u) x[u] = i + u < L.n ? L.S.logit[i + u] : -INFINITY;
         }
-        __device__ uint32_t operator()(const ListSource &, int, int u) const { return key[u]; }
+        __device__ float operator()(const ListSource &, int, int u) const { return x[u]; }
     };
     __device__ int index(int i) const { return S.index[i]; }
 };
-template <bool kF32>
+template <bool kF32, int kAhead>
 struct RowSource {
     const Args &A;
     int row, first, n;   // logits first .. first + n - 1 of the row
-    static constexpr int kDeep = 4;
+    static constexpr int kDeep = kAhead;
+    static constexpr bool kList = false;
     template <int kEach>
     struct Some {
         static_assert(kEach == 8, "as the loads are");
         Eight<kF32> x;
         __device__ void load(const RowSource &L, int i) { x.load(L.A, L.row, min(L.first + i, L.A.n_vocab)); }   // (past the end: nothing is read)
-        __device__ uint32_t operator()(const RowSource &L, int i, int u) const { return i + u < L.n ? key_of(x[u]) : 0; }
+        __device__ float operator()(const RowSource &L, int i, int u) const { return i + u < L.n ? x[u] : -INFINITY; }
     };
     __device__ int index(int i) const { return first + i; }
 };
 
-// use(i, keys) for all of a source, kEach * kThreads at a time. kDeep of them are loaded while those before
+// use(i, logits) for all of a source, kEach * kThreads at a time. kDeep of them are loaded while those before
 // are used (memory is 2 us away: with one of them ahead, converted as it came, a pass of 65536 took 28 us).
 template <int kEach, typename Source, typename Use>
 __device__ inline void each_tile(const Source &src, Use use) {
@@ -355,16 +355,19 @@ __device__ inline void each_tile(const Source &src, Use use) {
 #pragma unroll
         for (int d = 0; d < kDeep; ++d) {
             if (i0 + d * kStep >= src.n) break;
-            uint32_t key[kEach];
+            float x[kEach];
 #pragma unroll
-            for (int u = 0; u < kEach; ++u) key[u] = now[d](src, i + d * kStep, u);
-            use(i + d * kStep, key);
+            for (int u = 0; u < kEach; ++u) x[u] = now[d](src, i + d * kStep, u);
+            use(i + d * kStep, x);
         }
     }
 }
 
 constexpr double kUnit = 35184372088832.0;   // 2^45
-__device__ inline unsigned long long units(double w) { return (unsigned long long)rint(w * kUnit); }
+// (adding 2^52 rounds to a whole number and leaves it in the low bits)
+__device__ inline unsigned long long units(double w) {
+    return (unsigned long long)__double_as_longlong(fma(w, kUnit, 4503599627370496.0)) & 0xFFFFFFFFFFFFFull;
+}
 
 // A row's bins, 32 for each halving of the weight: kBins - 1 has the largest logit, 0 all whose weight is under
 // 2^-63.9. What is rounded on the way grows with the distance, so the bins keep the order of logits.
@@ -412,98 +415,142 @@ __device__ inline int find_bin(Pick &S, unsigned long long *need, double share =
     return S.found;
 }
 
-// The place of the last of the first k tokens from place `within` up (kWeigh: of those before which their weights' sum
-// is under the share p of `all` units; all 0: of their sum). 0: all of them. Bins of the weight first; where more
-// than kNear tokens are in the one that is found, its parts; then digits of the places, which all differ.
+// Which tokens of a source a cut is looked for in, and where: the place of the last of the first `need` of them
+// (kWeigh: the first one with which the sum of units reaches it), from place `within` up.
+struct Search {
+    unsigned long long need, within, prefix;
+    int level, below;   // levels of bins behind it, bits of the places below those that are found
+    int bin[2];         // bins of the first two levels: of the weight, parts of one of them
+};
+
+template <bool kWeigh>
+__device__ inline unsigned long long amount(const Pick &S, const Row &R, const Bins &bins, float x) {
+    return kWeigh ? units(weight(x, bins.top, R.c, S.table)) : 1;
+}
+
+// Whether a token lies in the bins of `levels` levels.
+template <typename Source>
+__device__ inline bool inside(const Search &Q, const Bins &bins, const Source &src, float x, int i, int levels) {
+    const int b = bins(x);
+    if (b == 0 || (levels > 0 && b != Q.bin[0]) || (levels > 1 && bins.part(x) != Q.bin[1])) return false;
+    if (!Q.within && Q.below == 64) return true;
+    const unsigned long long place = place_of(key_of(x), src.index(i));
+    return place >= Q.within && (Q.below == 64 || place >> Q.below == Q.prefix);
+}
+
+// use(item, logit) for the tokens of a source that are inside the found bins, one of a lane at a time: they are few, and
+// in different lanes. Most of the others are known by two comparisons.
+template <int kEach, typename Source, typename Use>
+__device__ inline void each_inside(const Search &Q, const Bins &bins, const Source &src, Use use) {
+    const float near = (float)(kBins - 1 - Q.bin[0]) / bins.scale, far = (float)(kBins - Q.bin[0]) / bins.scale,
+                slack = 1e-6f * (fabsf(bins.top) + far), from = bins.top - far - slack, to = bins.top - near + slack;
+    each_tile<kEach>(src, [&](int i, const float *x) {
+        uint32_t mine = 0;
+#pragma unroll
+        for (int u = 0; u < kEach; ++u) mine |= x[u] < from || x[u] > to ? 0 : 1u << u;
+        while (__any(mine != 0)) {
+            const int u = mine ? __builtin_ctz(mine) : 0;
+            float y = x[0];
+#pragma unroll
+            for (int v = 1; v < kEach; ++v) y = u == v ? x[v] : y;
+            if (mine && inside(Q, bins, src, y, i + u, Q.level)) use(i + u, y);
+            mine &= mine - 1;
+        }
+    });
+}
+
+// The place, among the n <= kNear tokens in S.near.
+template <bool kWeigh>
+__device__ inline unsigned long long cut_near(Pick &S, int n, const Row &R, const Bins &bins, unsigned long long need) {
+    const int tid = threadIdx.x;
+    if (kWeigh) {
+        if (tid < n) S.near_w[tid] = amount<true>(S, R, bins, value_of((uint32_t)(S.near[tid] >> 32)));
+        __syncthreads();
+    }
+    if (tid < n) {   // what lies before each of them
+        const unsigned long long mine = S.near[tid];
+        unsigned long long before = 0;
+#pragma unroll 4
+        for (int j = 0; j < n; ++j) before += S.near[j] > mine ? kWeigh ? S.near_w[j] : 1 : 0;
+        if (before < need && before + (kWeigh ? S.near_w[tid] : 1) >= need) S.place = mine;
+    }
+    __syncthreads();
+    return S.place;
+}
+
+// The tokens that are inside, counted in S.n_near; the first kNear of them in S.near.
+template <int kEach, typename Source>
+__device__ inline int gather_near(Pick &S, const Search &Q, const Bins &bins, const Source &src) {
+    __syncthreads();
+    if (threadIdx.x == 0) S.n_near = 0;
+    __syncthreads();
+    each_inside<kEach>(Q, bins, src, [&](int at, float x) {
+        const int to = atomicAdd(&S.n_near, 1);
+        if (to < kNear) S.near[to] = place_of(key_of(x), src.index(at));
+    });
+    __syncthreads();
+    return S.n_near;
+}
+
+// From the second level on: parts of the weight's bin, then digits of the places, which all differ, until kNear are left.
+template <bool kWeigh, int kEach, typename Source>
+__device__ inline unsigned long long cut_inside(Pick &S, Search Q, const Row &R, const Bins &bins, const Source &src) {
+    while (true) {
+        const int n = gather_near<kEach>(S, Q, bins, src);
+        if (n <= kNear) return cut_near<kWeigh>(S, n, R, bins, Q.need);
+        const int shift = Q.level == 1 ? 64 : Q.below - min(Q.below, 11);
+        clear_bins(S);
+        each_inside<kEach>(Q, bins, src, [&](int at, float x) {
+            const int b = shift == 64 ? bins.part(x)
+                                      : (int)(place_of(key_of(x), src.index(at)) >> shift & ((1ull << (Q.below - shift)) - 1));
+            atomicAdd(&S.bins[b], amount<kWeigh>(S, R, bins, x));
+        });
+        __syncthreads();
+        const int found = find_bin(S, &Q.need);
+        Q.need -= S.found_above;
+        if (Q.level == 1) {
+            Q.bin[1] = found;
+        } else {
+            Q.prefix = Q.prefix << (Q.below - shift) | (unsigned)found;
+            Q.below = shift;
+        }
+        ++Q.level;
+    }
+}
+
+// The cut of a source: the place of the last of the first k tokens from place `within` up (kWeigh: of those before which
+// their weights' sum is under the share p of `all` units; all 0: of their sum). 0: all of them. What is in the
+// weight's bin that has it goes to the list, where that is not the source and holds it.
 template <bool kWeigh, int kEach, typename Source>
 __device__ inline unsigned long long cut_at(Pick &S, const Source &src, const Row &R, const Bins &bins, int k,
                                             unsigned long long within, double all) {
-    const int tid = threadIdx.x;
-    unsigned long long need = kWeigh ? max((unsigned long long)ceil(R.p * all), 1ull) : k, prefix = 0;
-    int level = 0, below = 64, bin[2] = {0, 0};
-    // whether a token lies in the bins of the levels before this one
-    auto inside = [&](uint32_t key, int i, int levels) {
-        if (key == 0) return false;
-        const float x = value_of(key);
-        const int b = bins(x);
-        if (b == 0 || (levels > 0 && b != bin[0]) || (levels > 1 && bins.part(x) != bin[1])) return false;
-        if (!within && below == 64) return true;
-        const unsigned long long place = place_of(key, src.index(i));
-        return place >= within && (below == 64 || place >> below == prefix);
-    };
-    // use(item, key) for those inside, one of a lane at a time: they are few, and in different lanes
-    auto each_inside = [&](int i, const uint32_t *key, auto use) {
-        uint32_t mine = 0;
+    Search Q = {kWeigh ? max((unsigned long long)ceil(R.p * all), 1ull) : (unsigned long long)k, within, 0, 0, 64, {0, 0}};
+    clear_bins(S);
+    each_tile<kEach>(src, [&](int i, const float *x) {
+        unsigned long long w[kEach];
 #pragma unroll
-        for (int u = 0; u < kEach; ++u) mine |= inside(key[u], i + u, level) ? 1u << u : 0;
-        while (__any(mine != 0)) {
-            const int u = mine ? __builtin_ctz(mine) : 0;
-            uint32_t k = key[0];
+        for (int u = 0; u < kEach; ++u) w[u] = amount<kWeigh>(S, R, bins, x[u]);
 #pragma unroll
-            for (int v = 1; v < kEach; ++v) k = u == v ? key[v] : k;
-            if (mine) use(i + u, k);
-            mine &= mine - 1;
-        }
-    };
-    auto bin_of = [&](uint32_t key, int i) {   // (from the second level on)
-        if (level == 1) return bins.part(value_of(key));
-        const int shift = below - min(below, 11);
-        return (int)(place_of(key, src.index(i)) >> shift & ((1ull << (below - shift)) - 1));
-    };
-    while (true) {
-        clear_bins(S);
-        if (tid == 0) S.n_near = 0;
-        each_tile<kEach>(src, [&](int i, const uint32_t *key) {
-            if (level == 0) {   // most of them
-                unsigned long long x[kEach];
-#pragma unroll
-                for (int u = 0; u < kEach; ++u)
-                    x[u] = !inside(key[u], i + u, 0) ? 0 : kWeigh ? units(weight(value_of(key[u]), bins.top, R.c, S.table)) : 1;
-#pragma unroll
-                for (int u = 0; u < kEach; ++u)
-                    if (x[u]) atomicAdd(&S.bins[bins(value_of(key[u]))], x[u]);
-            } else {
-                each_inside(i, key, [&](int at, uint32_t k) {
-                    atomicAdd(&S.bins[bin_of(k, at)], kWeigh ? units(weight(value_of(k), bins.top, R.c, S.table)) : 1);
-                });
-            }
+        for (int u = 0; u < kEach; ++u)
+            if (w[u] && inside(Q, bins, src, x[u], i + u, 0)) atomicAdd(&S.bins[bins(x[u])], w[u]);
+    });
+    if (threadIdx.x == 0) S.n_list = 0;
+    __syncthreads();
+    const int found = find_bin(S, &Q.need, kWeigh && !(all > 0.0) ? fmax(R.p, 1e-300) : 0.0);
+    if (found < 0) return 0;
+    Q.need -= S.found_above;
+    Q.bin[0] = found;
+    Q.level = 1;
+    if constexpr (Source::kList) {
+        return cut_inside<kWeigh, kEach>(S, Q, R, bins, src);
+    } else {
+        each_inside<kEach>(Q, bins, src, [&](int at, float x) {
+            const int to = atomicAdd(&S.n_list, 1);
+            if (to < kList) S.logit[to] = x, S.index[to] = src.index(at);
         });
         __syncthreads();
-        const int found = find_bin(S, &need, kWeigh && level == 0 && !(all > 0.0) ? fmax(R.p, 1e-300) : 0.0);
-        if (found < 0) return 0;
-        need -= S.found_above;
-        if (level < 2) {
-            bin[level] = found;
-        } else {
-            const int shift = below - min(below, 11);
-            prefix = prefix << (below - shift) | (unsigned)found;
-            below = shift;
-        }
-        // the tokens in it
-        ++level;
-        each_tile<kEach>(src, [&](int i, const uint32_t *key) {
-            each_inside(i, key, [&](int at, uint32_t k) {
-                const int to = atomicAdd(&S.n_near, 1);
-                if (to < kNear) S.near[to] = place_of(k, src.index(at));
-            });
-        });
-        __syncthreads();
-        const int n = S.n_near;
-        if (n <= kNear) {
-            if (kWeigh) {
-                if (tid < n) S.near_w[tid] = units(weight(value_of((uint32_t)(S.near[tid] >> 32)), bins.top, R.c, S.table));
-                __syncthreads();
-            }
-            if (tid < n) {   // what lies before each of them
-                const unsigned long long mine = S.near[tid];
-                unsigned long long before = 0;
-#pragma unroll 4
-                for (int j = 0; j < n; ++j) before += S.near[j] > mine ? kWeigh ? S.near_w[j] : 1 : 0;
-                if (before < need && before + (kWeigh ? S.near_w[tid] : 1) >= need) S.place = mine;
-            }
-            __syncthreads();
-            return S.place;
-        }
+        const int n = S.n_list;
+        return n <= kList ? cut_inside<kWeigh, 1>(S, Q, R, bins, ListSource{S, n}) : cut_inside<kWeigh, kEach>(S, Q, R, bins, src);
     }
 }
 
@@ -514,24 +561,26 @@ template <int kEach, typename Source>
 __device__ inline void draw(const Args &A, Pick &S, const Source &src, const Row &R, int row, float top, unsigned long long cut,
                             double target, double all) {
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-    const uint32_t cut_key = (uint32_t)(cut >> 32);
+    const float cut_logit = cut ? value_of((uint32_t)(cut >> 32)) : -INFINITY;
     const int cut_index = (int)~(uint32_t)cut;
-    auto weights = [&](int i, const uint32_t *key, double *x) {
+    const double least = fmax(R.m, 0x1p-999);   // (weight()'s 0)
+    auto weights = [&](int i, const float *logit, double *x) {
         double sum = 0.0;
 #pragma unroll
         for (int u = 0; u < kEach; ++u) {
-            const bool in = key[u] != 0 && (key[u] > cut_key || (key[u] == cut_key && src.index(i + u) <= cut_index));
-            const double y = weight(value_of(key[u]), top, R.c, S.table);
-            x[u] = in && y >= R.m ? y : 0.0;
+            const bool in = logit[u] > cut_logit || (logit[u] == cut_logit && src.index(i + u) <= cut_index);
+            const double y = some_weight(logit[u], top, R.c, S.table);
+            x[u] = in && y >= least ? y : 0.0;
             sum += x[u];
         }
         return sum;
     };
-    double x[kEach];
+    double x[kEach], sum = 0.0;
     int n_sums = 0;
-    each_tile<kEach>(src, [&](int i, const uint32_t *key) {
-        const double sum = wave_scan(weights(i, key, x));
-        if (lane == 63) S.wave_sum[n_sums + w] = sum;
+    each_tile<kEach>(src, [&](int i, const float *logit) {
+        sum = weights(i, logit, x);
+        const double upto = wave_scan(sum);
+        if (lane == 63) S.wave_sum[n_sums + w] = upto;
         n_sums += kWaves;
     });
     if (tid == 0) S.found = 0x7FFFFFFF, S.n_near = -1;
@@ -552,14 +601,17 @@ __device__ inline void draw(const Args &A, Pick &S, const Source &src, const Row
     const int at = S.found < 0x7FFFFFFF ? S.found : max(S.n_near, 0);   // (the largest logit is always kept)
     if (tid == at) S.before = upto - mine;
     __syncthreads();
-    if (w != 0) return;
-    const int i = (at / kWaves * kThreads + (at % kWaves) * 64 + lane) * kEach;
-    typename Source::template Some<kEach> again;
-    again.load(src, i);
-    uint32_t key[kEach];
+    if (S.n_near < 0 || w != at % kWaves) return;
+    const int i = (at / kWaves * kThreads + tid) * kEach;
+    if (n_sums > kWaves) {   // (else x and sum are what they were)
+        typename Source::template Some<kEach> again;
+        again.load(src, i);
+        float logit[kEach];
 #pragma unroll
-    for (int u = 0; u < kEach; ++u) key[u] = again(src, i, u);
-    const double sum = weights(i, key, x), incl = S.before + wave_scan(sum);
+        for (int u = 0; u < kEach; ++u) logit[u] = again(src, i, u);
+        sum = weights(i, logit, x);
+    }
+    const double incl = S.before + wave_scan(sum);
     const uint64_t over = __ballot(sum > 0.0 && incl > target), any = __ballot(sum > 0.0);
     if (lane != (over ? __builtin_ctzll(over) : 63 - __builtin_clzll(any))) return;
     double run = incl - sum, share = 0.0;
@@ -582,8 +634,8 @@ __device__ inline void draw(const Args &A, Pick &S, const Source &src, const Row
 __device__ inline void pick_few(const Args &A, Pick &S, int n, const Row &R, int row, float top, double all) {
     const int tid = threadIdx.x;
     if (tid < n) {
-        S.near[tid] = place_of(S.key[tid], S.index[tid]);
-        S.near_w[tid] = units(weight(value_of(S.key[tid]), top, R.c, S.table));
+        S.near[tid] = place_of(key_of(S.logit[tid]), S.index[tid]);
+        S.near_w[tid] = units(weight(S.logit[tid], top, R.c, S.table));
     }
     __syncthreads();
     const int log_n = n > 1 ? 32 - __clz(n - 1) : 0, log_parts = min(31 - __clz(kThreads) - log_n, 4), parts = 1 << log_parts;
@@ -635,14 +687,19 @@ __global__ __launch_bounds__(kThreads) void pick_kernel(const Args A) {
 #pragma unroll
     for (int u = 0; u < kMost; u += 4)
         if (u < each && g0 + u < A.groups) __builtin_memcpy(g + u, group_max + g0 + u, 16);
-    // (every wave for itself; at most 32 parts)
-    const float pm = lane < A.parts ? A.part_max[(size_t)row * A.parts + lane] : -INFINITY;
-    const float top = wave_max(pm);
-    if (__any(pm != pm) || !(top > -INFINITY) || !R.valid) {
+    // (every wave for itself: a lane has two parts, of 128 at most and a multiple of four)
+    float pm[2] = {-INFINITY, -INFINITY};
+    double ps[2] = {0.0, 0.0};
+    if (2 * lane < A.parts) {
+        __builtin_memcpy(pm, A.part_max + (size_t)row * A.parts + 2 * lane, 8);
+        if (needs_sum(R)) __builtin_memcpy(ps, A.part_sum + (size_t)row * A.parts + 2 * lane, 16);
+    }
+    const float top = wave_max(fmaxf(pm[0], pm[1]));
+    if (__any(pm[0] != pm[0] || pm[1] != pm[1]) || !(top > -INFINITY) || !R.valid) {
         if (tid == 0) give(A, row, -1, __builtin_nan(""));
         return;
     }
-    fill_table(S.table);
+    if (tid < 64) S.table[tid] = kTable.v[tid];
     if (tid == 0) S.found = 0x7FFFFFFF;
     clear_bins(S);
     if (R.c == 0.0) {   // the first group that has the largest, the first of its logits that is it
@@ -650,7 +707,7 @@ __global__ __launch_bounds__(kThreads) void pick_kernel(const Args A) {
         for (int u = 0; u < kMost; ++u)
             if (u < each && g[u] == top) atomicMin(&S.found, g0 + u);
         __syncthreads();
-        if (w == 0) {
+        if (w == 0 && S.found < A.groups) {
             const int e = S.found * kGroup + lane;
             const uint64_t is = __ballot(lane < kGroup && e < A.n_vocab && load_one<kF32>(A, row, min(e, A.n_vocab - 1)) == top);
             if (lane == 0) give(A, row, S.found * kGroup + __builtin_ctzll(is), 1.0);
@@ -659,15 +716,20 @@ __global__ __launch_bounds__(kThreads) void pick_kernel(const Args A) {
     }
     double all = 0.0;   // of all weights
     if (needs_sum(R)) {
-        const double mine = lane < A.parts && pm > -INFINITY ? A.part_sum[(size_t)row * A.parts + lane] * weight(pm, top, R.c, S.table) : 0.0;
-        const double upto = wave_scan(mine);
-        all = __shfl(upto, 63);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) ps[u] = pm[u] > -INFINITY ? ps[u] * weight(pm[u], top, R.c, S.table) : 0.0;
+        const double mine = ps[0] + ps[1], upto = wave_scan(mine);
+        all = lane_of(upto, 63);
         if (!cuts_p(R) && !cuts_m(R)) {   // nothing is cut off
             const double target = R.u * all;
             const uint64_t over = __ballot(mine > 0.0 && upto > target), any = __ballot(mine > 0.0);
-            const int part = over ? __builtin_ctzll(over) : 63 - __builtin_clzll(any);
-            const double before = __shfl(upto - mine, part);
-            draw<8>(A, S, RowSource<kF32>{A, row, part * kPart, min(kPart, A.n_vocab - part * kPart)}, R, row, top, 0, target - before, all);
+            if (!any) return;   // (the largest logit's part weighs something)
+            const int pair = over ? __builtin_ctzll(over) : 63 - __builtin_clzll(any);
+            const double first = lane_of(ps[0], pair), begin = lane_of(upto - mine, pair);
+            const bool second = !(first > 0.0 && begin + first > target) && lane_of(ps[1], pair) > 0.0;
+            const int part = 2 * pair + second;
+            draw<8>(A, S, RowSource<kF32, 1>{A, row, part * kPart, min(kPart, A.n_vocab - part * kPart)}, R, row, top, 0,
+                    target - (second ? begin + first : begin), all);
             return;
         }
     }
@@ -726,7 +788,7 @@ __global__ __launch_bounds__(kThreads) void pick_kernel(const Args A) {
 #pragma unroll
             for (int u = 0; u < kGroup; ++u)
                 if (mine >> u & 1) {
-                    if (at < kList) S.key[at] = key_of(x[u >> 3][u & 7]), S.index[at] = e + u;
+                    if (at < kList) S.logit[at] = x[u >> 3][u & 7], S.index[at] = e + u;
                     ++at;
                 }
         }
@@ -742,7 +804,7 @@ __global__ __launch_bounds__(kThreads) void pick_kernel(const Args A) {
         if (cuts_p(R)) cut = cut_at<true, 1>(S, src, R, bins, 0, cut, all * kUnit);
         draw<1>(A, S, src, R, row, top, cut, 0.0, 0.0);
     } else {
-        const RowSource<kF32> src{A, row, 0, A.n_vocab};
+        const RowSource<kF32, 4> src{A, row, 0, A.n_vocab};
         unsigned long long cut = 0;
         if (R.k) cut = cut_at<false, 8>(S, src, R, bins, R.k, 0, 0.0);
         if (cuts_p(R)) cut = cut_at<true, 8>(S, src, R, bins, 0, cut, all * kUnit);
@@ -754,7 +816,7 @@ size_t up256(size_t b) { return (b + 255) & ~(size_t)255; }
 
 // The workspace, laid out from `base` (or only measured).
 size_t lay_out(Args *A, char *base, int n_rows, int n_vocab) {
-    const size_t parts = (n_vocab + kPart - 1) / kPart, groups = parts * (kPart / kGroup);
+    const size_t parts = (n_vocab + kPart * kScanParts - 1) / (kPart * kScanParts) * kScanParts, groups = parts * (kPart / kGroup);
     const size_t sums = up256(sizeof(double) * n_rows * parts), tops = up256(sizeof(float) * n_rows * parts);
     if (A) {
         A->parts = (int)parts;
@@ -802,7 +864,7 @@ extern "C" int ds4hip_sample_tokens(const ds4hip_sample *a, void *workspace, siz
     A.tokens = a->tokens;
     A.probs = a->probs;
     const hipStream_t st = (hipStream_t)stream;
-    const dim3 grid((unsigned)a->n_rows * A.parts);
+    const dim3 grid((unsigned)a->n_rows * (A.parts / kScanParts));
     if (a->logits_f32) {
         hipLaunchKernelGGL(scan_kernel<true>, grid, dim3(kScanThreads), 0, st, A);
         hipLaunchKernelGGL(pick_kernel<true>, dim3(a->n_rows), dim3(kThreads), 0, st, A);
