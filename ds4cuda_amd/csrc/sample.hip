@@ -28,12 +28,16 @@
 
 using namespace ds4hip;
 
+// (A call in a kernel of this file, anywhere, costs each launch of it 4 us: the stack that calls need.)
+#define DS4_INLINE __attribute__((always_inline))
+
 namespace {
 
 constexpr int kPart = 2048, kGroup = 32;   // logits of a part (a wave's), of a group
 constexpr int kMaxVocab = 1 << 18;         // (sums of 2^45 stay in 64 bits)
 constexpr int kScanThreads = 256, kScanParts = kScanThreads / 64;
 constexpr int kThreads = 512, kWaves = kThreads / 64;
+constexpr int kRow = 8192;       // logits of a row that has one launch
 constexpr int kBins = 2048;
 constexpr int kList = 4096;      // candidates in LDS
 constexpr int kFew = 512;        // candidates that are all compared with each other
@@ -64,7 +68,7 @@ struct Row {
     bool valid;
 };
 
-__device__ inline Row row_of(const Args &A, int row) {
+__device__ __forceinline__ Row row_of(const Args &A, int row) {
     Row R;
     const float t = A.temperature ? A.temperature[row] : A.all_temperature;
     const float p = A.top_p ? A.top_p[row] : A.all_top_p, m = A.min_p ? A.min_p[row] : A.all_min_p;
@@ -79,15 +83,15 @@ __device__ inline Row row_of(const Args &A, int row) {
     return R;
 }
 
-__device__ inline bool cuts_p(const Row &R) { return R.p < 1.0; }
-__device__ inline bool cuts_m(const Row &R) { return R.m > 0.0; }
+__device__ __forceinline__ bool cuts_p(const Row &R) { return R.p < 1.0; }
+__device__ __forceinline__ bool cuts_m(const Row &R) { return R.m > 0.0; }
 // Whether the sum of all weights is needed.
-__device__ inline bool needs_sum(const Row &R) { return R.c > 0.0 && R.k == 0 && (cuts_p(R) || !cuts_m(R)); }
+__device__ __forceinline__ bool needs_sum(const Row &R) { return R.c > 0.0 && R.k == 0 && (cuts_p(R) || !cuts_m(R)); }
 
 // 2^(t / 64) for t <= 0 (2^-1000 for all under -64000), from 2^(j/64) in LDS and the Taylor series of
 // 2^(r/64), |r| <= 1/2, up to r^4. Adding 1.5 x 2^52 rounds t to a whole number and leaves it in the low bits: 18
 // instructions, eight or more of them side by side (26 with the rounding and conversion instructions and a test).
-__device__ inline double pow2(double t, const double *table) {
+__device__ __forceinline__ double pow2(double t, const double *table) {
     constexpr double round = 6755399441055744.0, l = 0.69314718055994530942 / 64.0;
     t = fmax(t, -64000.0);
     const double s = t + round, r = t - (s - round);
@@ -117,27 +121,27 @@ struct Table {
 __constant__ const Table kTable = Table();
 
 // Weight of logit x where the row's largest is `top`; some_weight: 2^-1000 at least, also for -inf.
-__device__ inline double some_weight(float x, float top, double c, const double *table) {
+__device__ __forceinline__ double some_weight(float x, float top, double c, const double *table) {
     return pow2(((double)x - (double)top) * c, table);
 }
-__device__ inline double weight(float x, float top, double c, const double *table) {
+__device__ __forceinline__ double weight(float x, float top, double c, const double *table) {
     const double w = some_weight(x, top, c, table);
     return w > 0x1p-999 ? w : 0.0;
 }
 
 // Order of the logits as whole numbers (-0 is 0).
-__device__ inline uint32_t key_of(float x) {
+__device__ __forceinline__ uint32_t key_of(float x) {
     const uint32_t u = __float_as_uint(x + 0.0f);
     return u >> 31 ? ~u : u | 0x80000000u;
 }
-__device__ inline float value_of(uint32_t k) { return __uint_as_float(k >> 31 ? k & 0x7FFFFFFFu : ~k); }
+__device__ __forceinline__ float value_of(uint32_t k) { return __uint_as_float(k >> 31 ? k & 0x7FFFFFFFu : ~k); }
 
 // Eight logits of a row from e on (-inf past its end), as they lie in memory. Rows start at any multiple of
 // a logit's size.
 template <bool kF32>
 struct Eight {
     uint4_t v[kF32 ? 2 : 1];
-    __device__ void load(const Args &A, int row, int e) {
+    __device__ __forceinline__ void load(const Args &A, int row, int e) {
         if (kF32) {
             const float *src = static_cast<const float *>(A.logits) + row * A.stride + e;
             if (e + 8 <= A.n_vocab) {
@@ -157,18 +161,18 @@ struct Eight {
             }
         }
     }
-    __device__ float operator[](int i) const {
+    __device__ __forceinline__ float operator[](int i) const {
         return __uint_as_float(kF32 ? v[kF32 ? i >> 2 : 0][i & 3] : i & 1 ? v[0][i >> 1] & 0xFFFF0000u : v[0][i >> 1] << 16);
     }
 };
 
 template <bool kF32>
-__device__ inline float load_one(const Args &A, int row, int e) {
+__device__ __forceinline__ float load_one(const Args &A, int row, int e) {
     return kF32 ? static_cast<const float *>(A.logits)[row * A.stride + e]
                 : bf16_to_f32(static_cast<const uint16_t *>(A.logits)[row * A.stride + e]);
 }
 
-__device__ inline float wave_max(float v) {
+__device__ __forceinline__ float wave_max(float v) {
 #pragma unroll
     for (int off = 32; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor(v, off));
     return v;
@@ -225,6 +229,7 @@ __global__ __launch_bounds__(kScanThreads) void scan_kernel(const Args A) {
 struct Pick {
     double table[64];
     double sums[kWaves];
+    float tops[kWaves];
     unsigned long long scans[kWaves];
     int counts[kWaves];
     unsigned long long bins[kBins];        // weights, or numbers, of tokens
@@ -239,10 +244,10 @@ struct Pick {
 };
 
 // A token's place in the order of logits, as a whole number: the highest first, equal logits by index.
-__device__ inline unsigned long long place_of(uint32_t key, uint32_t index) { return (unsigned long long)key << 32 | ~index; }
+__device__ __forceinline__ unsigned long long place_of(uint32_t key, uint32_t index) { return (unsigned long long)key << 32 | ~index; }
 
 template <int kCtrl, int kRowMask, typename T>
-__device__ inline T dpp_or_0(T v) {
+__device__ __forceinline__ T dpp_or_0(T v) {
     if constexpr (sizeof(T) == 4) {
         return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), kCtrl, kRowMask, 0xF, false));
     } else {
@@ -255,7 +260,7 @@ __device__ inline T dpp_or_0(T v) {
 
 // Inclusive sum over the wave's lanes: in rows of 16, then the last lanes of the rows before.
 template <typename T>
-__device__ inline T wave_scan(T x) {
+__device__ __forceinline__ T wave_scan(T x) {
     x += dpp_or_0<0x111, 0xF>(x);   // the lane 1, 2, 4, 8 before
     x += dpp_or_0<0x112, 0xF>(x);
     x += dpp_or_0<0x114, 0xF>(x);
@@ -266,7 +271,7 @@ __device__ inline T wave_scan(T x) {
 }
 
 template <typename T>
-__device__ inline T lane_of(T v, int lane) {
+__device__ __forceinline__ T lane_of(T v, int lane) {
     if constexpr (sizeof(T) == 4) {
         return __builtin_bit_cast(T, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
     } else {
@@ -280,7 +285,7 @@ __device__ inline T lane_of(T v, int lane) {
 // Inclusive sum over the workgroup's threads, in their order; *total: of all. (Every wave sums the
 // waves' sums in its own lanes: with each thread adding them up, a sum took half a microsecond.)
 template <typename T>
-__device__ inline T block_scan(T v, T *sums, T *total) {
+__device__ __forceinline__ T block_scan(T v, T *sums, T *total) {
     static_assert(kWaves <= 16, "the waves' sums lie in a row of lanes");
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const T x = wave_scan(v);
@@ -296,7 +301,7 @@ __device__ inline T block_scan(T v, T *sums, T *total) {
     return w ? lane_of(y, w - 1) + x : x;
 }
 
-__device__ inline void give(const Args &A, int row, int token, double share) {
+__device__ __forceinline__ void give(const Args &A, int row, int token, double share) {
     A.tokens[row] = token;
     A.probs[row] = (float)share;
 }
@@ -311,13 +316,13 @@ struct ListSource {
     template <int kEach>
     struct Some {
         float x[kEach];
-        __device__ void load(const ListSource &L, int i) {
+        __device__ __forceinline__ void load(const ListSource &L, int i) {
 #pragma unroll
             for (int u = 0; u < kEach; ++u) x[u] = i + u < L.n ? L.S.logit[i + u] : -INFINITY;
         }
-        __device__ float operator()(const ListSource &, int, int u) const { return x[u]; }
+        __device__ __forceinline__ float operator()(const ListSource &, int, int u) const { return x[u]; }
     };
-    __device__ int index(int i) const { return S.index[i]; }
+    __device__ __forceinline__ int index(int i) const { return S.index[i]; }
 };
 template <bool kF32, int kAhead>
 struct RowSource {
@@ -325,20 +330,21 @@ struct RowSource {
     int row, first, n;   // logits first .. first + n - 1 of the row
     static constexpr int kDeep = kAhead;
     static constexpr bool kList = false;
+    __device__ __forceinline__ RowSource<kF32, 1> slow() const { return {A, row, first, n}; }   // (less code)
     template <int kEach>
     struct Some {
         static_assert(kEach == 8, "as the loads are");
         Eight<kF32> x;
-        __device__ void load(const RowSource &L, int i) { x.load(L.A, L.row, min(L.first + i, L.A.n_vocab)); }   // (past the end: nothing is read)
-        __device__ float operator()(const RowSource &L, int i, int u) const { return i + u < L.n ? x[u] : -INFINITY; }
+        __device__ __forceinline__ void load(const RowSource &L, int i) { x.load(L.A, L.row, min(L.first + i, L.A.n_vocab)); }   // (past the end: nothing is read)
+        __device__ __forceinline__ float operator()(const RowSource &L, int i, int u) const { return i + u < L.n ? x[u] : -INFINITY; }
     };
-    __device__ int index(int i) const { return first + i; }
+    __device__ __forceinline__ int index(int i) const { return first + i; }
 };
 
 // use(i, logits) for all of a source, kEach * kThreads at a time. kDeep of them are loaded while those before
 // are used (memory is 2 us away: with one of them ahead, converted as it came, a pass of 65536 took 28 us).
 template <int kEach, typename Source, typename Use>
-__device__ inline void each_tile(const Source &src, Use use) {
+__device__ __forceinline__ void each_tile(const Source &src, Use use) {
     constexpr int kStep = kEach * kThreads, kDeep = Source::kDeep;
     typename Source::template Some<kEach> next[kDeep];
     int i = kEach * threadIdx.x;
@@ -365,7 +371,7 @@ __device__ inline void each_tile(const Source &src, Use use) {
 
 constexpr double kUnit = 35184372088832.0;   // 2^45
 // (adding 2^52 rounds to a whole number and leaves it in the low bits)
-__device__ inline unsigned long long units(double w) {
+__device__ __forceinline__ unsigned long long units(double w) {
     return (unsigned long long)__double_as_longlong(fma(w, kUnit, 4503599627370496.0)) & 0xFFFFFFFFFFFFFull;
 }
 
@@ -373,16 +379,16 @@ __device__ inline unsigned long long units(double w) {
 // 2^-63.9. What is rounded on the way grows with the distance, so the bins keep the order of logits.
 struct Bins {
     float top, scale;
-    __device__ float steps(float x) const { return fminf((top - x) * scale, (float)(kBins - 1)); }
-    __device__ int operator()(float x) const { return kBins - 1 - (int)steps(x); }
+    __device__ __forceinline__ float steps(float x) const { return fminf((top - x) * scale, (float)(kBins - 1)); }
+    __device__ __forceinline__ int operator()(float x) const { return kBins - 1 - (int)steps(x); }
     // of x in its bin: the part of kBins that it lies in
-    __device__ int part(float x) const {
+    __device__ __forceinline__ int part(float x) const {
         const float d = steps(x);
         return kBins - 1 - (int)((d - floorf(d)) * (float)kBins);
     }
 };
 
-__device__ inline void clear_bins(Pick &S) {
+__device__ __forceinline__ void clear_bins(Pick &S) {
 #pragma unroll
     for (int i = 0; i < kBins; i += kThreads) S.bins[i + threadIdx.x] = 0;
     __syncthreads();
@@ -390,7 +396,7 @@ __device__ inline void clear_bins(Pick &S) {
 
 // After a barrier: the first bin, from the highest down, at which the bins' sum reaches need (-1: none), and in
 // S.found_above the sum of those above it. share: need is that of the bins' sum instead.
-__device__ inline int find_bin(Pick &S, unsigned long long *need, double share = 0.0) {
+__device__ __forceinline__ int find_bin(Pick &S, unsigned long long *need, double share = 0.0) {
     constexpr int kEach = kBins / kThreads;
     const int hi = kBins - 1 - kEach * (int)threadIdx.x;
     unsigned long long x[kEach], sum = 0, all;
@@ -424,13 +430,13 @@ struct Search {
 };
 
 template <bool kWeigh>
-__device__ inline unsigned long long amount(const Pick &S, const Row &R, const Bins &bins, float x) {
+__device__ __forceinline__ unsigned long long amount(const Pick &S, const Row &R, const Bins &bins, float x) {
     return kWeigh ? units(weight(x, bins.top, R.c, S.table)) : 1;
 }
 
 // Whether a token lies in the bins of `levels` levels.
 template <typename Source>
-__device__ inline bool inside(const Search &Q, const Bins &bins, const Source &src, float x, int i, int levels) {
+__device__ __forceinline__ bool inside(const Search &Q, const Bins &bins, const Source &src, float x, int i, int levels) {
     const int b = bins(x);
     if (b == 0 || (levels > 0 && b != Q.bin[0]) || (levels > 1 && bins.part(x) != Q.bin[1])) return false;
     if (!Q.within && Q.below == 64) return true;
@@ -441,10 +447,10 @@ __device__ inline bool inside(const Search &Q, const Bins &bins, const Source &s
 // use(item, logit) for the tokens of a source that are inside the found bins, one of a lane at a time: they are few, and
 // in different lanes. Most of the others are known by two comparisons.
 template <int kEach, typename Source, typename Use>
-__device__ inline void each_inside(const Search &Q, const Bins &bins, const Source &src, Use use) {
+__device__ __forceinline__ void each_inside(const Search &Q, const Bins &bins, const Source &src, Use use) {
     const float near = (float)(kBins - 1 - Q.bin[0]) / bins.scale, far = (float)(kBins - Q.bin[0]) / bins.scale,
                 slack = 1e-6f * (fabsf(bins.top) + far), from = bins.top - far - slack, to = bins.top - near + slack;
-    each_tile<kEach>(src, [&](int i, const float *x) {
+    each_tile<kEach>(src, [&](int i, const float *x) DS4_INLINE {
         uint32_t mine = 0;
 #pragma unroll
         for (int u = 0; u < kEach; ++u) mine |= x[u] < from || x[u] > to ? 0 : 1u << u;
@@ -461,7 +467,7 @@ __device__ inline void each_inside(const Search &Q, const Bins &bins, const Sour
 
 // The place, among the n <= kNear tokens in S.near.
 template <bool kWeigh>
-__device__ inline unsigned long long cut_near(Pick &S, int n, const Row &R, const Bins &bins, unsigned long long need) {
+__device__ __forceinline__ unsigned long long cut_near(Pick &S, int n, const Row &R, const Bins &bins, unsigned long long need) {
     const int tid = threadIdx.x;
     if (kWeigh) {
         if (tid < n) S.near_w[tid] = amount<true>(S, R, bins, value_of((uint32_t)(S.near[tid] >> 32)));
@@ -480,11 +486,11 @@ __device__ inline unsigned long long cut_near(Pick &S, int n, const Row &R, cons
 
 // The tokens that are inside, counted in S.n_near; the first kNear of them in S.near.
 template <int kEach, typename Source>
-__device__ inline int gather_near(Pick &S, const Search &Q, const Bins &bins, const Source &src) {
+__device__ __forceinline__ int gather_near(Pick &S, const Search &Q, const Bins &bins, const Source &src) {
     __syncthreads();
     if (threadIdx.x == 0) S.n_near = 0;
     __syncthreads();
-    each_inside<kEach>(Q, bins, src, [&](int at, float x) {
+    each_inside<kEach>(Q, bins, src, [&](int at, float x) DS4_INLINE {
         const int to = atomicAdd(&S.n_near, 1);
         if (to < kNear) S.near[to] = place_of(key_of(x), src.index(at));
     });
@@ -494,13 +500,13 @@ __device__ inline int gather_near(Pick &S, const Search &Q, const Bins &bins, co
 
 // From the second level on: parts of the weight's bin, then digits of the places, which all differ, until kNear are left.
 template <bool kWeigh, int kEach, typename Source>
-__device__ inline unsigned long long cut_inside(Pick &S, Search Q, const Row &R, const Bins &bins, const Source &src) {
+__device__ __forceinline__ unsigned long long cut_inside(Pick &S, Search Q, const Row &R, const Bins &bins, const Source &src) {
     while (true) {
         const int n = gather_near<kEach>(S, Q, bins, src);
         if (n <= kNear) return cut_near<kWeigh>(S, n, R, bins, Q.need);
         const int shift = Q.level == 1 ? 64 : Q.below - min(Q.below, 11);
         clear_bins(S);
-        each_inside<kEach>(Q, bins, src, [&](int at, float x) {
+        each_inside<kEach>(Q, bins, src, [&](int at, float x) DS4_INLINE {
             const int b = shift == 64 ? bins.part(x)
                                       : (int)(place_of(key_of(x), src.index(at)) >> shift & ((1ull << (Q.below - shift)) - 1));
             atomicAdd(&S.bins[b], amount<kWeigh>(S, R, bins, x));
@@ -522,11 +528,11 @@ __device__ inline unsigned long long cut_inside(Pick &S, Search Q, const Row &R,
 // their weights' sum is under the share p of `all` units; all 0: of their sum). 0: all of them. What is in the
 // weight's bin that has it goes to the list, where that is not the source and holds it.
 template <bool kWeigh, int kEach, typename Source>
-__device__ inline unsigned long long cut_at(Pick &S, const Source &src, const Row &R, const Bins &bins, int k,
+__device__ __forceinline__ unsigned long long cut_at(Pick &S, const Source &src, const Row &R, const Bins &bins, int k,
                                             unsigned long long within, double all) {
     Search Q = {kWeigh ? max((unsigned long long)ceil(R.p * all), 1ull) : (unsigned long long)k, within, 0, 0, 64, {0, 0}};
     clear_bins(S);
-    each_tile<kEach>(src, [&](int i, const float *x) {
+    each_tile<kEach>(src, [&](int i, const float *x) DS4_INLINE {
         unsigned long long w[kEach];
 #pragma unroll
         for (int u = 0; u < kEach; ++u) w[u] = amount<kWeigh>(S, R, bins, x[u]);
@@ -544,13 +550,13 @@ __device__ inline unsigned long long cut_at(Pick &S, const Source &src, const Ro
     if constexpr (Source::kList) {
         return cut_inside<kWeigh, kEach>(S, Q, R, bins, src);
     } else {
-        each_inside<kEach>(Q, bins, src, [&](int at, float x) {
+        each_inside<kEach>(Q, bins, src, [&](int at, float x) DS4_INLINE {
             const int to = atomicAdd(&S.n_list, 1);
             if (to < kList) S.logit[to] = x, S.index[to] = src.index(at);
         });
         __syncthreads();
         const int n = S.n_list;
-        return n <= kList ? cut_inside<kWeigh, 1>(S, Q, R, bins, ListSource{S, n}) : cut_inside<kWeigh, kEach>(S, Q, R, bins, src);
+        return n <= kList ? cut_inside<kWeigh, 1>(S, Q, R, bins, ListSource{S, n}) : cut_inside<kWeigh, kEach>(S, Q, R, bins, src.slow());
     }
 }
 
@@ -558,13 +564,13 @@ __device__ inline unsigned long long cut_at(Pick &S, const Source &src, const Ro
 // at least) passes the target, u of their sum, or the one given with the sum of all. A wave's kEach * 64 tokens
 // are summed together; the wave in which the target lies is looked through again.
 template <int kEach, typename Source>
-__device__ inline void draw(const Args &A, Pick &S, const Source &src, const Row &R, int row, float top, unsigned long long cut,
+__device__ __forceinline__ void draw(const Args &A, Pick &S, const Source &src, const Row &R, int row, float top, unsigned long long cut,
                             double target, double all) {
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
     const float cut_logit = cut ? value_of((uint32_t)(cut >> 32)) : -INFINITY;
     const int cut_index = (int)~(uint32_t)cut;
     const double least = fmax(R.m, 0x1p-999);   // (weight()'s 0)
-    auto weights = [&](int i, const float *logit, double *x) {
+    auto weights = [&](int i, const float *logit, double *x) DS4_INLINE {
         double sum = 0.0;
 #pragma unroll
         for (int u = 0; u < kEach; ++u) {
@@ -577,7 +583,7 @@ __device__ inline void draw(const Args &A, Pick &S, const Source &src, const Row
     };
     double x[kEach], sum = 0.0;
     int n_sums = 0;
-    each_tile<kEach>(src, [&](int i, const float *logit) {
+    each_tile<kEach>(src, [&](int i, const float *logit) DS4_INLINE {
         sum = weights(i, logit, x);
         const double upto = wave_scan(sum);
         if (lane == 63) S.wave_sum[n_sums + w] = upto;
@@ -631,7 +637,7 @@ __device__ inline void draw(const Args &A, Pick &S, const Source &src, const Row
 
 // The same and the cuts for a list of at most kFew candidates: each is compared with all others, by as many threads
 // side by side as there are for it, which gives its rank and the weights before it at once. All sums are units.
-__device__ inline void pick_few(const Args &A, Pick &S, int n, const Row &R, int row, float top, double all) {
+__device__ __forceinline__ void pick_few(const Args &A, Pick &S, int n, const Row &R, int row, float top, double all) {
     const int tid = threadIdx.x;
     if (tid < n) {
         S.near[tid] = place_of(key_of(S.logit[tid]), S.index[tid]);
@@ -670,6 +676,134 @@ __device__ inline void pick_few(const Args &A, Pick &S, int n, const Row &R, int
     const unsigned long long upto = block_scan(in ? w : 0, S.scans, &total);
     const unsigned long long target = (unsigned long long)(R.u * (double)total);   // the sum passes it: at least one more
     if (in && upto > target && upto - w <= target) give(A, row, (int)~(uint32_t)mine, (double)w / (double)total);
+}
+
+// The least logit of a candidate, from the lowest bin that all that is kept lies in (as one logit, with room for what is
+// rounded: more candidates do no harm). min-p gives a border too (the exact test comes later), but for
+// those that top-p counts among the first k.
+__device__ __forceinline__ float least_of(const Row &R, const Bins &bins, int border) {
+    const float top = bins.top, floor_m = cuts_m(R) ? top + (float)(64.0 * log2(R.m) / R.c) : -INFINITY;
+    const float least = floor_m > -INFINITY && !(R.k && cuts_p(R)) ? fminf(floor_m - 1e-5f * (fabsf(top) + fabsf(floor_m) + 1e-30f), top) : -INFINITY;
+    const float reach = (float)(kBins - border) / bins.scale;
+    return fmaxf(least, top - reach - 1e-6f * (fabsf(top) + reach));
+}
+
+// The n candidates in the list, or where it does not hold them the whole row: cut, and the token.
+template <bool kF32>
+__device__ __forceinline__ void settle(const Args &A, Pick &S, const Row &R, int row, const Bins &bins, int n, double all) {
+    const float top = bins.top;
+    if (n <= kFew) {
+        pick_few(A, S, n, R, row, top, all);
+    } else if (n <= kList) {
+        const ListSource src{S, n};
+        unsigned long long cut = 0;
+        if (R.k) cut = cut_at<false, 1>(S, src, R, bins, R.k, 0, 0.0);
+        if (cuts_p(R)) cut = cut_at<true, 1>(S, src, R, bins, 0, cut, all * kUnit);
+        draw<1>(A, S, src, R, row, top, cut, 0.0, 0.0);
+    } else {
+        const RowSource<kF32, 2> src{A, row, 0, A.n_vocab};
+        unsigned long long cut = 0;
+        if (R.k) cut = cut_at<false, 8>(S, src, R, bins, R.k, 0, 0.0);
+        if (cuts_p(R)) cut = cut_at<true, 8>(S, src, R, bins, 0, cut, all * kUnit);
+        draw<8>(A, S, src, R, row, top, cut, 0.0, 0.0);
+    }
+}
+
+// Rows of up to kRow logits, a workgroup each and one launch: sixteen logits of a thread in registers.
+template <bool kF32>
+__global__ __launch_bounds__(kThreads) void row_kernel(const Args A) {
+    static_assert(kRow == 16 * kThreads, "sixteen a thread");
+    __shared__ Pick S;
+    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, row = blockIdx.x;
+    Eight<kF32> x[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) x[j].load(A, row, min(j * (kRow / 2) + 8 * tid, A.n_vocab));
+    const Row R = row_of(A, row);
+    if (tid < 64) S.table[tid] = kTable.v[tid];
+    if (tid == 0) S.found = 0x7FFFFFFF;
+    float top = -INFINITY;
+    bool odd = false;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            top = fmaxf(top, x[j][u]);
+            odd = odd || !(x[j][u] < INFINITY);
+        }
+    odd = __any(odd);
+    top = wave_max(top);
+    if (lane == 0) S.tops[w] = odd ? __builtin_nanf("") : top;
+    clear_bins(S);
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) {
+        odd = odd || S.tops[i] != S.tops[i];
+        top = fmaxf(top, S.tops[i]);
+    }
+    if (odd || !(top > -INFINITY) || !R.valid) {
+        if (tid == 0) give(A, row, -1, __builtin_nan(""));
+        return;
+    }
+    if (R.c == 0.0) {
+#pragma unroll
+        for (int j = 1; j >= 0; --j)
+#pragma unroll
+            for (int u = 7; u >= 0; --u)
+                if (x[j][u] == top) atomicMin(&S.found, j * (kRow / 2) + 8 * tid + u);
+        __syncthreads();
+        if (tid == 0) give(A, row, S.found, 1.0);
+        return;
+    }
+    if (!R.k && !cuts_p(R) && !cuts_m(R)) {   // nothing is cut off
+        draw<8>(A, S, RowSource<kF32, 2>{A, row, 0, A.n_vocab}, R, row, top, 0, 0.0, 0.0);
+        return;
+    }
+    const Bins bins{top, (float)fmin(R.c * 0.5, 1e30)};
+    double all = 0.0;   // of all weights
+    int border = 1;
+    if (R.k || cuts_p(R)) {   // as in pick_kernel, with the tokens themselves
+        double sum = 0.0;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            unsigned long long n[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const double y = R.k ? 0.0 : weight(x[j][u], top, R.c, S.table);
+                sum += y;
+                n[u] = R.k ? 1 : units(y);
+            }
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const int b = bins(x[j][u]);
+                if (b && n[u]) atomicAdd(&S.bins[b], n[u]);
+            }
+        }
+        if (!R.k) block_scan(sum, S.sums, &all);
+        __syncthreads();
+        unsigned long long need = R.k ? R.k : (unsigned long long)(R.p * all * kUnit) + kRow;
+        border = max(find_bin(S, &need), 1);
+    }
+    const float from = least_of(R, bins, border);
+    // the candidates, by index: first those of the first half
+    uint32_t mine[2] = {0, 0};
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int u = 0; u < 8; ++u) mine[j] |= x[j][u] >= from && x[j][u] > -INFINITY ? 1u << u : 0;
+    const int both = (int)(__popc(mine[0]) | __popc(mine[1]) << 16);
+    int found;
+    const int before = block_scan(both, S.counts, &found) - both, n = (found & 0xFFFF) + (found >> 16);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        int at = j ? (found & 0xFFFF) + (before >> 16) : before & 0xFFFF;
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+            if (mine[j] >> u & 1) {
+                if (at < kList) S.logit[at] = x[j][u], S.index[at] = j * (kRow / 2) + 8 * tid + u;
+                ++at;
+            }
+    }
+    __syncthreads();
+    settle<kF32>(A, S, R, row, bins, n, all);
 }
 
 template <bool kF32>
@@ -753,13 +887,8 @@ __global__ __launch_bounds__(kThreads) void pick_kernel(const Args A) {
         unsigned long long need = R.k ? R.k : (unsigned long long)(R.p * all * kUnit) + A.groups;
         border = max(find_bin(S, &need), 1);
     }
-    // min-p is a border too (the exact test comes later), but for those that top-p counts among the first k
-    const float floor_m = cuts_m(R) ? top + (float)(64.0 * log2(R.m) / R.c) : -INFINITY;
-    const float least = floor_m > -INFINITY && !(R.k && cuts_p(R)) ? fminf(floor_m - 1e-5f * (fabsf(top) + fabsf(floor_m) + 1e-30f), top) : -INFINITY;
-    // (as one logit, with room for what is rounded: more candidates do no harm)
-    const float reach = (float)(kBins - border) / bins.scale;
-    const float from = fmaxf(least, top - reach - 1e-6f * (fabsf(top) + reach));
-    auto in = [&](float x) { return x >= from && x > -INFINITY; };
+    const float from = least_of(R, bins, border);
+    auto in = [&](float x) DS4_INLINE { return x >= from && x > -INFINITY; };
     // the groups that have a candidate, by index
     int n_groups = 0;
     {
@@ -795,21 +924,7 @@ __global__ __launch_bounds__(kThreads) void pick_kernel(const Args A) {
         n += found;
     }
     __syncthreads();
-    if (n <= kFew) {
-        pick_few(A, S, n, R, row, top, all);
-    } else if (n <= kList) {
-        const ListSource src{S, n};
-        unsigned long long cut = 0;
-        if (R.k) cut = cut_at<false, 1>(S, src, R, bins, R.k, 0, 0.0);
-        if (cuts_p(R)) cut = cut_at<true, 1>(S, src, R, bins, 0, cut, all * kUnit);
-        draw<1>(A, S, src, R, row, top, cut, 0.0, 0.0);
-    } else {
-        const RowSource<kF32, 4> src{A, row, 0, A.n_vocab};
-        unsigned long long cut = 0;
-        if (R.k) cut = cut_at<false, 8>(S, src, R, bins, R.k, 0, 0.0);
-        if (cuts_p(R)) cut = cut_at<true, 8>(S, src, R, bins, 0, cut, all * kUnit);
-        draw<8>(A, S, src, R, row, top, cut, 0.0, 0.0);
-    }
+    settle<kF32>(A, S, R, row, bins, n, all);
 }
 
 size_t up256(size_t b) { return (b + 255) & ~(size_t)255; }
@@ -865,6 +980,10 @@ extern "C" int ds4hip_sample_tokens(const ds4hip_sample *a, void *workspace, siz
     A.probs = a->probs;
     const hipStream_t st = (hipStream_t)stream;
     const dim3 grid((unsigned)a->n_rows * (A.parts / kScanParts));
+    if (a->n_vocab <= kRow) {
+        hipLaunchKernelGGL(a->logits_f32 ? row_kernel<true> : row_kernel<false>, dim3(a->n_rows), dim3(kThreads), 0, st, A);
+        return ds4hip_set_last_error(hip_status(hipGetLastError()));
+    }
     if (a->logits_f32) {
         hipLaunchKernelGGL(scan_kernel<true>, grid, dim3(kScanThreads), 0, st, A);
         hipLaunchKernelGGL(pick_kernel<true>, dim3(a->n_rows), dim3(kThreads), 0, st, A);
