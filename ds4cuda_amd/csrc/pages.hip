@@ -19,6 +19,7 @@
 #include "../../include/ds4hip_pages.h"
 
 #include <algorithm>
+#include <type_traits>
 
 using namespace ds4hip;
 
@@ -469,38 +470,26 @@ __global__ __launch_bounds__(256) void move_kernel(const ds4hip_kv_pages P, cons
 
 constexpr int kNodes = DS4HIP_TREE_MAX_NODES;
 
-// One wave a tree: from node 0 to the first child whose token is its parent's target, and so on. The tree lies
-// in LDS; a step is a look at 64 nodes at a time behind the last one (children follow their parents).
-__global__ __launch_bounds__(64) void walk_kernel(const int32_t *q_start, int n_jobs, const int32_t *parents, const int32_t *tokens,
-                                                  const int32_t *targets, int n_nodes, int32_t *path, int32_t *n_path,
-                                                  int32_t *next) {
-    __shared__ int parent_s[kNodes], token_s[kNodes], target_s[kNodes];
-    const int j = blockIdx.x, lane = threadIdx.x;
-    const int a = q_start[j], b = q_start[j + 1], n = b - a;
-    // nodes that no job names
-    if (j == 0)
-        for (int i = lane; i < min(a, n_nodes); i += 64) path[i] = -1;
-    if (j == n_jobs - 1)
-        for (int i = max(b, 0) + lane; i < n_nodes; i += 64) path[i] = -1;
-    if (a < 0 || b > n_nodes || n <= 0 || n > kNodes) {   // (the plan refuses what is not 0 nodes)
-        if (lane == 0) n_path[j] = 0, next[j] = -1;
-        return;
-    }
-    for (int i = lane; i < n; i += 64) {
-        parent_s[i] = parents[a + i];
-        token_s[i] = tokens[a + i];
-        target_s[i] = targets[a + i];
-    }
-    __syncthreads();
+// What walks read and write.
+struct Walk {
+    const int32_t *parents, *tokens, *targets;
+    int32_t *path, *n_path, *next;
+};
+
+// One wave: job j's path, from node 0 to the first child whose token is its parent's target, and so on; returns its
+// length. The tree's nodes lie in LDS at parent, token and target; a step is a look at 64 of them at a time behind
+// the last one (children follow their parents).
+__device__ inline int walk(const Walk &W, int j, int a, int n, const int *parent, const int *token, const int *target) {
+    const int lane = threadIdx.x & 63;
     int at = 0, length = 0, says;
     while (true) {
-        if (lane == 0) path[a + length] = at;
+        if (lane == 0) W.path[a + length] = at;
         ++length;
-        says = target_s[at];
+        says = target[at];
         int child = -1;
         for (int c0 = at + 1; says >= 0 && c0 < n; c0 += 64) {
-            const int c = c0 + lane;
-            const uint64_t fits = __ballot(c < n && parent_s[min(c, n - 1)] == at && token_s[min(c, n - 1)] == says);
+            const int c = min(c0 + lane, n - 1);
+            const uint64_t fits = __ballot(c0 + lane < n && parent[c] == at && token[c] == says);
             if (fits) {
                 child = c0 + __builtin_ctzll(fits);
                 break;
@@ -509,28 +498,105 @@ __global__ __launch_bounds__(64) void walk_kernel(const int32_t *q_start, int n_
         if (child < 0) break;
         at = child;
     }
-    for (int i = length + lane; i < n; i += 64) path[a + i] = -1;
+    for (int i = length + lane; i < n; i += 64) W.path[a + i] = -1;
     if (lane == 0) {
-        n_path[j] = length;
-        next[j] = says;
+        W.n_path[j] = length;
+        W.next[j] = says;
+    }
+    return length;
+}
+
+// -1 for the nodes that no job names, before the first job's and behind the last one's.
+__device__ inline void clear_path(const Walk &W, const int32_t *q_start, int n_jobs, int n_nodes, int tid, int threads) {
+    for (int i = tid; i < min(q_start[0], n_nodes); i += threads) W.path[i] = -1;
+    for (int i = max(q_start[n_jobs], 0) + tid; i < n_nodes; i += threads) W.path[i] = -1;
+}
+
+// A workgroup a job, of one wave, for calls of many nodes (the planning workgroup walks the others itself).
+__global__ __launch_bounds__(64) void walk_kernel(const int32_t *q_start, int n_jobs, int n_nodes, const Walk W) {
+    __shared__ int parent_s[kNodes], token_s[kNodes], target_s[kNodes];
+    const int j = blockIdx.x, lane = threadIdx.x;
+    const int a = q_start[j], b = q_start[j + 1], n = b - a;
+    if (j == 0) clear_path(W, q_start, n_jobs, n_nodes, lane, 64);
+    if (a < 0 || b > n_nodes || n <= 0 || n > kNodes) {   // (the plan refuses what is not 0 nodes)
+        if (lane == 0) W.n_path[j] = 0, W.next[j] = -1;
+        return;
+    }
+    for (int i = lane; i < n; i += 64) {
+        parent_s[i] = W.parents[a + i];
+        token_s[i] = W.tokens[a + i];
+        target_s[i] = W.targets[a + i];
+    }
+    __syncthreads();
+    walk(W, j, a, n, parent_s, token_s, target_s);
+}
+
+// Nodes of a call whose planning workgroup finds the paths itself: a launch less, all nodes loaded at once, and
+// all jobs' paths followed at once, a thread each, through the one child of each node that agrees. (64 jobs of 1195
+// nodes: the plan with it 9 us, with a wave a tree there 16, with walk_kernel before it 4.7 + 7.1.)
+constexpr int kWalkNodes = 4096;
+
+struct Trees {
+    int parent[kWalkNodes], token[kWalkNodes], target[kWalkNodes], next[kWalkNodes], start[kJobs + 1];
+};
+
+// All threads; length[j] receives the nodes of job j's path.
+__device__ inline void walk_all(const Walk &W, Trees &T, const int32_t *q_start, int n_jobs, int n_nodes, int *length) {
+    const int tid = threadIdx.x;
+    for (int i = tid; i < n_nodes; i += kThreads) {
+        T.parent[i] = W.parents[i];
+        T.token[i] = W.tokens[i];
+        T.target[i] = W.targets[i];
+        T.next[i] = kWalkNodes;
+    }
+    for (int i = tid; i <= n_jobs; i += kThreads) T.start[i] = q_start[i];
+    __syncthreads();
+    // the nodes of job j, none where the plan refuses them
+    auto nodes_of = [&](int j) {
+        const int a = T.start[j], b = T.start[j + 1];
+        return a >= 0 && b <= n_nodes && b - a <= kNodes ? b - a : 0;
+    };
+    for (int i = tid; i < n_nodes; i += kThreads) {
+        const int j = job_of(T.start, n_jobs, i), a = T.start[j], v = i - a, p = T.parent[i];
+        if (v > 0 && v < nodes_of(j) && p >= 0 && p < v && T.target[a + p] >= 0 && T.token[i] == T.target[a + p]) atomicMin(&T.next[a + p], v);
+    }
+    __syncthreads();
+    if (tid < n_jobs) {
+        const int a = T.start[tid], n = nodes_of(tid);
+        int k = 0, at = 0, says = -1;
+        while (at < n) {   // (kWalkNodes: no child agrees)
+            W.path[a + k++] = at;
+            says = T.target[a + at];
+            const int to = T.next[a + at];
+            at = to > at ? to : n;   // (a child comes later; where q_start goes back, trees lie over each other)
+        }
+        length[tid] = k;
+        W.n_path[tid] = k;
+        W.next[tid] = says;
+    }
+    __syncthreads();
+    for (int i = tid; i < n_nodes; i += kThreads) {
+        const int j = job_of(T.start, n_jobs, i), v = i - T.start[j];
+        if (v < 0 || v >= length[j]) W.path[i] = -1;   // (before the first job's nodes, behind a path, or behind the last job's)
     }
 }
 
 // Checks the jobs' paths, cuts their sequences and releases the pages behind them. kAccept: a refused call
-// takes back what the walk wrote.
-template <bool kAccept>
+// takes back what the walks wrote; kWalk: they are walked here.
+template <bool kAccept, bool kWalk>
 __global__ __launch_bounds__(kThreads) void keep_kernel(const ds4hip_kv_pages P, const int32_t *seqs, const int32_t *q_start,
-                                                        int n_jobs, int n_nodes, int32_t *path, int32_t *n_path, int32_t *next,
-                                                        const Moves M) {
+                                                        int n_jobs, int n_nodes, const Walk W, const Moves M) {
     __shared__ Plan S;
     __shared__ int kept_s[kJobs], nodes_s[kJobs];
+    __shared__ std::conditional_t<kWalk, Trees, int> T;
     const int tid = threadIdx.x, shift = __builtin_ctz(P.page_rows);
     start(S, P.n_seqs);
+    if constexpr (kWalk) walk_all(W, T, q_start, n_jobs, n_nodes, kept_s);
     int seq = -1, base = -1, n = 0, kept = 0, held_pages = 0;
     if (tid < n_jobs) {
         const int a = q_start[tid], b = q_start[tid + 1];
         seq = seqs[tid];
-        kept = n_path[tid];
+        kept = kWalk ? kept_s[tid] : W.n_path[tid];
         const long long count = (long long)b - a;
         if (a < 0 || count < 0 || b > n_nodes || seq < 0 || seq >= P.n_seqs || !first_named(S, seq) || kept < 0 || kept > count ||
             count > P.rows[seq] || (kAccept && count > kNodes) || pages_of(P, P.rows[seq]) > P.table_stride) {
@@ -562,7 +628,7 @@ __global__ __launch_bounds__(kThreads) void keep_kernel(const ds4hip_kv_pages P,
         if (!kAccept)
             for (int i = tid; i < rows; i += kThreads) {   // nodes in order
                 const int j = job_of(S.more, n_jobs, i), k = i - S.more[j];
-                const int v = path[nodes_s[j] + k], before = k ? path[nodes_s[j] + k - 1] : -1;
+                const int v = W.path[nodes_s[j] + k], before = k ? W.path[nodes_s[j] + k - 1] : -1;
                 if (v <= before || v >= q_start[j + 1] - nodes_s[j]) fail(S, kEINVAL);
             }
         if (failed(S, P)) {
@@ -587,63 +653,76 @@ __global__ __launch_bounds__(kThreads) void keep_kernel(const ds4hip_kv_pages P,
     }
 refuse:
     if (tid == 0) *M.n = 0;
-    for (int i = tid; i < n_nodes; i += kThreads) path[i] = -1;
-    if (tid < n_jobs) n_path[tid] = 0, next[tid] = -1;
+    for (int i = tid; i < n_nodes; i += kThreads) W.path[i] = -1;
+    if (tid < n_jobs) W.n_path[tid] = 0, W.next[tid] = -1;
 }
 
-// The paths' rows, a workgroup a job and layer: row path[i] of the drafts becomes row i, 64 at a time in order
-// (path[i] >= i: a row that is read later lies behind those already written), every load before the first store.
+// The paths' rows: row path[i] of the drafts becomes row i, from the first that moves on (those before it, which are
+// their own places, lie together). Every load comes before the first store, 64 rows at a time in order (path[i] >= i:
+// a row that is read later lies behind those already written). A job's layers go to `split` workgroups, each with as many
+// layers at once as make 64 rows: the places are looked up once for all of them, and little is left to wait for.
+// (64 jobs of 5 rows in 43 layers: a workgroup for each job and layer took 10.8 us.)
 __global__ __launch_bounds__(256) void keep_rows_kernel(const ds4hip_kv_pages P, const int32_t *seqs, const int32_t *q_start,
-                                                        const int32_t *path, const int32_t *n_path, const Moves M) {
+                                                        const int32_t *path, const int32_t *n_path, int split, const Moves M) {
     constexpr int kRows = 64;
     __shared__ long long from_s[kRows], to_s[kRows];
-    const int tid = threadIdx.x, n_jobs = *M.n, shift = __builtin_ctz(P.page_rows);   // (0 jobs: refused)
-    for (long long unit = blockIdx.x; unit < (long long)n_jobs * P.n_layers; unit += gridDim.x) {
-        const int j = (int)(unit / P.n_layers), kept = n_path[j], seq = seqs[j], base = M.base[j], a = q_start[j];
-        const long long first = (unit - (long long)j * P.n_layers) * P.layer_rows;
-        for (int i0 = 0; i0 < kept; i0 += kRows) {
-            const int rows = min(kRows, kept - i0);
-            __syncthreads();   // (the places before are read)
-            bool moves = false;
-            if (tid < rows) {
-                const int f = base + path[a + i0 + tid], t = base + i0 + tid;
-                moves = f != t;
-                from_s[tid] = first + ((long long)*entry(P, seq, f >> shift) << shift) + (f & (P.page_rows - 1));
-                to_s[tid] = first + ((long long)*entry(P, seq, t >> shift) << shift) + (t & (P.page_rows - 1));
-            }
-            if (!__syncthreads_or(moves)) continue;
+    const int tid = threadIdx.x, lane = tid & 63, shift = __builtin_ctz(P.page_rows);
+    const int j = blockIdx.x / split, part = blockIdx.x - j * split;
+    const int l0 = (int)((long long)P.n_layers * part / split), l1 = (int)((long long)P.n_layers * (part + 1) / split);
+    const int kept = n_path[j], seq = seqs[j], base = M.base[j], a = q_start[j];
+    if (*M.n == 0) return;   // refused
+    for (int i0 = 0; i0 < kept; i0 += kRows) {
+        const int i = i0 + lane, node = i < kept ? path[a + i] : i;
+        const uint64_t moved = __ballot(node != i);   // (the same in every wave)
+        if (!moved) continue;
+        const int first = __builtin_ctzll(moved), rows = min(kRows, kept - i0) - first;
+        __syncthreads();   // (the places before are read)
+        if (tid >= first && tid < first + rows) {
+            const int f = base + node, t = base + i;
+            from_s[tid - first] = ((long long)*entry(P, seq, f >> shift) << shift) + (f & (P.page_rows - 1));
+            to_s[tid - first] = ((long long)*entry(P, seq, t >> shift) << shift) + (t & (P.page_rows - 1));
+        }
+        __syncthreads();
+        const int per = kRows / rows;
+        for (int l = l0; l < l1; l += per) {
+            const int all = rows * min(per, l1 - l);   // rows of these layers
             constexpr int kUnits = 36, kEach = kRows * kUnits / 256;   // 16 bytes each: 28 of codes, 8 of the tail
+            auto place = [&](const long long *at, int r) {
+                const int layer = r / rows;
+                return (l + layer) * P.layer_rows + at[r - layer * rows];
+            };
             uint4_t v[kEach];
             uint2_t e = {0, 0};
 #pragma unroll
             for (int u = 0; u < kEach; ++u) {
-                const int i = tid + 256 * u, row = i / kUnits, k = i - row * kUnits;
-                if (row < rows)
-                    v[u] = k < 28 ? reinterpret_cast<const uint4_t *>(P.codes + from_s[row] * kCodes)[k]
-                                  : reinterpret_cast<const uint4_t *>(P.tail + from_s[row] * kRotD)[k - 28];
+                const int x = tid + 256 * u, r = x / kUnits, k = x - r * kUnits;
+                if (r < all) {
+                    const long long from = place(from_s, r);
+                    v[u] = k < 28 ? reinterpret_cast<const uint4_t *>(P.codes + from * kCodes)[k]
+                                  : reinterpret_cast<const uint4_t *>(P.tail + from * kRotD)[k - 28];
+                }
             }
-            if (tid < rows) e = *reinterpret_cast<const uint2_t *>(P.sexp + from_s[tid] * 8);
+            if (tid < all) e = *reinterpret_cast<const uint2_t *>(P.sexp + place(from_s, tid) * 8);
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");   // no other wave's store overtakes a load
             __syncthreads();
 #pragma unroll
             for (int u = 0; u < kEach; ++u) {
-                const int i = tid + 256 * u, row = i / kUnits, k = i - row * kUnits;
-                if (row < rows) {
+                const int x = tid + 256 * u, r = x / kUnits, k = x - r * kUnits;
+                if (r < all) {
+                    const long long to = place(to_s, r);
                     if (k < 28)
-                        reinterpret_cast<uint4_t *>(P.codes + to_s[row] * kCodes)[k] = v[u];
+                        reinterpret_cast<uint4_t *>(P.codes + to * kCodes)[k] = v[u];
                     else
-                        reinterpret_cast<uint4_t *>(P.tail + to_s[row] * kRotD)[k - 28] = v[u];
+                        reinterpret_cast<uint4_t *>(P.tail + to * kRotD)[k - 28] = v[u];
                 }
             }
-            if (tid < rows) *reinterpret_cast<uint2_t *>(P.sexp + to_s[tid] * 8) = e;
+            if (tid < all) *reinterpret_cast<uint2_t *>(P.sexp + place(to_s, tid) * 8) = e;
         }
     }
 }
 
-// Workgroups for n jobs' rows: whole rounds of the chip at most.
-unsigned keep_grid(const ds4hip_kv_pages *p, int n_jobs) {
-    return (unsigned)std::min<long long>((long long)n_jobs * p->n_layers, 256 * 16);
-}
+// Workgroups of a job's rows: two for each CU in all.
+int keep_split(const ds4hip_kv_pages *p, int n_jobs) { return std::max(1, std::min(p->n_layers, 512 / n_jobs)); }
 
 bool aligned(const void *p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
@@ -738,11 +817,10 @@ extern "C" int ds4hip_kv_pages_keep(const ds4hip_kv_pages *p, const int32_t *seq
     if (n_jobs == 0) return 0;
     const Moves M = moves_at(workspace, p->n_pages);
     const hipStream_t st = (hipStream_t)stream;
-    // (only read)
-    int32_t *nodes = const_cast<int32_t *>(path), *counts = const_cast<int32_t *>(n_path);
-    hipLaunchKernelGGL(keep_kernel<false>, dim3(1), dim3(kThreads), 0, st, *p, seqs, q_start, n_jobs, n_nodes, nodes, counts,
-                       nullptr, M);
-    hipLaunchKernelGGL(keep_rows_kernel, dim3(keep_grid(p, n_jobs)), dim3(256), 0, st, *p, seqs, q_start, path, n_path, M);
+    const Walk W = {nullptr, nullptr, nullptr, const_cast<int32_t *>(path), const_cast<int32_t *>(n_path), nullptr};   // (only read)
+    hipLaunchKernelGGL((keep_kernel<false, false>), dim3(1), dim3(kThreads), 0, st, *p, seqs, q_start, n_jobs, n_nodes, W, M);
+    const int split = keep_split(p, n_jobs);
+    hipLaunchKernelGGL(keep_rows_kernel, dim3(n_jobs * split), dim3(256), 0, st, *p, seqs, q_start, path, n_path, split, M);
     return ds4hip_set_last_error(hip_status(hipGetLastError()));
 }
 
@@ -757,10 +835,12 @@ extern "C" int ds4hip_kv_pages_accept(const ds4hip_kv_pages *p, const int32_t *s
     if (n_jobs == 0) return 0;
     const Moves M = moves_at(workspace, p->n_pages);
     const hipStream_t st = (hipStream_t)stream;
-    hipLaunchKernelGGL(walk_kernel, dim3(n_jobs), dim3(64), 0, st, q_start, n_jobs, parents, tokens, targets, n_nodes, path,
-                       n_path, next);
-    hipLaunchKernelGGL(keep_kernel<true>, dim3(1), dim3(kThreads), 0, st, *p, seqs, q_start, n_jobs, n_nodes, path, n_path, next,
-                       M);
-    hipLaunchKernelGGL(keep_rows_kernel, dim3(keep_grid(p, n_jobs)), dim3(256), 0, st, *p, seqs, q_start, path, n_path, M);
+    const Walk W = {parents, tokens, targets, path, n_path, next};
+    const bool here = n_nodes <= kWalkNodes;
+    if (!here) hipLaunchKernelGGL(walk_kernel, dim3(n_jobs), dim3(64), 0, st, q_start, n_jobs, n_nodes, W);
+    auto *plan = here ? keep_kernel<true, true> : keep_kernel<true, false>;
+    hipLaunchKernelGGL(plan, dim3(1), dim3(kThreads), 0, st, *p, seqs, q_start, n_jobs, n_nodes, W, M);
+    const int split = keep_split(p, n_jobs);
+    hipLaunchKernelGGL(keep_rows_kernel, dim3(n_jobs * split), dim3(256), 0, st, *p, seqs, q_start, path, n_path, split, M);
     return ds4hip_set_last_error(hip_status(hipGetLastError()));
 }

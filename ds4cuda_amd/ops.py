@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import ctypes as C
 from dataclasses import dataclass
+from functools import lru_cache
 
 import torch
 
@@ -318,6 +319,7 @@ def _same_gpu(t, index, name):
         raise Ds4HipError(f"{name}: on {t.device}, the cache is on GPU {index}", -22)
 
 
+@lru_cache(maxsize=256)
 def window_workspace_bytes(n_seqs, n_q, n_head) -> int:
     return lib().ds4hip_flash_attn_window_fp8_workspace_bytes(_int32(n_seqs, "n_seqs"), _int32(n_q, "n_q"),
                                                               _int32(n_head, "n_head"))
@@ -453,6 +455,7 @@ class Sample(C.Structure):
                 ("all_top_p", C.c_float), ("all_min_p", C.c_float), ("tokens", C.c_void_p), ("probs", C.c_void_p)]
 
 
+@lru_cache(maxsize=256)
 def sample_workspace_bytes(n_rows, n_vocab) -> int:
     return lib().ds4hip_sample_workspace_bytes(_int32(n_rows, "n_rows"), _int32(n_vocab, "n_vocab"))
 
@@ -470,43 +473,51 @@ def sample_tokens(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, 
     probability its share. Temperature 0: the first token of that order, probability 1. A row with a NaN or +inf, with no
     logit above -inf, or with a parameter or u outside its range gives -1 and NaN.
     """
-    if logits.dim() != 2 or logits.dtype not in (torch.bfloat16, torch.float32) or logits.device.type != "cuda":
+    f32, index = logits.dtype is torch.float32, logits.get_device()
+    if logits.dim() != 2 or index < 0 or not (f32 or logits.dtype is torch.bfloat16):
         raise Ds4HipError("logits must be bf16 or fp32 [n, vocab] on the GPU", -22)
-    n, vocab = (_int32(x, "logits") for x in logits.shape)
-    stride = logits.stride(0) if n > 1 else max(vocab, 1)
-    if vocab > 1 and logits.stride(1) != 1 or stride < vocab:
+    n, vocab = logits.shape
+    stride, step = logits.stride()
+    if n < 2:
+        stride = vocab
+    if (step != 1 and vocab > 1) or stride < vocab:
         raise Ds4HipError("logits: a row's values must be consecutive, and rows must not overlap", -22)
-    index = logits.get_device()
-    a = Sample(logits=logits.data_ptr(), logits_f32=logits.dtype == torch.float32, row_stride=stride, n_rows=n, n_vocab=vocab)
-    for t, dtype, name in ((temperature, torch.float32, "temperature"), (top_k, torch.int32, "top_k"),
-                           (top_p, torch.float32, "top_p"), (min_p, torch.float32, "min_p"), (u, torch.float32, "u")):
-        if isinstance(t, torch.Tensor) or name == "u":
+    a = Sample(logits.data_ptr(), f32, stride, _int32(n, "logits"), _int32(vocab, "logits"))
+    for t, dtype, name in ((u, torch.float32, "u"), (temperature, torch.float32, "temperature"), (top_k, torch.int32, "top_k"),
+                           (top_p, torch.float32, "top_p"), (min_p, torch.float32, "min_p")):
+        if isinstance(t, torch.Tensor):
             if not _ready(t, dtype, index) or t.numel() != n:
                 _check(t, dtype, n, name)
                 _same_gpu(t, index, name)
                 raise Ds4HipError(f"{name}: {n} entries expected, got {t.numel()}", -22)
             setattr(a, name, t.data_ptr())
+        elif name == "u":
+            raise Ds4HipError("u must be a tensor of one random number a row", -22)
         else:
             setattr(a, "all_" + name, _int32(t, name) if dtype is torch.int32 else t)
     with _on_stream(stream, logits.device):
         if tokens is None:
-            tokens = torch.empty(n, dtype=torch.int32, device=logits.device)
+            tokens = logits.new_empty(n, dtype=torch.int32)
+        else:
+            _check(tokens, torch.int32, n, "tokens")
+            _same_gpu(tokens, index, "tokens")
         if probs is None:
-            probs = torch.empty(n, dtype=torch.float32, device=logits.device)
-        for t, dtype, name in ((tokens, torch.int32, "tokens"), (probs, torch.float32, "probs")):
-            _check(t, dtype, n, name)
-            _same_gpu(t, index, name)
+            probs = logits.new_empty(n, dtype=torch.float32)
+        else:
+            _check(probs, torch.float32, n, "probs")
+            _same_gpu(probs, index, "probs")
         if n == 0:
             return tokens, probs
         need = sample_workspace_bytes(n, vocab)
         if workspace is None:
-            workspace = torch.empty(need, dtype=torch.uint8, device=logits.device)
+            workspace = logits.new_empty(need, dtype=torch.uint8)
+            size = need
         else:
             _dev(workspace, "workspace", need)
             _same_gpu(workspace, index, "workspace")
+            size = workspace.numel() * workspace.element_size()
         a.tokens, a.probs = tokens.data_ptr(), probs.data_ptr()
-        call("ds4hip_sample_tokens", C.byref(a), workspace.data_ptr(), workspace.numel() * workspace.element_size(),
-             _stream(stream))
+        call("ds4hip_sample_tokens", C.byref(a), workspace.data_ptr(), size, _stream(stream))
     return tokens, probs
 
 

@@ -165,24 +165,31 @@ class PagePool:
         self._jobs(keep, "keep", n)
         self._call("ds4hip_kv_pages_free", stream, _addr(seqs), _addr(keep), n)
 
-    def _nodes(self, q_start, n_jobs, tensors):
-        """Checks packed nodes: q_start of n_jobs trees and tensors of one int32 a node; their number."""
-        n = tensors[0][0].numel()
-        for t, want, name in ((q_start, n_jobs + 1, "q_start"), *((t, n, name) for t, name in tensors)):
-            if not _ready(t, torch.int32, self.index) or t.numel() != want:
-                _check(t, torch.int32, None, name)
-                _same_gpu(t, self.index, name)
-                raise Ds4HipError(f"{name}: {want} entries expected, got {t.numel()}", -22)
-        return _int32(n, "nodes")
+    def _nodes(self, seqs, q_start, *tensors):
+        """Checks packed nodes: the trees' sequences, their q_start, and (tensor, name) of one int32 a node; the
+        numbers of trees and of nodes."""
+        if seqs is None:
+            raise Ds4HipError("seqs: a tensor of the trees' sequences is required", -22)
+        k, n = self._jobs(seqs, "seqs"), tensors[0][0].numel()
+        if not _ready(q_start, torch.int32, self.index) or q_start.numel() != k + 1:
+            self._refuse(q_start, k + 1, "q_start")
+        for t, name in tensors:
+            if not _ready(t, torch.int32, self.index) or t.numel() != n:
+                self._refuse(t, n, name)
+        return k, _int32(n, "nodes")
+
+    def _refuse(self, t, want, name):
+        _check(t, torch.int32, None, name)
+        _same_gpu(t, self.index, name)
+        raise Ds4HipError(f"{name}: {want} entries expected, got {t.numel()}", -22)
 
     def keep(self, seqs, q_start, path, n_path, stream=None):
         """Of the drafted nodes q_start[j] .. q_start[j + 1] - 1, the last rows of sequence seqs[j],
         the n_path[j] ones path[q_start[j]], .. (ascending, counted from the tree's first) stay: their rows move to the
         front of the tree's in all layers, and the sequence is cut behind them. (int32 device
         tensors; path has an entry for every node.)"""
-        k = self._jobs(seqs, "seqs")
+        k, n = self._nodes(seqs, q_start, (path, "path"))
         self._jobs(n_path, "n_path", k)
-        n = self._nodes(q_start, k, ((path, "path"),))
         self._call("ds4hip_kv_pages_keep", stream, _addr(seqs), _addr(q_start), k, _addr(path), n, _addr(n_path),
                    *self._ws(stream))
 
@@ -192,19 +199,18 @@ class PagePool:
         drafted token, and the token sampled behind it. From a tree's first node the path goes on to the first
         child whose token is the target of its parent. Returns (path [nodes], the accepted nodes packed as
         q_start has them and -1 behind; n_path [jobs]; next [jobs], the last ones' targets)."""
-        k = self._jobs(seqs, "seqs")
-        n = self._nodes(q_start, k, ((parents, "parents"), (tokens, "tokens"), (targets, "targets")))
-        outs = []
+        k, n = self._nodes(seqs, q_start, (parents, "parents"), (tokens, "tokens"), (targets, "targets"))
         for t, size, name in ((path, n, "path"), (n_path, k, "n_path"), (next, k, "next")):
-            if t is None:
-                t = self._empty(size, torch.int32, stream)
-            else:
+            if t is not None:
                 _check(t, torch.int32, size, name)
                 _same_gpu(t, self.index, name)
-            outs.append(t)
-        self._call("ds4hip_kv_pages_accept", stream, _addr(seqs), _addr(q_start), k, _addr(parents), _addr(tokens),
-                   _addr(targets), n, *(t.data_ptr() for t in outs), *self._ws(stream))
-        return tuple(outs)
+        with _on_stream(stream, self.device):
+            path = tokens.new_empty(n) if path is None else path
+            n_path = tokens.new_empty(k) if n_path is None else n_path
+            next = tokens.new_empty(k) if next is None else next
+            call("ds4hip_kv_pages_accept", self._c, seqs.data_ptr(), q_start.data_ptr(), k, parents.data_ptr(), tokens.data_ptr(),
+                 targets.data_ptr(), n, path.data_ptr(), n_path.data_ptr(), next.data_ptr(), *self._ws(stream), _stream(stream))
+        return path, n_path, next
 
     def compact(self, n_live=None, stream=None):
         """Moves the held pages to the front of the pool; returns their number, an int32
