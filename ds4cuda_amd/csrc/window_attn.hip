@@ -25,6 +25,7 @@
 
 #include "attn_tile.h"
 #include "ds4hip_common.h"
+#include "scan.h"
 #include "../../include/ds4hip_pages.h"
 
 #include <algorithm>
@@ -72,6 +73,7 @@ struct WinArgs {
     int n_seqs, n_slots, n_q, log_head, window, first, stride, shift, n_pages;
     int log_rows;            // a problem has 2^log_rows rows (queries x heads)
     int n_wg;                // workgroups that the line is cut for
+    int uncut;               // 1: no problem is cut, however long
     // workspace
     int prob_cap;
     long long *line;         // [2] tiles per workgroup, tiles of a problem that stays whole
@@ -95,22 +97,29 @@ __device__ inline int2 queries_of(const WinArgs &A, int s) {
 // The heads of a query in one problem.
 __device__ inline int log_hpt(const WinArgs &A) { return min(A.log_head, A.log_rows); }
 
-// Problem `tile` of sequence s as the plan keeps it: its table row (-1: not a sequence of
-// the table, or one with more rows than its table row holds), first packed query, number of
-// queries, first head (times 256) and, of a tree, first node (times 65536; also -1: more nodes than
-// a tree may have, or than the sequence has rows), position (of a tree: row) of its first query.
+// Sequence s of the call: its first packed query and their number, its table row (-1: not a sequence of
+// the table, or one with more rows than its table row holds; of a tree also one with more nodes than a tree may have, or
+// than it has rows) and the rows before its queries.
 template <bool kTree>
-__device__ inline int4 record_of(const WinArgs &A, int s, int tile) {
-    const int lh = log_hpt(A), lg = A.log_head - lh, qpt = (1 << A.log_rows) >> lh;
+__device__ inline int4 sequence_of(const WinArgs &A, int s) {
+    const int slot = A.seq_ids ? A.seq_ids[s] : s;
     const int2 qs = queries_of(A, s);
-    const int q = (tile >> lg) * qpt, slot = A.seq_ids ? A.seq_ids[s] : s;
     const bool in = slot >= 0 && slot < A.n_slots;
     const int rows = in ? max(A.rows[slot], 0) : 0;
     const bool fits = in && rows <= kMaxRows && ((rows - 1) >> A.shift) < A.stride &&
                       (!kTree || (qs.y <= kMaxNodes && qs.y <= rows));
-    return make_int4(fits ? slot : -1, qs.x + q,
-                     min(qpt, qs.y - q) | ((tile & ((1 << lg) - 1)) << lh) << 8 | (kTree && fits ? q << 16 : 0),
-                     rows - qs.y + q);
+    return make_int4(qs.x, qs.y, fits ? slot : -1, rows - qs.y);
+}
+
+// Its problem `tile` as the plan keeps it: table row, first packed query, number of queries, first head
+// (times 256) and, of a tree, first node (times 65536), position (of a tree: row) of its first query.
+template <bool kTree>
+__device__ inline int4 record_of(const WinArgs &A, int4 seq, int tile) {
+    const int lh = log_hpt(A), lg = A.log_head - lh, qpt = (1 << A.log_rows) >> lh;
+    const int q = (tile >> lg) * qpt;
+    return make_int4(seq.z, seq.x + q,
+                     min(qpt, seq.y - q) | ((tile & ((1 << lg) - 1)) << lh) << 8 | (kTree && seq.z >= 0 ? q << 16 : 0),
+                     seq.w + q);
 }
 
 struct Problem {
@@ -174,10 +183,10 @@ struct Tree<true, kRows> {
     int pos[kRows / 8], base;
 };
 
-// All threads of the workgroup, between barriers of it; false in the threads whose query has an ancestor
-// whose parent is none. A thread walks one query's line to the root in LDS (twice: its depth first), 64 cycles
-// a step; parents come before their children, so every walk ends. parent: LDS that nothing else uses up to
-// the second barrier from here (the stage of a later tile).
+// All threads of the workgroup, after a barrier of it; false in the threads whose query has an ancestor
+// whose parent is none. A thread walks one query's line to the root in LDS, 64 cycles a step (again, where rows before the
+// tree's are fewer than the first ones, for what those keep visible); parents come before their children, so every walk
+// ends. parent: LDS that nothing else uses up to the second barrier from here (the stage of a later tile).
 template <int kThreads, int kRows>
 __device__ inline bool plant(const WinArgs &A, const Problem &P, Tree<true, kRows> &T, uint8_t *stage) {
     static_assert(2 * kMaxNodes <= kStageB, "a node's parent takes two bytes");
@@ -192,15 +201,24 @@ __device__ inline bool plant(const WinArgs &A, const Problem &P, Tree<true, kRow
     if (tid == 0) T.base = P.base;
     lds_barrier();
     if (tid >= P.n) return true;
-    int depth = 0, v = parent[P.node0 + tid];
-    for (; v >= 0; v = parent[v]) ++depth;
-    const bool good = v == -1;
-    const int pos = P.base + depth;
+    // the words of the line, from the node's own down; a word is written when the line leaves it
+    int v = P.node0 + tid, depth = 0, word = v >> 5;
+    uint32_t bits = 0;
+    for (; v >= 0; v = parent[v], ++depth) {
+        if (v >> 5 != word) {
+            T.mask[tid][1 + word] = bits;
+            word = v >> 5;
+            bits = 0;
+        }
+        if (A.window <= 0 || depth < A.window) bits |= 1u << (v & 31);
+    }
+    T.mask[tid][1 + word] = bits;
+    const int pos = P.base + depth - 1;
     T.pos[tid] = pos;
-    v = P.node0 + tid;
-    for (int at = pos; v >= 0; v = parent[v], --at)
-        if (A.window <= 0 || at > pos - A.window || at < A.first) T.mask[tid][1 + (v >> 5)] |= 1u << (v & 31);
-    return good;
+    if (A.window > 0 && P.base < A.first)
+        for (int u = P.node0 + tid, at = pos; u >= 0; u = parent[u], --at)
+            if (at < A.first) T.mask[tid][1 + (u >> 5)] |= 1u << (u & 31);
+    return v == -1;
 }
 
 // Whether the stretch of tiles up to i1 has any that the masks and positions are needed for.
@@ -208,72 +226,56 @@ __device__ inline bool needs_tree(const WinArgs &A, const Problem &P, int i1) {
     return A.window > 0 || tile_at(P, i1 - 1) >= P.whole_c;
 }
 
-// What a query sees of a tile, for its rows k = 0 .. 31.
+// What a query sees of the tile from key0 on, for its rows k = 0 .. 31. Of a tree: as bits.
 struct TreeSight {
-    int pos, base;
-    uint32_t bits;   // of the tree's rows in it
-    __device__ bool operator()(const WinArgs &A, int key0, int k) const {
-        const int key = key0 + k;
-        return key < base ? A.window <= 0 || key > pos - A.window || key < A.first : bits >> k & 1;
-    }
+    uint32_t seen;
+    __device__ bool operator()(const WinArgs &, int, int k) const { return seen >> k & 1; }
 };
 struct RowSight {
     int pos;
     __device__ bool operator()(const WinArgs &A, int key0, int k) const { return sees(A, pos, key0 + k); }
 };
+// The lowest n of 32 bits, of any n.
+__device__ inline uint32_t lowest(int n) { return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1; }
 template <int kRows>
-__device__ inline TreeSight sight_of(const Tree<true, kRows> &T, int, int qi, int key0) {
-    TreeSight v{T.pos[qi], T.base, 0};
-    const int at = key0 - v.base;
+__device__ inline TreeSight sight_of(const WinArgs &A, const Tree<true, kRows> &T, int, int qi, int key0) {
+    const int at = __builtin_amdgcn_readfirstlane(key0 - T.base);   // of the tile in the tree's rows
+    uint32_t seen = lowest(-at);
+    if (A.window > 0) seen &= ~lowest(T.pos[qi] - A.window + 1 - key0) | lowest(A.first - key0);
     if (at > -32) {
         const uint32_t *m = &T.mask[qi][1 + (at >> 5)];
-        v.bits = (uint32_t)((((uint64_t)m[1] << 32) | m[0]) >> (at & 31));
+        seen |= (uint32_t)((((uint64_t)m[1] << 32) | m[0]) >> (at & 31));
     }
-    return v;
+    return {seen};
 }
 template <int kRows>
-__device__ inline RowSight sight_of(const Tree<false, kRows> &, int pos, int, int) { return {pos}; }
+__device__ inline RowSight sight_of(const WinArgs &, const Tree<false, kRows> &, int pos, int, int) { return {pos}; }
 
 // ---- plan ------------------------------------------------------------------------
 
 // Exclusive sum of v over the workgroup's kThreads threads; *total receives the sum.
 template <int kThreads>
 __device__ inline long long block_scan(long long v, long long *sums, long long *total) {
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    long long x = v;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-        const long long y = __shfl_up(x, off);
-        if (lane >= off) x += y;
-    }
-    __syncthreads();
-    if (lane == 63) sums[w] = x;
-    __syncthreads();
-    long long before = 0, all = 0;
-#pragma unroll
-    for (int i = 0; i < kThreads / 64; ++i) {
-        const long long y = sums[i];
-        before += i < w ? y : 0;
-        all += y;
-    }
-    *total = all;
-    return before + x - v;
+    return wg_scan<kThreads / 64>(v, sums, total) - v;
 }
 
 // put(i, record, tiles before) for every problem; returns their number, *tiles and, in
-// *longest (shared, 0 before), the most of one. All threads of the workgroup; first_s: [n_seqs].
-template <bool kTree, int kThreads, int kEach, typename Put>
-__device__ inline int lay_line(const WinArgs &A, int *first_s, long long *sums, int *longest, long long *tiles, Put put) {
+// *longest (shared, 0 before), the most of one. All threads of the workgroup; first_s, seq_s: [n_seqs] (what the problems
+// need of their sequences is loaded once and at once: three loads that wait for each other less).
+template <bool kTree, int kThreads, int kEach, typename First, typename Put>
+__device__ inline int lay_line(const WinArgs &A, First *first_s, int4 *seq_s, long long *sums, int *longest, long long *tiles, Put put) {
     const int tid = threadIdx.x;
     const int lh = log_hpt(A), lg = A.log_head - lh, qpt = (1 << A.log_rows) >> lh;
     long long n_all = 0, t_all = 0;
     if (A.q_start) {
         for (int s0 = 0; s0 < A.n_seqs; s0 += kThreads) {
             const int s = s0 + tid;
-            const long long n = s < A.n_seqs ? (long long)((queries_of(A, s).y + qpt - 1) / qpt) << lg : 0;
+            int4 seq = make_int4(0, 0, 0, 0);
+            if (s < A.n_seqs) seq_s[s] = seq = sequence_of<kTree>(A, s);
+            const long long n = (long long)((seq.y + qpt - 1) / qpt) << lg;
             long long all;
             const long long before = n_all + block_scan<kThreads>(n, sums, &all);
-            if (s < A.n_seqs) first_s[s] = (int)min(before, (long long)A.prob_cap);
+            if (s < A.n_seqs) first_s[s] = (First)min(before, (long long)A.prob_cap);
             n_all += all;
         }
         __syncthreads();
@@ -299,7 +301,7 @@ __device__ inline int lay_line(const WinArgs &A, int *first_s, long long *sums, 
                     }
                     first = first_s[s];
                 }
-                rec[u] = record_of<kTree>(A, s, i - first);
+                rec[u] = record_of<kTree>(A, A.q_start ? seq_s[s] : sequence_of<kTree>(A, s), i - first);
             }
         }
 #pragma unroll
@@ -335,12 +337,13 @@ struct Cuts {
     int whole;   // tiles of a problem that stays whole; < 0: workgroup b has problem b
 };
 
-__device__ inline Cuts cuts_of(long long tiles, int n_wg, int n_prob, int longest) {
+__device__ inline Cuts cuts_of(const WinArgs &A, long long tiles, int n_prob, int longest) {
+    const int n_wg = A.n_wg;
     Cuts C;
     C.tiles = tiles;
     // at least sqrt(longest / 16) tiles: a long problem's merge takes 0.09 us a part, a tile 1.5
     C.per = max((tiles + n_wg - 1) / n_wg, (long long)max(kMinTiles, (int)sqrtf((float)longest * 0.0625f)));
-    C.whole = (int)min(max((long long)kWhole, C.per / 8), 1LL << 30);
+    C.whole = A.uncut ? 1 << 30 : (int)min(max((long long)kWhole, C.per / 8), 1LL << 30);
     if (n_prob <= n_wg && longest <= C.per + kPart) {
         C.whole = -1;
         C.per = tiles + 1;   // (no cut inside the line)
@@ -383,6 +386,7 @@ __device__ inline void leave(const WinArgs &A, const Cuts &C, int n_prob) {
 template <bool kTree>
 __global__ __launch_bounds__(1024) void plan_kernel(const WinArgs A) {
     __shared__ int first_s[kMaxSeqs];   // problems before each sequence
+    __shared__ int4 seq_s[kMaxSeqs];
     __shared__ long long sums[16];
     long long tiles;
     __shared__ int longest;
@@ -390,12 +394,12 @@ __global__ __launch_bounds__(1024) void plan_kernel(const WinArgs A) {
     constexpr int kHeld = 8192;   // (64 KB; the search below took half the kernel's time in memory)
     __shared__ long long pre_s[kHeld];
     // four problems a thread: their loads and one sum for 4096 (12 us; with one a thread 17)
-    const int n_prob = lay_line<kTree, 1024, 4>(A, first_s, sums, &longest, &tiles, [&](int i, int4 rec, long long before) {
+    const int n_prob = lay_line<kTree, 1024, 4>(A, first_s, seq_s, sums, &longest, &tiles, [&](int i, int4 rec, long long before) {
         A.prob[i] = rec;
         A.pre[i] = before;
         if (i < kHeld) pre_s[i] = before;
     });
-    const Cuts C = cuts_of(tiles, A.n_wg, n_prob, longest);
+    const Cuts C = cuts_of(A, tiles, n_prob, longest);
     if (threadIdx.x == 0) {
         A.pre[n_prob] = tiles;
         if (n_prob < kHeld) pre_s[n_prob] = tiles;
@@ -409,12 +413,22 @@ __global__ __launch_bounds__(1024) void plan_kernel(const WinArgs A) {
     A.wg_prob[b] = prob;
 }
 
+// The workgroup's place on the line. Trees: neighbours on the line have one XCD (workgroups are dealt to the eight in
+// turn), since a sequence's nodes, which read the same rows, are neighbours.
+template <bool kTree>
+__device__ inline int own_place(const WinArgs &A) {
+    const int b = blockIdx.x;
+    return kTree ? (b & 7) * (A.n_wg >> 3) + (b >> 3) : b;   // (n_wg is a multiple of 8)
+}
+
 // The workgroup's own copy of a line of at most kFew problems (0: none).
 template <int kFew>
 struct Line {
     int4 prob[kFew ? kFew : 1];
     long long pre[kFew + 1], sums[8];
-    int first[kFew ? kFew : 1], longest;
+    int4 seq[kFew ? kFew : 1];
+    uint16_t first[kFew ? kFew : 1];   // (at most kFew)
+    int longest;
 };
 
 // Where a workgroup stands: its first problem, and the tiles [t, end) of the line.
@@ -428,25 +442,25 @@ struct Place {
 // the first one leaves it to the merge; else the plan kernel did.
 template <bool kTree, int kFew, int kThreads>
 __device__ inline Place take_place(const WinArgs &A, Line<kFew> &L) {
-    const int tid = threadIdx.x, wg = blockIdx.x;
+    const int tid = threadIdx.x, wg = own_place<kTree>(A);
     Place at;
     at.part = 0;
     if constexpr (kFew != 0) {
         if (tid == 0) L.longest = 0;
         long long tiles;
-        at.n_prob = lay_line<kTree, kThreads, 1>(A, L.first, L.sums, &L.longest, &tiles, [&](int i, int4 rec, long long before) {
+        at.n_prob = lay_line<kTree, kThreads, 1>(A, L.first, L.seq, L.sums, &L.longest, &tiles, [&](int i, int4 rec, long long before) {
             L.prob[i] = rec;
             L.pre[i] = before;
         });
         if (tid == 0) L.pre[at.n_prob] = tiles;
         __syncthreads();
-        Cuts C = cuts_of(tiles, A.n_wg, at.n_prob, L.longest);
+        Cuts C = cuts_of(A, tiles, at.n_prob, L.longest);
         // Even parts: a problem is cut into equal ones and no workgroup has parts of two (the second's
         // queries and stores take as long as about kSecond tiles); the line then counts a problem as
         // a whole number of cuts. 16 long sequences: 70 us with parts that pass from one to the
         // next, 63 with even ones. Where the parts would be much longer for it (one long sequence among
         // a hundred short ones, whose workgroups are lost to it) they pass.
-        if (C.whole >= 0 && at.n_prob < A.n_wg) {
+        if (C.whole >= 0 && !A.uncut && at.n_prob < A.n_wg) {
             const long long per = max(C.per, (tiles + A.n_wg - at.n_prob - 1) / (A.n_wg - at.n_prob));
             if (per <= C.per + kSecond) {   // (a sum over problems of tiles / per, rounded up, is at most n_wg)
                 const long long n = tid < at.n_prob ? L.pre[tid + 1] - L.pre[tid] : 0;
@@ -720,7 +734,7 @@ __global__ __launch_bounds__(kF32 ? 256 : 512, kF32 ? 1 : 2) void window_kernel(
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n16 = lane & 15, g = lane >> 4, row = 16 * (w & 3) + n16;
     const int kh = w >> 2;   // the wave's (first) key half
-    const int wg = blockIdx.x;
+    const int wg = own_place<kTree>(A);
     constexpr int kFew = kInline ? kFewProbs : 0;
     __shared__ Line<kFew> line;
     __shared__ Tree<kTree, kRows> tree;
@@ -768,8 +782,6 @@ __global__ __launch_bounds__(kF32 ? 256 : 512, kF32 ? 1 : 2) void window_kernel(
             for (int b = 0; b < kDT; ++b) o[a][b] = float4_t{0, 0, 0, 0};
         if (tid == 0) bad_s = 0;
         if (P.pos1 >= 0) {   // else its one tile sees nothing
-            if constexpr (kTree)
-                if (needs_tree(A, P, i1)) bad |= !plant<64 * kW>(A, P, tree, stages[2]);   // (read after the tiles' first barrier)
             // row tiles in use; the waves of the others only share the rest
             const int n_rt = ((P.n << lh) + 15) >> 4;
             const bool scores_mine = (w & 3) < n_rt;
@@ -805,6 +817,8 @@ __global__ __launch_bounds__(kF32 ? 256 : 512, kF32 ? 1 : 2) void window_kernel(
                 load_row<kF32>(A, P, row, g, q);
                 kq = fragments_of<kF32>(q, qh, ql) * (kLog2e / 22.62741699796952f);   // 1 / sqrt(512)
             }
+            if constexpr (kTree)   // (under the first tile's loads; read after the tiles' first barrier)
+                if (needs_tree(A, P, i1)) bad |= !plant<64 * kW>(A, P, tree, stages[2]);
             const int pos = P.pos0 + min(row >> lh, P.n - 1);   // (rows past the queries repeat the last one's)
             float m = -INFINITY, l = 0.0f, sum = 0.0f;
             float ref = 0.0f;   // m, or 0 while there is none
@@ -980,7 +994,7 @@ __global__ __launch_bounds__(kF32 ? 256 : 512, kF32 ? 1 : 2) void window_kernel(
                 if (edge) {
                     uint32_t odd = 0;
                     const int lane_r = again(lane), g_r = lane_r >> 4;
-                    const auto sight = sight_of(tree, pos, min((16 * (w & 3) + (lane_r & 15)) >> lh, P.n - 1), key0);
+                    const auto sight = sight_of(A, tree, pos, min((16 * (w & 3) + (lane_r & 15)) >> lh, P.n - 1), key0);
 #pragma unroll
                     for (int u = 0; u < kN; ++u)
 #pragma unroll
@@ -1178,17 +1192,17 @@ __global__ __launch_bounds__(512, 2) void roles_kernel(const WinArgs A) {
             const Stretch T = S;
             const Problem &P = T.P;
             const bool whole = T.begins && T.ends;
-            const int slot = 2 * blockIdx.x + (T.begins ? 1 : 0), i0 = T.i0, i1 = T.i1;
+            const int slot = 2 * own_place<kTree>(A) + (T.begins ? 1 : 0), i0 = T.i0, i1 = T.i1;
             const int n_rt = ((P.n << lh) + 15) >> 4;   // row tiles in use
             F.bad = P.slot < 0;
             Ring G;
             if (tid == 0) bad_s = 0;
             const bool mine = 2 * rg < n_rt;   // else the wave only shares the rest
             if (P.pos1 >= 0) {
-                if constexpr (kTree)
-                    if (needs_tree(A, P, i1)) F.bad |= !plant<512>(A, P, tree, stages[2]);   // (with the other role's waves)
                 const uint32_t ka = pi_key(16 * kh + n16) * kRowB + 16 * g;
                 F.tile(A, T, i0, tid);
+                if constexpr (kTree)   // (with the other role's waves, under the tile's loads)
+                    if (needs_tree(A, P, i1)) F.bad |= !plant<512>(A, P, tree, stages[2]);
                 half8_t qh[2][16];
                 float kq[2] = {0.0f, 0.0f}, m[2], l[2], ref[2], sum[2];   // ref: m, or 0 while there is none
                 int pos[2];
@@ -1290,9 +1304,9 @@ __global__ __launch_bounds__(512, 2) void roles_kernel(const WinArgs A) {
                     if (edge_at(P, i)) {
                         const int key0 = kTile * tile_at(P, i), lane_r = again(lane), g_r = lane_r >> 4;
                         uint32_t odd = 0;
-                        const decltype(sight_of(tree, 0, 0, 0)) sight[2] = {
-                            sight_of(tree, pos[0], min((32 * rg + (lane_r & 15)) >> lh, P.n - 1), key0),
-                            sight_of(tree, pos[1], min((32 * rg + 16 + (lane_r & 15)) >> lh, P.n - 1), key0)};
+                        const decltype(sight_of(A, tree, 0, 0, 0)) sight[2] = {
+                            sight_of(A, tree, pos[0], min((32 * rg + (lane_r & 15)) >> lh, P.n - 1), key0),
+                            sight_of(A, tree, pos[1], min((32 * rg + 16 + (lane_r & 15)) >> lh, P.n - 1), key0)};
 #pragma unroll
                         for (int r = 0; r < 4; ++r) {
                             const int k = pi_key(16 * kh + 4 * g_r + r);
@@ -1340,7 +1354,7 @@ __global__ __launch_bounds__(512, 2) void roles_kernel(const WinArgs A) {
             const Stretch T = S;
             const Problem &P = T.P;
             const bool whole = T.begins && T.ends;
-            const int slot = 2 * blockIdx.x + (T.begins ? 1 : 0), i0 = T.i0, i1 = T.i1;
+            const int slot = 2 * own_place<kTree>(A) + (T.begins ? 1 : 0), i0 = T.i0, i1 = T.i1;
             const int n_rt = ((P.n << lh) + 15) >> 4;   // row tiles in use
             F.bad = P.slot < 0;
             Ring G;
@@ -1350,13 +1364,13 @@ __global__ __launch_bounds__(512, 2) void roles_kernel(const WinArgs A) {
 #pragma unroll
                 for (int b = 0; b < kDT; ++b) o[a][b] = float4_t{0, 0, 0, 0};
             if (P.pos1 >= 0) {
-                if constexpr (kTree)
-                    if (needs_tree(A, P, i1)) F.bad |= !plant<512>(A, P, tree, stages[2]);
                 uint32_t va[2];
 #pragma unroll
                 for (int kt = 0; kt < 2; ++kt)
                     va[kt] = lds_addr(stages[0]) + pi_key(16 * kt + 4 * (lane >> 4) + ((lane & 15) >> 2)) * kRowB + 256 * (w - 4) + 8 * (lane & 3);
                 F.tile(A, T, i0, tid);
+                if constexpr (kTree)
+                    if (needs_tree(A, P, i1)) F.bad |= !plant<512>(A, P, tree, stages[2]);
                 store_part(stages[0], tid, F.R);
                 F.tile(A, T, i0 + 1, tid);
                 for (int i = i0;; ++i) {
@@ -1488,8 +1502,6 @@ __global__ __launch_bounds__(256, 2) void few_rows_kernel(const WinArgs A) {
         for (int rt = 0; rt < kRT; ++rt) m[rt] = -INFINITY, l[rt] = kq[rt] = 0.0f;
         if (tid == 0) bad_s = 0;
         if (P.pos1 >= 0) {   // else its one tile sees nothing
-            if constexpr (kTree)
-                if (needs_tree(A, P, i1)) bad |= !plant<256>(A, P, tree, stages[1]);   // (read after the tiles' first barrier)
             // the thread's u-th row of tile i (past the last row seen: that row again, masked), and its page
             auto row_of = [&](int i, int u) { return min(kTile * tile_at(P, min(i, i1 - 1)) + (tid >> 4) + 16 * u, P.pos1); };
             auto page_of = [&](int i, int u) { return A.table[(long long)P.slot * A.stride + (row_of(i, u) >> A.shift)]; };
@@ -1514,6 +1526,8 @@ __global__ __launch_bounds__(256, 2) void few_rows_kernel(const WinArgs A) {
                 for (int u = 0; u < 2; ++u) store_part(stages[stage] + 16 * u * kRowB, tid, R[u]);
             };
             fetch(i0);
+            if constexpr (kTree)   // (under the tile's loads; read after the tiles' first barrier)
+                if (needs_tree(A, P, i1)) bad |= !plant<256>(A, P, tree, stages[1]);
             // the wave's quarter of the rows' dims, and its power of two from all quarters' largest values
             float x[kRT][4][8];
             int pos[kRT];
@@ -1586,10 +1600,10 @@ __global__ __launch_bounds__(256, 2) void few_rows_kernel(const WinArgs A) {
                 if (!(tile < P.whole_c && (tile >= P.whole_b || tile < P.whole_a))) {
                     uint32_t odd = 0;   // keys whose scores are not finite in any row
                     const int lane_r = again(lane), g_r = lane_r >> 4;
-                    decltype(sight_of(tree, 0, 0, 0)) sight[kRT];
+                    decltype(sight_of(A, tree, 0, 0, 0)) sight[kRT];
 #pragma unroll
                     for (int rt = 0; rt < kRT; ++rt)
-                        sight[rt] = sight_of(tree, pos[rt], min((16 * rt + (lane_r & 15)) >> lh, P.n - 1), key0);
+                        sight[rt] = sight_of(A, tree, pos[rt], min((16 * rt + (lane_r & 15)) >> lh, P.n - 1), key0);
 #pragma unroll
                     for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
@@ -1670,7 +1684,7 @@ __global__ __launch_bounds__(256, 2) void few_rows_kernel(const WinArgs A) {
         if (__any(bad) && lane == 0) bad_s = 1;
         lds_barrier();
         const float nan = bad_s ? __builtin_nanf("") : 0.0f;
-        const int slot = 2 * blockIdx.x + (S.begins ? 1 : 0);
+        const int slot = 2 * own_place<kTree>(A) + (S.begins ? 1 : 0);
 #pragma unroll
         for (int rt = 0; rt < kRT; ++rt) {
             const int row = 16 * rt + n16, qi = row >> lh, head = P.head0 + (row & ((1 << lh) - 1));
@@ -1888,12 +1902,16 @@ static int attend(const ds4hip_window_attn *a, const int32_t *parents, void *wor
     // (one query each: exactly as many problems)
     if (!a->q_start) A.prob_cap = a->n_seqs << (lh - std::min(lh, log_rows));
     const bool f32 = a->io_f32, in = A.prob_cap <= (log_rows == 4 ? kFewProbs16 : kFewProbs);
-    if (!in) hipLaunchKernelGGL(plan_kernel<kTree>, dim3(1), dim3(1024), 0, st, A);
     // tiles that a problem can have: of rows that the table can name, or of the window, the queries'
-    // own span and the first rows, with their ends inside tiles
+    // own span (a tree's: twice the average one's) and the first rows, with their ends inside tiles
     const long long held = (long long)a->table_stride << shift;
-    const long long span = std::min<long long>(held, (long long)a->window + (kTree ? kMaxNodes : (1 << log_rows) >> std::min(lh, log_rows)));
+    const long long own = kTree ? std::min(kMaxNodes, 2 * (a->n_q / a->n_seqs + 1)) : (1 << log_rows) >> std::min(lh, log_rows);
+    const long long span = std::min<long long>(held, (long long)a->window + own);
     const long long most = a->window > 0 ? span / kTile + 2 + (std::min<long long>(a->n_first, held) + kTile - 1) / kTile : held / kTile + 1;
+    // A tree in a short window is not cut: its problems have a tile more for 32 nodes before theirs, of which the
+    // host knows the average alone, and then need no merge (48 trees of up to 13 nodes: 37 us with it, 30 without).
+    A.uncut = kTree && a->window > 0 && most <= 16;
+    if (!in) hipLaunchKernelGGL(plan_kernel<kTree>, dim3(1), dim3(1024), 0, st, A);
     // Waves with roles for long problems of bf16 (us a call, with roles and without: problems of 34 tiles 1083, 1122,
     // of 1025 to 1152 22700, 24800, 16 sequences of up to 32768 rows 69.5, 72; problems of 6 tiles 176, 166; one
     // token over 4000 rows, in parts of 4 tiles, 30.5, 29.1)
@@ -1903,7 +1921,7 @@ static int attend(const ds4hip_window_attn *a, const int32_t *parents, void *wor
                  : most > 16   ? in ? roles_kernel<kTree, true> : roles_kernel<kTree, false>
                                : in ? window_kernel<kTree, false, true> : window_kernel<kTree, false, false>;
     hipLaunchKernelGGL(main, dim3(A.n_wg), dim3(log_rows < 6 || f32 ? 256 : 512), 0, st, A);
-    if (most > kWhole) {   // (else nothing is cut)
+    if (most > kWhole && !A.uncut) {   // (else nothing is cut)
         const int n = in ? A.prob_cap : A.n_wg - 1;
         // parts that a problem can have: its share of the workgroups, or as many as `per` leaves. Four rows a
         // workgroup from 17 problems on; a row's parts are shared by four waves, by eight from
