@@ -41,7 +41,7 @@ constexpr int kThreads = 512, kWaves = kThreads / 64;
 constexpr int kRow = 8192;       // logits of a row that has one launch
 constexpr int kBins = 2048;
 constexpr int kList = 4096;      // candidates in LDS
-constexpr int kFew = 512;        // candidates that are all compared with each other
+constexpr int kFew = 256;        // candidates that are all compared with each other
 constexpr int kNear = 512;       // tokens of a bin that are compared with each other
 constexpr double kLog2e = 1.4426950408889634074;
 
@@ -238,6 +238,7 @@ struct Pick {
     float logit[kList];                    // the candidates, by index
     uint32_t index[kList];
     unsigned long long near[kNear], near_w[kNear];   // the places and weights in a cut's bin
+    int rank[kFew];
     double wave_sum[kMaxVocab / 512];      // of 512 tokens of the row each
     int n_near, n_list, found;
     unsigned long long found_above, place;
@@ -428,7 +429,10 @@ __device__ __forceinline__ unsigned long long cut_near(Pick &S, int n, const Row
         const unsigned long long mine = S.near[tid];
         unsigned long long before = 0;
 #pragma unroll 4
-        for (int j = 0; j < n; ++j) before += S.near[j] > mine ? kWeigh ? S.near_w[j] : 1 : 0;
+        for (int j = 0; j < n; ++j) {
+            const unsigned long long w = kWeigh ? S.near_w[j] : 1;   // (read whether it counts or not: no branch)
+            before += S.near[j] > mine ? w : 0;
+        }
         if (before < need && before + (kWeigh ? S.near_w[tid] : 1) >= need) S.place = mine;
     }
     __syncthreads();
@@ -586,33 +590,50 @@ __device__ __forceinline__ void draw(const Args &A, Pick &S, const Source &src, 
     give(A, row, src.index(hit), share / all);
 }
 
-// The same and the cuts for a list of at most kFew candidates: each is compared with all others, by as many threads
-// side by side as there are for it, which gives its rank and the weights before it at once. All sums are units.
+// The same and the cuts for a list of at most kFew candidates: all are compared with all, which gives each one's rank and
+// the weights before it at once. A lane holds four of them and a wave has an eighth of the others to compare with, so that
+// what is read from LDS serves 256 comparisons (a read for each 64 took 4 us for 212 candidates). All sums are units.
 __device__ __forceinline__ void pick_few(const Args &A, Pick &S, int n, const Row &R, int row, float top, double all) {
-    const int tid = threadIdx.x;
+    constexpr int kHeld = kFew / 64;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     if (tid < n) {
         S.near[tid] = place_of(key_of(S.logit[tid]), S.index[tid]);
         S.near_w[tid] = units(weight(S.logit[tid], top, R.c, S.table));
     }
+    if (tid < kFew) S.rank[tid] = 0, S.bins[tid] = 0;   // (bins: the weights before each)
     __syncthreads();
-    const int log_n = n > 1 ? 32 - __clz(n - 1) : 0, log_parts = min(31 - __clz(kThreads) - log_n, 4), parts = 1 << log_parts;
-    const int i = tid >> log_parts, part = tid & (parts - 1);
-    const unsigned long long mine = i < n ? S.near[i] : 0, w = i < n ? S.near_w[i] : 0;
-    int rank = 0;
-    unsigned long long before = 0;
     if (R.k || cuts_p(R)) {
-#pragma unroll 4
-        for (int j = part; j < n; j += parts) {
-            const bool is = S.near[j] > mine;
-            rank += is;
-            before += is ? S.near_w[j] : 0;
+        unsigned long long place[kHeld], before[kHeld];
+        int rank[kHeld];
+#pragma unroll
+        for (int t = 0; t < kHeld; ++t) {
+            place[t] = S.near[min(lane + 64 * t, n - 1)];
+            rank[t] = 0;
+            before[t] = 0;
         }
-        for (int off = 1; off < parts; off <<= 1) {
-            rank += __shfl_xor(rank, off);
-            before += __shfl_xor(before, off);
+        const int each = (n + kWaves - 1) / kWaves, end = min(n, (wave + 1) * each);
+#pragma unroll 2
+        for (int j = wave * each; j < end; ++j) {
+            const unsigned long long other = S.near[j], w = S.near_w[j];
+#pragma unroll
+            for (int t = 0; t < kHeld; ++t) {
+                if (64 * t >= n) break;
+                const bool is = other > place[t];
+                rank[t] += is;
+                before[t] += is ? w : 0;
+            }
         }
+#pragma unroll
+        for (int t = 0; t < kHeld; ++t)
+            if (rank[t]) {
+                atomicAdd(&S.rank[lane + 64 * t], rank[t]);
+                atomicAdd(&S.bins[lane + 64 * t], before[t]);
+            }
+        __syncthreads();
     }
-    bool in = part == 0 && i < n && (!R.k || rank < R.k);
+    const int i = min(tid, n - 1), rank = S.rank[min(i, kFew - 1)];
+    const unsigned long long mine = S.near[i], w = S.near_w[i], before = S.bins[i];
+    bool in = tid < n && (!R.k || rank < R.k);
     unsigned long long total;
     if (cuts_p(R)) {
         double sum = all * kUnit;
