@@ -146,6 +146,44 @@ def test_the_largest_tree_and_all_jobs(gpu):
     b.check()
 
 
+@pytest.mark.parametrize("sizes", [[500] * 9, [1024] * 3 + [0, 1, 1023], [4096 // 64] * 64, [63] * 65 + [2]])
+def test_many_nodes(gpu, sizes):
+    """Around the number of nodes up to which the planning workgroup walks the trees itself (4096)."""
+    rng = random.Random(sum(sizes))
+    n = len(sizes)
+    b = Both(gpu, sum(sizes) // 16 + 3 * n, 16, n, 70, 1)
+    seqs = list(range(n))
+    rng.shuffle(seqs)
+    b.extend(seqs, [rng.randrange(1, 20) for _ in seqs])
+    b.extend(seqs, sizes)
+    trees = [random_tree(rng, k, rng.choice(["random", "chain", "star"])) for k in sizes]
+    tokens = [[rng.randrange(4) for _ in range(k)] for k in sizes]
+    targets = [[rng.randrange(4) for _ in range(k)] for k in sizes]
+    flat = lambda xs: i32([v for x in xs for v in x], gpu)
+    path, n_path, following = b.pool.accept(i32(seqs, gpu), i32(starts(sizes), gpu), flat(trees), flat(tokens), flat(targets))
+    want = [walk(t, k, y) for t, k, y in zip(trees, tokens, targets)]
+    assert path.tolist() == [v for (p, _), k in zip(want, sizes) for v in p + [-1] * (k - len(p))]
+    assert n_path.tolist() == [len(p) for p, _ in want] and following.tolist() == [y for _, y in want]
+    assert keep_model(b.model, seqs, sizes, [p for p, _ in want]) == 0
+    b.check()
+
+
+def test_trees_that_lie_over_each_other(gpu):
+    """A q_start that goes back names nodes twice: refused, whatever the nodes' links would make of it."""
+    from ds4cuda_amd import Ds4HipError
+    for nodes in (9, 5000):
+        b = Both(gpu, 600, 16, 3, 400, 1)
+        b.extend([0, 1, 2], [40, 40, 40])
+        for q in ([0, 5, 2, 6], [0, 9, 0, 9], [3, 9, 1, 8], [nodes, 0, 5, 7], [0, nodes, 0, nodes]):
+            x = i32([-1] + list(range(nodes - 1)), gpu)
+            path, n_path, following = b.pool.accept(i32([0, 1, 2], gpu), i32(q, gpu), x, torch.zeros_like(x), torch.zeros_like(x))
+            with pytest.raises(Ds4HipError) as e:
+                b.pool.check()
+            assert e.value.code == -22
+            assert (path == -1).all() and n_path.tolist() == [0] * 3 and following.tolist() == [-1] * 3
+            b.check()
+
+
 def test_refused_calls_change_nothing(gpu):
     from ds4cuda_amd import Ds4HipError
     b = Both(gpu, 60, 8, 6, 8, 2)

@@ -233,3 +233,22 @@ def test_captured_as_the_pool_grows(gpu):
         torch.cuda.synchronize()
         assert torch.equal(out, eager)
     pool.check()
+
+
+@pytest.mark.parametrize("heads,typ", [(64, "bf16"), (8, "bf16"), (16, "fp32")])
+def test_one_large_tree_among_small_ones_in_a_short_window(gpu, heads, typ):
+    """The small ones decide that nothing is cut; the large one's last nodes have many tiles of its own rows before them."""
+    rng = random.Random(25)
+    rows, new = [1100] + [40] * 30, [1000] + [1] * 29 + [3]
+    b = Batch(gpu, rows, 64, 26)
+    trees = [random_tree(rng, n, "random") for n in new]
+    q = queries(gpu, sum(new), heads, typ, 27)
+    out = run(b, q, trees, 64, 3)
+    from draft_check import rows_seen
+    from paged_check import attend_64
+    kv = b.values(0)
+    for v in list(range(0, 1000, 53)) + [998, 999]:
+        seen = kv[torch.tensor(rows_seen(100, trees[0], v, 64, 3), device=gpu)]
+        ref, size, err = attend_64(q[v:v + 1], seen, [seen.shape[0] - 1], 0, 0, None)
+        assert ((out[v:v + 1].double() - ref).abs() <= bound_of(ref, size, err, typ == "fp32")).all(), v
+    check(b, q[1000:], out[1000:], trees[1:], 64, 3, None, list(range(1, 31)))
