@@ -1,11 +1,13 @@
 // window_attn.hip — attention of packed queries over the pages of their
 // sequences' FP8 rows: a sliding window and a few first rows that stay visible,
-// for prompts and for single tokens, on gfx950 MFMA.
+// for prompts, for single tokens and for trees of drafted tokens, on gfx950 MFMA.
 //
 // Math, per query at position p and head h over the rows k it sees
 // (k <= p and (k > p - window or k < first)):
 //   out = sum_k exp(s_k - M) V_k / (exp(sink_h - M) + sum_k exp(s_k - M)),
 //   s_k = (q_h . K_k) / sqrt(512), K == V (one latent KV head).
+// The nodes of a tree are the last rows of their sequence. Node i at depth d sees of them its line to the root
+// alone, has position p = (rows before the tree's) + d, and sees an ancestor by that one's position.
 //
 // Work split. A problem is 64 rows (queries x heads of one sequence), or 16 where the
 // sequences have no more on the average, and the key tiles any of them sees. The tiles
@@ -22,6 +24,9 @@
 // of a few tiles are launch, the queries, the first rows and the outputs one after the other (about 20 us).
 // (A workgroup's place on the line by XCD, so that neighbours share an L2, changed nothing:
 // the rows come from there already.)
+// Trees of 64 heads: 16 of up to 24 nodes after up to 8192 rows (80 GFLOP) 177 us and 14 to merge, 75 tiles a
+// workgroup in 1.7 parts on the average; 512 nodes after 60000 rows 0.88 PFLOP/s; 48 of up to 13 in a window of 128 rows
+// 30 us, one of 7 after 1500 rows 28 and 6.4 to merge: launch, line (4), queries and first rows (7), tiles (1.6), outputs (3).
 
 #include "attn_tile.h"
 #include "ds4hip_common.h"
@@ -413,14 +418,6 @@ __global__ __launch_bounds__(1024) void plan_kernel(const WinArgs A) {
     A.wg_prob[b] = prob;
 }
 
-// The workgroup's place on the line. Trees: neighbours on the line have one XCD (workgroups are dealt to the eight in
-// turn), since a sequence's nodes, which read the same rows, are neighbours.
-template <bool kTree>
-__device__ inline int own_place(const WinArgs &A) {
-    const int b = blockIdx.x;
-    return kTree ? (b & 7) * (A.n_wg >> 3) + (b >> 3) : b;   // (n_wg is a multiple of 8)
-}
-
 // The workgroup's own copy of a line of at most kFew problems (0: none).
 template <int kFew>
 struct Line {
@@ -442,7 +439,7 @@ struct Place {
 // the first one leaves it to the merge; else the plan kernel did.
 template <bool kTree, int kFew, int kThreads>
 __device__ inline Place take_place(const WinArgs &A, Line<kFew> &L) {
-    const int tid = threadIdx.x, wg = own_place<kTree>(A);
+    const int tid = threadIdx.x, wg = blockIdx.x;
     Place at;
     at.part = 0;
     if constexpr (kFew != 0) {
@@ -734,7 +731,7 @@ __global__ __launch_bounds__(kF32 ? 256 : 512, kF32 ? 1 : 2) void window_kernel(
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int n16 = lane & 15, g = lane >> 4, row = 16 * (w & 3) + n16;
     const int kh = w >> 2;   // the wave's (first) key half
-    const int wg = own_place<kTree>(A);
+    const int wg = blockIdx.x;
     constexpr int kFew = kInline ? kFewProbs : 0;
     __shared__ Line<kFew> line;
     __shared__ Tree<kTree, kRows> tree;
@@ -1192,7 +1189,7 @@ __global__ __launch_bounds__(512, 2) void roles_kernel(const WinArgs A) {
             const Stretch T = S;
             const Problem &P = T.P;
             const bool whole = T.begins && T.ends;
-            const int slot = 2 * own_place<kTree>(A) + (T.begins ? 1 : 0), i0 = T.i0, i1 = T.i1;
+            const int slot = 2 * blockIdx.x + (T.begins ? 1 : 0), i0 = T.i0, i1 = T.i1;
             const int n_rt = ((P.n << lh) + 15) >> 4;   // row tiles in use
             F.bad = P.slot < 0;
             Ring G;
@@ -1354,7 +1351,7 @@ __global__ __launch_bounds__(512, 2) void roles_kernel(const WinArgs A) {
             const Stretch T = S;
             const Problem &P = T.P;
             const bool whole = T.begins && T.ends;
-            const int slot = 2 * own_place<kTree>(A) + (T.begins ? 1 : 0), i0 = T.i0, i1 = T.i1;
+            const int slot = 2 * blockIdx.x + (T.begins ? 1 : 0), i0 = T.i0, i1 = T.i1;
             const int n_rt = ((P.n << lh) + 15) >> 4;   // row tiles in use
             F.bad = P.slot < 0;
             Ring G;
@@ -1684,7 +1681,7 @@ __global__ __launch_bounds__(256, 2) void few_rows_kernel(const WinArgs A) {
         if (__any(bad) && lane == 0) bad_s = 1;
         lds_barrier();
         const float nan = bad_s ? __builtin_nanf("") : 0.0f;
-        const int slot = 2 * own_place<kTree>(A) + (S.begins ? 1 : 0);
+        const int slot = 2 * blockIdx.x + (S.begins ? 1 : 0);
 #pragma unroll
         for (int rt = 0; rt < kRT; ++rt) {
             const int row = 16 * rt + n16, qi = row >> lh, head = P.head0 + (row & ((1 << lh) - 1));
