@@ -320,9 +320,13 @@ def _same_gpu(t, index, name):
 
 
 @lru_cache(maxsize=256)
+def _workspace_bytes(name, *sizes) -> int:
+    return getattr(lib(), name)(*sizes)
+
+
 def window_workspace_bytes(n_seqs, n_q, n_head) -> int:
-    return lib().ds4hip_flash_attn_window_fp8_workspace_bytes(_int32(n_seqs, "n_seqs"), _int32(n_q, "n_q"),
-                                                              _int32(n_head, "n_head"))
+    return _workspace_bytes("ds4hip_flash_attn_window_fp8_workspace_bytes", _int32(n_seqs, "n_seqs"), _int32(n_q, "n_q"),
+                            _int32(n_head, "n_head"))
 
 
 class _Here:
@@ -455,9 +459,8 @@ class Sample(C.Structure):
                 ("all_top_p", C.c_float), ("all_min_p", C.c_float), ("tokens", C.c_void_p), ("probs", C.c_void_p)]
 
 
-@lru_cache(maxsize=256)
 def sample_workspace_bytes(n_rows, n_vocab) -> int:
-    return lib().ds4hip_sample_workspace_bytes(_int32(n_rows, "n_rows"), _int32(n_vocab, "n_vocab"))
+    return _workspace_bytes("ds4hip_sample_workspace_bytes", _int32(n_rows, "n_rows"), _int32(n_vocab, "n_vocab"))
 
 
 def sample_tokens(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, tokens=None, probs=None, workspace=None,

@@ -89,3 +89,16 @@ def test_python_refuses_host_tensors_and_shapes():
                            torch.zeros((64, 64), dtype=torch.int16))
     with pytest.raises(Ds4HipError):
         ops.flash_attn_tree_fp8(f(2, 64, 512), i(2), cache, i(2, 4), i(2), page_rows=16)
+
+
+def test_workspace_sizes_of_any_integers():
+    import numpy as np
+    from ds4cuda_amd import ops
+    n = torch.tensor(4)
+    for f, rest in ((ops.window_workspace_bytes, (64, 64)), (ops.sample_workspace_bytes, (4096,))):
+        sizes = []
+        for k in (4, 4000):
+            n.fill_(k)   # (the same tensor with another value)
+            sizes.append(f(n, *rest))
+            assert sizes[-1] == f(k, *rest) == f(np.array(k), *rest) > 0
+        assert sizes[0] < sizes[1]
