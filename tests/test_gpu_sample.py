@@ -195,3 +195,45 @@ def test_another_stream(gpu):
     got = sample(x, u, 1.0, 0, 0.9, 0.0, stream=side)
     side.synchronize()
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_temperatures_and_logits_of_any_size(gpu):
+    for scale, t in ((1e-30, 1e-30), (1e-30, 1.0), (1e30, 1e30), (1e30, 1.0), (1.0, 1e-30), (1.0, 1e-3), (1.0, 1e3),
+                     (1.0, 3e38), (1e36, 3e38)):
+        for vocab in (500, 12000):
+            x, u = scale * logits_of(gpu, 4, vocab, "fp32", 18), randoms(gpu, 4, 19)
+            for k, p, m in ((0, 1.0, 0.0), (20, 1.0, 0.0), (0, 0.9, 0.0), (0, 1.0, 0.1), (700, 0.99, 0.001)):
+                check(x, u, t, k, p, m, sample(x, u, t, k, p, m))
+
+
+def test_rows_past_32_bits(gpu):
+    stride, vocab = 1300000007, 9001   # the last row begins 5.2 GB behind the first
+    x = torch.empty(2 * stride + vocab, dtype=torch.bfloat16, device=gpu).as_strided((3, vocab), (stride, 1))
+    x.copy_(logits_of(gpu, 3, vocab, "bf16", 20))
+    u = randoms(gpu, 3, 21)
+    for t, k, p, m in FILTERS:
+        check(x, u, t, k, p, m, sample(x, u, t, k, p, m))
+
+
+def test_the_most_rows(gpu):
+    x, u = logits_of(gpu, 64, 8256, "bf16", 22).repeat(1024, 1), randoms(gpu, 65536, 23)
+    some = torch.arange(0, 65536, 1009, device=gpu)
+    for t, k, p, m in ((0.8, 10, 0.9, 0.0), (1.0, 0, 1.0, 0.0), (3.0, 0, 0.95, 0.0)):
+        got = sample(x, u, t, k, p, m)
+        check(x[some], u[some], t, k, p, m, (got[0][some], got[1][some]))
+
+
+def test_two_streams_at_once(gpu):
+    """Calls that run at the same time, each with its own workspace."""
+    inputs = [(logits_of(gpu, 40, 40001, "bf16", 24 + i, 0.5 + i), randoms(gpu, 40, 26 + i)) for i in range(2)]
+    want = [sample(x, u, 0.9, 0, 0.9, 0.0) for x, u in inputs]
+    streams = [torch.cuda.Stream(gpu) for _ in range(2)]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for i, (x, u) in enumerate(inputs):
+            got[i].append(sample(x, u, 0.9, 0, 0.9, 0.0, stream=streams[i]))
+    torch.cuda.synchronize()
+    for w, all_got in zip(want, got):
+        for g in all_got:
+            assert torch.equal(w[0], g[0]) and torch.equal(w[1], g[1])
