@@ -45,6 +45,7 @@ constexpr int kMinTiles = 4;         // tiles of a part
 constexpr int kWhole = 8;            // tiles of a problem that is never cut
 constexpr int kPart = 12;            // tiles whose time a cut costs: its parts' 256 KB and their merge
 constexpr int kSecond = 4;           // tiles whose time a workgroup's second problem costs
+constexpr int kHead = 10;            // tiles whose time a problem of trees costs besides its own
 constexpr int kMaxSeqs = 4096;
 constexpr int kMaxRows = 0x7FFFFF00; // rows of a sequence: a tile's keys stay in 32 bits
 constexpr int kFewProbs = 512, kFewProbs16 = 128;   // problems of 64, 16 rows that a workgroup lays out itself
@@ -340,12 +341,29 @@ __device__ inline int lay_line(const WinArgs &A, First *first_s, int4 *seq_s, lo
 struct Cuts {
     long long tiles, per;
     int whole;   // tiles of a problem that stays whole; < 0: workgroup b has problem b
+    int head;    // tiles that the line counts for a problem besides its own
 };
+
+// Trees: the line counts kHead tiles more for a problem, the time of its queries, mask and outputs, where workgroups have
+// several of them; else one with many short ones ends last. Problems of 64 rows, us with and without, tiles of a
+// workgroup in brackets: 12 to 16 trees of up to 32 nodes after 128 to 8192 rows 131, 178 [45], 135, 236 [53], 182, 335 [84];
+// after 32 to 2048 rows 79, 121 [13], 107, 212 [26]; 16 of up to 24 after up to 8192 164, 185 [75]; fp32 250, 391 [49]; of
+// 16 rows 68, 72 [31]. (14 tiles: 0 to 5% more, 18: up to 30%, 6: up to 10%.) Cuts lie further apart than a head is long, so that every part has a tile.
+__device__ inline int head_of(const WinArgs &A, const Cuts &C, int n_prob) {
+    const long long per = (C.tiles + (long long)kHead * n_prob + A.n_wg - 1) / A.n_wg;
+    return C.whole >= 0 && !A.uncut && per > kHead + 2 ? kHead : 0;
+}
+__device__ inline void add_heads(const WinArgs &A, Cuts &C, int n_prob) {
+    C.tiles += (long long)C.head * n_prob;
+    C.per = max(C.per, (C.tiles + A.n_wg - 1) / A.n_wg);
+    C.whole += C.head;   // (so what is cut has nine tiles or more)
+}
 
 __device__ inline Cuts cuts_of(const WinArgs &A, long long tiles, int n_prob, int longest) {
     const int n_wg = A.n_wg;
     Cuts C;
     C.tiles = tiles;
+    C.head = 0;
     // at least sqrt(longest / 16) tiles: a long problem's merge takes 0.09 us a part, a tile 1.5
     C.per = max((tiles + n_wg - 1) / n_wg, (long long)max(kMinTiles, (int)sqrtf((float)longest * 0.0625f)));
     C.whole = A.uncut ? 1 << 30 : (int)min(max((long long)kWhole, C.per / 8), 1LL << 30);
@@ -384,6 +402,7 @@ __device__ inline void leave(const WinArgs &A, const Cuts &C, int n_prob) {
     *A.n_prob = n_prob;
     A.line[0] = C.per;
     A.line[1] = C.whole;
+    A.line[2] = C.head;
 }
 
 // One workgroup, for lines of many problems: latency of a few loads, scans and a search in LDS,
@@ -404,10 +423,21 @@ __global__ __launch_bounds__(1024) void plan_kernel(const WinArgs A) {
         A.pre[i] = before;
         if (i < kHeld) pre_s[i] = before;
     });
-    const Cuts C = cuts_of(A, tiles, n_prob, longest);
+    Cuts C = cuts_of(A, tiles, n_prob, longest);
+    if constexpr (kTree) {
+        C.head = head_of(A, C, n_prob);
+        if (C.head) {
+            add_heads(A, C, n_prob);
+            for (int i = threadIdx.x; i < n_prob; i += 1024) {
+                const long long before = (i < kHeld ? pre_s[i] : A.pre[i]) + (long long)C.head * i;
+                A.pre[i] = before;
+                if (i < kHeld) pre_s[i] = before;
+            }
+        }
+    }
     if (threadIdx.x == 0) {
-        A.pre[n_prob] = tiles;
-        if (n_prob < kHeld) pre_s[n_prob] = tiles;
+        A.pre[n_prob] = C.tiles;
+        if (n_prob < kHeld) pre_s[n_prob] = C.tiles;
         leave(A, C, n_prob);
     }
     __syncthreads();
@@ -433,6 +463,7 @@ struct Place {
     int n_prob, prob;
     long long t, end;
     int part;   // > 0: even parts of that many tiles at most
+    int head;   // tiles that the line counts before each problem's own
 };
 
 // Few problems: every workgroup lays out the line itself (a launch and a wait less), and
@@ -441,7 +472,7 @@ template <bool kTree, int kFew, int kThreads>
 __device__ inline Place take_place(const WinArgs &A, Line<kFew> &L) {
     const int tid = threadIdx.x, wg = blockIdx.x;
     Place at;
-    at.part = 0;
+    at.part = at.head = 0;
     if constexpr (kFew != 0) {
         if (tid == 0) L.longest = 0;
         long long tiles;
@@ -472,6 +503,15 @@ __device__ inline Place take_place(const WinArgs &A, Line<kFew> &L) {
                 at.part = (int)per;
             }
         }
+        if constexpr (kTree) {
+            C.head = at.part ? 0 : head_of(A, C, at.n_prob);
+            if (C.head) {
+                add_heads(A, C, at.n_prob);
+                for (int i = tid; i <= at.n_prob; i += kThreads) L.pre[i] += (long long)C.head * i;
+                __syncthreads();
+            }
+            at.head = C.head;
+        }
         if (wg == 0) {
             for (int i = tid; i <= at.n_prob; i += kThreads) {
                 if (i < at.n_prob) A.prob[i] = L.prob[i];
@@ -487,6 +527,7 @@ __device__ inline Place take_place(const WinArgs &A, Line<kFew> &L) {
         at.prob = A.wg_prob[wg];
         at.t = A.wg_tile[wg];
         at.end = A.wg_tile[wg + 1];
+        if constexpr (kTree) at.head = (int)A.line[2];
     }
     return at;
 }
@@ -509,6 +550,13 @@ __device__ inline bool next_stretch(const WinArgs &A, const Line<kFew> &L, Place
     S.begins = at.t == begin;
     S.ends = end <= at.end;
     int i0 = (int)(at.t - begin), i1 = (int)(min(end, at.end) - begin);
+    if constexpr (kTree) {   // (a cut leaves both sides a tile; cuts lie further apart than heads are long)
+        const int last = S.P.tiles - 1;
+        if (at.head) {
+            i0 = S.begins ? 0 : min(max(i0 - at.head, 1), last);
+            i1 = S.ends ? last + 1 : min(max(i1 - at.head, 1), last);
+        }
+    }
     if (kFew && at.part) {
         const int parts = (int)(end - begin) / at.part, k = i0 / at.part, n = S.P.tiles / parts, more = S.P.tiles - n * parts;
         i0 = n * k + min(k, more);
@@ -1813,7 +1861,7 @@ size_t lay_out(WinArgs *A, char *base, long long cap, int log_rows) {
         at += up256(bytes);
         return p;
     };
-    char *line = take(2 * sizeof(long long)), *n_prob = take(sizeof(int)), *prob = take(sizeof(int4) * cap),
+    char *line = take(3 * sizeof(long long)), *n_prob = take(sizeof(int)), *prob = take(sizeof(int4) * cap),
          *pre = take(sizeof(long long) * (cap + 1)), *wg_tile = take(sizeof(long long) * (n_wg + 1)),
          *wg_prob = take(sizeof(int) * (n_wg + 1)), *ml = take(sizeof(float) * 2 * n_wg * 3 * rows),
          *o = take(sizeof(float) * 2 * n_wg * rows * kD);

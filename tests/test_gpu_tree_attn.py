@@ -252,3 +252,20 @@ def test_one_large_tree_among_small_ones_in_a_short_window(gpu, heads, typ):
         ref, size, err = attend_64(q[v:v + 1], seen, [seen.shape[0] - 1], 0, 0, None)
         assert ((out[v:v + 1].double() - ref).abs() <= bound_of(ref, size, err, typ == "fp32")).all(), v
     check(b, q[1000:], out[1000:], trees[1:], 64, 3, None, list(range(1, 31)))
+
+
+@pytest.mark.parametrize("long,short,new,heads,typ", [(3, 14, 24, 64, "bf16"), (3, 22, 24, 64, "bf16"), (5, 30, 13, 64, "fp32"),
+                                                      (60, 60, 2, 8, "bf16"), (60, 60, 2, 8, "fp32")])
+def test_long_trees_and_many_short_ones(gpu, long, short, new, heads, typ):
+    """Workgroups with parts of several trees, cut in any place, from the few problems that each workgroup lays out itself and
+    the many that a kernel does."""
+    rng = random.Random(long + short)
+    rows = [rng.choice([8000, 8031, 7990])] * long + [rng.randint(40, 300) for _ in range(short)]
+    rng.shuffle(rows)
+    b = Batch(gpu, rows, 64, short)
+    trees = [random_tree(rng, new - rng.randint(0, 1), "random") for _ in rows]
+    q = queries(gpu, sum(map(len, trees)), heads, typ, 12)
+    sinks = torch.randn(heads, device=gpu)
+    out = run(b, q, trees, 0, 0, sinks)
+    check(b, q, out, trees, 0, 0, sinks)
+    assert torch.equal(out, run(b, q, trees, 0, 0, sinks))
