@@ -269,3 +269,14 @@ def test_long_trees_and_many_short_ones(gpu, long, short, new, heads, typ):
     out = run(b, q, trees, 0, 0, sinks)
     check(b, q, out, trees, 0, 0, sinks)
     assert torch.equal(out, run(b, q, trees, 0, 0, sinks))
+
+
+def test_more_problems_than_the_plan_holds_in_shared_memory(gpu):
+    rng = random.Random(13)
+    rows = [270 + rng.randint(0, 140) for _ in range(17)]
+    b = Batch(gpu, rows, 32, 14)
+    trees = [random_tree(rng, 250 + rng.randint(0, 20), "random") for _ in rows]
+    q = queries(gpu, sum(map(len, trees)), 128, "bf16", 15)   # two problems a node, more than 8192
+    out = run(b, q, trees)
+    assert 2 * q.shape[0] > 8192
+    check(b, q, out, trees, 0, 0, None)
