@@ -15,6 +15,7 @@
 // (647 MB read and written) 140 us, 4.6 TB/s of the 5.1 that a large copy reaches.
 
 #include "ds4hip_common.h"
+#include "node_range.h"
 #include "step_bodies.h"
 #include "../../include/ds4hip_pages.h"
 
@@ -508,17 +509,18 @@ __device__ inline int walk(const Walk &W, int j, int a, int n, const int *parent
 
 // -1 for the nodes that no job names, before the first job's and behind the last one's.
 __device__ inline void clear_path(const Walk &W, const int32_t *q_start, int n_jobs, int n_nodes, int tid, int threads) {
-    for (int i = tid; i < min(q_start[0], n_nodes); i += threads) W.path[i] = -1;
-    for (int i = max(q_start[n_jobs], 0) + tid; i < n_nodes; i += threads) W.path[i] = -1;
+    for (int i = tid; i < start_in(q_start[0], n_nodes); i += threads) W.path[i] = -1;
+    for (int i = start_in(q_start[n_jobs], n_nodes) + tid; i < n_nodes; i += threads) W.path[i] = -1;
 }
 
 // A workgroup a job, of one wave, for calls of many nodes (the planning workgroup walks the others itself).
 __global__ __launch_bounds__(64) void walk_kernel(const int32_t *q_start, int n_jobs, int n_nodes, const Walk W) {
     __shared__ int parent_s[kNodes], token_s[kNodes], target_s[kNodes];
     const int j = blockIdx.x, lane = threadIdx.x;
-    const int a = q_start[j], b = q_start[j + 1], n = b - a;
+    const NodeRange own = nodes_between(q_start[j], q_start[j + 1], n_nodes, kNodes);
+    const int a = own.first, n = own.n;
     if (j == 0) clear_path(W, q_start, n_jobs, n_nodes, lane, 64);
-    if (a < 0 || b > n_nodes || n <= 0 || n > kNodes) {   // (the plan refuses what is not 0 nodes)
+    if (n == 0) {   // (the plan refuses starts that do not say so)
         if (lane == 0) W.n_path[j] = 0, W.next[j] = -1;
         return;
     }
@@ -549,13 +551,10 @@ __device__ inline void walk_all(const Walk &W, Trees &T, const int32_t *q_start,
         T.target[i] = W.targets[i];
         T.next[i] = kWalkNodes;
     }
-    for (int i = tid; i <= n_jobs; i += kThreads) T.start[i] = q_start[i];
+    for (int i = tid; i <= n_jobs; i += kThreads) T.start[i] = start_in(q_start[i], n_nodes);
     __syncthreads();
-    // the nodes of job j, none where the plan refuses them
-    auto nodes_of = [&](int j) {
-        const int a = T.start[j], b = T.start[j + 1];
-        return a >= 0 && b <= n_nodes && b - a <= kNodes ? b - a : 0;
-    };
+    // (the plan looks at the starts as they are, and refuses those that were moved here)
+    auto nodes_of = [&](int j) { return nodes_between(T.start[j], T.start[j + 1], n_nodes, kNodes).n; };
     for (int i = tid; i < n_nodes; i += kThreads) {
         const int j = job_of(T.start, n_jobs, i), a = T.start[j], v = i - a, p = T.parent[i];
         if (v > 0 && v < nodes_of(j) && p >= 0 && p < v && T.target[a + p] >= 0 && T.token[i] == T.target[a + p]) atomicMin(&T.next[a + p], v);
