@@ -598,7 +598,8 @@ __device__ __forceinline__ void draw(const Args &A, Pick &S, const Source &src, 
 
 // The same and the cuts for a list of at most kFew candidates: all are compared with all, which gives each one's rank and
 // the weights before it at once. A lane holds four of them and a wave has an eighth of the others to compare with, so that
-// what is read from LDS serves 256 comparisons (a read for each 64 took 4 us for 212 candidates). All sums are units.
+// what is read from LDS serves 256 comparisons (a read for each 64 took 4 us for 212 candidates). All sums are units: that of
+// all that is kept is off by 2^-38 of itself at most.
 __device__ __forceinline__ void pick_few(const Args &A, Pick &S, int n, const Row &R, int row, float top, double all) {
     constexpr int kHeld = kFew / 64;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -653,7 +654,9 @@ __device__ __forceinline__ void pick_few(const Args &A, Pick &S, int n, const Ro
     if (cuts_m(R)) in = in && (rank == 0 && (R.k || cuts_p(R)) ? true : weight(value_of((uint32_t)(mine >> 32)), top, R.c, S.table) >= R.m);
     const unsigned long long upto = block_scan(in ? w : 0, S.scans, &total);
     const unsigned long long target = (unsigned long long)(R.u * (double)total);   // the sum passes it: at least one more
-    if (in && upto > target && upto - w <= target) give(A, row, (int)~(uint32_t)mine, (double)w / (double)total);
+    // (the token's own weight not in units: of a small one they keep only the leading bits)
+    if (in && upto > target && upto - w <= target)
+        give(A, row, (int)~(uint32_t)mine, weight(value_of((uint32_t)(mine >> 32)), top, R.c, S.table) * kUnit / (double)total);
 }
 
 // The least logit of a candidate, from the lowest bin that all that is kept lies in (as one logit, with room for what is
