@@ -30,3 +30,18 @@ def test_shares_of_small_weights(gpu, vocab, many):
         for k, p, m in ((0, 1.0, 0.0), (vocab, 1.0, 0.0), (vocab - 1, 1.0, 0.0), (0, 1.0, 2.0 ** -46), (vocab - 1, 1.0, 2.0 ** -46),
                         (0, 1.0 - 2.0 ** -24, 0.0)):
             check(x, u, t, k, p, m, sample(x, u, t, k, p, m))
+
+
+@pytest.mark.parametrize("vocab", [300, 900, 8000, 12000, 70000])
+def test_differences_past_fp32(gpu, vocab):
+    """Logits from -3.2e38 to 3.2e38 at temperatures of that size: their differences pass fp32's range, while even the
+    smallest weight is e^-6.4 of the largest."""
+    g = torch.Generator(gpu).manual_seed(vocab)
+    for t in (3e38, 1e38):
+        x = (2.0 * torch.rand((3, vocab), generator=g, device=gpu) - 1.0) * 3.2e38
+        x[1] = torch.where(x[1] > 0, 3.2e38, -3.2e38)
+        x[2, ::3] = -math.inf
+        u = torch.rand(3, generator=g, device=gpu)
+        for k, p, m in ((0, 1.0, 0.0), (vocab - vocab // 10, 1.0, 0.0), (vocab // 2 + vocab // 4, 0.9, 0.0), (0, 0.95, 0.0), (0, 0.8, 0.0),
+                        (0, 1.0, 0.2), (50, 1.0, 0.0), (vocab - 1, 0.99, 0.001)):
+            check(x, u, t, k, p, m, sample(x, u, t, k, p, m))
