@@ -39,15 +39,13 @@ struct Moves {
     int *n_live;   // held pages (compact)
     int *src, *dst, *count;   // [n_pages] pages, and the rows of each
     int *now;      // [n_pages] where a page went (compact)
-    int *base;     // [kJobs] a sequence's rows before its drafts (keep)
 };
 
-size_t moves_bytes(int n_pages) { return sizeof(int) * (64 + 4 * (size_t)n_pages + kJobs); }
+size_t moves_bytes(int n_pages) { return sizeof(int) * (64 + 4 * (size_t)n_pages); }
 
 Moves moves_at(void *ws, int n_pages) {
     int *p = static_cast<int *>(ws);
-    return {p, p + 1, p + 64, p + 64 + (size_t)n_pages, p + 64 + 2 * (size_t)n_pages, p + 64 + 3 * (size_t)n_pages,
-            p + 64 + 4 * (size_t)n_pages};
+    return {p, p + 1, p + 64, p + 64 + (size_t)n_pages, p + 64 + 2 * (size_t)n_pages, p + 64 + 3 * (size_t)n_pages};
 }
 
 struct Plan {
@@ -643,10 +641,7 @@ __global__ __launch_bounds__(kThreads) void keep_kernel(const ds4hip_kv_pages P,
             if (k >= pages_of(P, now)) P.refs[*entry(P, s, k)] = 0;
         }
         __syncthreads();
-        if (tid < n_jobs) {
-            P.rows[seq] = base + kept;
-            M.base[tid] = base;
-        }
+        if (tid < n_jobs) P.rows[seq] = base + kept;
         if (tid == 0) *M.n = n_jobs;
         return;
     }
@@ -669,8 +664,9 @@ __global__ __launch_bounds__(256) void keep_rows_kernel(const ds4hip_kv_pages P,
     const int tid = threadIdx.x, lane = tid & 63, shift = __builtin_ctz(P.page_rows);
     const int j = blockIdx.x / split, part = blockIdx.x - j * split;
     const int l0 = (int)((long long)P.n_layers * part / split), l1 = (int)((long long)P.n_layers * (part + 1) / split);
-    const int kept = n_path[j], seq = seqs[j], base = M.base[j], a = q_start[j];
+    const int kept = n_path[j], seq = seqs[j], a = q_start[j];
     if (*M.n == 0) return;   // refused
+    const int base = P.rows[seq] - kept;   // (the plan has cut the sequence)
     for (int i0 = 0; i0 < kept; i0 += kRows) {
         const int i = i0 + lane, node = i < kept ? path[a + i] : i;
         const uint64_t moved = __ballot(node != i);   // (the same in every wave)
