@@ -511,6 +511,12 @@ __device__ inline void clear_path(const Walk &W, const int32_t *q_start, int n_j
     for (int i = start_in(q_start[n_jobs], n_nodes) + tid; i < n_nodes; i += threads) W.path[i] = -1;
 }
 
+// A call without jobs: its nodes are no job's.
+__global__ __launch_bounds__(256) void no_path_kernel(int32_t *path, int n_nodes) {
+    const int i = blockIdx.x * 256 + threadIdx.x;
+    if (i < n_nodes) path[i] = -1;
+}
+
 // A workgroup a job, of one wave, for calls of many nodes (the planning workgroup walks the others itself).
 __global__ __launch_bounds__(64) void walk_kernel(const int32_t *q_start, int n_jobs, int n_nodes, const Walk W) {
     __shared__ int parent_s[kNodes], token_s[kNodes], target_s[kNodes];
@@ -824,13 +830,17 @@ extern "C" int ds4hip_kv_pages_accept(const ds4hip_kv_pages *p, const int32_t *s
                                       const int32_t *parents, const int32_t *tokens, const int32_t *targets, int n_nodes,
                                       int32_t *path, int32_t *n_path, int32_t *next, void *workspace, size_t workspace_bytes,
                                       void *stream) {
-    if (!pool_ok(p) || n_jobs < 0 || n_jobs > kJobs || n_nodes < 0 || n_nodes > (1 << 24) ||
-        (n_jobs && (!seqs || !q_start || !n_path || !next || (n_nodes && (!parents || !tokens || !targets || !path)) ||
+    if (!pool_ok(p) || n_jobs < 0 || n_jobs > kJobs || n_nodes < 0 || n_nodes > (1 << 24) || (n_nodes && !path) ||
+        (n_jobs && (!seqs || !q_start || !n_path || !next || (n_nodes && (!parents || !tokens || !targets)) ||
                     !workspace || !aligned(workspace, 8) || workspace_bytes < moves_bytes(p->n_pages))))
         return ds4hip_set_last_error(kEINVAL);
-    if (n_jobs == 0) return 0;
-    const Moves M = moves_at(workspace, p->n_pages);
     const hipStream_t st = (hipStream_t)stream;
+    if (n_jobs == 0) {
+        if (n_nodes == 0) return 0;
+        hipLaunchKernelGGL(no_path_kernel, dim3((unsigned)(n_nodes + 255) / 256), dim3(256), 0, st, path, n_nodes);
+        return ds4hip_set_last_error(hip_status(hipGetLastError()));
+    }
+    const Moves M = moves_at(workspace, p->n_pages);
     const Walk W = {parents, tokens, targets, path, n_path, next};
     const bool here = n_nodes <= kWalkNodes;
     if (!here) hipLaunchKernelGGL(walk_kernel, dim3(n_jobs), dim3(64), 0, st, q_start, n_jobs, n_nodes, W);
