@@ -82,7 +82,7 @@ struct WinArgs {
     int uncut;               // 1: no problem is cut, however long
     // workspace
     int prob_cap;
-    long long *line;         // [2] tiles per workgroup, tiles of a problem that stays whole
+    long long *line;         // [3] tiles per workgroup, tiles of a problem that stays whole, of a problem's head (trees)
     int *n_prob;
     int4 *prob;              // [prob_cap] records
     long long *pre;          // [prob_cap + 1] tiles before each problem
@@ -1522,6 +1522,9 @@ __global__ __launch_bounds__(256, 2) void few_rows_kernel(const WinArgs A) {
     __shared__ int bad_s;
     __shared__ Line<kFew> line;
     __shared__ Tree<kTree, kRows> tree;
+    // (each on 16 bytes at most)
+    static_assert(sizeof(stages) + sizeof(sum_s) + sizeof(top_s) + sizeof(bad_s) + sizeof(line) + sizeof(tree) + 6 * 16 <= 160 * 1024 / 2,
+                  "two workgroups a CU");
     const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
     const int n16 = lane & 15, g = lane >> 4;
     Place at = take_place<kTree, kFew, 256>(A, line);
