@@ -785,18 +785,15 @@ __global__ __launch_bounds__(kF32 ? 256 : 512, kF32 ? 1 : 2) void window_kernel(
     __shared__ Tree<kTree, kRows> tree;
     Place at = take_place<kTree, kFew, 64 * kW>(A, line);
     const int lh = log_hpt(A);
-    uint32_t ka[kN], va[2];
-    {
+    // (the other key half is kHalf further. With a register for it, and one for that of va, the fp32 kernels read three
+    // spilled fragments a tile and not two, in one form or the other: 16 queries of 64 heads over 20000 rows 180 us and not 174)
+    constexpr uint32_t kHalf = 16 * kRowB;
+    const uint32_t ka = pi_key(16 * kh + n16) * kRowB + 16 * g;
+    uint32_t va[2];
 #pragma unroll
-        for (int u = 0; u < kN; ++u) {
-            const int r = pi_key(16 * (kh + u) + n16);
-            ka[u] = r * kRowB + 16 * g;
-        }
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt) {
-            const int v = pi_key(16 * kt + 4 * g + (n16 >> 2));
-            va[kt] = lds_addr(stages[0]) + v * kRowB + kDB * w + 8 * (n16 & 3);
-        }
+    for (int kt = 0; kt < 2; ++kt) {
+        const int v = pi_key(16 * kt + 4 * g + (n16 >> 2));
+        va[kt] = lds_addr(stages[0]) + v * kRowB + kDB * w + 8 * (n16 & 3);
     }
 
     // The page of the thread's u-th row of the first tile is looked up before the outputs of the
@@ -1002,7 +999,7 @@ __global__ __launch_bounds__(kF32 ? 256 : 512, kF32 ? 1 : 2) void window_kernel(
 #pragma unroll
                     for (int u = 0; u < kN; ++u)
 #pragma unroll
-                        for (int v = 0; v < 2; ++v) k[0][u][v] = *reinterpret_cast<const half8_t *>(st + ka[u] + 64 * v);
+                        for (int v = 0; v < 2; ++v) k[0][u][v] = *reinterpret_cast<const half8_t *>(st + ka + kHalf * u + 64 * v);
 #pragma unroll
                     for (int s0 = 0; s0 < 16; s0 += 2) {
                         const int now = (s0 / 2) & 1;
@@ -1010,7 +1007,7 @@ __global__ __launch_bounds__(kF32 ? 256 : 512, kF32 ? 1 : 2) void window_kernel(
                         for (int u = 0; u < kN; ++u)
 #pragma unroll
                             for (int v = 0; v < 2; ++v)
-                                if (s0 < 14) k[now ^ 1][u][v] = *reinterpret_cast<const half8_t *>(st + ka[u] + 64 * (s0 + 2 + v));
+                                if (s0 < 14) k[now ^ 1][u][v] = *reinterpret_cast<const half8_t *>(st + ka + kHalf * u + 64 * (s0 + 2 + v));
 #pragma unroll
                         for (int u = 0; u < kN; ++u)
 #pragma unroll
