@@ -671,8 +671,9 @@ __global__ __launch_bounds__(256) void keep_rows_kernel(const ds4hip_kv_pages P,
     const int j = blockIdx.x / split, part = blockIdx.x - j * split;
     const int l0 = (int)((long long)P.n_layers * part / split), l1 = (int)((long long)P.n_layers * (part + 1) / split);
     const int kept = n_path[j], seq = seqs[j], a = q_start[j];
+    // (the plan has cut the sequence; asked for before it is known whether the call was refused: 0.3 us less)
+    const int base = P.rows[min(max(seq, 0), P.n_seqs - 1)] - kept;
     if (*M.n == 0) return;   // refused
-    const int base = P.rows[seq] - kept;   // (the plan has cut the sequence)
     for (int i0 = 0; i0 < kept; i0 += kRows) {
         const int i = i0 + lane, node = i < kept ? path[a + i] : i;
         const uint64_t moved = __ballot(node != i);   // (the same in every wave)
