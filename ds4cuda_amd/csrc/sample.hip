@@ -337,8 +337,8 @@ __device__ __forceinline__ unsigned long long units(double w) {
 // 2^-63.9. What is rounded on the way grows with the distance, so the bins keep the order of logits.
 struct Bins {
     float top, scale;
-    // (half the difference of two logits stays in fp32's range, and twice the scale does)
-    __device__ __forceinline__ float steps(float x) const { return fminf(fmaf(x, -0.5f, 0.5f * top) * (2.0f * scale), (float)(kBins - 1)); }
+    float half = 0.5f * top, twice = 2.0f * scale;   // (half the difference of two logits stays in fp32's range, and twice the scale does)
+    __device__ __forceinline__ float steps(float x) const { return fminf(fmaf(x, -0.5f, half) * twice, (float)(kBins - 1)); }
     __device__ __forceinline__ int operator()(float x) const { return kBins - 1 - (int)steps(x); }
     // of x in its bin: the part of kBins that it lies in
     __device__ __forceinline__ int part(float x) const {
