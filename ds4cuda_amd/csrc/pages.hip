@@ -10,7 +10,7 @@
 //
 // What bounds them. A plan is a chain of loads that wait for each other (jobs, rows, table
 // entries, counts) and of barriers: 4.0 us to extend 6 sequences, 8.2 to fork 6, 3.4 to free
-// them, 7.4 to compact a pool of 352 pages, 5.2 to accept 2 trees of up to 9 nodes, 9.6 for 64 of
+// them, 7.4 to compact a pool of 352 pages, 4.8 to accept 2 trees of up to 9 nodes, 8.1 for 64 of
 // up to 48. The moves run at memory speed: deep copies of four sequences of 7001 rows in 43 layers
 // (647 MB read and written) 140 us, 4.6 TB/s of the 5.1 that a large copy reaches.
 

@@ -24,7 +24,8 @@
 // What bounds it. The scan: bytes where no row needs a sum (256 rows of 129280 bf16, 66 MB: 12.0 us, 5.5 TB/s, as a
 // large copy), the weights' 18 instructions a logit where all do (30 us; filters that differ: 21). The pick: a chain of
 // loads that wait for each other (parameters and maxima 1.3 us, the border 2, the candidates' groups 3.4, their
-// comparison 1 and up, the sums 0.7), and in a flat row the fp64 weights of all its logits, twice, on one CU.
+// comparison 1 and up, the sums 0.7), and in a flat row the fp64 weights of all its logits, twice, on one CU: one row of
+// 129280 of which thousands stay adds 110 us to a call of any number of rows (256 rows 36 us without such a row, 145 to 153 with).
 
 #include "ds4hip_common.h"
 #include "scan.h"
@@ -788,8 +789,8 @@ __global__ __launch_bounds__(kThreads) void row_kernel(const Args A) {
     settle<kF32>(A, S, R, row, bins, n, all);
 }
 
-// A workgroup a row, the groups' maxima in registers. One row of 129280 with k and p: 8.6 us; 256 rows with filters of
-// their own: 15 (k = 200: 13 alone); 24 flat rows of 65536 with p: 85, of which bins of all weights 25, the cut's
+// A workgroup a row, the groups' maxima in registers. One row of 129280 with k and p: 9.0 us; 256 rows with filters of
+// their own: 15 (k = 200: 13 alone); 24 flat rows of 65536 with p: 86, of which bins of all weights 25, the cut's
 // bin gathered 10, the draw 27 (a row on one CU: the host does not know which rows are flat, and
 // further launches for them would cost the others about 3 us each).
 template <bool kF32>

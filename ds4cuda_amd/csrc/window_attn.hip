@@ -24,8 +24,8 @@
 // of a few tiles are launch, the queries, the first rows and the outputs one after the other (about 20 us).
 // (A workgroup's place on the line by XCD, so that neighbours share an L2, changed nothing:
 // the rows come from there already.)
-// Trees of 64 heads: 16 of up to 24 nodes after up to 8192 rows (80 GFLOP) 160 us with 14 to merge, 75 tiles a
-// workgroup in 1.7 parts on the average; 512 nodes after 60000 rows 0.88 PFLOP/s; 48 of up to 13 in a window of 128 rows
+// Trees of 64 heads: 16 of up to 24 nodes after up to 8192 rows (80 GFLOP) 159 us a call (traced, one after the other,
+// 164 and 14 to merge), 75 tiles a workgroup in 1.7 parts on the average; 512 nodes after 60000 rows 0.88 PFLOP/s; 48 of up to 13 in a window of 128 rows
 // 30 us, one of 7 after 1500 rows 28 and 6.4 to merge: launch, line (4), queries and first rows (7), tiles (1.6), outputs (3).
 
 #include "attn_tile.h"
