@@ -110,8 +110,8 @@ int ds4hip_kv_pages_keep(const ds4hip_kv_pages *p, const int32_t *seqs, const in
  * [n_nodes], as ds4hip_flash_attn_tree_fp8 takes the nodes): each node's parent, its drafted token, and
  * the token that follows it (sampled; < 0 agrees with no draft). A path begins with node 0 and goes on with the first
  * node that has its last one as parent and that one's target as token, until there is none. path receives the
- * nodes (-1 behind them and where no job has nodes), n_path their numbers and next [n_jobs] the target of
- * each last one: the token that the step adds behind the drafts (no nodes: 0 and -1). Where the call is
+ * nodes (-1 behind them and where no job has nodes, also where there are no jobs), n_path their numbers and next [n_jobs] the
+ * target of each last one: the token that the step adds behind the drafts (no nodes: 0 and -1). Where the call is
  * refused, path and next are -1 and n_path 0. -22: also more than DS4HIP_TREE_MAX_NODES nodes. */
 int ds4hip_kv_pages_accept(const ds4hip_kv_pages *p, const int32_t *seqs, const int32_t *q_start, int n_jobs,
                            const int32_t *parents, const int32_t *tokens, const int32_t *targets, int n_nodes,
